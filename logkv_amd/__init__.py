@@ -13,3 +13,4 @@ from . import beta_log_kv  # noqa: F401
 from .kv_compression import cache_compression_snapshot, summarize_compression  # noqa: F401
 from .streaming import LogKVStreamingAttention  # noqa: F401
 from .flush_group import flush_grouping, set_flush_grouping  # noqa: F401
+from .row_attention import EvictedRows, log_kv_evict, log_kv_tree_attention, log_kv_weight_attention  # noqa: F401

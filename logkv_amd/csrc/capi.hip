@@ -9,6 +9,7 @@
 #include <mutex>
 
 #include "route.hpp"
+#include "rows.hpp"
 #include "unified.hpp"
 
 thread_local const char* logkv::g_refusal = nullptr;
@@ -816,6 +817,96 @@ int logkv_chunk_attention_backward(const logkv_attention_args* a, const int32_t*
   const int rc = logkv::launch_chunk_backward(*a, table + table_ints - 1, *gr, static_cast<float*>(ws),
                                               static_cast<hipStream_t>(stream));
   if (rc) return launch_failed(rc, "attention backward");
+  return LOGKV_OK;
+}
+
+namespace {
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Whether rows of 16-bit features can be read in 16-byte units: the first one and every stride.
+bool unit_rows(const void* p, int64_t sb, int64_t sg, int64_t st) {
+  return aligned16(p) && sb % 8 == 0 && sg % 8 == 0 && st % 8 == 0;
+}
+
+int check_rows_shape(const logkv_rows_args* a) {
+  if (!a) return fail(LOGKV_EINVAL, "row attention args are NULL");
+  if (a->n_batch < 1 || a->n_groups < 1 || a->n_heads < 1 || a->n_heads % a->n_groups || a->tq < 1)
+    return fail(LOGKV_EINVAL, "row attention shape: batch %d, heads %d, groups %d, queries %d", a->n_batch, a->n_heads,
+                a->n_groups, a->tq);
+  if (int64_t(a->n_batch) * a->n_groups > 65535 || int64_t(a->n_heads / a->n_groups) * a->tq > 1 << 19)
+    return fail(LOGKV_EINVAL, "row attention takes at most 65535 lanes and 2^19 query rows per KV group");
+  if (a->dk < 8 || a->dv < 8 || a->dk % 8 || a->dv % 8 || a->dk > 256 || a->dv > 256)
+    return fail(LOGKV_EINVAL, "row attention widths must be multiples of 8 in [8, 256], got %d/%d", a->dk, a->dv);
+  if (a->cap < 0 || a->cap > 1 << 30) return fail(LOGKV_EINVAL, "cache capacity %d outside [0, 2^30]", a->cap);
+  if (a->dtype != LOGKV_BF16 && a->dtype != LOGKV_F16) return fail(LOGKV_EINVAL, "row attention takes bf16 or fp16");
+  return LOGKV_OK;
+}
+
+int check_rows(const logkv_rows_args* a, const void* ws, int64_t ws_bytes, bool weights) {
+  int rc = check_rows_shape(a);
+  if (rc) return rc;
+  if (!a->q || !a->k || !a->v || !a->out || (a->cap && (!a->cache_k || !a->cache_v)))
+    return fail(LOGKV_EINVAL, "row attention buffer is NULL");
+  if (!unit_rows(a->q, a->q_sb, a->q_sh, a->q_st) || !unit_rows(a->k, a->k_sb, a->k_sg, a->k_st) ||
+      !unit_rows(a->v, a->v_sb, a->v_sg, a->v_st) ||
+      (a->cap && (!unit_rows(a->cache_k, a->ck_sb, a->ck_sg, a->ck_st) ||
+                  !unit_rows(a->cache_v, a->cv_sb, a->cv_sg, a->cv_st))))
+    return fail(LOGKV_EINVAL, "row attention rows must be 16-byte aligned (strides multiples of 8 elements)");
+  if (reinterpret_cast<uintptr_t>(a->out) % 8 || a->o_sb % 4 || a->o_sh % 4 || a->o_st % 4)
+    return fail(LOGKV_EINVAL, "row attention output rows must be 8-byte aligned");
+  if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return fail(LOGKV_EINVAL, "attention scale must be positive");
+  if (weights ? !a->weights || a->visible || a->bias : !a->visible || a->weights || a->counts)
+    return fail(LOGKV_EINVAL, weights ? "weight attention takes weights, no bias and no mask"
+                                      : "tree attention takes a mask of the own rows, no weights and no counts");
+  if (!aligned16(ws) || !ws || ws_bytes < logkv::rows_launch(*a, weights, nullptr).bytes)
+    return fail(LOGKV_EINVAL, "row attention workspace too small");
+  return LOGKV_OK;
+}
+
+}  // namespace
+
+int64_t logkv_rows_workspace_bytes(const logkv_rows_args* a) {
+  if (check_rows_shape(a)) return -1;
+  return logkv::rows_launch(*a, a->weights != nullptr, nullptr).bytes;
+}
+
+int logkv_tree_attention(const logkv_rows_args* a, void* ws, int64_t ws_bytes, void* stream) {
+  int rc = check_rows(a, ws, ws_bytes, false);
+  if (rc) return rc;
+  rc = logkv::launch_rows_attention(*a, logkv::rows_launch(*a, false, ws), static_cast<hipStream_t>(stream));
+  if (rc) return launch_failed(rc, "tree attention");
+  return LOGKV_OK;
+}
+
+int logkv_weight_attention(const logkv_rows_args* a, void* ws, int64_t ws_bytes, void* stream) {
+  int rc = check_rows(a, ws, ws_bytes, true);
+  if (rc) return rc;
+  rc = logkv::launch_rows_attention(*a, logkv::rows_launch(*a, true, ws), static_cast<hipStream_t>(stream));
+  if (rc) return launch_failed(rc, "weight attention");
+  return LOGKV_OK;
+}
+
+int logkv_evict_rows(const logkv_evict_args* a, void* stream) {
+  if (!a) return fail(LOGKV_EINVAL, "eviction args are NULL");
+  if (a->n_batch < 1 || a->n_groups < 1 || int64_t(a->n_batch) * a->n_groups > 65535 || a->cap < 1 || a->cap > 1 << 30)
+    return fail(LOGKV_EINVAL, "eviction shape: batch %d, groups %d, capacity %d", a->n_batch, a->n_groups, a->cap);
+  if (a->keep < 1 || a->recent < 0 || a->recent > a->keep)
+    return fail(LOGKV_EINVAL, "eviction keeps %d rows, the last %d among them", a->keep, a->recent);
+  if (a->size != 1 && a->size != 2 && a->size != 4) return fail(LOGKV_EINVAL, "features of %d bytes", a->size);
+  if (a->dk < 1 || a->dv < 1 || a->dk > 4096 || a->dv > 4096 || int64_t(a->dk) * a->size % 16 || int64_t(a->dv) * a->size % 16)
+    return fail(LOGKV_EINVAL, "evicted rows must be multiples of 16 bytes, got %d and %d features of %d bytes", a->dk,
+                a->dv, a->size);
+  if (!a->cache_k || !a->cache_v || !a->weights || !a->out_k || !a->out_v || !a->out_weights || !a->kept ||
+      !a->out_lengths || !a->positions != !a->out_positions)
+    return fail(LOGKV_EINVAL, "eviction buffer is NULL");
+  if (!aligned16(a->cache_k) || !aligned16(a->cache_v) || !aligned16(a->out_k) || !aligned16(a->out_v))
+    return fail(LOGKV_EINVAL, "evicted rows must be 16-byte aligned");
+  for (int64_t s : {a->ck_sb, a->ck_sg, a->ck_st, a->cv_sb, a->cv_sg, a->cv_st, a->ok_sb, a->ok_sg, a->ok_st, a->ov_sb,
+                    a->ov_sg, a->ov_st})
+    if (s * a->size % 16) return fail(LOGKV_EINVAL, "evicted rows must be 16-byte aligned (strides)");
+  const int rc = logkv::launch_evict(*a, static_cast<hipStream_t>(stream));
+  if (rc) return launch_failed(rc, "eviction");
   return LOGKV_OK;
 }
 

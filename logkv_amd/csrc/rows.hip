@@ -1,0 +1,348 @@
+// Attention over a cache's rows and the call's own rows: what follows the streamed products
+// (rows_stream.hip), and the sizes of a launch.
+#include <algorithm>
+
+#include "rows.hpp"
+
+namespace logkv {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWeightRows = 4 * kThreads;   // score columns per block of the weight sums
+constexpr int kAppendUnits = 4 * kThreads;  // 16-byte units per block of the append
+
+int64_t align256(int64_t x) { return (x + 255) & ~int64_t(255); }
+
+// Partials join under the largest maximum; an empty one has maximum -inf and zero sums, one of NaN
+// logits alone -inf and NaN, so a sum of zero (and only that) means that a query sees no row.
+
+// Maximum and sum of a query over its splits' partials; `threads` lanes of a wave (a power of two)
+// take every threads-th split and fold theirs by xor.
+__device__ __forceinline__ void fold_splits(const float* base, int64_t step, int splits, int dv, int j, int threads,
+                                            float& m, float& lsum) {
+  m = -__builtin_inff();
+  for (int sp = j; sp < splits; sp += threads) m = fmaxf(m, base[sp * step + dv]);
+  for (int off = threads / 2; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
+  lsum = 0.f;
+  const float top = m == -__builtin_inff() ? 0.f : m;
+  for (int sp = j; sp < splits; sp += threads)
+    lsum += base[sp * step + dv + 1] * __builtin_amdgcn_exp2f(base[sp * step + dv] - top);
+  for (int off = threads / 2; off >= 1; off >>= 1) lsum += __shfl_xor(lsum, off, kWave);
+}
+
+}  // namespace
+
+// Roles by blockIdx.x, all of one launch:
+//  * [0, out_blocks): outputs. TQ threads per query, four features each; the block's other factor
+//    is shared by queries and by groups of splits (QPB queries x SG groups), whose sums are
+//    joined in group order.
+//  * [out_blocks, + weight_blocks): weights of up to 16 queries from the stored products,
+//    p = 2^(s c2 - m) / l, one score column a thread and four at a time.
+//  * the rest: the own rows copied behind the cache's rows.
+template <int DT, int TQ, int SG>
+__global__ __launch_bounds__(kThreads) void rows_finish_kernel(logkv_rows_args a, RowsLaunch r, int out_blocks,
+                                                               int weight_blocks) {
+  typedef Elem<DT> E;
+  constexpr int QPB = kThreads / (TQ * SG);
+  const int lane = blockIdx.y, G = a.n_groups, b = lane / G, g = lane % G;
+  const int rep = a.n_heads / G, nq = rep * a.tq, tid = threadIdx.x;
+  const int stride = a.dv + kRowsPartTail;
+  const int64_t step = static_cast<int64_t>(nq) * stride;
+  const float* lane_part = r.part + static_cast<int64_t>(lane) * r.splits * step;
+  int blk = blockIdx.x;
+  if (blk < out_blocks) {
+    __shared__ __align__(16) float acc_s[QPB][SG][4 * TQ];
+    __shared__ float m_s[QPB][SG], l_s[QPB][SG];
+    const int qs = tid / (TQ * SG), sg = tid / TQ % SG, d = 4 * (tid % TQ);
+    const int qi = blk * QPB + qs;
+    const bool there = qi < nq && d < a.dv;
+    const float* base = lane_part + static_cast<int64_t>(min(qi, nq - 1)) * stride;
+    float m = -__builtin_inff(), lsum = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    // Eight splits' loads at a time, joined under the running maximum.
+    for (int s0 = sg; s0 < r.splits; s0 += 8 * SG) {
+      float2 ml[8];
+      f32x4 x[8];
+      float mx = m;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int sp = s0 + k * SG;
+        ml[k] = make_float2(-__builtin_inff(), 0.f);
+        x[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (there && sp < r.splits) {
+          ml[k] = *reinterpret_cast<const float2*>(base + sp * step + a.dv);
+          x[k] = *reinterpret_cast<const f32x4*>(base + sp * step + d);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mx = fmaxf(mx, ml[k].x);
+      const float top = mx == -__builtin_inff() ? 0.f : mx;
+      const float corr = __builtin_amdgcn_exp2f(m - top);
+      lsum *= corr;
+      acc *= corr;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float f = __builtin_amdgcn_exp2f(ml[k].x - top);
+        lsum += ml[k].y * f;
+        acc += x[k] * f;
+      }
+      m = mx;
+    }
+    if constexpr (SG > 1) {
+      *reinterpret_cast<f32x4*>(&acc_s[qs][sg][d]) = acc;
+      if (d == 0) {
+        m_s[qs][sg] = m;
+        l_s[qs][sg] = lsum;
+      }
+      __syncthreads();
+      if (sg) return;
+      float mx = m;
+#pragma unroll
+      for (int k = 1; k < SG; ++k) mx = fmaxf(mx, m_s[qs][k]);
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+      float total = 0.f;
+      const float top = mx == -__builtin_inff() ? 0.f : mx;
+#pragma unroll
+      for (int k = 0; k < SG; ++k) {
+        const float f = __builtin_amdgcn_exp2f(m_s[qs][k] - top);
+        total += l_s[qs][k] * f;
+        sum += *reinterpret_cast<const f32x4*>(&acc_s[qs][k][d]) * f;
+      }
+      m = mx;
+      lsum = total;
+      acc = sum;
+    }
+    if (!there) return;
+    const bool empty = lsum == 0.f;
+    if (r.lse && d == 0)
+      r.lse[static_cast<int64_t>(lane) * nq + qi] = empty ? __builtin_inff() : m + __builtin_amdgcn_logf(lsum) - E::kShift;
+    uint16_t y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = empty ? uint16_t(0) : E::from_f32(acc[k] / lsum);
+    LOGKV_G uint16_t* o = gp(a.out) + b * a.o_sb + (g * rep + qi / a.tq) * a.o_sh + qi % a.tq * a.o_st + d;
+    *reinterpret_cast<LOGKV_G uint2*>(o) =
+        make_uint2(y[0] | static_cast<uint32_t>(y[1]) << 16, y[2] | static_cast<uint32_t>(y[3]) << 16);
+    return;
+  }
+  blk -= out_blocks;
+  const int n = rows_in_use(a, b), own = own_rows(a, b);
+  if (blk < weight_blocks) {
+    __shared__ float qm[16], ql[16];
+    const int np = (n + kRowTile - 1) / kRowTile * kRowTile;
+    const int c0 = blk * kWeightRows;
+    if (c0 >= np + own) return;
+    {
+      const int q = tid / 16;
+      if (q < nq) {
+        float m, lsum;
+        fold_splits(lane_part + static_cast<int64_t>(q) * stride, step, r.splits, a.dv, tid % 16, 16, m, lsum);
+        if (tid % 16 == 0) {
+          qm[q] = E::kShift - (m == -__builtin_inff() ? 0.f : m);
+          ql[q] = lsum == 0.f ? 0.f : 1.f / lsum;
+        }
+      }
+    }
+    __syncthreads();
+    const int c = c0 + 4 * tid;
+    if (c >= np + own) return;
+    const float c2 = a.scale * kLog2e;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    const float* row = r.scores + static_cast<int64_t>(lane) * nq * r.score_st + c;
+#pragma unroll 4
+    for (int q = 0; q < nq; ++q) {
+      const f32x4 s = *reinterpret_cast<const f32x4*>(row + q * r.score_st);
+      if (ql[q] == 0.f) continue;   // a query that sees nothing
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum[k] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], c2, qm[q])) * ql[q];
+    }
+    LOGKV_G float* wrow = gp(a.weights) + b * a.w_sb + g * a.w_sg;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (c + k < n) wrow[c + k] += sum[k];
+      else if (c + k >= np && c + k < np + own && n + (c + k - np) < a.cap) wrow[n + (c + k - np)] = sum[k];
+    }
+    return;
+  }
+  blk -= weight_blocks;
+  const int ku = a.dk / 8, vu = a.dv / 8, total = min(own, a.cap - n) * (ku + vu);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int i = blk * kAppendUnits + k * kThreads + tid;
+    if (i >= total) return;
+    const int t = i / (ku + vu), u = i % (ku + vu);
+    if (u < ku)
+      *(LOGKV_G uint4*)(gp(a.cache_k) + b * a.ck_sb + g * a.ck_sg + (n + t) * a.ck_st + 8 * u) =
+          *(const LOGKV_G uint4*)(gp(a.k) + b * a.k_sb + g * a.k_sg + t * a.k_st + 8 * u);
+    else
+      *(LOGKV_G uint4*)(gp(a.cache_v) + b * a.cv_sb + g * a.cv_sg + (n + t) * a.cv_st + 8 * (u - ku)) =
+          *(const LOGKV_G uint4*)(gp(a.v) + b * a.v_sb + g * a.v_sg + t * a.v_st + 8 * (u - ku));
+  }
+}
+
+// Weights of more than 16 queries: with a query's log-sum-exp L known, p = 2^(s c2 - L), summed over
+// the queries. S = Q K^T with the keys as columns, so a lane sums its own key over all queries in
+// registers: a wave holds 64 keys' operands for good and the block's queries pass through LDS, 16
+// rows a product. One wave owns a key: no atomics, a fixed order.
+constexpr int kSumKeys = 64;       // per wave
+constexpr int kSumQueries = 64;    // per staged tile
+template <int DT, int NS>
+__global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_args a, RowsLaunch r, int cache_blocks) {
+  typedef Elem<DT> E;
+  typedef typename E::vec8 vec8;
+  constexpr int kLd = 32 * NS + 8;
+  __shared__ __align__(16) uint16_t q_s[kSumQueries * kLd];
+  __shared__ __align__(16) float l_s[kSumQueries];
+  const int lane = blockIdx.y, G = a.n_groups, b = lane / G, g = lane % G;
+  const int rep = a.n_heads / G, nq = rep * a.tq, units = a.dk / 8;
+  const int w = wave_id(), l = lane_id(), col = l & 15, hq = l >> 4;
+  const int n = rows_in_use(a, b), own = own_rows(a, b);
+  // Blocks of the cache's rows, then of the own rows.
+  const bool of_cache = static_cast<int>(blockIdx.x) < cache_blocks;
+  const int rows = of_cache ? n : own;
+  const int b0 = (static_cast<int>(blockIdx.x) - (of_cache ? 0 : cache_blocks)) * 4 * kSumKeys;
+  if (b0 >= rows) return;
+  const int k0 = b0 + w * kSumKeys;
+  const LOGKV_G uint16_t* kr = of_cache ? gp(a.cache_k) + b * a.ck_sb + g * a.ck_sg : gp(a.k) + b * a.k_sb + g * a.k_sg;
+  const int64_t kst = of_cache ? a.ck_st : a.k_st;
+  vec8 kf[4][NS];
+#pragma unroll
+  for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (4 * s + hq < units) x = *(const LOGKV_G uint4*)(kr + min(k0 + 16 * kb + col, rows - 1) * kst + 32 * s + 8 * hq);
+      kf[kb][s] = __builtin_bit_cast(vec8, x);
+    }
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  const float c2 = a.scale * kLog2e;
+  for (int q0 = 0; q0 < nq; q0 += kSumQueries) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < kSumQueries * 4 * NS; i += kThreads) {
+      const int qq = i / (4 * NS), u = i % (4 * NS), qi = min(q0 + qq, nq - 1);
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (u < units)
+        x = *(const LOGKV_G uint4*)(gp(a.q) + b * a.q_sb + (g * rep + qi / a.tq) * a.q_sh + qi % a.tq * a.q_st + 8 * u);
+      *reinterpret_cast<uint4*>(&q_s[qq * kLd + 8 * u]) = x;
+    }
+    if (threadIdx.x < kSumQueries) {
+      const int qi = q0 + static_cast<int>(threadIdx.x);
+      l_s[threadIdx.x] = qi < nq ? r.lse[static_cast<int64_t>(lane) * nq + qi] : __builtin_inff();
+    }
+    __syncthreads();
+#pragma unroll
+    for (int qb = 0; qb < kSumQueries / 16; ++qb) {
+      f32x4 s[4];
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int st = 0; st < NS; ++st) {
+        const vec8 qf = *reinterpret_cast<const vec8*>(&q_s[(16 * qb + col) * kLd + 32 * st + 8 * hq]);
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) s[kb] = E::mfma16(qf, kf[kb][st], s[kb]);
+      }
+      // Element i is query 16 qb + 4 hq + i against key 16 kb + col.
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(&l_s[16 * qb + 4 * hq]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int qi = q0 + 16 * qb + 4 * hq + i, t = of_cache ? 0 : qi % a.tq;
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], c2, -lse[i]));
+          if (lse[i] == __builtin_inff() || (!of_cache && k0 + 16 * kb + col > t)) p = 0.f;
+          sum[kb] += p;
+        }
+      }
+    }
+  }
+  LOGKV_G float* wrow = gp(a.weights) + b * a.w_sb + g * a.w_sg;
+#pragma unroll
+  for (int kb = 0; kb < 4; ++kb) {
+    sum[kb] += __shfl_xor(sum[kb], 16, kWave);
+    sum[kb] += __shfl_xor(sum[kb], 32, kWave);
+    const int j = k0 + 16 * kb + col;
+    if (hq || j >= rows) continue;
+    if (of_cache) wrow[j] += sum[kb];
+    else if (n + j < a.cap) wrow[n + j] = sum[kb];
+  }
+}
+
+namespace {
+
+template <int DT, int TQ, int SG>
+void launch_finish(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
+  const int nq = a.n_heads / a.n_groups * a.tq, qpb = kThreads / (TQ * SG);
+  const int out_blocks = (nq + qpb - 1) / qpb;
+  const int weight_blocks = r.scores ? static_cast<int>((r.score_st + kWeightRows - 1) / kWeightRows) : 0;
+  const int append_blocks = r.causal ? (a.tq * (a.dk / 8 + a.dv / 8) + kAppendUnits - 1) / kAppendUnits : 0;
+  hipLaunchKernelGGL((rows_finish_kernel<DT, TQ, SG>), dim3(out_blocks + weight_blocks + append_blocks, a.n_batch * a.n_groups),
+                     dim3(kThreads), 0, stream, a, r, out_blocks, weight_blocks);
+}
+
+template <int DT>
+void launch_finish_type(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
+  const bool many = r.splits > 8;
+  if (a.dv <= 128) {
+    if (many) launch_finish<DT, 32, 8>(a, r, stream);
+    else launch_finish<DT, 32, 1>(a, r, stream);
+  } else {
+    if (many) launch_finish<DT, 64, 4>(a, r, stream);
+    else launch_finish<DT, 64, 1>(a, r, stream);
+  }
+}
+
+template <int DT>
+void launch_weights(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
+  constexpr int kKeys = 4 * kSumKeys;
+  const int cache_blocks = (a.cap + kKeys - 1) / kKeys;
+  const dim3 grid(cache_blocks + (a.tq + kKeys - 1) / kKeys, a.n_batch * a.n_groups);
+  if (a.dk <= 64) hipLaunchKernelGGL((rows_weight_kernel<DT, 2>), grid, dim3(kThreads), 0, stream, a, r, cache_blocks);
+  else if (a.dk <= 128) hipLaunchKernelGGL((rows_weight_kernel<DT, 4>), grid, dim3(kThreads), 0, stream, a, r, cache_blocks);
+  else hipLaunchKernelGGL((rows_weight_kernel<DT, 8>), grid, dim3(kThreads), 0, stream, a, r, cache_blocks);
+}
+
+}  // namespace
+
+RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws) {
+  const int64_t lanes = static_cast<int64_t>(a.n_batch) * a.n_groups, nq = static_cast<int64_t>(a.n_heads / a.n_groups) * a.tq;
+  const bool wide = a.dk > 128 || a.dv > 128;
+  RowsLaunch r{};
+  r.causal = causal ? 1 : 0;
+  r.cols = nq <= 16 ? 1 : nq <= 32 || wide ? 2 : 4;
+  const int64_t q_blocks = (nq + 16 * r.cols - 1) / (16 * r.cols);
+  const int64_t tiles = (a.cap + kRowTile - 1) / kRowTile + (a.tq + kRowTile - 1) / kRowTile;
+  // One share per resident block, none shorter than a tile for each of its waves.
+  const int64_t resident = wide || r.cols == 4 ? 256 : 512;
+  r.splits = static_cast<int>(std::max<int64_t>(
+      1, std::min<int64_t>({kMaxRowSplits, (tiles + 3) / 4, resident / std::max<int64_t>(1, lanes * q_blocks)})));
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  int64_t off = 0;
+  auto take = [&](int64_t floats) {
+    float* p = base ? reinterpret_cast<float*>(base + off) : nullptr;
+    off += align256(4 * floats);
+    return p;
+  };
+  r.part = take(lanes * r.splits * nq * (a.dv + kRowsPartTail));
+  if (causal && nq <= 16) {
+    r.score_st = tiles * kRowTile;
+    r.scores = take(lanes * nq * r.score_st);
+  } else if (causal) {
+    r.lse = take(lanes * nq);
+  }
+  r.bytes = off;
+  return r;
+}
+
+int launch_rows_attention(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
+  const int rc = launch_rows_stream(a, r, stream);
+  if (rc) return rc;
+  if (a.dtype == LOGKV_BF16) launch_finish_type<LOGKV_BF16>(a, r, stream);
+  else launch_finish_type<LOGKV_F16>(a, r, stream);
+  if (r.lse) {
+    if (a.dtype == LOGKV_BF16) launch_weights<LOGKV_BF16>(a, r, stream);
+    else launch_weights<LOGKV_F16>(a, r, stream);
+  }
+  return hipGetLastError() == hipSuccess ? LOGKV_OK : LOGKV_ERUNTIME;
+}
+
+}  // namespace logkv

@@ -1,0 +1,273 @@
+"""Attention over an exact cache's rows and the rows of the call itself, and eviction by attention weight.
+
+Rows are ``[batch, groups, capacity, features]`` (bfloat16 or float16), ``lengths`` the rows in use per
+batch row. No counterpart in the reference, whose LogKV path masks nothing among its in-flight rows but
+the causal tail and keeps no exact cache that attention weight cuts:
+
+* ``log_kv_tree_attention``: a tree of drafted tokens over a cache that is only read, for the
+  verification step of speculative decoding (``LogKVStreamingAttention.draft`` runs it over the
+  compressed cache's packed rows, with their log-mass as bias);
+* ``log_kv_weight_attention``: causal attention of new tokens that adds each row's probability to its
+  running weight and stores the new rows behind the cache's;
+* ``log_kv_evict``: the rows of every (batch row, KV head) cut to a budget by those weights.
+
+All run in liblogkv_hip.so on the current stream of the tensors' device, allocate their outputs and
+scratch through torch, never wait for the host and can be captured into a HIP graph. They are for
+inference: none has a gradient.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import math
+from contextlib import nullcontext
+from typing import NamedTuple
+
+import torch
+
+from ._lib import check, check_activation_dtype, ptr, require_device, stream_of
+from ._rows import BF16, F16, EvictArgs, RowsArgs, rows_lib
+
+_ROW_DTYPES = {torch.bfloat16: BF16, torch.float16: F16}
+
+
+class EvictedRows(NamedTuple):
+    """What ``log_kv_evict`` keeps: rows ``k / v [B, G, keep, d]``, ``weights`` and ``positions [B, G, keep]``,
+    ``kept`` (int32 ``[B, G, keep]``, the rows' indices before, -1 behind the last) and ``lengths`` (int32 ``[B]``)."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    weights: torch.Tensor
+    positions: torch.Tensor | None
+    kept: torch.Tensor
+    lengths: torch.Tensor
+
+
+def _on(device):
+    """The device as the current one while a launch is issued."""
+    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _no_grad(*tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise NotImplementedError("row attention is for inference: it has no gradient (run it under torch.no_grad())")
+
+
+def _small_rows(x, dtype):
+    """Rows of the call in the cache's dtype, readable in 16-byte units."""
+    if x.dtype != dtype:
+        check_activation_dtype(x.dtype)
+        x = x.to(dtype)
+    sb, sh, st, sd = x.stride()
+    if sd != 1 or (sb | sh | st) % 8 or x.data_ptr() % 16:
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    return x
+
+
+def _lengths(lengths, batch, cap, device, room=0):
+    """(tensor or None, stride, added rows) of an int or an int32 tensor ``[B]``."""
+    if isinstance(lengths, torch.Tensor):
+        if lengths.shape != (batch,) or lengths.device != device or lengths.dtype not in (torch.int32, torch.int64):
+            raise ValueError("lengths must be an int or an int32 tensor [batch] on the cache's device")
+        return lengths.to(torch.int32).contiguous(), 1, 0
+    lengths = int(lengths)
+    if not 0 <= lengths <= cap - room:
+        raise ValueError(f"{lengths} rows and {room} new ones do not fit the cache's {cap}")
+    return None, 0, lengths
+
+
+def _attention(q, k, v, cache_k, cache_v, scale, lengths, room, *, bias=None, visible=None, counts=None, weights=None,
+               lengths2=None, len_add=0):
+    """Checks and launch of both attentions."""
+    if q.ndim != 4 or k.ndim != 4 or v.ndim != 4 or cache_k.ndim != 4 or cache_v.ndim != 4:
+        raise ValueError("queries, rows and cache must be 4-dimensional")
+    batch, heads, tq, dk = q.shape
+    groups, cap, dv = cache_k.size(1), cache_k.size(2), cache_v.size(3)
+    device, dtype = cache_k.device, cache_k.dtype
+    if dtype not in _ROW_DTYPES or cache_v.dtype != dtype:
+        raise ValueError("the cache must be bfloat16 or float16")
+    if (cache_k.shape != (batch, groups, cap, dk) or cache_v.shape != (batch, groups, cap, dv) or groups < 1
+            or heads % groups or heads < 1 or tq < 1 or batch < 1):
+        raise ValueError("cache rows must be [B, G, capacity, d] with G dividing the query heads")
+    if k.shape != (batch, groups, tq, dk) or v.shape != (batch, groups, tq, dv):
+        raise ValueError("the call's rows must be [B, G, T, d], one per query position")
+    for t, what in ((cache_k, "cache_k"), (cache_v, "cache_v")):
+        require_device(t, what)
+        if cap and (t.stride(3) != 1 or (t.stride(0) | t.stride(1) | t.stride(2)) % 8 or t.data_ptr() % 16):
+            raise ValueError(f"{what} rows must be 16-byte aligned with contiguous features")
+    if cache_v.device != device or q.device != device or k.device != device or v.device != device:
+        raise ValueError("all tensors must be on the cache's device")
+    if not (math.isfinite(scale) and scale > 0.0):
+        raise ValueError("attention scale must be positive")
+    _no_grad(q, k, v, cache_k, cache_v)
+    out_dtype = q.dtype
+    q, k, v = _small_rows(q, dtype), _small_rows(k, dtype), _small_rows(v, dtype)
+    if lengths2 is None:
+        lengths, len_stride, len_add = _lengths(lengths, batch, cap, device, room)
+    else:
+        len_stride = 0
+    if bias is not None:
+        if bias.shape != (batch, groups, cap) or bias.device != device or bias.dtype not in (torch.float32, dtype):
+            raise ValueError("bias must be [B, G, capacity] on the cache's device, float32 or the cache's dtype")
+        _no_grad(bias)
+    out = torch.empty((batch, heads, tq, dv), dtype=dtype, device=device)
+    args = RowsArgs(
+        q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
+        cache_k.data_ptr(), *cache_k.stride()[:3], cache_v.data_ptr(), *cache_v.stride()[:3],
+        ptr(bias), *(bias.stride() if bias is not None else (0, 0, 0)), ptr(lengths), ptr(lengths2),
+        ptr(visible), *(visible.stride()[:2] if visible is not None else (0, 0)), ptr(counts),
+        ptr(weights), *(weights.stride()[:2] if weights is not None else (0, 0)),
+        out.data_ptr(), *out.stride()[:3], batch, heads, groups, tq, cap, dk, dv, _ROW_DTYPES[dtype], len_stride,
+        len_add, 0 if bias is None or bias.dtype == torch.float32 else 1, scale)
+    handle = rows_lib()
+    need = handle.logkv_rows_workspace_bytes(C.byref(args))
+    if need < 0:
+        raise ValueError("row attention: " + handle.logkv_last_error().decode(errors="replace"))
+    workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    with _on(device):
+        if weights is None:
+            check(handle.logkv_tree_attention(C.byref(args), workspace.data_ptr(), need, stream_of(device)),
+                  "logkv_tree_attention")
+        else:
+            check(handle.logkv_weight_attention(C.byref(args), workspace.data_ptr(), need, stream_of(device)),
+                  "logkv_weight_attention")
+    return out if out_dtype == dtype else out.to(out_dtype)
+
+
+def _visible(visible, batch, tq, device):
+    """The drafted rows' mask as uint8 ``[B, T, T]`` (batch stride 0 where it is shared)."""
+    if (not isinstance(visible, torch.Tensor) or visible.dtype not in (torch.bool, torch.uint8)
+            or visible.shape not in ((tq, tq), (batch, tq, tq)) or visible.device != device):
+        raise ValueError("visible must be a bool tensor [T, T] or [B, T, T] on the cache's device")
+    if visible.dtype == torch.bool:
+        visible = visible.view(torch.uint8)
+    if visible.stride(-1) != 1:
+        visible = visible.contiguous()
+    return visible.expand(batch, tq, tq)
+
+
+def log_kv_tree_attention(q, k, v, cache_k, cache_v, lengths, visible, scale, *, bias=None):
+    """Attention of T drafted tokens over a cache and each other, ``[B, n_heads, T, dv]``.
+
+    ``q [B, n_heads, T, dk]``, the drafted rows ``k [B, G, T, dk]`` and ``v [B, G, T, dv]``; ``cache_k / cache_v
+    [B, G, capacity, d]`` with ``lengths`` rows in use (an int, or an int32 tensor ``[B]`` read on the device and
+    held to the capacity). Every token sees all rows in use, and the drafted row r where ``visible[t, r]`` (bool,
+    ``[T, T]`` or ``[B, T, T]``; a tree's mask has each token's ancestors and itself). ``bias`` (``[B, G, capacity]``,
+    float32 or the cache's dtype, any strides) is added to the scaled logits; -inf hides a row. A token that sees
+    nothing gets zeros, and what hidden rows hold (NaN, infinities) reaches no output.
+
+    Queries and drafted rows of another activation dtype are rounded to the cache's, and the output is returned
+    in the queries'. The cache is only read: commit the accepted tokens with the cache's own call."""
+    visible = _visible(visible, q.size(0), q.size(2), cache_k.device)
+    return _attention(q, k, v, cache_k, cache_v, float(scale), lengths, 0, bias=bias, visible=visible)
+
+
+def log_kv_weight_attention(q, k, v, cache_k, cache_v, weights, lengths, scale, *, counts=None):
+    """Causal attention of T new tokens over a cache and themselves, ``[B, n_heads, T, dv]``, that keeps the
+    rows' attention weights.
+
+    In place, with n = ``lengths[b]`` rows in use: ``weights[b, g, j] += sum of row j's probabilities`` over the KV
+    head's query heads and the T queries for j < n, ``weights[b, g, n + t]`` set to new row t's sum, and the new rows
+    stored at cache rows n + t. ``lengths`` itself is left to the caller (the rows in use are n + T afterwards); as
+    an int tensor it is read on the device, and rows past the capacity are attended to but not stored. ``counts``
+    (int32 ``[B]``) gives the tokens that really exist per batch row of a padded batch: the others' outputs are zeros,
+    they add no weight and are not stored. ``weights`` is float32 ``[B, G, capacity]`` with contiguous rows."""
+    batch, groups, cap = cache_k.shape[:3]
+    if (weights.shape != (batch, groups, cap) or weights.dtype != torch.float32 or weights.device != cache_k.device
+            or weights.stride(2) != 1 or cap < 1):
+        raise ValueError("weights must be float32 [B, G, capacity] on the cache's device with contiguous rows")
+    if counts is not None:
+        if counts.shape != (batch,) or counts.device != cache_k.device or counts.dtype not in (torch.int32, torch.int64):
+            raise ValueError("counts must be an int32 tensor [batch] on the cache's device")
+        counts = counts.to(torch.int32).contiguous()
+    return _attention(q, k, v, cache_k, cache_v, float(scale), lengths, q.size(2), counts=counts, weights=weights)
+
+
+def _span(t):
+    """First and one past the last byte that a tensor's elements occupy."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+    return t.data_ptr(), t.data_ptr() + last * t.element_size()
+
+
+def _evict_rows_ok(t):
+    size = t.element_size()
+    return t.stride(3) == 1 and not any(s * size % 16 for s in t.stride()[:3]) and t.data_ptr() % 16 == 0
+
+
+def log_kv_evict(cache_k, cache_v, weights, lengths, keep, *, recent=0, positions=None, out=None):
+    """Cut every (batch row, KV head) of a cache to its last ``recent`` rows and, up to ``keep`` in all, its other
+    rows of largest weight, kept in their order; returns ``EvictedRows``.
+
+    ``cache_k / cache_v [B, G, capacity, d]`` (rows of a multiple of 16 bytes, of 1, 2 or 4 byte elements), ``weights``
+    float32 ``[B, G, capacity]``, ``lengths`` an int or an int32 tensor ``[B]``, ``positions`` optionally int64
+    ``[B, G, capacity]``. Equal weights keep the lowest index, NaN counts as the largest. A sequence of at most
+    ``keep`` rows keeps them all; rows behind a sequence's last are zeros (-1 in ``kept`` and ``positions``).
+
+    The result is new tensors, or ``out``: an ``EvictedRows`` of buffers of at least ``keep`` rows that do not overlap
+    the inputs (a cache's second buffer set), of which the first ``keep`` rows are written."""
+    if cache_k.ndim != 4 or cache_v.ndim != 4 or cache_k.shape[:3] != cache_v.shape[:3]:
+        raise ValueError("cache rows must be [B, G, capacity, d]")
+    batch, groups, cap, dk = cache_k.shape
+    dv, device = cache_v.size(3), cache_k.device
+    keep, recent = int(keep), int(recent)
+    if keep < 1 or not 0 <= recent <= keep:
+        raise ValueError("keep must be at least 1, recent between 0 and keep")
+    require_device(cache_k, "cache_k")
+    if cache_v.device != device or cache_v.dtype != cache_k.dtype or weights.device != device:
+        raise ValueError("all tensors must be on the cache's device, keys and values of one dtype")
+    if weights.shape != (batch, groups, cap) or weights.dtype != torch.float32 or weights.stride(2) != 1:
+        raise ValueError("weights must be float32 [B, G, capacity] with contiguous rows")
+    if positions is not None and (positions.shape != (batch, groups, cap) or positions.dtype != torch.int64
+                                  or positions.stride(2) != 1 or positions.device != device):
+        raise ValueError("positions must be int64 [B, G, capacity] with contiguous rows")
+    if not (_evict_rows_ok(cache_k) and _evict_rows_ok(cache_v)):
+        raise ValueError("cache rows must be 16-byte aligned with contiguous features")
+    _no_grad(cache_k, cache_v, weights)
+    lengths, _, len_add = _lengths(lengths, batch, cap, device)
+    if out is None:
+        out = EvictedRows(
+            torch.empty((batch, groups, keep, dk), dtype=cache_k.dtype, device=device),
+            torch.empty((batch, groups, keep, dv), dtype=cache_k.dtype, device=device),
+            torch.empty((batch, groups, keep), dtype=torch.float32, device=device),
+            None if positions is None else torch.empty((batch, groups, keep), dtype=torch.int64, device=device),
+            torch.empty((batch, groups, keep), dtype=torch.int32, device=device),
+            torch.empty(batch, dtype=torch.int32, device=device))
+    else:
+        _check_evict_out(out, cache_k, cache_v, weights, positions, lengths, keep)
+    k, v, w, p, kept, n = out
+    args = EvictArgs(
+        cache_k.data_ptr(), *cache_k.stride()[:3], cache_v.data_ptr(), *cache_v.stride()[:3], weights.data_ptr(),
+        *weights.stride()[:2], ptr(positions), *(positions.stride()[:2] if positions is not None else (0, 0)),
+        ptr(lengths), k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], w.data_ptr(), *w.stride()[:2],
+        ptr(p), *(p.stride()[:2] if p is not None else (0, 0)), kept.data_ptr(), n.data_ptr(), batch, groups, cap, dk,
+        dv, cache_k.element_size(), len_add, keep, recent)
+    with _on(device):
+        check(rows_lib().logkv_evict_rows(C.byref(args), stream_of(device)), "logkv_evict_rows")
+    return out
+
+
+def _check_evict_out(out, cache_k, cache_v, weights, positions, lengths, keep):
+    batch, groups, _, dk = cache_k.shape
+    dv, device = cache_v.size(3), cache_k.device
+    k, v, w, p, kept, n = out
+
+    def rows(t, dtype, *rest):
+        return (t.ndim == 3 + len(rest) and t.shape[:2] == (batch, groups) and t.size(2) >= keep and t.shape[3:] == rest
+                and t.dtype == dtype and t.device == device and t.stride(2 if not rest else 3) == 1)
+
+    if not (rows(k, cache_k.dtype, dk) and rows(v, cache_k.dtype, dv) and rows(w, torch.float32)
+            and _evict_rows_ok(k) and _evict_rows_ok(v) and (p is None) == (positions is None)
+            and (p is None or rows(p, torch.int64)) and kept.shape == (batch, groups, keep) and kept.is_contiguous()
+            and kept.dtype == torch.int32 and kept.device == device and n.shape == (batch,) and n.is_contiguous()
+            and n.dtype == torch.int32 and n.device == device):
+        raise ValueError("out must be EvictedRows buffers of at least keep rows that match the cache")
+    given = [t for t in (cache_k, cache_v, weights, positions, lengths) if t is not None]
+    results = [t for t in out if t is not None]
+    for i, t in enumerate(results):
+        a, b = _span(t)
+        for other in given + results[:i]:
+            c, d = _span(other)
+            if a < d and c < b:
+                raise ValueError("out must not overlap the inputs or itself")
