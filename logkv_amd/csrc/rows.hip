@@ -116,7 +116,7 @@ __global__ __launch_bounds__(kThreads) void rows_finish_kernel(logkv_rows_args a
     if (!there) return;
     const bool empty = lsum == 0.f;
     if (r.lse && d == 0)
-      r.lse[static_cast<int64_t>(lane) * nq + qi] = empty ? __builtin_inff() : m + __builtin_amdgcn_logf(lsum) - E::kShift;
+      r.lse[static_cast<int64_t>(lane) * nq + qi] = empty ? __builtin_inff() : m + __builtin_amdgcn_logf(lsum) - r.shift;
     uint16_t y[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) y[k] = empty ? uint16_t(0) : E::from_f32(acc[k] / lsum);
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kThreads) void rows_finish_kernel(logkv_rows_args a
         float m, lsum;
         fold_splits(lane_part + static_cast<int64_t>(q) * stride, step, r.splits, a.dv, tid % 16, 16, m, lsum);
         if (tid % 16 == 0) {
-          qm[q] = E::kShift - (m == -__builtin_inff() ? 0.f : m);
+          qm[q] = r.shift - (m == -__builtin_inff() ? 0.f : m);
           ql[q] = lsum == 0.f ? 0.f : 1.f / lsum;
         }
       }
@@ -301,6 +301,24 @@ void launch_weights(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t s
   else hipLaunchKernelGGL((rows_weight_kernel<DT, 8>), grid, dim3(kThreads), 0, stream, a, r, cache_blocks);
 }
 
+// Splits of the tiled kernel: rounds of blocks over the CUs, each of a split's tiles and two more
+// for its start and end, and for more than one split two tiles' time for the join and the partials.
+int tile_splits(const logkv_rows_args& a, int64_t blocks, int q_waves) {
+  const int rows = q_waves == 8 ? 64 : 128;
+  const int64_t tiles = (a.cap + rows - 1) / rows + (a.tq + rows - 1) / rows;
+  int best = 1;
+  int64_t best_cost = INT64_MAX;
+  for (int64_t s = 1; s <= std::min<int64_t>(kMaxRowSplits, tiles); ++s) {
+    const int64_t rounds = (blocks * s + 255) / 256;
+    const int64_t cost = 32 * (rounds * ((tiles + s - 1) / s + 2) + (s > 1 ? 2 : 0)) + (s > 1 ? blocks * s * q_waves / 8 : 0);
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = static_cast<int>(s);
+    }
+  }
+  return best;
+}
+
 }  // namespace
 
 RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws) {
@@ -308,13 +326,20 @@ RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws) {
   const bool wide = a.dk > 128 || a.dv > 128;
   RowsLaunch r{};
   r.causal = causal ? 1 : 0;
-  r.cols = nq <= 16 ? 1 : nq <= 32 || wide ? 2 : 4;
-  const int64_t q_blocks = (nq + 16 * r.cols - 1) / (16 * r.cols);
   const int64_t tiles = (a.cap + kRowTile - 1) / kRowTile + (a.tq + kRowTile - 1) / kRowTile;
-  // One share per resident block, none shorter than a tile for each of its waves.
-  const int64_t resident = wide || r.cols == 4 ? 256 : 512;
-  r.splits = static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>({kMaxRowSplits, (tiles + 3) / 4, resident / std::max<int64_t>(1, lanes * q_blocks)})));
+  if (nq > 32 && !wide) {
+    r.q_waves = nq <= 64 ? 2 : nq <= 128 ? 4 : 8;
+    r.shift = 15.f;
+    r.splits = tile_splits(a, lanes * ((nq + 32 * r.q_waves - 1) / (32 * r.q_waves)), r.q_waves);
+  } else {
+    r.cols = nq <= 16 ? 1 : 2;
+    r.shift = a.dtype == LOGKV_F16 ? Elem<LOGKV_F16>::kShift : Elem<LOGKV_BF16>::kShift;
+    const int64_t q_blocks = (nq + 16 * r.cols - 1) / (16 * r.cols);
+    // One share per resident block, none shorter than a tile for each of its waves.
+    const int64_t resident = wide ? 256 : 512;
+    r.splits = static_cast<int>(std::max<int64_t>(
+        1, std::min<int64_t>({kMaxRowSplits, (tiles + 3) / 4, resident / std::max<int64_t>(1, lanes * q_blocks)})));
+  }
   uint8_t* base = static_cast<uint8_t*>(ws);
   int64_t off = 0;
   auto take = [&](int64_t floats) {
@@ -334,7 +359,7 @@ RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws) {
 }
 
 int launch_rows_attention(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
-  const int rc = launch_rows_stream(a, r, stream);
+  const int rc = r.q_waves ? launch_rows_tile(a, r, stream) : launch_rows_stream(a, r, stream);
   if (rc) return rc;
   if (a.dtype == LOGKV_BF16) launch_finish_type<LOGKV_BF16>(a, r, stream);
   else launch_finish_type<LOGKV_F16>(a, r, stream);

@@ -23,12 +23,15 @@ struct RowsLaunch {
   int64_t score_st;
   int64_t bytes;
   int splits;
-  int cols;       // 16-query column blocks per wave
+  int cols;       // streamed kernel: 16-query column blocks per wave
+  int q_waves;    // tiled kernel: waves with 32 queries each (0: the streamed kernel)
+  float shift;    // the partials' sums carry 2^shift
   int causal;     // weight attention; otherwise the visible mask
 };
 
 RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws);
 int launch_rows_stream(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream);
+int launch_rows_tile(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream);
 int launch_rows_attention(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream);
 int launch_evict(const logkv_evict_args& a, hipStream_t stream);
 
@@ -41,6 +44,13 @@ __device__ __forceinline__ int rows_in_use(const logkv_rows_args& a, int b) {
 }
 __device__ __forceinline__ int own_rows(const logkv_rows_args& a, int b) {
   return a.counts ? max(0, min(a.counts[b], a.tq)) : a.tq;
+}
+
+// A bias in base 2. A finite one stays finite (a mask of the type's lowest value hides a row only
+// beside larger logits).
+__device__ __forceinline__ float bias_base2(float x) {
+  const float y = x * kLog2e;
+  return __builtin_isinf(y) && !__builtin_isinf(x) ? __builtin_copysignf(3.402823466e38f, x) : y;
 }
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));

@@ -29,13 +29,6 @@ constexpr int kWaves = 4;
 // distinct banks.
 constexpr int v_stride(int blocks) { return 16 * blocks + 16; }
 
-// A bias in base 2. A finite one stays finite (a mask of the type's lowest value hides a row only
-// beside larger logits).
-__device__ __forceinline__ float base2(float x) {
-  const float y = x * kLog2e;
-  return __builtin_isinf(y) && !__builtin_isinf(x) ? __builtin_copysignf(3.402823466e38f, x) : y;
-}
-
 }  // namespace
 
 // NS 32-wide steps of dk, NB 16-wide blocks of dv, NC 16-query column blocks. Units past dk and dv
@@ -116,7 +109,7 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
           const int64_t at = b * a.b_sb + g * a.b_sg + (t0 + rr) * a.b_st;
           const float x = a.bias_half ? E::to_f32(gp(static_cast<const uint16_t*>(a.bias))[at])
                                       : gp(static_cast<const float*>(a.bias))[at];
-          bx[j] = base2(x);
+          bx[j] = bias_base2(x);
         }
       }
     }
@@ -157,7 +150,7 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
     // The wave's own V tile: written and read by this wave only (LDS accesses of a wave complete
     // in order; the fences keep the compiler's order).
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (!finite) {
+    if (__builtin_expect(!finite, 0)) {
       for (int e = l; e < 3 * 16 * NB; e += 64) (&odd_s[w][0][0])[e] = 0;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
@@ -229,7 +222,7 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
         for (int nb = 0; nb < NB; ++nb) o[c][nb] *= corr;
       }
       m[c] = m_new;
-      if (!finite) {
+      if (__builtin_expect(!finite, 0)) {
         seen[c] = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -262,7 +255,7 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
 #pragma unroll
         for (int c = 0; c < NC; ++c) o[c][nb] = E::mfma16(vf, pf[c][q], o[c][nb]);
     }
-    if (!finite) {
+    if (__builtin_expect(!finite, 0)) {
       // The infinities and NaNs left out of the products, for the queries that see their rows.
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
@@ -333,12 +326,10 @@ template <int DT>
 void launch_type(const logkv_rows_args& a, const RowsLaunch& r, dim3 grid, hipStream_t stream) {
   if (a.dk <= 64 && a.dv <= 64) {
     if (r.cols == 1) launch_one<DT, 2, 4, 1>(a, r, grid, stream);
-    else if (r.cols == 2) launch_one<DT, 2, 4, 2>(a, r, grid, stream);
-    else launch_one<DT, 2, 4, 4>(a, r, grid, stream);
+    else launch_one<DT, 2, 4, 2>(a, r, grid, stream);
   } else if (a.dk <= 128 && a.dv <= 128) {
     if (r.cols == 1) launch_one<DT, 4, 8, 1>(a, r, grid, stream);
-    else if (r.cols == 2) launch_one<DT, 4, 8, 2>(a, r, grid, stream);
-    else launch_one<DT, 4, 8, 4>(a, r, grid, stream);
+    else launch_one<DT, 4, 8, 2>(a, r, grid, stream);
   } else {
     if (r.cols == 1) launch_one<DT, 8, 16, 1>(a, r, grid, stream);
     else launch_one<DT, 8, 16, 2>(a, r, grid, stream);

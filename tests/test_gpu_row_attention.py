@@ -139,6 +139,26 @@ def test_infinities_reach_only_who_sees_them(dtype, rep, T, d):
     check_close(out, want, bound)
 
 
+@pytest.mark.parametrize("dtype,size", [(BF16, 1e-30), (BF16, 1e-9), (BF16, 1e-3), (BF16, 700.0), (BF16, 1e25), (BF16, "mixed"),
+                                        (F16, 1e-6), (F16, 1e-3), (F16, 2e4), (F16, "mixed")])
+@pytest.mark.parametrize("rep,T", [(2, 4), (2, 20), (2, 40), (4, 50)])
+def test_value_magnitudes(dtype, size, rep, T):
+    """Values of any exponent: tiny, huge (fp16: some beyond its range, infinite), and features of very different sizes in one row (some tiles with a huge row)."""
+    d, cap = 64, 300
+    q, k, v, ck, cv = inputs(1, 1, rep, T, cap, d, d, torch.float32, 25)
+    if size == "mixed":
+        power = torch.arange(d, device="cuda") % 16 * (2.0 if dtype == BF16 else 0.8) - 24.0 * (dtype == BF16) - 8.0 * (dtype == F16)
+        v, cv = v * 2.0 ** power, cv * 2.0 ** power
+        cv[:, :, 200] *= 2.0 ** (14 if dtype == BF16 else 10)
+    else:
+        v, cv = v * size, cv * size
+    q, k, v, ck, cv = (x.to(dtype) for x in (q, k, v, ck, cv))
+    visible = tree_mask(T, 6)
+    out = log_kv_tree_attention(q, k, v, ck, cv, cap, visible.cuda(), d ** -0.5)
+    want, _, bound, _ = reference(q, k, v, ck, cv, [cap], visible[None], d ** -0.5)
+    check_close(out, want, bound + 1e-38)
+
+
 WEIGHTS = [
     (1, 1, 1, 1, [1], 2, 64, 64, BF16, "rows"),
     (1, 2, 2, 1, [0], 8, 64, 64, BF16, "rows"),
