@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes as C
 from functools import lru_cache
+from struct import Struct
 
 from ._lib import _i32, _i64, _p, lib
 
@@ -43,12 +44,26 @@ class EvictArgs(C.Structure):
     ]
 
 
-# Exported symbol -> (restype, argtypes); the tests check this table against the header.
+# The structs as packed bytes, a third of a ctypes structure's cost to fill on a call's path (the layouts above
+# have no padding but the last field's, which the tests check against the header).
+_CODES = {_p: "Q", _i64: "q", _i32: "i", C.c_float: "f"}
+
+
+def _packer(struct) -> Struct:
+    fmt = Struct("=" + "".join(_CODES[t] for _, t in struct._fields_))
+    return Struct(f"{fmt.format}{C.sizeof(struct) - fmt.size}x")
+
+
+pack_rows = _packer(RowsArgs).pack
+pack_evict = _packer(EvictArgs).pack
+
+# Exported symbol -> (restype, argtypes); the tests check this table against the header. The structs are passed as
+# their bytes or by reference.
 SIGNATURES = {
-    "logkv_rows_workspace_bytes": (_i64, [C.POINTER(RowsArgs)]),
-    "logkv_tree_attention": (_i32, [C.POINTER(RowsArgs), _p, _i64, _p]),
-    "logkv_weight_attention": (_i32, [C.POINTER(RowsArgs), _p, _i64, _p]),
-    "logkv_evict_rows": (_i32, [C.POINTER(EvictArgs), _p]),
+    "logkv_rows_workspace_bytes": (_i64, [_p]),
+    "logkv_tree_attention": (_i32, [_p, _p, _i64, _p]),
+    "logkv_weight_attention": (_i32, [_p, _p, _i64, _p]),
+    "logkv_evict_rows": (_i32, [_p, _p]),
 }
 
 

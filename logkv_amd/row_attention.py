@@ -18,17 +18,18 @@ inference: none has a gradient.
 
 from __future__ import annotations
 
-import ctypes as C
 import math
-from contextlib import nullcontext
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
 
-from ._lib import check, check_activation_dtype, ptr, require_device, stream_of
-from ._rows import BF16, F16, EvictArgs, RowsArgs, rows_lib
+from ._lib import check, check_activation_dtype, require_device
+from ._rows import BF16, F16, RowsArgs, pack_evict, pack_rows, rows_lib
 
 _ROW_DTYPES = {torch.bfloat16: BF16, torch.float16: F16}
+_LENGTH_DTYPES = (torch.int32, torch.int64)
+_NO_STRIDES = (0, 0, 0)
 
 
 class EvictedRows(NamedTuple):
@@ -43,13 +44,16 @@ class EvictedRows(NamedTuple):
     lengths: torch.Tensor
 
 
-def _on(device):
-    """The device as the current one while a launch is issued."""
-    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _launch(entry, what, index, *args):
+    """Calls a C entry point on the current stream of the device ``index``, made the current one."""
+    if torch._C._cuda_getDevice() == index:
+        return check(entry(*args, torch._C._cuda_getCurrentRawStream(index)), what)
+    with torch.cuda.device(index):
+        return check(entry(*args, torch._C._cuda_getCurrentRawStream(index)), what)
 
 
-def _no_grad(*tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+def _refuse_grad(*tensors):
+    if any(t.requires_grad for t in tensors):
         raise NotImplementedError("row attention is for inference: it has no gradient (run it under torch.no_grad())")
 
 
@@ -59,93 +63,98 @@ def _small_rows(x, dtype):
         check_activation_dtype(x.dtype)
         x = x.to(dtype)
     sb, sh, st, sd = x.stride()
-    if sd != 1 or (sb | sh | st) % 8 or x.data_ptr() % 16:
+    if sd != 1 or (sb | sh | st) & 7 or x.data_ptr() & 15:
         x = x.contiguous()
-        if x.data_ptr() % 16:
+        if x.data_ptr() & 15:
             x = x.clone()
-    return x
+        sb, sh, st, sd = x.stride()
+    return x, sb, sh, st
 
 
-def _lengths(lengths, batch, cap, device, room=0):
-    """(tensor or None, stride, added rows) of an int or an int32 tensor ``[B]``."""
+def _lengths(lengths, batch, cap, index, room=0):
+    """(int32 tensor or None, its address, its stride, added rows) of an int or an int tensor ``[B]``."""
     if isinstance(lengths, torch.Tensor):
-        if lengths.shape != (batch,) or lengths.device != device or lengths.dtype not in (torch.int32, torch.int64):
+        if lengths.shape != (batch,) or lengths.get_device() != index or lengths.dtype not in _LENGTH_DTYPES:
             raise ValueError("lengths must be an int or an int32 tensor [batch] on the cache's device")
-        return lengths.to(torch.int32).contiguous(), 1, 0
+        if lengths.dtype != torch.int32 or not lengths.is_contiguous():
+            lengths = lengths.to(torch.int32).contiguous()
+        return lengths, lengths.data_ptr(), 1, 0
     lengths = int(lengths)
     if not 0 <= lengths <= cap - room:
         raise ValueError(f"{lengths} rows and {room} new ones do not fit the cache's {cap}")
-    return None, 0, lengths
+    return None, 0, 0, lengths
+
+
+@lru_cache(maxsize=256)
+def _workspace_bytes(weights, batch, heads, groups, tq, cap, dk, dv, dtype):
+    """Scratch of a call of these sizes."""
+    args = RowsArgs(n_batch=batch, n_heads=heads, n_groups=groups, tq=tq, cap=cap, dk=dk, dv=dv, dtype=dtype,
+                    weights=1 if weights else 0)
+    need = rows_lib().logkv_rows_workspace_bytes(bytes(args))
+    if need < 0:
+        raise ValueError("row attention: " + rows_lib().logkv_last_error().decode(errors="replace"))
+    return need
 
 
 def _attention(q, k, v, cache_k, cache_v, scale, lengths, room, *, bias=None, visible=None, counts=None, weights=None,
                lengths2=None, len_add=0):
     """Checks and launch of both attentions."""
-    if q.ndim != 4 or k.ndim != 4 or v.ndim != 4 or cache_k.ndim != 4 or cache_v.ndim != 4:
+    if not q.ndim == k.ndim == v.ndim == cache_k.ndim == cache_v.ndim == 4:
         raise ValueError("queries, rows and cache must be 4-dimensional")
     batch, heads, tq, dk = q.shape
-    groups, cap, dv = cache_k.size(1), cache_k.size(2), cache_v.size(3)
-    device, dtype = cache_k.device, cache_k.dtype
-    if dtype not in _ROW_DTYPES or cache_v.dtype != dtype:
+    _, groups, cap, _ = cache_k.shape
+    dv, dtype, index = cache_v.size(3), cache_k.dtype, cache_k.get_device()
+    code = _ROW_DTYPES.get(dtype)
+    if code is None or cache_v.dtype != dtype:
         raise ValueError("the cache must be bfloat16 or float16")
     if (cache_k.shape != (batch, groups, cap, dk) or cache_v.shape != (batch, groups, cap, dv) or groups < 1
             or heads % groups or heads < 1 or tq < 1 or batch < 1):
         raise ValueError("cache rows must be [B, G, capacity, d] with G dividing the query heads")
     if k.shape != (batch, groups, tq, dk) or v.shape != (batch, groups, tq, dv):
         raise ValueError("the call's rows must be [B, G, T, d], one per query position")
-    for t, what in ((cache_k, "cache_k"), (cache_v, "cache_v")):
-        require_device(t, what)
-        if cap and (t.stride(3) != 1 or (t.stride(0) | t.stride(1) | t.stride(2)) % 8 or t.data_ptr() % 16):
-            raise ValueError(f"{what} rows must be 16-byte aligned with contiguous features")
-    if cache_v.device != device or q.device != device or k.device != device or v.device != device:
+    require_device(cache_k, "cache_k")
+    if not cache_v.get_device() == q.get_device() == k.get_device() == v.get_device() == index:
         raise ValueError("all tensors must be on the cache's device")
-    if not (math.isfinite(scale) and scale > 0.0):
+    if not (0.0 < scale < math.inf):
         raise ValueError("attention scale must be positive")
-    _no_grad(q, k, v, cache_k, cache_v)
+    if torch.is_grad_enabled():
+        _refuse_grad(q, k, v, cache_k, cache_v, *(() if bias is None else (bias,)))
+    ck, cv = cache_k.data_ptr(), cache_v.data_ptr()
+    ck_sb, ck_sg, ck_st, ck_sd = cache_k.stride()
+    cv_sb, cv_sg, cv_st, cv_sd = cache_v.stride()
+    if cap and (ck_sd != 1 or cv_sd != 1 or (ck_sb | ck_sg | ck_st | cv_sb | cv_sg | cv_st) & 7 or (ck | cv) & 15):
+        raise ValueError("cache rows must be 16-byte aligned with contiguous features")
     out_dtype = q.dtype
-    q, k, v = _small_rows(q, dtype), _small_rows(k, dtype), _small_rows(v, dtype)
+    (q, *q_st), (k, *k_st), (v, *v_st) = _small_rows(q, dtype), _small_rows(k, dtype), _small_rows(v, dtype)
     if lengths2 is None:
-        lengths, len_stride, len_add = _lengths(lengths, batch, cap, device, room)
+        lengths, n_ptr, n_st, len_add = _lengths(lengths, batch, cap, index, room)
     else:
-        len_stride = 0
+        n_ptr, n_st = lengths.data_ptr(), 0
+    b_ptr, b_st, b_half = 0, _NO_STRIDES, 0
     if bias is not None:
-        if bias.shape != (batch, groups, cap) or bias.device != device or bias.dtype not in (torch.float32, dtype):
+        if bias.shape != (batch, groups, cap) or bias.get_device() != index or bias.dtype not in (torch.float32, dtype):
             raise ValueError("bias must be [B, G, capacity] on the cache's device, float32 or the cache's dtype")
-        _no_grad(bias)
-    out = torch.empty((batch, heads, tq, dv), dtype=dtype, device=device)
-    args = RowsArgs(
-        q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
-        cache_k.data_ptr(), *cache_k.stride()[:3], cache_v.data_ptr(), *cache_v.stride()[:3],
-        ptr(bias), *(bias.stride() if bias is not None else (0, 0, 0)), ptr(lengths), ptr(lengths2),
-        ptr(visible), *(visible.stride()[:2] if visible is not None else (0, 0)), ptr(counts),
-        ptr(weights), *(weights.stride()[:2] if weights is not None else (0, 0)),
-        out.data_ptr(), *out.stride()[:3], batch, heads, groups, tq, cap, dk, dv, _ROW_DTYPES[dtype], len_stride,
-        len_add, 0 if bias is None or bias.dtype == torch.float32 else 1, scale)
+        b_ptr, b_st, b_half = bias.data_ptr(), bias.stride(), int(bias.dtype == dtype)
+    vis_ptr = vis_sb = vis_st = w_ptr = w_sb = w_sg = 0
+    if visible is not None:
+        vis_ptr, vis_sb, vis_st = visible.data_ptr(), visible.stride(0) if visible.ndim == 3 else 0, visible.stride(-2)
+    else:
+        w_ptr, (w_sb, w_sg, _) = weights.data_ptr(), weights.stride()
+    out = torch.empty((batch, heads, tq, dv), dtype=dtype, device=cache_k.device)
+    need = _workspace_bytes(weights is not None, batch, heads, groups, tq, cap, dk, dv, code)
+    workspace = torch.empty(need, dtype=torch.uint8, device=cache_k.device)
+    o_sh = tq * dv
+    args = pack_rows(
+        q.data_ptr(), *q_st, k.data_ptr(), *k_st, v.data_ptr(), *v_st, ck, ck_sb, ck_sg, ck_st, cv, cv_sb, cv_sg, cv_st,
+        b_ptr, *b_st, n_ptr, 0 if lengths2 is None else lengths2.data_ptr(), vis_ptr, vis_sb, vis_st,
+        0 if counts is None else counts.data_ptr(), w_ptr, w_sb, w_sg, out.data_ptr(), heads * o_sh, o_sh, dv,
+        batch, heads, groups, tq, cap, dk, dv, code, n_st, len_add, b_half, scale)
     handle = rows_lib()
-    need = handle.logkv_rows_workspace_bytes(C.byref(args))
-    if need < 0:
-        raise ValueError("row attention: " + handle.logkv_last_error().decode(errors="replace"))
-    workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    with _on(device):
-        if weights is None:
-            check(handle.logkv_tree_attention(C.byref(args), workspace.data_ptr(), need, stream_of(device)),
-                  "logkv_tree_attention")
-        else:
-            check(handle.logkv_weight_attention(C.byref(args), workspace.data_ptr(), need, stream_of(device)),
-                  "logkv_weight_attention")
+    if weights is None:
+        _launch(handle.logkv_tree_attention, "logkv_tree_attention", index, args, workspace.data_ptr(), need)
+    else:
+        _launch(handle.logkv_weight_attention, "logkv_weight_attention", index, args, workspace.data_ptr(), need)
     return out if out_dtype == dtype else out.to(out_dtype)
-
-
-def _visible(visible, batch, tq, device):
-    """The drafted rows' mask as uint8 ``[B, T, T]`` (batch stride 0 where it is shared)."""
-    if (not isinstance(visible, torch.Tensor) or visible.dtype not in (torch.bool, torch.uint8)
-            or visible.shape not in ((tq, tq), (batch, tq, tq)) or visible.device != device):
-        raise ValueError("visible must be a bool tensor [T, T] or [B, T, T] on the cache's device")
-    if visible.dtype == torch.bool:
-        visible = visible.view(torch.uint8)
-    if visible.stride(-1) != 1:
-        visible = visible.contiguous()
-    return visible.expand(batch, tq, tq)
 
 
 def log_kv_tree_attention(q, k, v, cache_k, cache_v, lengths, visible, scale, *, bias=None):
@@ -160,7 +169,12 @@ def log_kv_tree_attention(q, k, v, cache_k, cache_v, lengths, visible, scale, *,
 
     Queries and drafted rows of another activation dtype are rounded to the cache's, and the output is returned
     in the queries'. The cache is only read: commit the accepted tokens with the cache's own call."""
-    visible = _visible(visible, q.size(0), q.size(2), cache_k.device)
+    if (not isinstance(visible, torch.Tensor) or visible.dtype not in (torch.bool, torch.uint8) or q.ndim != 4
+            or visible.shape not in ((q.size(2),) * 2, (q.size(0), q.size(2), q.size(2)))
+            or visible.get_device() != cache_k.get_device()):
+        raise ValueError("visible must be a bool tensor [T, T] or [B, T, T] on the cache's device")
+    if visible.stride(-1) != 1:
+        visible = visible.contiguous()
     return _attention(q, k, v, cache_k, cache_v, float(scale), lengths, 0, bias=bias, visible=visible)
 
 
@@ -174,12 +188,13 @@ def log_kv_weight_attention(q, k, v, cache_k, cache_v, weights, lengths, scale, 
     an int tensor it is read on the device, and rows past the capacity are attended to but not stored. ``counts``
     (int32 ``[B]``) gives the tokens that really exist per batch row of a padded batch: the others' outputs are zeros,
     they add no weight and are not stored. ``weights`` is float32 ``[B, G, capacity]`` with contiguous rows."""
-    batch, groups, cap = cache_k.shape[:3]
-    if (weights.shape != (batch, groups, cap) or weights.dtype != torch.float32 or weights.device != cache_k.device
+    batch, _, cap = shape = cache_k.shape[:3]
+    if (weights.shape != shape or weights.dtype != torch.float32 or weights.get_device() != cache_k.get_device()
             or weights.stride(2) != 1 or cap < 1):
         raise ValueError("weights must be float32 [B, G, capacity] on the cache's device with contiguous rows")
     if counts is not None:
-        if counts.shape != (batch,) or counts.device != cache_k.device or counts.dtype not in (torch.int32, torch.int64):
+        if (counts.shape != (batch,) or counts.get_device() != cache_k.get_device()
+                or counts.dtype not in _LENGTH_DTYPES):
             raise ValueError("counts must be an int32 tensor [batch] on the cache's device")
         counts = counts.to(torch.int32).contiguous()
     return _attention(q, k, v, cache_k, cache_v, float(scale), lengths, q.size(2), counts=counts, weights=weights)
@@ -192,8 +207,8 @@ def _span(t):
 
 
 def _evict_rows_ok(t):
-    size = t.element_size()
-    return t.stride(3) == 1 and not any(s * size % 16 for s in t.stride()[:3]) and t.data_ptr() % 16 == 0
+    sb, sg, st, sd = t.stride()
+    return sd == 1 and ((sb | sg | st) * t.element_size() | t.data_ptr()) & 15 == 0
 
 
 def log_kv_evict(cache_k, cache_v, weights, lengths, keep, *, recent=0, positions=None, out=None):
@@ -210,41 +225,45 @@ def log_kv_evict(cache_k, cache_v, weights, lengths, keep, *, recent=0, position
     if cache_k.ndim != 4 or cache_v.ndim != 4 or cache_k.shape[:3] != cache_v.shape[:3]:
         raise ValueError("cache rows must be [B, G, capacity, d]")
     batch, groups, cap, dk = cache_k.shape
-    dv, device = cache_v.size(3), cache_k.device
+    dv, device, dtype, index = cache_v.size(3), cache_k.device, cache_k.dtype, cache_k.get_device()
     keep, recent = int(keep), int(recent)
     if keep < 1 or not 0 <= recent <= keep:
         raise ValueError("keep must be at least 1, recent between 0 and keep")
     require_device(cache_k, "cache_k")
-    if cache_v.device != device or cache_v.dtype != cache_k.dtype or weights.device != device:
+    if cache_v.dtype != dtype or not cache_v.get_device() == weights.get_device() == index:
         raise ValueError("all tensors must be on the cache's device, keys and values of one dtype")
     if weights.shape != (batch, groups, cap) or weights.dtype != torch.float32 or weights.stride(2) != 1:
         raise ValueError("weights must be float32 [B, G, capacity] with contiguous rows")
-    if positions is not None and (positions.shape != (batch, groups, cap) or positions.dtype != torch.int64
-                                  or positions.stride(2) != 1 or positions.device != device):
-        raise ValueError("positions must be int64 [B, G, capacity] with contiguous rows")
+    p_in = p_out = _NO_STRIDES
+    if positions is not None:
+        p_in = (positions.data_ptr(), *positions.stride()[:2])
+        if (positions.shape != (batch, groups, cap) or positions.dtype != torch.int64 or positions.stride(2) != 1
+                or positions.get_device() != index):
+            raise ValueError("positions must be int64 [B, G, capacity] with contiguous rows")
     if not (_evict_rows_ok(cache_k) and _evict_rows_ok(cache_v)):
         raise ValueError("cache rows must be 16-byte aligned with contiguous features")
-    _no_grad(cache_k, cache_v, weights)
-    lengths, _, len_add = _lengths(lengths, batch, cap, device)
+    if torch.is_grad_enabled():
+        _refuse_grad(cache_k, cache_v, weights)
+    lengths, n_ptr, _, len_add = _lengths(lengths, batch, cap, index)
     if out is None:
+        kept = torch.empty((batch, groups, keep), dtype=torch.int32, device=device)
         out = EvictedRows(
-            torch.empty((batch, groups, keep, dk), dtype=cache_k.dtype, device=device),
-            torch.empty((batch, groups, keep, dv), dtype=cache_k.dtype, device=device),
+            torch.empty((batch, groups, keep, dk), dtype=dtype, device=device),
+            torch.empty((batch, groups, keep, dv), dtype=dtype, device=device),
             torch.empty((batch, groups, keep), dtype=torch.float32, device=device),
             None if positions is None else torch.empty((batch, groups, keep), dtype=torch.int64, device=device),
-            torch.empty((batch, groups, keep), dtype=torch.int32, device=device),
-            torch.empty(batch, dtype=torch.int32, device=device))
+            kept, torch.empty(batch, dtype=torch.int32, device=device))
     else:
         _check_evict_out(out, cache_k, cache_v, weights, positions, lengths, keep)
     k, v, w, p, kept, n = out
-    args = EvictArgs(
+    if p is not None:
+        p_out = (p.data_ptr(), *p.stride()[:2])
+    args = pack_evict(
         cache_k.data_ptr(), *cache_k.stride()[:3], cache_v.data_ptr(), *cache_v.stride()[:3], weights.data_ptr(),
-        *weights.stride()[:2], ptr(positions), *(positions.stride()[:2] if positions is not None else (0, 0)),
-        ptr(lengths), k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], w.data_ptr(), *w.stride()[:2],
-        ptr(p), *(p.stride()[:2] if p is not None else (0, 0)), kept.data_ptr(), n.data_ptr(), batch, groups, cap, dk,
-        dv, cache_k.element_size(), len_add, keep, recent)
-    with _on(device):
-        check(rows_lib().logkv_evict_rows(C.byref(args), stream_of(device)), "logkv_evict_rows")
+        *weights.stride()[:2], *p_in, n_ptr, k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], w.data_ptr(),
+        *w.stride()[:2], *p_out, kept.data_ptr(), n.data_ptr(), batch, groups, cap, dk, dv, cache_k.element_size(),
+        len_add, keep, recent)
+    _launch(rows_lib().logkv_evict_rows, "logkv_evict_rows", index, args)
     return out
 
 

@@ -46,6 +46,11 @@ def test_ctypes_structs_match_the_header(tmp_path):
     got = [int(x) for x in subprocess.run([str(tmp_path / "probe")], check=True, capture_output=True, text=True).stdout.split()]
     want = [x for n, c in structs.items() for x in [C.sizeof(c)] + [getattr(c, f).offset for f, _ in c._fields_]]
     assert got == want
+    # The packed form of the structs.
+    for cls, pack in ((_rows.RowsArgs, _rows.pack_rows), (_rows.EvictArgs, _rows.pack_evict)):
+        values = [3 * i + 1 for i in range(len(cls._fields_))]
+        a = cls.from_buffer_copy(pack(*values))
+        assert [getattr(a, f) for f, _ in cls._fields_] == values
 
 
 def rows_args(**over):
