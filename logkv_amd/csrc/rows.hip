@@ -180,93 +180,6 @@ __global__ __launch_bounds__(kThreads) void rows_finish_kernel(logkv_rows_args a
   }
 }
 
-// Weights of more than 16 queries: with a query's log-sum-exp L known, p = 2^(s c2 - L), summed over
-// the queries. S = Q K^T with the keys as columns, so a lane sums its own key over all queries in
-// registers: a wave holds 64 keys' operands for good and the block's queries pass through LDS, 16
-// rows a product. One wave owns a key: no atomics, a fixed order.
-constexpr int kSumKeys = 64;       // per wave
-constexpr int kSumQueries = 64;    // per staged tile
-template <int DT, int NS>
-__global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_args a, RowsLaunch r, int cache_blocks) {
-  typedef Elem<DT> E;
-  typedef typename E::vec8 vec8;
-  constexpr int kLd = 32 * NS + 8;
-  __shared__ __align__(16) uint16_t q_s[kSumQueries * kLd];
-  __shared__ __align__(16) float l_s[kSumQueries];
-  const int lane = blockIdx.y, G = a.n_groups, b = lane / G, g = lane % G;
-  const int rep = a.n_heads / G, nq = rep * a.tq, units = a.dk / 8;
-  const int w = wave_id(), l = lane_id(), col = l & 15, hq = l >> 4;
-  const int n = rows_in_use(a, b), own = own_rows(a, b);
-  // Blocks of the cache's rows, then of the own rows.
-  const bool of_cache = static_cast<int>(blockIdx.x) < cache_blocks;
-  const int rows = of_cache ? n : own;
-  const int b0 = (static_cast<int>(blockIdx.x) - (of_cache ? 0 : cache_blocks)) * 4 * kSumKeys;
-  if (b0 >= rows) return;
-  const int k0 = b0 + w * kSumKeys;
-  const LOGKV_G uint16_t* kr = of_cache ? gp(a.cache_k) + b * a.ck_sb + g * a.ck_sg : gp(a.k) + b * a.k_sb + g * a.k_sg;
-  const int64_t kst = of_cache ? a.ck_st : a.k_st;
-  vec8 kf[4][NS];
-#pragma unroll
-  for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (4 * s + hq < units) x = *(const LOGKV_G uint4*)(kr + min(k0 + 16 * kb + col, rows - 1) * kst + 32 * s + 8 * hq);
-      kf[kb][s] = __builtin_bit_cast(vec8, x);
-    }
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  const float c2 = a.scale * kLog2e;
-  for (int q0 = 0; q0 < nq; q0 += kSumQueries) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kSumQueries * 4 * NS; i += kThreads) {
-      const int qq = i / (4 * NS), u = i % (4 * NS), qi = min(q0 + qq, nq - 1);
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (u < units)
-        x = *(const LOGKV_G uint4*)(gp(a.q) + b * a.q_sb + (g * rep + qi / a.tq) * a.q_sh + qi % a.tq * a.q_st + 8 * u);
-      *reinterpret_cast<uint4*>(&q_s[qq * kLd + 8 * u]) = x;
-    }
-    if (threadIdx.x < kSumQueries) {
-      const int qi = q0 + static_cast<int>(threadIdx.x);
-      l_s[threadIdx.x] = qi < nq ? r.lse[static_cast<int64_t>(lane) * nq + qi] : __builtin_inff();
-    }
-    __syncthreads();
-#pragma unroll
-    for (int qb = 0; qb < kSumQueries / 16; ++qb) {
-      f32x4 s[4];
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb) s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int st = 0; st < NS; ++st) {
-        const vec8 qf = *reinterpret_cast<const vec8*>(&q_s[(16 * qb + col) * kLd + 32 * st + 8 * hq]);
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb) s[kb] = E::mfma16(qf, kf[kb][st], s[kb]);
-      }
-      // Element i is query 16 qb + 4 hq + i against key 16 kb + col.
-      const f32x4 lse = *reinterpret_cast<const f32x4*>(&l_s[16 * qb + 4 * hq]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int qi = q0 + 16 * qb + 4 * hq + i, t = of_cache ? 0 : qi % a.tq;
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], c2, -lse[i]));
-          if (lse[i] == __builtin_inff() || (!of_cache && k0 + 16 * kb + col > t)) p = 0.f;
-          sum[kb] += p;
-        }
-      }
-    }
-  }
-  LOGKV_G float* wrow = gp(a.weights) + b * a.w_sb + g * a.w_sg;
-#pragma unroll
-  for (int kb = 0; kb < 4; ++kb) {
-    sum[kb] += __shfl_xor(sum[kb], 16, kWave);
-    sum[kb] += __shfl_xor(sum[kb], 32, kWave);
-    const int j = k0 + 16 * kb + col;
-    if (hq || j >= rows) continue;
-    if (of_cache) wrow[j] += sum[kb];
-    else if (n + j < a.cap) wrow[n + j] = sum[kb];
-  }
-}
-
 namespace {
 
 template <int DT, int TQ, int SG>
@@ -291,26 +204,16 @@ void launch_finish_type(const logkv_rows_args& a, const RowsLaunch& r, hipStream
   }
 }
 
-template <int DT>
-void launch_weights(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
-  constexpr int kKeys = 4 * kSumKeys;
-  const int cache_blocks = (a.cap + kKeys - 1) / kKeys;
-  const dim3 grid(cache_blocks + (a.tq + kKeys - 1) / kKeys, a.n_batch * a.n_groups);
-  if (a.dk <= 64) hipLaunchKernelGGL((rows_weight_kernel<DT, 2>), grid, dim3(kThreads), 0, stream, a, r, cache_blocks);
-  else if (a.dk <= 128) hipLaunchKernelGGL((rows_weight_kernel<DT, 4>), grid, dim3(kThreads), 0, stream, a, r, cache_blocks);
-  else hipLaunchKernelGGL((rows_weight_kernel<DT, 8>), grid, dim3(kThreads), 0, stream, a, r, cache_blocks);
-}
-
 // Splits of the tiled kernel: rounds of blocks over the CUs, each of a split's tiles and two more
 // for its start and end, and for more than one split two tiles' time for the join and the partials.
 int tile_splits(const logkv_rows_args& a, int64_t blocks, int q_waves) {
-  const int rows = q_waves == 8 ? 64 : 128;
+  const int rows = q_waves == 2 ? 128 : 64, resident = 256;
   const int64_t tiles = (a.cap + rows - 1) / rows + (a.tq + rows - 1) / rows;
   int best = 1;
   int64_t best_cost = INT64_MAX;
   for (int64_t s = 1; s <= std::min<int64_t>(kMaxRowSplits, tiles); ++s) {
-    const int64_t rounds = (blocks * s + 255) / 256;
-    const int64_t cost = 32 * (rounds * ((tiles + s - 1) / s + 2) + (s > 1 ? 2 : 0)) + (s > 1 ? blocks * s * q_waves / 8 : 0);
+    const int64_t rounds = (blocks * s + resident - 1) / resident;
+    const int64_t cost = 32 * (rounds * ((tiles + s - 1) / s + 2) + (s > 1 ? 2 : 0)) + (s > 1 ? blocks * s / 2 : 0);
     if (cost < best_cost) {
       best_cost = cost;
       best = static_cast<int>(s);
@@ -329,7 +232,7 @@ RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws) {
   const int64_t tiles = (a.cap + kRowTile - 1) / kRowTile + (a.tq + kRowTile - 1) / kRowTile;
   if (nq > 32 && !wide) {
     r.q_waves = nq <= 64 ? 2 : nq <= 128 ? 4 : 8;
-    r.shift = 15.f;
+    r.shift = kTileShift;
     r.splits = tile_splits(a, lanes * ((nq + 32 * r.q_waves - 1) / (32 * r.q_waves)), r.q_waves);
   } else {
     r.cols = nq <= 16 ? 1 : 2;
@@ -348,6 +251,7 @@ RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws) {
     return p;
   };
   r.part = take(lanes * r.splits * nq * (a.dv + kRowsPartTail));
+  if (r.q_waves) r.redo = reinterpret_cast<int*>(take(lanes * r.splits * ((nq + 32 * r.q_waves - 1) / (32 * r.q_waves))));
   if (causal && nq <= 16) {
     r.score_st = tiles * kRowTile;
     r.scores = take(lanes * nq * r.score_st);
@@ -363,10 +267,7 @@ int launch_rows_attention(const logkv_rows_args& a, const RowsLaunch& r, hipStre
   if (rc) return rc;
   if (a.dtype == LOGKV_BF16) launch_finish_type<LOGKV_BF16>(a, r, stream);
   else launch_finish_type<LOGKV_F16>(a, r, stream);
-  if (r.lse) {
-    if (a.dtype == LOGKV_BF16) launch_weights<LOGKV_BF16>(a, r, stream);
-    else launch_weights<LOGKV_F16>(a, r, stream);
-  }
+  if (r.lse) return launch_rows_weight(a, r, stream);
   return hipGetLastError() == hipSuccess ? LOGKV_OK : LOGKV_ERUNTIME;
 }
 

@@ -10,21 +10,24 @@ namespace logkv {
 constexpr int kRowTile = 32;        // cache rows (or own rows) per tile
 constexpr int kRowsPartTail = 4;    // a partial's maximum and sum, padded to 16 bytes
 constexpr int kMaxRowSplits = 64;
+constexpr float kTileShift = 7.f;   // tiled kernel: P times 2^7 (below 2^15: its base may lag the maximum by 2^8)
 constexpr float kLog2e = 1.44269504088896341f;
 
 // Launch parameters beside the caller's arguments. Workspace regions, 256-byte aligned:
 // part [lanes, splits, nq, dv + kRowsPartTail]: unnormalised sums, then the base-2 maximum and sum;
 // scores [lanes, nq, score_st]: raw products q . k of up to 16 queries (weight attention);
+// redo: one flag per block of the tiled kernel;
 // lse [lanes, nq]: base-2 log-sum-exp of longer ones (+inf where a query sees nothing).
 struct RowsLaunch {
   float* part;
   float* scores;
   float* lse;
+  int* redo;      // tiled kernel: per block whether its share is left to the second launch
   int64_t score_st;
   int64_t bytes;
   int splits;
   int cols;       // streamed kernel: 16-query column blocks per wave
-  int q_waves;    // tiled kernel: waves with 32 queries each (0: the streamed kernel)
+  int q_waves;    // tiled kernel: waves with 64 queries each (0: the streamed kernel)
   float shift;    // the partials' sums carry 2^shift
   int causal;     // weight attention; otherwise the visible mask
 };
@@ -32,6 +35,7 @@ struct RowsLaunch {
 RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws);
 int launch_rows_stream(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream);
 int launch_rows_tile(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream);
+int launch_rows_weight(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream);
 int launch_rows_attention(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream);
 int launch_evict(const logkv_evict_args& a, hipStream_t stream);
 

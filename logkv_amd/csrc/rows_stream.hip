@@ -187,12 +187,17 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
       for (int c = 0; c < NC; ++c) {
         const int lim = (!of_cache && r.causal ? min(rows, tq[c] + 1 - t0) : rows) - 4 * hq;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int rr = 16 * (j / 4) + j % 4;
-          bool see = rr < lim;
-          if (!of_cache && !r.causal && see)
-            see = gp(a.visible)[b * a.vis_sb + tq[c] * a.vis_st + t0 + 4 * hq + rr] != 0;
-          if (!see) s[c][j / 4][j % 4] = -__builtin_inff();
+        for (int j = 0; j < 8; ++j)
+          if (16 * (j / 4) + j % 4 >= lim) s[c][j / 4][j % 4] = -__builtin_inff();
+        if (!of_cache && !r.causal) {
+          // All flags loaded at once, those past the line's end its last one.
+          const LOGKV_G uint8_t* line = gp(a.visible) + b * a.vis_sb + tq[c] * a.vis_st;
+          uint8_t see[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) see[j] = line[min(t0 + 4 * hq + 16 * (j / 4) + j % 4, a.tq - 1)];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (!see[j]) s[c][j / 4][j % 4] = -__builtin_inff();
         }
       }
     }

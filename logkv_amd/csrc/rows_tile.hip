@@ -1,22 +1,29 @@
 // Attention over a cache's rows and the call's own rows for more queries than a wave's columns:
-// tiles of K and V in LDS, shared by a block's eight waves.
+// tiles of K and V in LDS, shared by a block's four waves.
 //
-// Same mathematics as rows_stream.hip (one pass with a running maximum). QW waves hold 32 queries
-// each (one per lane column, in registers for the whole range), and 8 / QW groups of them take
-// 32 RB rows each of a tile:
-//   S^T = K Q^T by 32x32x16 matrix products (a lane holds 16 rows of its own query per 32 rows);
+// Same mathematics as rows_stream.hip (one pass with a running maximum). QW waves hold 64 queries
+// each (two column blocks of 32, in registers for the whole range), and 4 / QW groups of them take
+// 32 RB rows each of a tile. Per 32 rows:
+//   S^T = K Q^T by 32x32x16 matrix products (a lane holds 16 rows of its own query);
 //   O^T += V^T P^T, where P^T's operand is the lane's own score registers (operand element j of a
 //   16-row step st is row 16 st + 8 (j / 4) + 4 (l / 32) + j % 4) and V is read transposed.
-// bf16 caches: V enters the products as fp16, converted as it is staged (times 2^6: exact from 2^-23
-// up, below that to 2^-31 absolute), and P as fp16 times 2^15 (11 bits): one product per step, a
+// A block has a CU to itself, a wave its SIMD and 512 registers, so nothing hides a wave's waits but
+// the wave: the score products of the next 32 rows are interleaved with the maxima and half of the
+// exponentials of these, the value products with the other half and with the staging of the next
+// tile, one product and the vector work of its 32 cycles at a time. With 64 queries a wave an operand
+// read from LDS serves two products (32 queries a wave, two waves a SIMD, all in step: the reads
+// alone took the products' time).
+// bf16 caches: V enters the products as fp16, converted as it is staged (exact from 2^-17 up,
+// below that to 2^-25 absolute), and P as fp16 times 2^7 (11 bits): one product per step, a
 // third less matrix work than two bf16 parts of P, and P's error stays an eighth of the output's
-// rounding. A share with a tile whose largest magnitude is not in [2^-8, 2^9) is done again in a
-// second form: V as bf16, P as two parts. fp16 caches: P as two fp16 parts in both forms, since one
+// rounding. A share with a tile whose largest magnitude is not in [2^-8, 2^16) is done again by a
+// second launch (in one kernel the second form's registers spilled in the first's loop, and a
+// reload there waits for every load ahead) in a second form: V as bf16, P as two parts. fp16 caches: P as two fp16 parts in both forms, since one
 // part's rounding would equal the output's; the second form is for infinities and NaNs in V, which
 // it adds row by row for the queries that see them.
 // Rows are stored without padding, their 16-byte units permuted by row so that the operand reads
-// and the transposed reads meet every bank once. Two buffers, one barrier per tile, the next
-// tile's rows on their way in registers.
+// and the transposed reads meet every bank once. Two buffers, one barrier per tile, the following
+// tiles' rows on their way in registers.
 #include <algorithm>
 #include <type_traits>
 
@@ -28,10 +35,11 @@ namespace {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 512;
-constexpr float kVScale = 64.f;          // bf16 V as fp16: times 2^6
-constexpr float kPShift = 15.f;          // P times 2^15
+constexpr int kWaves = 8;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kCols = 1;                 // 32-query column blocks per wave
 
 // Where 16-byte unit u of row r is stored: u ^ swizzle. 16 units a row: four consecutive rows fall
 // into distinct 64-byte quarters of the 256-byte bank row, sixteen into distinct units. 8 units a
@@ -58,9 +66,23 @@ __device__ __forceinline__ f32x16 mfma32(uint4 x, uint4 y, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
 }
 
-// Two bf16 values as fp16 times 2^6, exact in the range above.
+// x, not known to be the same from one use to the next: keeps the addresses of rarely taken branches
+// from being computed ahead and held in registers through the loop.
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// A place in program order that x is computed before: products and exponentials stay interleaved as
+// written (the compiler moves them otherwise, to their next use).
+template <typename T>
+__device__ __forceinline__ void here(T& x) {
+  asm volatile("" : "+v"(x));
+}
+
+// Two bf16 values as fp16, exact in the range above.
 __device__ __forceinline__ uint32_t half_of_bf16(uint32_t x) {
-  const f32x2 f = {__uint_as_float(x << 16) * kVScale, __uint_as_float(x & 0xffff0000u) * kVScale};
+  const f32x2 f = {__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)};
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, f16x2));
 }
 
@@ -80,273 +102,508 @@ __device__ __forceinline__ RowsBlock rows_block() {
   return RowsBlock{lin % nx, lin / nx % ny, lin / (nx * ny)};
 }
 
-// What a block's share needs beside its tiles, and what it leaves: a lane's query column with 16
-// features of each 32 per register block.
+// What a block's share needs beside its tiles, and what it leaves: per column block a lane's query
+// with 16 features of each 32 per register block.
 template <int NKS, int NDV>
 struct RowsShare {
-  int b, g, t, n, own, np, begin, end;
-  uint4 qf[NKS];
-  f32x16 o[NDV];
-  float m, lsum;
+  int b, g, n, own, np, begin, end;
+  int t[kCols];
+  uint4 qf[kCols][NKS];
+  f32x16 o[kCols][NDV];
+  float m[kCols], lsum[kCols];
 };
 
-// A share's tiles. False where the first form (SECOND false) meets a tile that it cannot take.
-// NKS 16-wide steps of dk, NDV 32-wide blocks of dv.
-template <int DT, int NKS, int NDV, int QW, int RB, bool BIAS, bool SECOND>
+template <int NKS, int NDV>
+__device__ __forceinline__ void clear_sums(RowsShare<NKS, NDV>& c) {
+#pragma unroll
+  for (int k = 0; k < kCols; ++k) {
+#pragma unroll
+    for (int nb = 0; nb < NDV; ++nb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) c.o[k][nb][i] = 0.f;
+    c.m[k] = -__builtin_inff();
+    c.lsum[k] = 0.f;
+  }
+}
+
+// A share's tiles in the first form; false where it meets one that it cannot take. NKS 16-wide steps
+// of dk, NDV 32-wide blocks of dv.
+template <int DT, int NKS, int NDV, int QW, int RB, bool BIAS>
 __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const RowsLaunch& r, RowsShare<NKS, NDV>& c,
-                                                uint8_t* buf, float (*bias_s)[32 * RB * 8 / QW], int* flag_s) {
+                                                uint8_t* buf, float (*bias_s)[32 * RB * kWaves / QW], int* flag_s) {
   typedef __attribute__((address_space(3))) s16x4* lds4;
-  constexpr int RW = 8 / QW, TR = 32 * RB * RW;        // row groups, rows per tile
+  typedef __attribute__((address_space(3))) const uint8_t* ldsb;
+  typedef __attribute__((address_space(3))) const u32x4* ldsq;
+  constexpr int RW = kWaves / QW, TR = 32 * RB * RW;   // row groups, rows per tile
   constexpr int KU = 2 * NKS, VU = 4 * NDV;            // 16-byte units of a staged row
   constexpr int kKTasks = TR * KU / kThreads, kVTasks = TR * VU / kThreads;
   constexpr int kTileBytes = TR * (KU + VU) * 16;
-  constexpr bool kHalfV = DT == LOGKV_BF16 && !SECOND; // V converted to fp16
-  constexpr int kPDT = kHalfV ? LOGKV_F16 : DT;        // type of the value products
-  constexpr float kVFactor = DT == LOGKV_BF16 && SECOND ? kVScale : 1.f;   // both forms' sums carry V's scale
-  static_assert(8 * 16 * 32 * 4 <= kTileBytes, "a tile buffer holds 16 rows' probabilities of every wave");
-  const int tid = threadIdx.x, w = wave_id(), l = lane_id(), h = l >> 5, col = l & 31, rw = w / QW;
-  const int kunits = a.dk / 8, vunits = a.dv / 8, b = c.b, g = c.g, t = c.t, np = c.np, begin = c.begin, end = c.end;
+  constexpr bool kHalfV = DT == LOGKV_BF16;            // V converted to fp16
+  const int tid = threadIdx.x, l = lane_id(), h = l >> 5, col = l & 31, rw = wave_id() / QW;
+  const int kunits = a.dk / 8, vunits = a.dv / 8, b = c.b, g = c.g, np = c.np, begin = c.begin, end = c.end;
+  auto k_tile = [&](int bf) { return reinterpret_cast<uint4*>(buf + bf * kTileBytes); };
+  auto v_tile = [&](int bf) { return reinterpret_cast<uint4*>(buf + bf * kTileBytes + TR * KU * 16); };
+
+  // Registers of the tiles on their way: K two tiles ahead of the sums, V one. A thread's units are
+  // rows tid / KU + kThreads / KU q of a tile. The loads are issued on one path for every tile (values
+  // merged from two would be waited for at the merge): rows past a tile's are its last one, units past
+  // dk and dv the last ones. When stored, V's extra rows and K's extra units become zero (extra rows of
+  // K are masked in the scores, extra units of V reach only features that are not written out).
+  uint4 kx[kKTasks], vx[kVTasks];
+  uint16_t bx[2] = {0, 0};
+  const int ku = tid % KU, kr0 = tid / KU, vr0 = tid / VU;
+  const int ku8 = 8 * min(ku, kunits - 1), vu8 = 8 * min(tid % VU, vunits - 1);
   const LOGKV_G uint16_t* kc = gp(a.cache_k) + b * a.ck_sb + g * a.ck_sg;
   const LOGKV_G uint16_t* vc = gp(a.cache_v) + b * a.cv_sb + g * a.cv_sg;
   const LOGKV_G uint16_t* ko = gp(a.k) + b * a.k_sb + g * a.k_sg;
   const LOGKV_G uint16_t* vo = gp(a.v) + b * a.v_sb + g * a.v_sg;
-  auto k_tile = [&](int bf) { return reinterpret_cast<uint4*>(buf + bf * kTileBytes); };
-  auto v_tile = [&](int bf) { return reinterpret_cast<uint4*>(buf + bf * kTileBytes + TR * KU * 16); };
-
-  // Registers of the tile on its way. Rows past the tile's: K repeats the last one (masked in the
-  // scores), V is zero; units past dk and dv are zero.
-  uint4 kx[kKTasks], vx[kVTasks];
-  float bx = 0.f;
-  auto load = [&](int ti) {
-    const bool of_cache = ti < np;
-    const int t0 = TR * (of_cache ? ti : ti - np), rows = min(TR, (of_cache ? c.n : c.own) - t0);
-    const int64_t kst = of_cache ? a.ck_st : a.k_st, vst = of_cache ? a.cv_st : a.v_st;
-    const LOGKV_G uint16_t* kr = (of_cache ? kc : ko) + t0 * kst;
-    const LOGKV_G uint16_t* vr = (of_cache ? vc : vo) + t0 * vst;
+  auto rows_in = [&](int ti) { return ti < np ? min(TR, c.n - TR * ti) : min(TR, c.own - TR * (ti - np)); };
+  auto load_k = [&](int ti) {
+    const int t0 = TR * (ti < np ? ti : ti - np), last = rows_in(ti) - 1;
+    const int64_t st = ti < np ? a.ck_st : a.k_st;
+    const LOGKV_G uint16_t* base = (ti < np ? kc : ko) + t0 * st;
 #pragma unroll
-    for (int q = 0; q < kKTasks; ++q) {
-      const int i = tid + kThreads * q, rr = min(i / KU, rows - 1), u = i % KU;
-      kx[q] = make_uint4(0, 0, 0, 0);
-      if (u < kunits) kx[q] = *(const LOGKV_G uint4*)(kr + rr * kst + 8 * u);
-    }
-#pragma unroll
-    for (int q = 0; q < kVTasks; ++q) {
-      const int i = tid + kThreads * q, rr = i / VU, u = i % VU;
-      vx[q] = make_uint4(0, 0, 0, 0);
-      if (u < vunits && rr < rows) vx[q] = *(const LOGKV_G uint4*)(vr + rr * vst + 8 * u);
-    }
+    for (int q = 0; q < kKTasks; ++q) kx[q] = *(const LOGKV_G uint4*)(base + min(kr0 + kThreads / KU * q, last) * st + ku8);
     if constexpr (BIAS) {
-      if (tid < TR) {
-        bx = 0.f;
-        if (of_cache) {
-          const int64_t at = b * a.b_sb + g * a.b_sg + (t0 + min(tid, rows - 1)) * a.b_st;
-          bx = bias_base2(a.bias_half ? Elem<DT>::to_f32(gp(static_cast<const uint16_t*>(a.bias))[at])
-                                      : gp(static_cast<const float*>(a.bias))[at]);
-        }
+      // A bias as its 16-bit halves (behind the cache's rows: any 4 bytes, not used).
+      const LOGKV_G uint16_t* at = gp(a.q);
+      if (ti < np) at = gp(static_cast<const uint16_t*>(a.bias)) + (a.bias_half ? 1 : 2) * (b * a.b_sb + g * a.b_sg + (t0 + min(tid % TR, last)) * a.b_st);
+      bx[0] = at[0];
+      bx[1] = at[a.bias_half ? 0 : 1];
+    }
+  };
+  auto load_v = [&](int ti) {
+    const int t0 = TR * (ti < np ? ti : ti - np), last = rows_in(ti) - 1;
+    const int64_t st = ti < np ? a.cv_st : a.v_st;
+    const LOGKV_G uint16_t* base = (ti < np ? vc : vo) + t0 * st;
+#pragma unroll
+    for (int q = 0; q < kVTasks; ++q) vx[q] = *(const LOGKV_G uint4*)(base + min(vr0 + kThreads / VU * q, last) * st + vu8);
+  };
+  auto store_k = [&](int ti, int bf, int q) {
+    const int rr = kr0 + kThreads / KU * q;
+    if (kunits < KU && ku >= kunits) kx[q] = make_uint4(0, 0, 0, 0);
+    k_tile(bf)[rr * KU + (ku ^ swizzle<KU>(rr))] = kx[q];
+    if constexpr (BIAS) {
+      if (q == 0 && tid < TR) {
+        const float x = a.bias_half ? Elem<DT>::to_f32(bx[0]) : __uint_as_float(bx[0] | static_cast<uint32_t>(bx[1]) << 16);
+        bias_s[bf][tid] = ti < np ? bias_base2(x) : 0.f;
       }
     }
   };
-  // Flags of a tile's V magnitudes: 1 some at 2^9 (fp16 caches and the second form: not finite) or
-  // above, 2 some nonzero, 4 some at 2^-8 or above.
-  auto store = [&](int ti, int bf) {
+  // V stored, its magnitudes gathered in top.
+  u16x2 top = {0, 0};
+  auto store_v = [&](int ti, int bf, int q) {
+    const int rr = vr0 + kThreads / VU * q, rows = rows_in(ti);
+    if (rows < TR && rr >= rows) vx[q] = make_uint4(0, 0, 0, 0);
+    uint32_t x4[4] = {vx[q].x, vx[q].y, vx[q].z, vx[q].w};
 #pragma unroll
-    for (int q = 0; q < kKTasks; ++q) {
-      const int i = tid + kThreads * q, rr = i / KU, u = i % KU;
-      k_tile(bf)[rr * KU + (u ^ swizzle<KU>(rr))] = kx[q];
+    for (int j = 0; j < 4; ++j) {
+      top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, x4[j] & 0x7fff7fffu));
+      if constexpr (kHalfV) x4[j] = half_of_bf16(x4[j]);
     }
-    u16x2 top = {0, 0};
-#pragma unroll
-    for (int q = 0; q < kVTasks; ++q) {
-      const int i = tid + kThreads * q, rr = i / VU, u = i % VU;
-      uint32_t x4[4] = {vx[q].x, vx[q].y, vx[q].z, vx[q].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, x4[j] & 0x7fff7fffu));
-        if constexpr (kHalfV) x4[j] = half_of_bf16(x4[j]);
-      }
-      v_tile(bf)[rr * VU + (u ^ swizzle<VU>(rr))] = make_uint4(x4[0], x4[1], x4[2], x4[3]);
-    }
+    v_tile(bf)[rr * VU + (tid % VU ^ swizzle<VU>(rr))] = make_uint4(x4[0], x4[1], x4[2], x4[3]);
+  };
+  // Flags of tile ti's V: 1 some magnitude at 2^16 (fp16 caches: not finite) or above, 2 some nonzero,
+  // 4 some at 2^-8 or above.
+  auto store_flags = [&](int ti) {
     const int mag = max(static_cast<int>(top[0]), static_cast<int>(top[1]));
-    constexpr int kMost = kHalfV ? (127 + 9) << 7 : static_cast<int>(Elem<DT>::kInf), kLeast = (127 - 8) << 7;
+    constexpr int kMost = kHalfV ? (127 + 16) << 7 : static_cast<int>(Elem<DT>::kInf), kLeast = (127 - 8) << 7;
     const int bits = (__ballot(mag >= kMost) ? 1 : 0) | (kHalfV ? (__ballot(mag != 0) ? 2 : 0) | (__ballot(mag >= kLeast) ? 4 : 0) : 0);
     if (bits && l == 0) atomicOr(&flag_s[(ti - begin) % 3], bits);
-    if constexpr (BIAS) {
-      if (tid < TR) bias_s[bf][tid] = bx;
-    }
+    top = u16x2{0, 0};
   };
-#pragma unroll
-  for (int nb = 0; nb < NDV; ++nb)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) c.o[nb][i] = 0.f;
-  c.m = -__builtin_inff();
-  c.lsum = 0.f;
+  clear_sums(c);
+  if (begin >= end) return true;
   const float c2 = a.scale * kLog2e;
-  if (tid < 3) flag_s[tid] = 0;
-  __syncthreads();   // the flags are clear
-  if (begin < end) {
-    load(begin);
-    store(begin, 0);
-    if (begin + 1 < end) load(begin + 1);
-  }
   const int r0 = 32 * RB * rw;   // this wave's rows of a tile
-  for (int ti = begin; ti < end; ++ti) {
-    const int it = ti - begin, bf = it & 1;
-    __syncthreads();   // tile ti is stored, tile ti - 1 has been read
-    const int flags = flag_s[it % 3];
-    if (!SECOND && ((flags & 1) || (flags & 6) == 2)) return false;
-    if (tid == 0) flag_s[(it + 2) % 3] = 0;
-    const bool own = ti >= np;
-    const int t0 = TR * (own ? ti - np : ti), rows = min(TR, (own ? c.own : c.n) - t0);
-    // V^T operand of rows 16 st .. + 15 (in P's order), features 32 nb + l % 32.
-    auto load_vt = [&](int nb, int st) {
-      const int i = l & 15, ra = r0 + 16 * st + 4 * h + (i >> 2), rb = ra + 8, f = 32 * nb + (l & 16) + 4 * (i & 3);
-      const uint16_t* base = reinterpret_cast<const uint16_t*>(v_tile(bf));
-      const uint16_t* p0 = base + ra * (8 * VU) + 8 * ((f >> 3) ^ swizzle<VU>(ra)) + (f & 7);
-      const uint16_t* p1 = base + rb * (8 * VU) + 8 * ((f >> 3) ^ swizzle<VU>(rb)) + (f & 7);
-      const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p0)));
-      const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p1)));
-      return make_uint4(x.x, x.y, y.x, y.y);
-    };
-    f32x16 s[RB];
+  if (tid < 3) flag_s[tid] = 0;
+  load_k(begin);
+  load_v(begin);
 #pragma unroll
-    for (int kb = 0; kb < RB; ++kb)
+  for (int q = 0; q < kKTasks; ++q) store_k(begin, 0, q);
+  load_k(min(begin + 1, end - 1));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
+  for (int q = 0; q < kKTasks; ++q) store_k(min(begin + 1, end - 1), 1, q);
+  __syncthreads();   // the flags are clear, K of the first tiles is stored
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks)
+  for (int q = 0; q < kVTasks; ++q) store_v(begin, 0, q);
+  store_flags(begin);
+  load_k(min(begin + 2, end - 1));
+  load_v(min(begin + 1, end - 1));
+
+  // LDS addresses of this lane's operands in buffer 0: K of its row (unit 2 ks + h), V of its
+  // transposed reads (features 32 nb + l % 32 of rows 4 h .. and 8 + 4 h ..).
+  ldsb k_at[NKS], v_at[NDV][2];
+  {
+    const int rr = r0 + col, i = l & 15;
 #pragma unroll
-      for (int kb = 0; kb < RB; ++kb) {
-        const int rr = r0 + 32 * kb + col;
-        s[kb] = mfma32<DT>(k_tile(bf)[rr * KU + ((2 * ks + h) ^ swizzle<KU>(rr))], c.qf[ks], s[kb]);
+    for (int ks = 0; ks < NKS; ++ks) k_at[ks] = (ldsb)(buf + 16 * (rr * KU + ((2 * ks + h) ^ swizzle<KU>(rr))));
+#pragma unroll
+    for (int nb = 0; nb < NDV; ++nb)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int rv = r0 + 4 * h + (i >> 2) + 8 * half, f = 32 * nb + (l & 16) + 4 * (i & 3);
+        v_at[nb][half] = (ldsb)(buf + TR * KU * 16 + 16 * (rv * VU + ((f >> 3) ^ swizzle<VU>(rv))) + 2 * (f & 7));
       }
+  }
+  // K operand ks of 32-row block kb, V^T operand nb of the 16 rows st (in P's order) of a tile.
+  auto k_frag = [&](int bf, int kb, int ks) { return __builtin_bit_cast(uint4, *(ldsq)(k_at[ks] + bf * kTileBytes + kb * 32 * KU * 16)); };
+  auto v_frag = [&](int bf, int st, int nb) {
+    const int at = bf * kTileBytes + st * 16 * VU * 16;
+    const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(v_at[nb][0] + at)));
+    const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(v_at[nb][1] + at)));
+    return make_uint4(x.x, x.y, y.x, y.y);
+  };
+  // Scores of the next 32 rows, then with their bias and masks; the first half of their products'
+  // operands is read ahead.
+  constexpr int kHalf = NKS / 2;
+  f32x16 next[kCols];
+  uint4 kf[kHalf];
+  float mx[kCols], arg0[kCols];
+#pragma unroll
+  for (int k = 0; k < kCols; ++k) arg0[k] = kTileShift;
+  // Element i is row r0 + 32 kb + 8 (i / 4) + 4 h + i % 4 of tile ti.
+  auto finish_scores = [&](int ti, int kb) {
+    const bool own = ti >= np;
+    const int bf = (ti - begin) & 1, t0 = TR * (own ? ti - np : ti), rows = min(TR, (own ? c.own : c.n) - t0);
     if constexpr (BIAS) {
 #pragma unroll
-      for (int kb = 0; kb < RB; ++kb)
+      for (int i4 = 0; i4 < 4; ++i4) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(&bias_s[bf][r0 + 32 * kb + 8 * i4 + 4 * h]);
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(&bias_s[bf][r0 + 32 * kb + 8 * i4 + 4 * h]);
+        for (int k = 0; k < kCols; ++k)
 #pragma unroll
           for (int i = 0; i < 4; ++i)   // a row hidden by -inf stays hidden whatever its key holds
-            s[kb][4 * i4 + i] = x[i] == -__builtin_inff() ? x[i] : __builtin_fmaf(s[kb][4 * i4 + i], c2, x[i]);
-        }
+            next[k][4 * i4 + i] = x[i] == -__builtin_inff() ? x[i] : __builtin_fmaf(next[k][4 * i4 + i], c2, x[i]);
+      }
     }
-    // Masks: element i of block kb is row r0 + 32 kb + 8 (i / 4) + 4 h + i % 4 of the tile.
     if (own || rows < TR) {
-      const int lim = (own && r.causal ? min(rows, t + 1 - t0) : rows) - r0 - 4 * h;
 #pragma unroll
-      for (int kb = 0; kb < RB; ++kb)
+      for (int k = 0; k < kCols; ++k) {
+        const int lim = (own && r.causal ? min(rows, fresh(c.t[k]) + 1 - t0) : rows) - r0 - 32 * kb - 4 * h;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int rr = 32 * kb + 8 * (i / 4) + i % 4;
-          bool see = rr < lim;
-          if (own && !r.causal && see)
-            see = gp(a.visible)[b * a.vis_sb + t * a.vis_st + t0 + r0 + 4 * h + rr] != 0;
-          if (!see) s[kb][i] = -__builtin_inff();
+        for (int i = 0; i < 16; ++i)
+          if (8 * (i / 4) + i % 4 >= lim) next[k][i] = -__builtin_inff();
+        if (own && !r.causal) {
+          // All flags loaded at once, those past the line's end its last one.
+          const LOGKV_G uint8_t* line = gp(a.visible) + b * a.vis_sb + fresh(c.t[k]) * a.vis_st;
+          const int first = t0 + r0 + 32 * kb + 4 * h;
+          uint8_t see[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) see[i] = line[min(first + 8 * (i / 4) + i % 4, a.tq - 1)];
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (!see[i]) next[k][i] = -__builtin_inff();
         }
+      }
     }
-    float mx = -__builtin_inff();
 #pragma unroll
-    for (int kb = 0; kb < RB; ++kb)
+    for (int k = 0; k < kCols; ++k) mx[k] = -__builtin_inff();
+  };
+  // The sums' base moves when a maximum passes it by more than 2^8 (P stays below 2^(8 + kTileShift)):
+  // a few times a share instead of at every new maximum.
+  auto move_base = [&]() {
+    float y[kCols];
+    bool past = false;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-    mx = pair_max32(mx);
-    const float m_new = fmaxf(c.m, BIAS ? mx : mx * c2);
-    const float mb = m_new == -__builtin_inff() ? 0.f : m_new;
-    const float corr = __builtin_amdgcn_exp2f(c.m - mb);
-    c.m = m_new;
-    if (__ballot(corr != 1.f)) {
-      c.lsum *= corr;
+    for (int k = 0; k < kCols; ++k) {
+      const float x = pair_max32(mx[k]);
+      y[k] = BIAS ? x : x * c2;
+      past |= y[k] > c.m[k] + 8.f;
+    }
+    if (!__ballot(past)) return;
+#pragma unroll
+    for (int k = 0; k < kCols; ++k) {
+      const float m_new = fmaxf(c.m[k], y[k]), mb = m_new == -__builtin_inff() ? 0.f : m_new;
+      const float corr = __builtin_amdgcn_exp2f(c.m[k] - mb);
+      c.m[k] = m_new;
+      arg0[k] = kTileShift - mb;
+      c.lsum[k] *= corr;
 #pragma unroll
       for (int nb = 0; nb < NDV; ++nb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) c.o[nb][i] *= corr;
+        for (int i = 0; i < 16; ++i) c.o[k][nb][i] *= corr;
     }
-    uint32_t seen[RB];   // the second form: rows that the query sees
-    if constexpr (SECOND) {
+  };
 #pragma unroll
-      for (int kb = 0; kb < RB; ++kb) {
-        seen[kb] = 0;
+  for (int k = 0; k < kCols; ++k)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) seen[kb] |= (s[kb][i] != -__builtin_inff() ? 1u : 0u) << (8 * (i / 4) + 4 * h + i % 4);
-        seen[kb] |= __shfl_xor(seen[kb], 32, kWave);
+    for (int i = 0; i < 16; ++i) next[k][i] = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks) {
+    kf[ks % kHalf] = k_frag(0, 0, ks);
+#pragma unroll
+    for (int k = 0; k < kCols; ++k) next[k] = mfma32<DT>(kf[ks % kHalf], c.qf[k][ks], next[k]);
+  }
+  finish_scores(begin, 0);
+#pragma unroll
+  for (int k = 0; k < kCols; ++k)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx[k] = fmaxf(mx[k], next[k][i]);
+  move_base();
+#pragma unroll
+  for (int ks = 0; ks < kHalf; ++ks) kf[ks] = k_frag(RB > 1 ? 0 : 1, RB > 1 ? 1 : 0, ks);
+
+  for (int ti = begin; ti < end; ++ti) {
+    const int it = ti - begin, bf = it & 1;
+    __syncthreads();   // V of tile ti and K of tile ti + 1 are stored, V of tile ti - 1 and K of tile ti have been read
+    const int flags = flag_s[it % 3];
+    if ((flags & 1) || (flags & 6) == 2) return false;
+    if (tid == 0) flag_s[(it + 2) % 3] = 0;
+#pragma unroll
+    for (int kb = 0; kb < RB; ++kb) {
+      // 32 rows: their exponentials among the score products of the next 32, then their value products
+      // among the maxima of those and, behind a tile's last rows, the staging of the next tiles. (Behind
+      // the share's last rows the scores are of what the buffer holds, and unused.)
+      f32x16 s[kCols];
+#pragma unroll
+      for (int k = 0; k < kCols; ++k) {
+        s[k] = next[k];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) next[k][i] = 0.f;
       }
-    }
-    const float arg0 = kPShift - mb;
-    float sum = 0.f;
+      const int nbf = kb + 1 < RB ? bf : bf ^ 1, nkb = kb + 1 < RB ? kb + 1 : 0;
+      uint4 vf[NDV];
+      if constexpr (RB == 1) {
 #pragma unroll
-    for (int kb = 0; kb < RB; ++kb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[kb][i] = __builtin_amdgcn_exp2f(BIAS ? s[kb][i] + arg0 : __builtin_fmaf(s[kb][i], c2, arg0));
-        sum += s[kb][i];
+        for (int ks = 0; ks < kHalf; ++ks) kf[ks] = k_frag(nbf, nkb, ks);
       }
-    c.lsum += sum;
-    if (!SECOND || !(flags & 1)) {
 #pragma unroll
-      for (int st = 0; st < 2 * RB; ++st) {
-        uint32_t hi[4], lo[4];
+      for (int nb = 0; nb < NDV; ++nb) vf[nb] = v_frag(bf, 2 * kb, nb);
+      uint32_t hi[kCols][2][4], lo[kCols][2][4];
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float p0 = s[st / 2][8 * (st % 2) + 2 * j], p1 = s[st / 2][8 * (st % 2) + 2 * j + 1];
-          if constexpr (kHalfV) hi[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{p0, p1}, f16x2));
-          else Elem<DT>::parts(kVFactor * p0, kVFactor * p1, hi[j], lo[j]);
+      for (int ks = 0; ks < NKS; ++ks)
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) {
+          next[k] = mfma32<DT>(kf[ks % kHalf], c.qf[k][ks], next[k]);
+          if (k == kCols - 1 && ks < kHalf) kf[ks] = k_frag(nbf, nkb, ks + kHalf);
+          here(next[k]);
+#pragma unroll
+          for (int i = 16 / NKS * ks; i < 16 / NKS * (ks + 1); i += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(BIAS ? s[k][i] + arg0[k] : __builtin_fmaf(s[k][i], c2, arg0[k]));
+            const float p1 = __builtin_amdgcn_exp2f(BIAS ? s[k][i + 1] + arg0[k] : __builtin_fmaf(s[k][i + 1], c2, arg0[k]));
+            c.lsum[k] += p0;
+            c.lsum[k] += p1;
+            if constexpr (kHalfV) hi[k][i / 8][i / 2 % 4] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{p0, p1}, f16x2));
+            else Elem<DT>::parts(p0, p1, hi[k][i / 8][i / 2 % 4], lo[k][i / 8][i / 2 % 4]);
+            here(hi[k][i / 8][i / 2 % 4]);
+            here(c.lsum[k]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
+      const bool last = kb + 1 == RB, stage_k = last && ti + 2 < end, stage_v = last && ti + 1 < end;
+      if (!last || ti + 1 < end) finish_scores(last ? ti + 1 : ti, nkb);
+      constexpr int kSlots = 2 * NDV * kCols;
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int nb = 0; nb < NDV; ++nb) {
-          const uint4 v = load_vt(nb, st);
-          c.o[nb] = mfma32<kPDT>(v, make_uint4(hi[0], hi[1], hi[2], hi[3]), c.o[nb]);
-          if constexpr (!kHalfV) c.o[nb] = mfma32<kPDT>(v, make_uint4(lo[0], lo[1], lo[2], lo[3]), c.o[nb]);
-        }
-      }
-    } else if constexpr (SECOND) {
-      // Not finite: row by row in float32, each for the queries that see it. The probabilities pass
-      // through the other tile buffer, which holds nothing now.
-      float* p_s = reinterpret_cast<float*>(buf + (bf ^ 1) * kTileBytes) + w * 16 * 32;
+      for (int st = 0; st < 2; ++st)
 #pragma unroll
-      for (int st = 0; st < 2 * RB; ++st) {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int nb = 0; nb < NDV; ++nb)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p_s[32 * (8 * (j / 4) + 4 * h + j % 4) + col] = kVFactor * s[st / 2][8 * (st % 2) + j];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-        for (int k = 0; k < 16; ++k) {
-          const int rr = r0 + 16 * st + k;
-          const float pk = p_s[32 * k + col];
-          const bool see = seen[st / 2] >> (16 * (st % 2) + k) & 1;
+          for (int k = 0; k < kCols; ++k) {
+            const int j = (st * NDV + nb) * kCols + k;
+            c.o[k][nb] = mfma32<LOGKV_F16>(vf[nb], make_uint4(hi[k][st][0], hi[k][st][1], hi[k][st][2], hi[k][st][3]), c.o[k][nb]);
+            if constexpr (!kHalfV)
+              c.o[k][nb] = mfma32<LOGKV_F16>(vf[nb], make_uint4(lo[k][st][0], lo[k][st][1], lo[k][st][2], lo[k][st][3]), c.o[k][nb]);
+            if (k == kCols - 1 && st == 0) vf[nb] = v_frag(bf, 2 * kb + 1, nb);
+            here(c.o[k][nb]);
 #pragma unroll
-          for (int nb = 0; nb < NDV; ++nb)
+            for (int kk = 0; kk < kCols; ++kk) {
 #pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4) {
-              const uint16_t* v = reinterpret_cast<const uint16_t*>(v_tile(bf) + rr * VU + ((4 * nb + i4) ^ swizzle<VU>(rr))) + 4 * h;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float x = pk * Elem<DT>::to_f32(v[i]);
-                c.o[nb][4 * i4 + i] += see ? x : 0.f;
-              }
+              for (int i = 16 / kSlots * j; i < 16 / kSlots * (j + 1); ++i) mx[kk] = fmaxf(mx[kk], next[kk][i]);
+              here(mx[kk]);
             }
-        }
+            if constexpr (RB > 1) {
+              // After (ti, 0) the products were of (ti, 1), the ones to come are of (ti + 1, 0); after (ti, 1),
+              // of (ti + 1, 1).
+              if (j < kHalf) kf[j] = k_frag(bf ^ 1, kb, j);
+            }
+            if (stage_v) {
+              constexpr int kStores = (kVTasks + kSlots - 1) / kSlots;
+#pragma unroll
+              for (int q = kStores * j; q < min(kStores * (j + 1), kVTasks); ++q) store_v(ti + 1, bf ^ 1, q);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+      if (!last || ti + 1 < end) move_base();
+      if (stage_k) {
+#pragma unroll
+        for (int q = 0; q < kKTasks; ++q) store_k(ti + 2, bf, q);
       }
-      __syncthreads();
+      if (stage_v) store_flags(ti + 1);
     }
-    if (ti + 1 < end) {
-      store(ti + 1, bf ^ 1);
-      if (ti + 2 < end) load(ti + 2);
-    }
+    load_k(min(ti + 3, end - 1));
+    load_v(min(ti + 2, end - 1));
   }
   return true;
 }
 
+// The same in the second form: V in its own type, P as two parts of that type, and a tile that is not
+// finite row by row in float32, each row for the queries that see it. Plain steps (one buffer, nothing
+// ahead): shares that need it are rare.
 template <int DT, int NKS, int NDV, int QW, int RB, bool BIAS>
+__device__ __forceinline__ void rows_tile_share2(const logkv_rows_args& a, const RowsLaunch& r, RowsShare<NKS, NDV>& c,
+                                                 uint8_t* buf, float (*bias_s)[32 * RB * kWaves / QW], int* flag_s) {
+  typedef __attribute__((address_space(3))) s16x4* lds4;
+  constexpr int RW = kWaves / QW, TR = 32 * RB * RW, KU = 2 * NKS, VU = 4 * NDV;
+  static_assert(kWaves * 16 * 32 * 4 <= TR * (KU + VU) * 16, "the second buffer holds 16 rows' probabilities of every wave");
+  const int tid = threadIdx.x, w = wave_id(), l = lane_id(), h = l >> 5, col = l & 31, r0 = 32 * RB * (w / QW);
+  uint4* ks_ = reinterpret_cast<uint4*>(buf);
+  uint4* vs_ = reinterpret_cast<uint4*>(buf + TR * KU * 16);
+  float* p_s = reinterpret_cast<float*>(buf + TR * (KU + VU) * 16) + w * 16 * 32;
+  clear_sums(c);
+  const float c2 = a.scale * kLog2e;
+#pragma unroll 1
+  for (int ti = c.begin; ti < c.end; ++ti) {
+    const bool own = ti >= c.np;
+    const int t0 = TR * (own ? ti - c.np : ti), rows = min(TR, (own ? c.own : c.n) - t0);
+    const int64_t kst = own ? a.k_st : a.ck_st, vst = own ? a.v_st : a.cv_st;
+    const LOGKV_G uint16_t* kr = (own ? gp(a.k) + c.b * a.k_sb + c.g * a.k_sg : gp(a.cache_k) + c.b * a.ck_sb + c.g * a.ck_sg) + t0 * kst;
+    const LOGKV_G uint16_t* vr = (own ? gp(a.v) + c.b * a.v_sb + c.g * a.v_sg : gp(a.cache_v) + c.b * a.cv_sb + c.g * a.cv_sg) + t0 * vst;
+    __syncthreads();   // the last tile has been read
+    if (tid == 0) flag_s[0] = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < TR * KU; i += kThreads) {
+      const int rr = i / KU, u = i % KU;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (8 * u < a.dk) x = *(const LOGKV_G uint4*)(kr + min(rr, rows - 1) * kst + 8 * u);
+      ks_[rr * KU + (u ^ swizzle<KU>(rr))] = x;
+    }
+#pragma unroll 1
+    for (int i = tid; i < TR * VU; i += kThreads) {
+      const int rr = i / VU, u = i % VU;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (8 * u < a.dv && rr < rows) x = *(const LOGKV_G uint4*)(vr + rr * vst + 8 * u);
+      const uint32_t x4[4] = {x.x, x.y, x.z, x.w};
+      uint32_t most = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) most = max(most, max(x4[j] & 0x7fffu, x4[j] >> 16 & 0x7fffu));
+      if (most >= Elem<DT>::kInf) flag_s[0] = 1;
+      vs_[rr * VU + (u ^ swizzle<VU>(rr))] = x;
+    }
+    if constexpr (BIAS) {
+      if (tid < TR) {
+        float x = 0.f;
+        if (!own) {
+          const int64_t at = c.b * a.b_sb + c.g * a.b_sg + (t0 + min(tid, rows - 1)) * a.b_st;
+          x = bias_base2(a.bias_half ? Elem<DT>::to_f32(gp(static_cast<const uint16_t*>(a.bias))[at])
+                                     : gp(static_cast<const float*>(a.bias))[at]);
+        }
+        bias_s[0][tid] = x;
+      }
+    }
+    __syncthreads();
+    const bool finite = flag_s[0] == 0;
+#pragma unroll 1
+    for (int kb = 0; kb < RB; ++kb) {
+#pragma unroll
+      for (int k = 0; k < kCols; ++k) {
+        f32x16 s;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = 0.f;
+        const int rk = r0 + 32 * kb + col;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) {
+          s = mfma32<DT>(ks_[rk * KU + ((2 * ks + h) ^ swizzle<KU>(rk))], c.qf[k][ks], s);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        const int lim = (own && r.causal ? min(rows, c.t[k] + 1 - t0) : rows) - r0 - 32 * kb - 4 * h;
+        const LOGKV_G uint8_t* line = gp(a.visible) + c.b * a.vis_sb + c.t[k] * a.vis_st + t0 + r0 + 32 * kb + 4 * h;
+        uint32_t seen = 0;
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int rr = 8 * (i / 4) + i % 4;
+          if constexpr (BIAS) {
+            const float x = bias_s[0][r0 + 32 * kb + 4 * h + rr];
+            s[i] = x == -__builtin_inff() ? x : __builtin_fmaf(s[i], c2, x);
+          }
+          bool see = rr < lim;
+          if (own && !r.causal && see) see = line[rr] != 0;
+          if (!see) s[i] = -__builtin_inff();
+          mx = fmaxf(mx, s[i]);
+          seen |= (s[i] != -__builtin_inff() ? 1u : 0u) << (rr + 4 * h);
+        }
+        seen |= __shfl_xor(seen, 32, kWave);
+        mx = pair_max32(mx);
+        const float m_new = fmaxf(c.m[k], BIAS ? mx : mx * c2);
+        const float mb = m_new == -__builtin_inff() ? 0.f : m_new, corr = __builtin_amdgcn_exp2f(c.m[k] - mb);
+        c.m[k] = m_new;
+        c.lsum[k] *= corr;
+#pragma unroll
+        for (int nb = 0; nb < NDV; ++nb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) c.o[k][nb][i] *= corr;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[i] = __builtin_amdgcn_exp2f(BIAS ? s[i] + (kTileShift - mb) : __builtin_fmaf(s[i], c2, kTileShift - mb));
+          c.lsum[k] += s[i];
+        }
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          if (finite) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) Elem<DT>::parts(s[8 * st + 2 * j], s[8 * st + 2 * j + 1], hi[j], lo[j]);
+#pragma unroll
+            for (int nb = 0; nb < NDV; ++nb) {
+              const int i = l & 15, ra = r0 + 32 * kb + 16 * st + 4 * h + (i >> 2), rb = ra + 8, f = 32 * nb + (l & 16) + 4 * (i & 3);
+              const uint16_t* base = reinterpret_cast<const uint16_t*>(vs_);
+              const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(base + ra * (8 * VU) + 8 * ((f >> 3) ^ swizzle<VU>(ra)) + (f & 7))));
+              const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(base + rb * (8 * VU) + 8 * ((f >> 3) ^ swizzle<VU>(rb)) + (f & 7))));
+              const uint4 v = make_uint4(x.x, x.y, y.x, y.y);
+              c.o[k][nb] = mfma32<DT>(v, make_uint4(hi[0], hi[1], hi[2], hi[3]), c.o[k][nb]);
+              c.o[k][nb] = mfma32<DT>(v, make_uint4(lo[0], lo[1], lo[2], lo[3]), c.o[k][nb]);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          } else {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p_s[32 * (8 * (j / 4) + 4 * h + j % 4) + col] = s[8 * st + j];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+            for (int j = 0; j < 16; ++j) {
+              const int rr = r0 + 32 * kb + 16 * st + j;
+              const float pk = p_s[32 * j + col];
+              const bool see = seen >> (16 * st + j) & 1;
+#pragma unroll
+              for (int nb = 0; nb < NDV; ++nb) {
+#pragma unroll
+                for (int i4 = 0; i4 < 4; ++i4) {
+                  const uint16_t* v = reinterpret_cast<const uint16_t*>(vs_ + rr * VU + ((4 * nb + i4) ^ swizzle<VU>(rr))) + 4 * h;
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    const float x = pk * Elem<DT>::to_f32(v[i]);
+                    c.o[k][nb][4 * i4 + i] += see ? x : 0.f;
+                  }
+                  __builtin_amdgcn_sched_barrier(0);
+                }
+              }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          }
+        }
+      }
+    }
+  }
+}
+
+// SECOND: the launch that follows, whose blocks do again what the first left (r.redo, one flag a block).
+template <int DT, int NKS, int NDV, int QW, int RB, bool BIAS, bool SECOND>
 __global__ __launch_bounds__(kThreads, 2) void rows_tile_kernel(logkv_rows_args a, RowsLaunch r) {
-  constexpr int RW = 8 / QW, TR = 32 * RB * RW;
+  constexpr int RW = kWaves / QW, TR = 32 * RB * RW, kQueries = 32 * kCols;   // per wave
   constexpr int kTileBytes = TR * (2 * NKS + 4 * NDV) * 16;
-  constexpr int kOutBytes = RW > 1 ? 8 * 32 * 32 * NDV * 4 : 0;
+  constexpr int kOutBytes = RW > 1 ? kWaves * kQueries * 32 * NDV * 4 : 0;
   __shared__ __align__(16) uint8_t buf[2 * kTileBytes > kOutBytes ? 2 * kTileBytes : kOutBytes];
   __shared__ __align__(16) float bias_s[BIAS ? 2 : 1][TR];
   __shared__ int flag_s[3];
-  __shared__ float m_s[8][32], l_s[8][32];
+  __shared__ float m_s[kWaves][kQueries], l_s[kWaves][kQueries];
   const RowsBlock id = rows_block();
+  int* redo = r.redo + (static_cast<int64_t>(id.lane) * gridDim.y + id.split) * gridDim.x + id.qb;
+  if (SECOND && *redo == 0) return;
   const int lane = id.lane, G = a.n_groups, tid = threadIdx.x;
   const int rep = a.n_heads / G, nq = rep * a.tq, w = wave_id(), l = lane_id(), h = l >> 5, col = l & 31;
   RowsShare<NKS, NDV> c;
@@ -354,9 +611,8 @@ __global__ __launch_bounds__(kThreads, 2) void rows_tile_kernel(logkv_rows_args 
   c.g = lane % G;
   c.n = rows_in_use(a, c.b);
   c.own = own_rows(a, c.b);
-  const int q_first = id.qb * 32 * QW, q_last = min(q_first + 32 * QW, nq) - 1;
-  const int qi = q_first + 32 * (w % QW) + col, qc = min(qi, nq - 1);
-  c.t = qc % a.tq;
+  const int q_first = id.qb * kQueries * QW, q_last = min(q_first + kQueries * QW, nq) - 1;
+  const int q0 = q_first + kQueries * (w % QW) + col;   // the first column block's query
   // Own rows that some query of the block may see.
   const int t_max = q_first / a.tq == q_last / a.tq ? q_last % a.tq : a.tq - 1;
   const int own_end = r.causal ? min(c.own, t_max + 1) : c.own;
@@ -364,63 +620,76 @@ __global__ __launch_bounds__(kThreads, 2) void rows_tile_kernel(logkv_rows_args 
   const int tiles = c.np + (own_end + TR - 1) / TR, share = (tiles + r.splits - 1) / r.splits;
   c.begin = min(id.split * share, tiles);
   c.end = min(c.begin + share, tiles);
-  const LOGKV_G uint16_t* qrow = gp(a.q) + c.b * a.q_sb + (c.g * rep + qc / a.tq) * a.q_sh + c.t * a.q_st;
 #pragma unroll
-  for (int ks = 0; ks < NKS; ++ks) {
-    c.qf[ks] = make_uint4(0, 0, 0, 0);
-    if (2 * ks + h < a.dk / 8) c.qf[ks] = *(const LOGKV_G uint4*)(qrow + 16 * ks + 8 * h);
-  }
-  if (!rows_tile_share<DT, NKS, NDV, QW, RB, BIAS, false>(a, r, c, buf, bias_s, flag_s)) {
-    __syncthreads();
-    rows_tile_share<DT, NKS, NDV, QW, RB, BIAS, true>(a, r, c, buf, bias_s, flag_s);
-  }
-  c.lsum = pair_sum32(c.lsum);
-  if (c.t >= c.own || qi >= nq) {   // a query past its batch row's count sees nothing
-    c.m = -__builtin_inff();
-    c.lsum = 0.f;
+  for (int k = 0; k < kCols; ++k) {
+    const int qc = min(q0 + 32 * k, nq - 1);
+    c.t[k] = qc % a.tq;
+    const LOGKV_G uint16_t* qrow = gp(a.q) + c.b * a.q_sb + (c.g * rep + qc / a.tq) * a.q_sh + c.t[k] * a.q_st;
 #pragma unroll
-    for (int nb = 0; nb < NDV; ++nb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) c.o[nb][i] = 0.f;
+    for (int ks = 0; ks < NKS; ++ks) {
+      c.qf[k][ks] = make_uint4(0, 0, 0, 0);
+      if (2 * ks + h < a.dk / 8) c.qf[k][ks] = *(const LOGKV_G uint4*)(qrow + 16 * ks + 8 * h);
+    }
   }
-  const float vscale = DT == LOGKV_BF16 ? 1.f / kVScale : 1.f;
+  if constexpr (SECOND) {
+    rows_tile_share2<DT, NKS, NDV, QW, RB, BIAS>(a, r, c, buf, bias_s, flag_s);
+  } else {
+    const bool done = rows_tile_share<DT, NKS, NDV, QW, RB, BIAS>(a, r, c, buf, bias_s, flag_s);
+    if (tid == 0) *redo = done ? 0 : 1;
+    if (!done) return;
+  }
+#pragma unroll
+  for (int k = 0; k < kCols; ++k) {
+    c.lsum[k] = pair_sum32(c.lsum[k]);
+    if (c.t[k] >= c.own) {   // a query past its batch row's count sees nothing
+      c.m[k] = -__builtin_inff();
+      c.lsum[k] = 0.f;
+#pragma unroll
+      for (int nb = 0; nb < NDV; ++nb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) c.o[k][nb][i] = 0.f;
+    }
+  }
   float* part = r.part + (static_cast<int64_t>(lane) * r.splits + id.split) * nq * (a.dv + kRowsPartTail);
   if constexpr (RW == 1) {
-    if (qi >= nq) return;
-    float* out = part + static_cast<int64_t>(qi) * (a.dv + kRowsPartTail);
-    if (h == 0) *reinterpret_cast<float2*>(out + a.dv) = make_float2(c.m, c.lsum);
 #pragma unroll
-    for (int nb = 0; nb < NDV; ++nb)
+    for (int k = 0; k < kCols; ++k) {
+      const int qi = q0 + 32 * k;
+      if (qi >= nq) continue;
+      float* out = part + static_cast<int64_t>(qi) * (a.dv + kRowsPartTail);
+      if (h == 0) *reinterpret_cast<float2*>(out + a.dv) = make_float2(c.m[k], c.lsum[k]);
 #pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4) {
-        const int d = 32 * nb + 8 * i4 + 4 * h;
-        f32x4 y;
+      for (int nb = 0; nb < NDV; ++nb)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = c.o[nb][4 * i4 + i] * vscale;
-        if (d < a.dv) *reinterpret_cast<f32x4*>(out + d) = y;
-      }
+        for (int i4 = 0; i4 < 4; ++i4) {
+          const int d = 32 * nb + 8 * i4 + 4 * h;
+          const f32x4 y = {c.o[k][nb][4 * i4], c.o[k][nb][4 * i4 + 1], c.o[k][nb][4 * i4 + 2], c.o[k][nb][4 * i4 + 3]};
+          if (d < a.dv) *reinterpret_cast<f32x4*>(out + d) = y;
+        }
+    }
   } else {
     // The row groups joined in their order.
     constexpr int kLd = 32 * NDV;
     __syncthreads();
-    float* acc = reinterpret_cast<float*>(buf) + w * 32 * kLd;
 #pragma unroll
-    for (int nb = 0; nb < NDV; ++nb)
+    for (int k = 0; k < kCols; ++k) {
+      float* acc = reinterpret_cast<float*>(buf) + (w * kQueries + 32 * k + col) * kLd;
 #pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4) {
-        f32x4 y;
+      for (int nb = 0; nb < NDV; ++nb)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = c.o[nb][4 * i4 + i] * vscale;
-        *reinterpret_cast<f32x4*>(acc + col * kLd + 4 * ((8 * nb + 2 * i4 + h) ^ (col & 7))) = y;
+        for (int i4 = 0; i4 < 4; ++i4) {
+          const f32x4 y = {c.o[k][nb][4 * i4], c.o[k][nb][4 * i4 + 1], c.o[k][nb][4 * i4 + 2], c.o[k][nb][4 * i4 + 3]};
+          *reinterpret_cast<f32x4*>(acc + 4 * ((8 * nb + 2 * i4 + h) ^ (col & 7))) = y;
+        }
+      if (h == 0) {
+        m_s[w][32 * k + col] = c.m[k];
+        l_s[w][32 * k + col] = c.lsum[k];
       }
-    if (h == 0) {
-      m_s[w][col] = c.m;
-      l_s[w][col] = c.lsum;
     }
     __syncthreads();
-    const int queries = min(32 * QW, nq - q_first), units = a.dv / 4 + 1;
+    const int queries = min(kQueries * QW, nq - q_first), units = a.dv / 4 + 1;
     for (int e = tid; e < queries * units; e += kThreads) {
-      const int q = e / units, u = e % units, qq = q / 32, cc = q % 32;
+      const int q = e / units, u = e % units, qq = q / kQueries, cc = q % kQueries;
       float mx = -__builtin_inff();
 #pragma unroll
       for (int k = 0; k < RW; ++k) mx = fmaxf(mx, m_s[k * QW + qq][cc]);
@@ -431,7 +700,7 @@ __global__ __launch_bounds__(kThreads, 2) void rows_tile_kernel(logkv_rows_args 
         const int ww = k * QW + qq;
         const float f = __builtin_amdgcn_exp2f(m_s[ww][cc] - top);
         if (u == units - 1) sum[1] += l_s[ww][cc] * f;
-        else sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(buf) + (ww * 32 + cc) * kLd + 4 * (u ^ (cc & 7))) * f;
+        else sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(buf) + (ww * kQueries + cc) * kLd + 4 * (u ^ (cc & 7))) * f;
       }
       if (u == units - 1) sum[0] = mx;
       *reinterpret_cast<f32x4*>(part + static_cast<int64_t>(q_first + q) * (a.dv + kRowsPartTail) + 4 * u) = sum;
@@ -442,31 +711,36 @@ __global__ __launch_bounds__(kThreads, 2) void rows_tile_kernel(logkv_rows_args 
 namespace {
 
 template <int DT, int NKS, int NDV, int QW, int RB>
-void launch_one(const logkv_rows_args& a, const RowsLaunch& r, dim3 grid, hipStream_t stream) {
-  if (a.bias) hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, QW, RB, true>), grid, dim3(kThreads), 0, stream, a, r);
-  else hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, QW, RB, false>), grid, dim3(kThreads), 0, stream, a, r);
+void launch_one(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
+  const int nq = a.n_heads / a.n_groups * a.tq, queries = 32 * kCols * QW;
+  const dim3 grid((nq + queries - 1) / queries, r.splits, a.n_batch * a.n_groups);
+  if (a.bias) {
+    hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, QW, RB, true, false>), grid, dim3(kThreads), 0, stream, a, r);
+    hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, QW, RB, true, true>), grid, dim3(kThreads), 0, stream, a, r);
+  } else {
+    hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, QW, RB, false, false>), grid, dim3(kThreads), 0, stream, a, r);
+    hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, QW, RB, false, true>), grid, dim3(kThreads), 0, stream, a, r);
+  }
 }
 
 template <int DT, int NKS, int NDV>
-void launch_width(const logkv_rows_args& a, const RowsLaunch& r, dim3 grid, hipStream_t stream) {
-  if (r.q_waves == 2) launch_one<DT, NKS, NDV, 2, 1>(a, r, grid, stream);
-  else if (r.q_waves == 4) launch_one<DT, NKS, NDV, 4, 2>(a, r, grid, stream);
-  else launch_one<DT, NKS, NDV, 8, 2>(a, r, grid, stream);
+void launch_width(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
+  if (r.q_waves == 2) launch_one<DT, NKS, NDV, 2, 1>(a, r, stream);
+  else if (r.q_waves == 4) launch_one<DT, NKS, NDV, 4, 1>(a, r, stream);
+  else launch_one<DT, NKS, NDV, 8, 2>(a, r, stream);
 }
 
 template <int DT>
-void launch_type(const logkv_rows_args& a, const RowsLaunch& r, dim3 grid, hipStream_t stream) {
-  if (a.dk <= 64 && a.dv <= 64) launch_width<DT, 4, 2>(a, r, grid, stream);
-  else launch_width<DT, 8, 4>(a, r, grid, stream);
+void launch_type(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
+  if (a.dk <= 64 && a.dv <= 64) launch_width<DT, 4, 2>(a, r, stream);
+  else launch_width<DT, 8, 4>(a, r, stream);
 }
 
 }  // namespace
 
 int launch_rows_tile(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
-  const int nq = a.n_heads / a.n_groups * a.tq;
-  const dim3 grid((nq + 32 * r.q_waves - 1) / (32 * r.q_waves), r.splits, a.n_batch * a.n_groups);
-  if (a.dtype == LOGKV_BF16) launch_type<LOGKV_BF16>(a, r, grid, stream);
-  else launch_type<LOGKV_F16>(a, r, grid, stream);
+  if (a.dtype == LOGKV_BF16) launch_type<LOGKV_BF16>(a, r, stream);
+  else launch_type<LOGKV_F16>(a, r, stream);
   return hipGetLastError() == hipSuccess ? LOGKV_OK : LOGKV_ERUNTIME;
 }
 

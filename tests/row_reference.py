@@ -7,8 +7,8 @@ Error of an attention output against the exact value of the same (rounded) input
  * a probability as two parts: 2^-14 relative (bf16, cut) or 2^-22 (fp16, rounded; 2^-44 absolute where the second
    part is subnormal);
  * the float32 sums over rows: each partial sum within 2^-24 per addition, at most `rows` of them;
- * bf16 values as fp16 (times 2^6; more than 32 queries): 2^-31 absolute below 2^-23, where a tile's largest is 2^-8 or
-   more, and exact otherwise;
+ * bf16 values as fp16 (more than 32 queries): 2^-25 absolute below 2^-17, where a tile's largest is 2^-8 or more, and
+   exact otherwise;
  * the output's rounding: half a step, 2^-8 (bf16) or 2^-11 (fp16, 2^-25 absolute) of the value.
 All but the last scale with sum p |v|."""
 
@@ -61,7 +61,7 @@ def reference(q, k, v, cache_k, cache_v, lengths, visible, scale, bias=None, cou
                     spread = p @ vv.abs()
                     bound[b, h, t] = half * out[b, h, t].abs() + (1 + half) * factor * spread
                     bound[b, h, t] += 2.0 ** -24 if cache_k.dtype == torch.float16 else (
-                        2.0 ** -31 if float(vv.abs().nan_to_num(0.0, 0.0, 0.0).max()) >= 2.0 ** -8 else 0.0)
+                        2.0 ** -25 if float(vv.abs().nan_to_num(0.0, 0.0, 0.0).max()) >= 2.0 ** -8 else 0.0)
                     column = torch.zeros(n + live, dtype=torch.float64)
                     column[see] = p
                     weights[b, g, :n] += column[:n]
