@@ -207,7 +207,7 @@ void launch_finish_type(const logkv_rows_args& a, const RowsLaunch& r, hipStream
 // Splits of the tiled kernel: rounds of blocks over the CUs, each of a split's tiles and two more
 // for its start and end, and for more than one split two tiles' time for the join and the partials.
 int tile_splits(const logkv_rows_args& a, int64_t blocks, int q_waves) {
-  const int rows = q_waves == 2 ? 128 : 64, resident = 256;
+  const int rows = 64, resident = q_waves == 2 ? 512 : 256;
   const int64_t tiles = (a.cap + rows - 1) / rows + (a.tq + rows - 1) / rows;
   int best = 1;
   int64_t best_cost = INT64_MAX;

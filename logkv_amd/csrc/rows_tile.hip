@@ -37,8 +37,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 8;
-constexpr int kThreads = 64 * kWaves;
 constexpr int kCols = 1;                 // 32-query column blocks per wave
 
 // Where 16-byte unit u of row r is stored: u ^ swizzle. 16 units a row: four consecutive rows fall
@@ -128,13 +126,13 @@ __device__ __forceinline__ void clear_sums(RowsShare<NKS, NDV>& c) {
 
 // A share's tiles in the first form; false where it meets one that it cannot take. NKS 16-wide steps
 // of dk, NDV 32-wide blocks of dv.
-template <int DT, int NKS, int NDV, int QW, int RB, bool BIAS>
+template <int DT, int NKS, int NDV, int NW, int QW, int RB, bool BIAS>
 __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const RowsLaunch& r, RowsShare<NKS, NDV>& c,
-                                                uint8_t* buf, float (*bias_s)[32 * RB * kWaves / QW], int* flag_s) {
+                                                uint8_t* buf, float (*bias_s)[32 * RB * NW / QW], int* flag_s) {
   typedef __attribute__((address_space(3))) s16x4* lds4;
   typedef __attribute__((address_space(3))) const uint8_t* ldsb;
   typedef __attribute__((address_space(3))) const u32x4* ldsq;
-  constexpr int RW = kWaves / QW, TR = 32 * RB * RW;   // row groups, rows per tile
+  constexpr int kThreads = 64 * NW, RW = NW / QW, TR = 32 * RB * RW;   // row groups, rows per tile
   constexpr int KU = 2 * NKS, VU = 4 * NDV;            // 16-byte units of a staged row
   constexpr int kKTasks = TR * KU / kThreads, kVTasks = TR * VU / kThreads;
   constexpr int kTileBytes = TR * (KU + VU) * 16;
@@ -442,12 +440,12 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
 // The same in the second form: V in its own type, P as two parts of that type, and a tile that is not
 // finite row by row in float32, each row for the queries that see it. Plain steps (one buffer, nothing
 // ahead): shares that need it are rare.
-template <int DT, int NKS, int NDV, int QW, int RB, bool BIAS>
+template <int DT, int NKS, int NDV, int NW, int QW, int RB, bool BIAS>
 __device__ __forceinline__ void rows_tile_share2(const logkv_rows_args& a, const RowsLaunch& r, RowsShare<NKS, NDV>& c,
-                                                 uint8_t* buf, float (*bias_s)[32 * RB * kWaves / QW], int* flag_s) {
+                                                 uint8_t* buf, float (*bias_s)[32 * RB * NW / QW], int* flag_s) {
   typedef __attribute__((address_space(3))) s16x4* lds4;
-  constexpr int RW = kWaves / QW, TR = 32 * RB * RW, KU = 2 * NKS, VU = 4 * NDV;
-  static_assert(kWaves * 16 * 32 * 4 <= TR * (KU + VU) * 16, "the second buffer holds 16 rows' probabilities of every wave");
+  constexpr int kThreads = 64 * NW, RW = NW / QW, TR = 32 * RB * RW, KU = 2 * NKS, VU = 4 * NDV;
+  static_assert(NW * 16 * 32 * 4 <= TR * (KU + VU) * 16, "the second buffer holds 16 rows' probabilities of every wave");
   const int tid = threadIdx.x, w = wave_id(), l = lane_id(), h = l >> 5, col = l & 31, r0 = 32 * RB * (w / QW);
   uint4* ks_ = reinterpret_cast<uint4*>(buf);
   uint4* vs_ = reinterpret_cast<uint4*>(buf + TR * KU * 16);
@@ -592,15 +590,15 @@ __device__ __forceinline__ void rows_tile_share2(const logkv_rows_args& a, const
 }
 
 // SECOND: the launch that follows, whose blocks do again what the first left (r.redo, one flag a block).
-template <int DT, int NKS, int NDV, int QW, int RB, bool BIAS, bool SECOND>
-__global__ __launch_bounds__(kThreads, 2) void rows_tile_kernel(logkv_rows_args a, RowsLaunch r) {
-  constexpr int RW = kWaves / QW, TR = 32 * RB * RW, kQueries = 32 * kCols;   // per wave
+template <int DT, int NKS, int NDV, int NW, int QW, int RB, bool BIAS, bool SECOND>
+__global__ __launch_bounds__(64 * NW, 2) void rows_tile_kernel(logkv_rows_args a, RowsLaunch r) {
+  constexpr int kThreads = 64 * NW, RW = NW / QW, TR = 32 * RB * RW, kQueries = 32 * kCols;   // per wave
   constexpr int kTileBytes = TR * (2 * NKS + 4 * NDV) * 16;
-  constexpr int kOutBytes = RW > 1 ? kWaves * kQueries * 32 * NDV * 4 : 0;
+  constexpr int kOutBytes = RW > 1 ? NW * kQueries * 32 * NDV * 4 : 0;
   __shared__ __align__(16) uint8_t buf[2 * kTileBytes > kOutBytes ? 2 * kTileBytes : kOutBytes];
   __shared__ __align__(16) float bias_s[BIAS ? 2 : 1][TR];
   __shared__ int flag_s[3];
-  __shared__ float m_s[kWaves][kQueries], l_s[kWaves][kQueries];
+  __shared__ float m_s[NW][kQueries], l_s[NW][kQueries];
   const RowsBlock id = rows_block();
   int* redo = r.redo + (static_cast<int64_t>(id.lane) * gridDim.y + id.split) * gridDim.x + id.qb;
   if (SECOND && *redo == 0) return;
@@ -632,9 +630,9 @@ __global__ __launch_bounds__(kThreads, 2) void rows_tile_kernel(logkv_rows_args 
     }
   }
   if constexpr (SECOND) {
-    rows_tile_share2<DT, NKS, NDV, QW, RB, BIAS>(a, r, c, buf, bias_s, flag_s);
+    rows_tile_share2<DT, NKS, NDV, NW, QW, RB, BIAS>(a, r, c, buf, bias_s, flag_s);
   } else {
-    const bool done = rows_tile_share<DT, NKS, NDV, QW, RB, BIAS>(a, r, c, buf, bias_s, flag_s);
+    const bool done = rows_tile_share<DT, NKS, NDV, NW, QW, RB, BIAS>(a, r, c, buf, bias_s, flag_s);
     if (tid == 0) *redo = done ? 0 : 1;
     if (!done) return;
   }
@@ -710,24 +708,24 @@ __global__ __launch_bounds__(kThreads, 2) void rows_tile_kernel(logkv_rows_args 
 
 namespace {
 
-template <int DT, int NKS, int NDV, int QW, int RB>
+template <int DT, int NKS, int NDV, int NW, int QW, int RB>
 void launch_one(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
   const int nq = a.n_heads / a.n_groups * a.tq, queries = 32 * kCols * QW;
   const dim3 grid((nq + queries - 1) / queries, r.splits, a.n_batch * a.n_groups);
   if (a.bias) {
-    hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, QW, RB, true, false>), grid, dim3(kThreads), 0, stream, a, r);
-    hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, QW, RB, true, true>), grid, dim3(kThreads), 0, stream, a, r);
+    hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, NW, QW, RB, true, false>), grid, dim3(64 * NW), 0, stream, a, r);
+    hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, NW, QW, RB, true, true>), grid, dim3(64 * NW), 0, stream, a, r);
   } else {
-    hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, QW, RB, false, false>), grid, dim3(kThreads), 0, stream, a, r);
-    hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, QW, RB, false, true>), grid, dim3(kThreads), 0, stream, a, r);
+    hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, NW, QW, RB, false, false>), grid, dim3(64 * NW), 0, stream, a, r);
+    hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, NW, QW, RB, false, true>), grid, dim3(64 * NW), 0, stream, a, r);
   }
 }
 
 template <int DT, int NKS, int NDV>
 void launch_width(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
-  if (r.q_waves == 2) launch_one<DT, NKS, NDV, 2, 1>(a, r, stream);
-  else if (r.q_waves == 4) launch_one<DT, NKS, NDV, 4, 1>(a, r, stream);
-  else launch_one<DT, NKS, NDV, 8, 2>(a, r, stream);
+  if (r.q_waves == 2) launch_one<DT, NKS, NDV, 4, 2, 1>(a, r, stream);
+  else if (r.q_waves == 4) launch_one<DT, NKS, NDV, 8, 4, 1>(a, r, stream);
+  else launch_one<DT, NKS, NDV, 8, 8, 2>(a, r, stream);
 }
 
 template <int DT>
