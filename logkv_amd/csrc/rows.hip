@@ -9,7 +9,8 @@ namespace logkv {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWeightRows = 4 * kThreads;   // score columns per block of the weight sums
+constexpr int kColumns = 2;                       // score columns per thread of the weight sums
+constexpr int kWeightRows = kColumns * kThreads;
 constexpr int kAppendUnits = 4 * kThreads;  // 16-byte units per block of the append
 
 int64_t align256(int64_t x) { return (x + 255) & ~int64_t(255); }
@@ -38,7 +39,7 @@ __device__ __forceinline__ void fold_splits(const float* base, int64_t step, int
 //    is shared by queries and by groups of splits (QPB queries x SG groups), whose sums are
 //    joined in group order.
 //  * [out_blocks, + weight_blocks): weights of up to 16 queries from the stored products,
-//    p = 2^(s c2 - m) / l, one score column a thread and four at a time.
+//    p = 2^(s c2 - m) / l, kColumns score columns a thread.
 //  * the rest: the own rows copied behind the cache's rows.
 template <int DT, int TQ, int SG>
 __global__ __launch_bounds__(kThreads) void rows_finish_kernel(logkv_rows_args a, RowsLaunch r, int out_blocks,
@@ -144,21 +145,28 @@ __global__ __launch_bounds__(kThreads) void rows_finish_kernel(logkv_rows_args a
       }
     }
     __syncthreads();
-    const int c = c0 + 4 * tid;
+    const int c = c0 + kColumns * tid;
     if (c >= np + own) return;
     const float c2 = a.scale * kLog2e;
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    typedef float columns __attribute__((ext_vector_type(kColumns)));
+    float sum[kColumns] = {};
     const float* row = r.scores + static_cast<int64_t>(lane) * nq * r.score_st + c;
-#pragma unroll 4
-    for (int q = 0; q < nq; ++q) {
-      const f32x4 s = *reinterpret_cast<const f32x4*>(row + q * r.score_st);
-      if (ql[q] == 0.f) continue;   // a query that sees nothing
+    // All of a query block's products loaded at once.
+    for (int q0 = 0; q0 < nq; q0 += 8) {
+      columns s[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sum[k] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], c2, qm[q])) * ql[q];
+      for (int q = 0; q < 8; ++q) s[q] = *reinterpret_cast<const columns*>(row + min(q0 + q, nq - 1) * r.score_st);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        if (q0 + q >= nq || ql[q0 + q] == 0.f) continue;   // a query that sees nothing
+#pragma unroll
+        for (int k = 0; k < kColumns; ++k)
+          sum[k] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[q][k], c2, qm[q0 + q])) * ql[q0 + q];
+      }
     }
     LOGKV_G float* wrow = gp(a.weights) + b * a.w_sb + g * a.w_sg;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kColumns; ++k) {
       if (c + k < n) wrow[c + k] += sum[k];
       else if (c + k >= np && c + k < np + own && n + (c + k - np) < a.cap) wrow[n + (c + k - np)] = sum[k];
     }
