@@ -28,6 +28,7 @@ import torch
 
 from ._lib import (AttentionArgs, AttentionGradArgs, PackArgs, ReadoutView, SlotPackArgs, as_storage, check, lib, ptr,
                    require_device, stream_of)
+from .row_attention import _attention, _tree
 
 _BACKENDS = ("auto", "triton", "hip")
 
@@ -298,6 +299,22 @@ def _decode_capacity(cache, t: int) -> int:
     return cache.K_max * cache.L_alloc * cache.B_prime + cache.alpha_exact_tokens + cache.recent_capacity + max(2, t)
 
 
+def _pack_prefix(cache, view, k, v, dim, reuse, attention_plan=None):
+    """The packed ``[cache state | k, v]`` rows: (state key, plan, buffers, attention workspace). With ``reuse`` the
+    prefix that an earlier call left on the cache is taken, and only the rows after it are packed."""
+    key = (k.device, k.dtype, dim, id(cache.cos_cache), id(cache.sin_cache))
+    saved = cache._mid_decode_state if reuse else None
+    if saved is not None and saved[0] == key:
+        _, plan, buffers, recent_start, workspace = saved
+        _launch_pack(cache, view, plan, k, v, dim, *buffers, True, recent_start)
+        return key, plan, buffers, workspace
+    plan = semantic_mid_attention_plan(cache, view) if attention_plan is None else attention_plan
+    cap = _decode_capacity(cache, k.size(2))
+    buffers = (k.new_empty(*k.shape[:2], cap, dim), v.new_empty(*v.shape[:2], cap, dim))
+    _launch_pack(cache, view, plan, k, v, dim, *buffers, False, 0)
+    return key, plan, buffers, None
+
+
 def log_kv_chunk_attention(cache, q_b, k_b, v_b, scale, second_order_scale=1.0, attention_plan=None, *,
                            causal_tail=None, reuse_prefix=False):
     """One streaming attention step over ``[cache state | current chunk (causal)]``, without committing the chunk.
@@ -341,26 +358,8 @@ def log_kv_chunk_attention(cache, q_b, k_b, v_b, scale, second_order_scale=1.0, 
                                       causal_tail, v_b.size(-1), cache.n_groups, exact, None)
     reuse = (reuse_prefix and not torch.is_grad_enabled() and q_b.size(2) <= 2
              and not k_b.requires_grad and not v_b.requires_grad)
-    key = (k_b.device, k_b.dtype, dim, id(cache.cos_cache), id(cache.sin_cache))
-    buffers, skip_pooled, recent_start = None, False, 0
-    if reuse:
-        saved = cache._mid_decode_state
-        if saved is not None and saved[0] == key:
-            _, plan, buffers, recent_start, workspace = saved
-            skip_pooled = True
-        else:
-            plan = semantic_mid_attention_plan(cache, view) if attention_plan is None else attention_plan
-            workspace = None
-        if buffers is None:
-            cap = _decode_capacity(cache, k_b.size(2))
-            buffers = (k_b.new_empty(*k_b.shape[:2], cap, dim), v_b.new_empty(*v_b.shape[:2], cap, dim))
-    else:
-        plan = semantic_mid_attention_plan(cache, view) if attention_plan is None else attention_plan
-        workspace = None
-        cap = _decode_capacity(cache, k_b.size(2))
-        buffers = (k_b.new_empty(*k_b.shape[:2], cap, dim), v_b.new_empty(*v_b.shape[:2], cap, dim))
+    key, plan, buffers, workspace = _pack_prefix(cache, view, k_b, v_b, dim, reuse, attention_plan)
     ka, va = buffers
-    _launch_pack(cache, view, plan, k_b, v_b, dim, ka, va, skip_pooled, recent_start)
     exact = cache.alpha_count_dev if cache.alpha_exact_tokens else None
     tail = cache.recent_count + k_b.size(2)
     out, workspace = packed_attention(q_b, ka, va, plan, tail, scale, causal_tail, v_b.size(-1), cache.n_groups,
@@ -368,6 +367,40 @@ def log_kv_chunk_attention(cache, q_b, k_b, v_b, scale, second_order_scale=1.0, 
     if reuse:
         cache._mid_decode_state = (key, plan, buffers, cache.recent_count, workspace)
     return out
+
+
+def log_kv_draft_attention(cache, q, k, v, visible, scale, *, pending=None):
+    """Attention of a tree of T drafted tokens over ``[cache state | pending row | the drafted rows visible to each]``,
+    ``[B, n_heads, T, v_dim]``, without committing any. For inference: it has no gradient.
+
+    ``q [B, n_heads, T, k_dim]``, ``k / v [B, G, T, .]`` post-RoPE at the tokens' depths; ``visible`` (bool, ``[T, T]``
+    or ``[B, T, T]``) gives the drafted rows that each token sees, its ancestors and itself; ``pending`` is an optional
+    ``(k, v)`` of one attended but uncommitted row, which every token sees. A slot's logit is ``scale * q.k + log w``
+    with its log-mass as packed. The packed prefix is shared with ``log_kv_chunk_attention(reuse_prefix=True)``."""
+    if not cache.semantic_clusters or cache.semantic_anchor_mode != "mid":
+        raise NotImplementedError("logkv_amd reads out the first-order mid-anchor path (second_order_scale=0)")
+    _check_backend(cache.semantic_pack_backend)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, *(pending or ()))):
+        raise NotImplementedError("draft attention is for inference: it has no gradient (run it under torch.no_grad())")
+    k, v = as_storage(k), as_storage(v)
+    pk, pv = (k[:, :, :0], v[:, :, :0]) if pending is None else (as_storage(x) for x in pending)
+    _check_kv(cache, k, v)
+    _check_kv(cache, pk, pv)
+    if pk.size(2) > 1:
+        raise ValueError("at most one token can be pending")
+    if q.ndim != 4 or q.size(0) != cache.batch_size or q.device != k.device:
+        raise ValueError("queries must be [B, n_heads, T, k_dim] on the cache's device")
+    visible = _tree(visible, q, k)
+    dim = packed_dim(cache.k_dim, cache.v_dim)
+    with torch.no_grad():
+        key, plan, (ka, va), workspace = _pack_prefix(cache, readout_view(cache), pk, pv, dim, True)
+        recent = cache.recent_count
+        cache._mid_decode_state = (key, plan, (ka, va), recent, workspace)
+        # The plan's width and the exact pool's rows are read on the device.
+        in_use = (plan.table[-1:].data_ptr(), 0, cache.alpha_count_dev.data_ptr() if cache.alpha_exact_tokens else 0,
+                  recent + pk.size(2))
+        return _attention(q, k, v, ka[..., :cache.k_dim], va[..., :cache.v_dim], float(scale), None, 0,
+                          bias=ka[..., cache.k_dim], visible=visible, in_use=in_use)
 
 
 def attention_state(cache, plan):

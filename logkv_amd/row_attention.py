@@ -9,7 +9,8 @@ the causal tail and keeps no exact cache that attention weight cuts:
   compressed cache's packed rows, with their log-mass as bias);
 * ``log_kv_weight_attention``: causal attention of new tokens that adds each row's probability to its
   running weight and stores the new rows behind the cache's;
-* ``log_kv_evict``: the rows of every (batch row, KV head) cut to a budget by those weights.
+* ``log_kv_evict``: the rows of every (batch row, KV head) cut to a budget by those weights
+  (``EvictingKVCache`` runs the three of them over its own rows).
 
 All run in liblogkv_hip.so on the current stream of the tensors' device, allocate their outputs and
 scratch through torch, never wait for the host and can be captured into a HIP graph. They are for
@@ -97,8 +98,9 @@ def _workspace_bytes(weights, batch, heads, groups, tq, cap, dk, dv, dtype):
 
 
 def _attention(q, k, v, cache_k, cache_v, scale, lengths, room, *, bias=None, visible=None, counts=None, weights=None,
-               lengths2=None, len_add=0):
-    """Checks and launch of both attentions."""
+               in_use=None):
+    """Checks and launch of both attentions. ``in_use`` in place of ``lengths``: (address, stride) of device counts
+    per batch row, a second count's address (0: none) and rows to add to both."""
     if not q.ndim == k.ndim == v.ndim == cache_k.ndim == cache_v.ndim == 4:
         raise ValueError("queries, rows and cache must be 4-dimensional")
     batch, heads, tq, dk = q.shape
@@ -126,10 +128,11 @@ def _attention(q, k, v, cache_k, cache_v, scale, lengths, room, *, bias=None, vi
         raise ValueError("cache rows must be 16-byte aligned with contiguous features")
     out_dtype = q.dtype
     (q, *q_st), (k, *k_st), (v, *v_st) = _small_rows(q, dtype), _small_rows(k, dtype), _small_rows(v, dtype)
-    if lengths2 is None:
+    n2_ptr = 0
+    if in_use is None:
         lengths, n_ptr, n_st, len_add = _lengths(lengths, batch, cap, index, room)
     else:
-        n_ptr, n_st = lengths.data_ptr(), 0
+        n_ptr, n_st, n2_ptr, len_add = in_use
     b_ptr, b_st, b_half = 0, _NO_STRIDES, 0
     if bias is not None:
         if bias.shape != (batch, groups, cap) or bias.get_device() != index or bias.dtype not in (torch.float32, dtype):
@@ -146,7 +149,7 @@ def _attention(q, k, v, cache_k, cache_v, scale, lengths, room, *, bias=None, vi
     o_sh = tq * dv
     args = pack_rows(
         q.data_ptr(), *q_st, k.data_ptr(), *k_st, v.data_ptr(), *v_st, ck, ck_sb, ck_sg, ck_st, cv, cv_sb, cv_sg, cv_st,
-        b_ptr, *b_st, n_ptr, 0 if lengths2 is None else lengths2.data_ptr(), vis_ptr, vis_sb, vis_st,
+        b_ptr, *b_st, n_ptr, n2_ptr, vis_ptr, vis_sb, vis_st,
         0 if counts is None else counts.data_ptr(), w_ptr, w_sb, w_sg, out.data_ptr(), heads * o_sh, o_sh, dv,
         batch, heads, groups, tq, cap, dk, dv, code, n_st, len_add, b_half, scale)
     handle = rows_lib()
@@ -169,13 +172,17 @@ def log_kv_tree_attention(q, k, v, cache_k, cache_v, lengths, visible, scale, *,
 
     Queries and drafted rows of another activation dtype are rounded to the cache's, and the output is returned
     in the queries'. The cache is only read: commit the accepted tokens with the cache's own call."""
+    return _attention(q, k, v, cache_k, cache_v, float(scale), lengths, 0, bias=bias,
+                      visible=_tree(visible, q, cache_k))
+
+
+def _tree(visible, q, cache_k):
+    """The checked mask of a draft, with contiguous rows."""
     if (not isinstance(visible, torch.Tensor) or visible.dtype not in (torch.bool, torch.uint8) or q.ndim != 4
             or visible.shape not in ((q.size(2),) * 2, (q.size(0), q.size(2), q.size(2)))
             or visible.get_device() != cache_k.get_device()):
         raise ValueError("visible must be a bool tensor [T, T] or [B, T, T] on the cache's device")
-    if visible.stride(-1) != 1:
-        visible = visible.contiguous()
-    return _attention(q, k, v, cache_k, cache_v, float(scale), lengths, 0, bias=bias, visible=visible)
+    return visible if visible.stride(-1) == 1 else visible.contiguous()
 
 
 def log_kv_weight_attention(q, k, v, cache_k, cache_v, weights, lengths, scale, *, counts=None):
