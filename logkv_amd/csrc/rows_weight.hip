@@ -65,32 +65,33 @@ __global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_arg
         kf[kb][ks] = *(const LOGKV_G uint4*)(kr + min(k0 + 32 * kb + col, rows - 1) * kst + 16 * ks + 8 * h);
     }
   const LOGKV_G float* lse = gp(r.lse) + static_cast<int64_t>(lane) * nq;
-  // Each task's query of the tile on its way, as (head, position), moved on by a tile without division.
-  const LOGKV_G uint16_t* qbase = gp(a.q) + b * a.q_sb + g * rep * a.q_sh;
-  const int step_head = kQueries / a.tq, step_t = kQueries % a.tq;
-  int head[kTasks], pos[kTasks];
+  // Each task's unit of the tile on its way, moved on by a tile without a product or a division.
+  static_assert(kThreads % KU == 0, "a thread's tasks share a unit");
+  const int unit = tid % KU, step_t = kQueries % a.tq;
+  const int64_t step = kQueries / a.tq * a.q_sh + step_t * a.q_st, wrap = a.q_sh - a.tq * a.q_st;
+  const LOGKV_G uint16_t* qp[kTasks];
+  int pos[kTasks];
 #pragma unroll
   for (int k = 0; k < kTasks; ++k) {
     const int qq = (tid + kThreads * k) / KU;
-    head[k] = qq / a.tq;
     pos[k] = qq % a.tq;
+    qp[k] = gp(a.q) + b * a.q_sb + (g * rep + qq / a.tq) * a.q_sh + pos[k] * a.q_st + 8 * unit;
   }
   int my_t = tid % a.tq;   // of query tid of the tile (tid < kQueries)
   uint4 qx[kTasks];
-  float lq[kTasks], lx = 0.f;
+  float lx = 0.f;
   int tx = 0;
+  // Queries past the row's tokens see nothing (L = +inf, probabilities 2^-inf) and are stored as zeros.
   auto load = [&](int q0) {
 #pragma unroll
     for (int k = 0; k < kTasks; ++k) {
-      const int i = tid + kThreads * k, qi = q0 + i / KU, u = i % KU;
       qx[k] = make_uint4(0, 0, 0, 0);
-      lq[k] = lse[min(qi, nq - 1)];
-      if (u < units && qi < nq) qx[k] = *(const LOGKV_G uint4*)(qbase + head[k] * a.q_sh + pos[k] * a.q_st + 8 * u);
-      head[k] += step_head;
+      if (unit < units && q0 + (tid + kThreads * k) / KU < nq && pos[k] < own) qx[k] = *(const LOGKV_G uint4*)qp[k];
+      qp[k] += step;
       pos[k] += step_t;
       if (pos[k] >= a.tq) {
         pos[k] -= a.tq;
-        ++head[k];
+        qp[k] += wrap;
       }
     }
     if (tid < kQueries) lx = q0 + tid < nq ? lse[q0 + tid] : __builtin_inff();
@@ -98,13 +99,11 @@ __global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_arg
     my_t += step_t;
     if (my_t >= a.tq) my_t -= a.tq;
   };
-  // A query that sees nothing (L = +inf) is stored as zero: its probabilities are 2^-inf.
   auto store = [&](int bf) {
 #pragma unroll
     for (int k = 0; k < kTasks; ++k) {
-      const int i = tid + kThreads * k, qq = i / KU, u = i % KU;
-      if (lq[k] == __builtin_inff()) qx[k] = make_uint4(0, 0, 0, 0);
-      q_s[bf][qq * KU + (u ^ swizzle<KU>(qq))] = qx[k];
+      const int qq = (tid + kThreads * k) / KU;
+      q_s[bf][qq * KU + (unit ^ swizzle<KU>(qq))] = qx[k];
     }
     if (tid < kQueries) {
       l_s[bf][tid] = lx;

@@ -53,13 +53,12 @@ def _launch(entry, what, index, *args):
         return check(entry(*args, torch._C._cuda_getCurrentRawStream(index)), what)
 
 
-def _refuse_grad(*tensors):
-    if any(t.requires_grad for t in tensors):
-        raise NotImplementedError("row attention is for inference: it has no gradient (run it under torch.no_grad())")
+def _no_gradient():
+    return NotImplementedError("row attention is for inference: it has no gradient (run it under torch.no_grad())")
 
 
 def _small_rows(x, dtype):
-    """Rows of the call in the cache's dtype, readable in 16-byte units."""
+    """Rows of the call in the cache's dtype, readable in 16-byte units, and their strides."""
     if x.dtype != dtype:
         check_activation_dtype(x.dtype)
         x = x.to(dtype)
@@ -104,12 +103,13 @@ def _attention(q, k, v, cache_k, cache_v, scale, lengths, room, *, bias=None, vi
     if not q.ndim == k.ndim == v.ndim == cache_k.ndim == cache_v.ndim == 4:
         raise ValueError("queries, rows and cache must be 4-dimensional")
     batch, heads, tq, dk = q.shape
-    _, groups, cap, _ = cache_k.shape
-    dv, dtype, index = cache_v.size(3), cache_k.dtype, cache_k.get_device()
+    k_shape, v_shape = cache_k.shape, cache_v.shape
+    groups, cap, dv = k_shape[1], k_shape[2], v_shape[3]
+    dtype, index = cache_k.dtype, cache_k.get_device()
     code = _ROW_DTYPES.get(dtype)
     if code is None or cache_v.dtype != dtype:
         raise ValueError("the cache must be bfloat16 or float16")
-    if (cache_k.shape != (batch, groups, cap, dk) or cache_v.shape != (batch, groups, cap, dv) or groups < 1
+    if (k_shape != (batch, groups, cap, dk) or v_shape != (batch, groups, cap, dv) or groups < 1
             or heads % groups or heads < 1 or tq < 1 or batch < 1):
         raise ValueError("cache rows must be [B, G, capacity, d] with G dividing the query heads")
     if k.shape != (batch, groups, tq, dk) or v.shape != (batch, groups, tq, dv):
@@ -119,8 +119,9 @@ def _attention(q, k, v, cache_k, cache_v, scale, lengths, room, *, bias=None, vi
         raise ValueError("all tensors must be on the cache's device")
     if not (0.0 < scale < math.inf):
         raise ValueError("attention scale must be positive")
-    if torch.is_grad_enabled():
-        _refuse_grad(q, k, v, cache_k, cache_v, *(() if bias is None else (bias,)))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or cache_k.requires_grad
+                                    or cache_v.requires_grad or bias is not None and bias.requires_grad):
+        raise _no_gradient()
     ck, cv = cache_k.data_ptr(), cache_v.data_ptr()
     ck_sb, ck_sg, ck_st, ck_sd = cache_k.stride()
     cv_sb, cv_sg, cv_st, cv_sd = cache_v.stride()
@@ -143,9 +144,9 @@ def _attention(q, k, v, cache_k, cache_v, scale, lengths, room, *, bias=None, vi
         vis_ptr, vis_sb, vis_st = visible.data_ptr(), visible.stride(0) if visible.ndim == 3 else 0, visible.stride(-2)
     else:
         w_ptr, (w_sb, w_sg, _) = weights.data_ptr(), weights.stride()
-    out = torch.empty((batch, heads, tq, dv), dtype=dtype, device=cache_k.device)
+    out = cache_k.new_empty((batch, heads, tq, dv))
     need = _workspace_bytes(weights is not None, batch, heads, groups, tq, cap, dk, dv, code)
-    workspace = torch.empty(need, dtype=torch.uint8, device=cache_k.device)
+    workspace = cache_k.new_empty(need // 2)
     o_sh = tq * dv
     args = pack_rows(
         q.data_ptr(), *q_st, k.data_ptr(), *k_st, v.data_ptr(), *v_st, ck, ck_sb, ck_sg, ck_st, cv, cv_sb, cv_sg, cv_st,
@@ -232,7 +233,7 @@ def log_kv_evict(cache_k, cache_v, weights, lengths, keep, *, recent=0, position
     if cache_k.ndim != 4 or cache_v.ndim != 4 or cache_k.shape[:3] != cache_v.shape[:3]:
         raise ValueError("cache rows must be [B, G, capacity, d]")
     batch, groups, cap, dk = cache_k.shape
-    dv, device, dtype, index = cache_v.size(3), cache_k.device, cache_k.dtype, cache_k.get_device()
+    dv, dtype, index = cache_v.size(3), cache_k.dtype, cache_k.get_device()
     keep, recent = int(keep), int(recent)
     if keep < 1 or not 0 <= recent <= keep:
         raise ValueError("keep must be at least 1, recent between 0 and keep")
@@ -249,17 +250,15 @@ def log_kv_evict(cache_k, cache_v, weights, lengths, keep, *, recent=0, position
             raise ValueError("positions must be int64 [B, G, capacity] with contiguous rows")
     if not (_evict_rows_ok(cache_k) and _evict_rows_ok(cache_v)):
         raise ValueError("cache rows must be 16-byte aligned with contiguous features")
-    if torch.is_grad_enabled():
-        _refuse_grad(cache_k, cache_v, weights)
+    if torch.is_grad_enabled() and (cache_k.requires_grad or cache_v.requires_grad or weights.requires_grad):
+        raise _no_gradient()
     lengths, n_ptr, _, len_add = _lengths(lengths, batch, cap, index)
     if out is None:
-        kept = torch.empty((batch, groups, keep), dtype=torch.int32, device=device)
+        kept = weights.new_empty((batch, groups, keep), dtype=torch.int32)
         out = EvictedRows(
-            torch.empty((batch, groups, keep, dk), dtype=dtype, device=device),
-            torch.empty((batch, groups, keep, dv), dtype=dtype, device=device),
-            torch.empty((batch, groups, keep), dtype=torch.float32, device=device),
-            None if positions is None else torch.empty((batch, groups, keep), dtype=torch.int64, device=device),
-            kept, torch.empty(batch, dtype=torch.int32, device=device))
+            cache_k.new_empty((batch, groups, keep, dk)), cache_v.new_empty((batch, groups, keep, dv)),
+            weights.new_empty((batch, groups, keep)),
+            None if positions is None else positions.new_empty((batch, groups, keep)), kept, kept.new_empty(batch))
     else:
         _check_evict_out(out, cache_k, cache_v, weights, positions, lengths, keep)
     k, v, w, p, kept, n = out
