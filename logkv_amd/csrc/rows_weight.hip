@@ -48,9 +48,12 @@ __global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_arg
   const int rep = a.n_heads / G, nq = rep * a.tq, units = a.dk / 8;
   const int w = wave_id(), l = lane_id(), col = l & 31, h = l >> 5;
   const int n = rows_in_use(a, b), own = own_rows(a, b);
-  // Blocks of the cache's rows, then of the own rows.
-  const bool of_cache = static_cast<int>(blockIdx.x) < cache_blocks;
-  const int rows = of_cache ? n : own, b0 = (static_cast<int>(blockIdx.x) - (of_cache ? 0 : cache_blocks)) * kKeys;
+  // Blocks of the cache's rows, then of the own rows. Fewer queries see a later own block: lanes take them in turned
+  // order, or the XCD that a multiple of eight blocks a lane hands all first ones ends last (30720 rows and 2048 new
+  // ones: 439 us against 340 on the XCD of the last ones).
+  const int x = blockIdx.x, own_blocks = gridDim.x - cache_blocks;
+  const bool of_cache = x < cache_blocks;
+  const int rows = of_cache ? n : own, b0 = (of_cache ? x : (x - cache_blocks + lane) % own_blocks) * kKeys;
   if (b0 >= rows || own == 0) return;
   const int k0 = b0 + w * 32 * KB;
   const LOGKV_G uint16_t* kr = of_cache ? gp(a.cache_k) + b * a.ck_sb + g * a.ck_sg : gp(a.k) + b * a.k_sb + g * a.k_sg;

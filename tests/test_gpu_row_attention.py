@@ -338,3 +338,26 @@ def test_captured_and_replayed(T, rep):
         torch.cuda.synchronize()
         assert torch.equal(a, want_a) and torch.equal(b, want_b), i
         assert torch.equal(ck, sk) and torch.equal(cv, sv) and torch.equal(w, sw) and torch.equal(n, sn), i
+
+
+@pytest.mark.parametrize("rep,T,dk,dv", [(2, 12, 128, 128), (1, 17, 96, 128), (4, 8, 80, 64)])
+def test_17_to_32_queries_over_many_rows(rep, T, dk, dv):
+    """Both operators where 17 to 32 queries take the tiled kernel: bf16, more than 64 features, a cache of many rows
+    (in use: a few, and past a split's tiles)."""
+    B, G, cap = 2, 1, 65600
+    lengths = [4099, 33]
+    q, k, v, ck, cv = inputs(B, G, rep, T, cap, dk, dv, BF16, 77)
+    n, scale = torch.tensor(lengths, dtype=torch.int32, device="cuda"), dk ** -0.5
+    visible = torch.stack([tree_mask(T, 60 + b, empty=(T - 1,)) for b in range(B)])
+    want, _, bound, _ = reference(q, k, v, ck, cv, lengths, visible, scale)
+    check_close(log_kv_tree_attention(q, k, v, ck, cv, n, visible.cuda(), scale), want, bound)
+    causal = torch.ones(T, T, dtype=torch.bool).tril()[None].expand(B, T, T)
+    want, column, bound, rel = reference(q, k, v, ck, cv, lengths, causal, scale)
+    w = torch.rand(B, G, cap, generator=torch.Generator().manual_seed(8)).cuda()
+    total = w.cpu().double()
+    check_close(log_kv_weight_attention(q, k, v, ck, cv, w, n, scale), want, bound)
+    for b, m in enumerate(lengths):
+        total[b, :, :m] += column[b, :, :m]
+        total[b, :, m:m + T] = column[b, :, cap:cap + T]
+        check_close(w[b], total[b], (rel + (rep * T + 4) * 2.0 ** -23) * total[b].abs() + 1e-30)
+        assert torch.equal(ck[b, :, m:m + T], k[b]) and torch.equal(cv[b, :, m:m + T], v[b])
