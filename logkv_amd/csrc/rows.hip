@@ -1,6 +1,7 @@
 // Attention over a cache's rows and the call's own rows: what follows the streamed products
 // (rows_stream.hip), and the sizes of a launch.
 #include <algorithm>
+#include <type_traits>
 
 #include "rows.hpp"
 
@@ -9,8 +10,6 @@ namespace logkv {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kColumns = 2;                       // score columns per thread of the weight sums
-constexpr int kWeightRows = kColumns * kThreads;
 constexpr int kAppendUnits = 4 * kThreads;  // 16-byte units per block of the append
 
 int64_t align256(int64_t x) { return (x + 255) & ~int64_t(255); }
@@ -39,9 +38,9 @@ __device__ __forceinline__ void fold_splits(const float* base, int64_t step, int
 //    is shared by queries and by groups of splits (QPB queries x SG groups), whose sums are
 //    joined in group order.
 //  * [out_blocks, + weight_blocks): weights of up to 16 queries from the stored products,
-//    p = 2^(s c2 - m) / l, kColumns score columns a thread.
+//    p = 2^(s c2 - m) / l, COLS score columns a thread.
 //  * the rest: the own rows copied behind the cache's rows.
-template <int DT, int TQ, int SG>
+template <int DT, int TQ, int SG, int COLS>
 __global__ __launch_bounds__(kThreads) void rows_finish_kernel(logkv_rows_args a, RowsLaunch r, int out_blocks,
                                                                int weight_blocks) {
   typedef Elem<DT> E;
@@ -131,7 +130,7 @@ __global__ __launch_bounds__(kThreads) void rows_finish_kernel(logkv_rows_args a
   if (blk < weight_blocks) {
     __shared__ float qm[16], ql[16];
     const int np = (n + kRowTile - 1) / kRowTile * kRowTile;
-    const int c0 = blk * kWeightRows;
+    const int c0 = blk * COLS * kThreads;
     if (c0 >= np + own) return;
     {
       const int q = tid / 16;
@@ -145,29 +144,37 @@ __global__ __launch_bounds__(kThreads) void rows_finish_kernel(logkv_rows_args a
       }
     }
     __syncthreads();
-    const int c = c0 + kColumns * tid;
+    const int c = c0 + COLS * tid;
     if (c >= np + own) return;
     const float c2 = a.scale * kLog2e;
-    typedef float columns __attribute__((ext_vector_type(kColumns)));
-    float sum[kColumns] = {};
+    typedef float columns __attribute__((ext_vector_type(COLS)));
+    float sum[COLS] = {};
     const float* row = r.scores + static_cast<int64_t>(lane) * nq * r.score_st + c;
-    // All of a query block's products loaded at once.
-    for (int q0 = 0; q0 < nq; q0 += 8) {
-      columns s[8];
-#pragma unroll
-      for (int q = 0; q < 8; ++q) s[q] = *reinterpret_cast<const columns*>(row + min(q0 + q, nq - 1) * r.score_st);
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        if (q0 + q >= nq || ql[q0 + q] == 0.f) continue;   // a query that sees nothing
-#pragma unroll
-        for (int k = 0; k < kColumns; ++k)
-          sum[k] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[q][k], c2, qm[q0 + q])) * ql[q0 + q];
-      }
-    }
     LOGKV_G float* wrow = gp(a.weights) + b * a.w_sb + g * a.w_sg;
+    float before[COLS];
 #pragma unroll
-    for (int k = 0; k < kColumns; ++k) {
-      if (c + k < n) wrow[c + k] += sum[k];
+    for (int k = 0; k < COLS; ++k) before[k] = wrow[min(c + k, a.cap - 1)];
+    // QB queries' products loaded at once.
+    auto add = [&](auto qb) {
+      constexpr int QB = decltype(qb)::value;
+      for (int q0 = 0; q0 < nq; q0 += QB) {
+        columns s[QB];
+#pragma unroll
+        for (int q = 0; q < QB; ++q) s[q] = *reinterpret_cast<const columns*>(row + min(q0 + q, nq - 1) * r.score_st);
+#pragma unroll
+        for (int q = 0; q < QB; ++q) {
+          if (q0 + q >= nq || ql[q0 + q] == 0.f) continue;   // a query that sees nothing
+#pragma unroll
+          for (int k = 0; k < COLS; ++k)
+            sum[k] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[q][k], c2, qm[q0 + q])) * ql[q0 + q];
+        }
+      }
+    };
+    if (nq <= 2) add(std::integral_constant<int, 2>{});
+    else add(std::integral_constant<int, 8>{});
+#pragma unroll
+    for (int k = 0; k < COLS; ++k) {
+      if (c + k < n) wrow[c + k] = before[k] + sum[k];
       else if (c + k >= np && c + k < np + own && n + (c + k - np) < a.cap) wrow[n + (c + k - np)] = sum[k];
     }
     return;
@@ -190,14 +197,24 @@ __global__ __launch_bounds__(kThreads) void rows_finish_kernel(logkv_rows_args a
 
 namespace {
 
-template <int DT, int TQ, int SG>
+template <int DT, int TQ, int SG, int COLS>
 void launch_finish(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
+  constexpr int kWeightRows = COLS * kThreads;
   const int nq = a.n_heads / a.n_groups * a.tq, qpb = kThreads / (TQ * SG);
   const int out_blocks = (nq + qpb - 1) / qpb;
   const int weight_blocks = r.scores ? static_cast<int>((r.score_st + kWeightRows - 1) / kWeightRows) : 0;
   const int append_blocks = r.causal ? (a.tq * (a.dk / 8 + a.dv / 8) + kAppendUnits - 1) / kAppendUnits : 0;
-  hipLaunchKernelGGL((rows_finish_kernel<DT, TQ, SG>), dim3(out_blocks + weight_blocks + append_blocks, a.n_batch * a.n_groups),
-                     dim3(kThreads), 0, stream, a, r, out_blocks, weight_blocks);
+  hipLaunchKernelGGL((rows_finish_kernel<DT, TQ, SG, COLS>),
+                     dim3(out_blocks + weight_blocks + append_blocks, a.n_batch * a.n_groups), dim3(kThreads), 0, stream, a, r,
+                     out_blocks, weight_blocks);
+}
+
+template <int DT, int TQ, int SG>
+void launch_finish_cols(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
+  // Four columns a thread where two would make more blocks than stay resident: 64 lanes of 32768 rows 14.1 us (two:
+  // 17.8), 64 lanes of 4096 rows 9.1 (8.0).
+  if (r.scores && r.score_st * a.n_batch * a.n_groups >= 2048 * 2 * kThreads) launch_finish<DT, TQ, SG, 4>(a, r, stream);
+  else launch_finish<DT, TQ, SG, 2>(a, r, stream);
 }
 
 template <int DT>
@@ -206,11 +223,11 @@ void launch_finish_type(const logkv_rows_args& a, const RowsLaunch& r, hipStream
   // 512 queries without them 120 us, with them 123; 4096 rows and 666 queries 54.6 and 60.9 us.
   const bool many = r.splits > 8 && static_cast<int64_t>(a.n_batch) * a.n_heads * a.tq < 8 * 256;
   if (a.dv <= 128) {
-    if (many) launch_finish<DT, 32, 8>(a, r, stream);
-    else launch_finish<DT, 32, 1>(a, r, stream);
+    if (many) launch_finish_cols<DT, 32, 8>(a, r, stream);
+    else launch_finish_cols<DT, 32, 1>(a, r, stream);
   } else {
-    if (many) launch_finish<DT, 64, 4>(a, r, stream);
-    else launch_finish<DT, 64, 1>(a, r, stream);
+    if (many) launch_finish_cols<DT, 64, 4>(a, r, stream);
+    else launch_finish_cols<DT, 64, 1>(a, r, stream);
   }
 }
 

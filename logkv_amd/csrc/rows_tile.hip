@@ -1,26 +1,30 @@
-// Attention over a cache's rows and the call's own rows for more queries than a wave's columns:
-// tiles of K and V in LDS, shared by a block's four waves.
+// Attention over a cache's rows and the call's own rows for many queries per KV group (rows.hip's rule):
+// tiles of K and V in LDS, shared by a block's NW waves.
 //
-// Same mathematics as rows_stream.hip (one pass with a running maximum). QW waves hold 64 queries
-// each (two column blocks of 32, in registers for the whole range), and 4 / QW groups of them take
-// 32 RB rows each of a tile. Per 32 rows:
+// Same mathematics as rows_stream.hip (one pass with a running maximum). QW waves hold 32 queries
+// each, in registers for the whole range, and NW / QW groups of them take 32 RB rows each of a
+// tile. Per 32 rows:
 //   S^T = K Q^T by 32x32x16 matrix products (a lane holds 16 rows of its own query);
 //   O^T += V^T P^T, where P^T's operand is the lane's own score registers (operand element j of a
 //   16-row step st is row 16 st + 8 (j / 4) + 4 (l / 32) + j % 4) and V is read transposed.
-// A block has a CU to itself, a wave its SIMD and 512 registers, so nothing hides a wave's waits but
-// the wave: the score products of the next 32 rows are interleaved with the maxima and half of the
-// exponentials of these, the value products with the other half and with the staging of the next
-// tile, one product and the vector work of its 32 cycles at a time. With 64 queries a wave an operand
-// read from LDS serves two products (32 queries a wave, two waves a SIMD, all in step: the reads
-// alone took the products' time).
+// Bound by the vector unit beside the matrix cores: two waves a SIMD issue a vector operation every
+// 4.7 cycles (one wave: 8), and the exponentials, maxima and conversions of 32 rows take about as
+// long as their products. So two waves a SIMD, and in each the score products of the next 32 rows
+// are interleaved with the maxima and half of the exponentials of these, the value products with
+// the other half and with the staging of the next tile. 32768 rows of 128 features, 8 lanes of 512 queries: 107 us, 645
+// TFLOP/s of the 1207 of a large matrix product (one wave a SIMD with 64 queries was slower: nothing
+// hid its waits); 30720 rows and 2048 new ones, 8 lanes of 4096 queries: 700 us, 760 TFLOP/s.
+// Up to 64 queries: two blocks of four waves a CU (two waves of queries, two of rows): 64 lanes of
+// 8192 rows, 52 queries 80 us, in one block of eight waves 85.
 // bf16 caches: V enters the products as fp16, converted as it is staged (exact from 2^-17 up,
 // below that to 2^-25 absolute), and P as fp16 times 2^7 (11 bits): one product per step, a
 // third less matrix work than two bf16 parts of P, and P's error stays an eighth of the output's
 // rounding. A share with a tile whose largest magnitude is not in [2^-8, 2^16) is done again by a
 // second launch (in one kernel the second form's registers spilled in the first's loop, and a
-// reload there waits for every load ahead) in a second form: V as bf16, P as two parts. fp16 caches: P as two fp16 parts in both forms, since one
-// part's rounding would equal the output's; the second form is for infinities and NaNs in V, which
-// it adds row by row for the queries that see them.
+// reload there waits for every load ahead) in a second form: V as bf16, P as two parts. fp16
+// caches: P as two fp16 parts in both forms, since one part's rounding would equal the output's;
+// the second form is for infinities and NaNs in V, which it adds row by row for the queries that
+// see them. The second launch's blocks read a flag and end: 4.7 us.
 // Rows are stored without padding, their 16-byte units permuted by row so that the operand reads
 // and the transposed reads meet every bank once. Two buffers, one barrier per tile, the following
 // tiles' rows on their way in registers.
