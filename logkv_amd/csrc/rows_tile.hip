@@ -11,9 +11,10 @@
 // 4.7 cycles (one wave: 8), and the exponentials, maxima and conversions of 32 rows take about as
 // long as their products. So two waves a SIMD, and in each the score products of the next 32 rows
 // are interleaved with the maxima and half of the exponentials of these, the value products with
-// the other half and with the staging of the next tile. 32768 rows of 128 features, 8 lanes of 512 queries: 107 us, 645
-// TFLOP/s of the 1207 of a large matrix product (one wave a SIMD with 64 queries was slower: nothing
-// hid its waits); 30720 rows and 2048 new ones, 8 lanes of 4096 queries: 700 us, 760 TFLOP/s.
+// the other half and with the staging of the next tile. 32768 rows of 128 features, 8 lanes of 512
+// queries: 107 us, 645 TFLOP/s of the 1207 of a large matrix product (one wave a SIMD with 64
+// queries was slower: nothing hid its waits); 30720 rows and 2048 new ones, 8 lanes of 4096
+// queries: 700 us, 760 TFLOP/s.
 // Up to 64 queries: two blocks of four waves a CU (two waves of queries, two of rows): 64 lanes of
 // 8192 rows, 52 queries 80 us, in one block of eight waves 85.
 // bf16 caches: V enters the products as fp16, converted as it is staged (exact from 2^-17 up,
