@@ -859,6 +859,7 @@ int check_rows(const logkv_rows_args* a, const void* ws, int64_t ws_bytes, bool 
   if (weights ? !a->weights || a->visible || a->bias : !a->visible || a->weights || a->counts)
     return fail(LOGKV_EINVAL, weights ? "weight attention takes weights, no bias and no mask"
                                       : "tree attention takes a mask of the own rows, no weights and no counts");
+  if (weights && a->cap < 1) return fail(LOGKV_EINVAL, "weight attention needs a cache of at least one row");
   if (!aligned16(ws) || !ws || ws_bytes < logkv::rows_launch(*a, weights, nullptr).bytes)
     return fail(LOGKV_EINVAL, "row attention workspace too small");
   return LOGKV_OK;

@@ -200,12 +200,21 @@ def log_kv_weight_attention(q, k, v, cache_k, cache_v, weights, lengths, scale, 
     if (weights.shape != shape or weights.dtype != torch.float32 or weights.get_device() != cache_k.get_device()
             or weights.stride(2) != 1 or cap < 1):
         raise ValueError("weights must be float32 [B, G, capacity] on the cache's device with contiguous rows")
+    if _repeats(weights) or _repeats(cache_k) or _repeats(cache_v):
+        raise ValueError("weights and cache are written: their rows must not share memory (expanded tensors)")
+    if weights.requires_grad and torch.is_grad_enabled():
+        raise _no_gradient()
     if counts is not None:
         if (counts.shape != (batch,) or counts.get_device() != cache_k.get_device()
                 or counts.dtype not in _LENGTH_DTYPES):
             raise ValueError("counts must be an int32 tensor [batch] on the cache's device")
         counts = counts.to(torch.int32).contiguous()
     return _attention(q, k, v, cache_k, cache_v, float(scale), lengths, q.size(2), counts=counts, weights=weights)
+
+
+def _repeats(t):
+    """Whether elements of an expanded tensor share memory."""
+    return 0 in t.stride() and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape))
 
 
 def _span(t):
@@ -286,7 +295,8 @@ def _check_evict_out(out, cache_k, cache_v, weights, positions, lengths, keep):
             and _evict_rows_ok(k) and _evict_rows_ok(v) and (p is None) == (positions is None)
             and (p is None or rows(p, torch.int64)) and kept.shape == (batch, groups, keep) and kept.is_contiguous()
             and kept.dtype == torch.int32 and kept.device == device and n.shape == (batch,) and n.is_contiguous()
-            and n.dtype == torch.int32 and n.device == device):
+            and n.dtype == torch.int32 and n.device == device and not any(_repeats(t) for t in (k, v, w))
+            and (p is None or not _repeats(p))):
         raise ValueError("out must be EvictedRows buffers of at least keep rows that match the cache")
     given = [t for t in (cache_k, cache_v, weights, positions, lengths) if t is not None]
     results = [t for t in out if t is not None]

@@ -161,3 +161,36 @@ def test_python_refusals_on_the_host():
     for keep, recent in ((0, 0), (3, 4), (3, -1)):
         with pytest.raises(ValueError, match="keep"):
             log_kv_evict(ck, ck, w, 5, keep, recent=recent)
+
+
+@no_device
+def test_weight_attention_needs_a_cache():
+    lib, a = _rows.rows_lib(), rows_args(weights=FAKE, visible=0, cap=0)
+    assert lib.logkv_weight_attention(C.byref(a), FAKE, 1 << 40, None) == _lib.LOGKV_EINVAL
+    assert "at least one row" in lib.logkv_last_error().decode()
+
+
+def test_rows_written_must_not_share_memory():
+    """Expanded tensors where a call writes."""
+    from logkv_amd import EvictedRows, log_kv_weight_attention
+    from logkv_amd.row_attention import _check_evict_out, _repeats
+
+    bf = torch.bfloat16
+    q, k, ck = torch.zeros(2, 4, 3, 64, dtype=bf), torch.zeros(2, 2, 3, 64, dtype=bf), torch.zeros(2, 2, 10, 64, dtype=bf)
+    w = torch.zeros(2, 2, 10)
+    for cache, weights in ((ck, w[:1].expand(2, -1, -1)), (ck[:, :1].expand(-1, 2, -1, -1), w)):
+        with pytest.raises(ValueError, match="share memory"):
+            log_kv_weight_attention(q, k, k, cache, ck, weights, 5, 0.1)
+    with pytest.raises(NotImplementedError, match="gradient"):
+        log_kv_weight_attention(q, k, k, ck, ck, w.clone().requires_grad_(), 5, 0.1)
+    assert not _repeats(ck[:1].expand(1, -1, -1, -1)) and _repeats(ck[:1].expand(2, -1, -1, -1))
+
+    def out(**over):
+        fields = {"k": ck.clone(), "v": ck.clone(), "weights": w.clone(), "positions": None,
+                  "kept": torch.zeros(2, 2, 4, dtype=torch.int32), "lengths": torch.zeros(2, dtype=torch.int32), **over}
+        return EvictedRows(**fields)
+
+    _check_evict_out(out(), ck, ck.clone(), w, None, None, 4)
+    for over in ({"k": ck[:1].clone().expand(2, -1, -1, -1)}, {"weights": w[:, :1].clone().expand(-1, 2, -1)}):
+        with pytest.raises(ValueError, match="out must be"):
+            _check_evict_out(out(**over), ck, ck.clone(), w, None, None, 4)
