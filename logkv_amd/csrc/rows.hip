@@ -49,7 +49,8 @@ __global__ __launch_bounds__(kThreads) void rows_finish_kernel(logkv_rows_args a
   const int rep = a.n_heads / G, nq = rep * a.tq, tid = threadIdx.x;
   const int stride = a.dv + kRowsPartTail;
   const int64_t step = static_cast<int64_t>(nq) * stride;
-  const float* lane_part = r.part + static_cast<int64_t>(lane) * r.splits * step;
+  const float* lane_part = r.part + static_cast<int64_t>(lane) * r.room * step;
+  const int splits = r.shares ? r.shares[lane] : r.splits;
   int blk = blockIdx.x;
   if (blk < out_blocks) {
     __shared__ __align__(16) float acc_s[QPB][SG][4 * TQ];
@@ -61,7 +62,7 @@ __global__ __launch_bounds__(kThreads) void rows_finish_kernel(logkv_rows_args a
     float m = -__builtin_inff(), lsum = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     // Eight splits' loads at a time, joined under the running maximum.
-    for (int s0 = sg; s0 < r.splits; s0 += 8 * SG) {
+    for (int s0 = sg; s0 < splits; s0 += 8 * SG) {
       float2 ml[8];
       f32x4 x[8];
       float mx = m;
@@ -70,7 +71,7 @@ __global__ __launch_bounds__(kThreads) void rows_finish_kernel(logkv_rows_args a
         const int sp = s0 + k * SG;
         ml[k] = make_float2(-__builtin_inff(), 0.f);
         x[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (there && sp < r.splits) {
+        if (there && sp < splits) {
           ml[k] = *reinterpret_cast<const float2*>(base + sp * step + a.dv);
           x[k] = *reinterpret_cast<const f32x4*>(base + sp * step + d);
         }
@@ -136,7 +137,7 @@ __global__ __launch_bounds__(kThreads) void rows_finish_kernel(logkv_rows_args a
       const int q = tid / 16;
       if (q < nq) {
         float m, lsum;
-        fold_splits(lane_part + static_cast<int64_t>(q) * stride, step, r.splits, a.dv, tid % 16, 16, m, lsum);
+        fold_splits(lane_part + static_cast<int64_t>(q) * stride, step, splits, a.dv, tid % 16, 16, m, lsum);
         if (tid % 16 == 0) {
           qm[q] = r.shift - (m == -__builtin_inff() ? 0.f : m);
           ql[q] = lsum == 0.f ? 0.f : 1.f / lsum;
@@ -282,13 +283,20 @@ RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws) {
     off += align256(4 * floats);
     return p;
   };
-  r.part = take(lanes * r.splits * nq * (a.dv + kRowsPartTail));
+  // Shares by length (rows_tile.hip): a lane may take up to twice the equal number.
+  const bool by_length = r.q_waves && r.splits > 1 && a.n_batch > 1 && a.n_batch <= kWave;
+  r.room = by_length ? 2 * r.splits : r.splits;
+  r.part = take(lanes * r.room * nq * (a.dv + kRowsPartTail));
   if (r.q_waves) r.redo = reinterpret_cast<int*>(take(lanes * r.splits * ((nq + 32 * r.q_waves - 1) / (32 * r.q_waves))));
   if (causal && nq <= 16) {
     r.score_st = tiles * kRowTile;
     r.scores = take(lanes * nq * r.score_st);
   } else if (causal) {
     r.lse = take(lanes * nq);
+  }
+  if (by_length) {
+    r.shares = reinterpret_cast<int*>(take(lanes));
+    if (!a.lengths || !a.len_stride) r.shares = nullptr;   // sequences of one length
   }
   r.bytes = off;
   return r;

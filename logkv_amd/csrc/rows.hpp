@@ -14,20 +14,23 @@ constexpr float kTileShift = 7.f;   // tiled kernel: P times 2^7 (below 2^15: it
 constexpr float kLog2e = 1.44269504088896341f;
 
 // Launch parameters beside the caller's arguments. Workspace regions, 256-byte aligned:
-// part [lanes, splits, nq, dv + kRowsPartTail]: unnormalised sums, then the base-2 maximum and sum;
+// part [lanes, room, nq, dv + kRowsPartTail]: unnormalised sums, then the base-2 maximum and sum;
 // scores [lanes, nq, score_st]: raw products q . k of up to 16 queries (weight attention);
 // redo: one flag per block of the tiled kernel;
+// shares [lanes]: the partials of a lane where lengths decide (null: splits of them);
 // lse [lanes, nq]: base-2 log-sum-exp of longer ones (+inf where a query sees nothing).
 struct RowsLaunch {
   float* part;
   float* scores;
   float* lse;
   int* redo;      // tiled kernel: per block whether its share is left to the second launch
+  int* shares;
   int64_t score_st;
   int64_t bytes;
   int splits;
+  int room;       // partials that a lane has memory for
   int cols;       // streamed kernel: 16-query column blocks per wave
-  int q_waves;    // tiled kernel: waves with 64 queries each (0: the streamed kernel)
+  int q_waves;    // tiled kernel: waves with 32 queries each (0: the streamed kernel)
   float shift;    // the partials' sums carry 2^shift
   int causal;     // weight attention; otherwise the visible mask
 };

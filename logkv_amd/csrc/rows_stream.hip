@@ -302,7 +302,7 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
     }
     __syncthreads();
     const int qb = q0 + 16 * c, queries = min(16, nq - qb);
-    float* out = r.part + ((static_cast<int64_t>(lane) * r.splits + blockIdx.x) * nq + qb) * (a.dv + kRowsPartTail);
+    float* out = r.part + ((static_cast<int64_t>(lane) * r.room + blockIdx.x) * nq + qb) * (a.dv + kRowsPartTail);
     for (int e = threadIdx.x; e < queries * (a.dv + 2); e += blockDim.x) {
       const int q = e / (a.dv + 2), d = e % (a.dv + 2);
       float mx = -__builtin_inff();

@@ -105,6 +105,48 @@ __device__ __forceinline__ RowsBlock rows_block() {
   return RowsBlock{lin % nx, lin / nx % ny, lin / (nx * ny)};
 }
 
+__device__ __forceinline__ int wave_total(int x) {
+#pragma unroll
+  for (int off = kWave / 2; off; off >>= 1) x += __shfl_xor(x, off, kWave);
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
+// Of sequences of different lengths: the equal number of shares a lane (splits) is dealt out anew, to
+// each batch row as many as its tiles take at R a share, for the smallest R that needs no more shares
+// than there are and no more than `room` for a row. Found by every wave for itself, a batch row in each
+// of its lanes. Changes the block's place and the shares of its lane; false for a block left over.
+template <int TR>
+__device__ __forceinline__ bool share_by_length(const logkv_rows_args& a, const RowsLaunch& r, RowsBlock& id, int& splits) {
+  const int B = a.n_batch, G = a.n_groups, l = lane_id(), i = min(l, B - 1), slots = B * r.splits;
+  const int tiles = max(1, (rows_in_use(a, i) + TR - 1) / TR + (own_rows(a, i) + TR - 1) / TR), t = l < B ? tiles : 0;
+  if (__ballot(tiles != __builtin_amdgcn_readfirstlane(tiles)) == 0) return true;   // as they are
+  int most = t;
+#pragma unroll
+  for (int off = kWave / 2; off; off >>= 1) most = max(most, __shfl_xor(most, off, kWave));
+  most = __builtin_amdgcn_readfirstlane(most);
+  int lo = max((wave_total(t) + slots - 1) / slots, (most + r.room - 1) / r.room), hi = (most + r.splits - 1) / r.splits;
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (wave_total((t + mid - 1) / mid) <= slots) hi = mid;
+    else lo = mid + 1;
+  }
+  const int mine = (t + lo - 1) / lo;
+  int up_to = mine;
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const int up = __shfl_up(up_to, off, kWave);
+    if (l >= off) up_to += up;
+  }
+  const int slot = id.lane / G * r.splits + id.split;
+  const uint64_t later = __ballot(l < B && up_to > slot);
+  if (!later) return false;
+  const int b = __ffsll(static_cast<unsigned long long>(later)) - 1;
+  splits = __builtin_amdgcn_readlane(mine, b);
+  id.split = slot - (__builtin_amdgcn_readlane(up_to, b) - splits);
+  id.lane = b * G + id.lane % G;
+  return true;
+}
+
 // What a block's share needs beside its tiles, and what it leaves: per column block a lane's query
 // with 16 features of each 32 per register block.
 template <int NKS, int NDV>
@@ -604,9 +646,17 @@ __global__ __launch_bounds__(64 * NW, 2) void rows_tile_kernel(logkv_rows_args a
   __shared__ __align__(16) float bias_s[BIAS ? 2 : 1][TR];
   __shared__ int flag_s[3];
   __shared__ float m_s[NW][kQueries], l_s[NW][kQueries];
-  const RowsBlock id = rows_block();
+  RowsBlock id = rows_block();
   int* redo = r.redo + (static_cast<int64_t>(id.lane) * gridDim.y + id.split) * gridDim.x + id.qb;
   if (SECOND && *redo == 0) return;
+  int splits = r.splits;
+  if (r.shares) {
+    if (!share_by_length<TR>(a, r, id, splits)) {
+      if (threadIdx.x == 0) *redo = 0;
+      return;
+    }
+    if (id.split == 0 && id.qb == 0 && threadIdx.x == 0) r.shares[id.lane] = splits;
+  }
   const int lane = id.lane, G = a.n_groups, tid = threadIdx.x;
   const int rep = a.n_heads / G, nq = rep * a.tq, w = wave_id(), l = lane_id(), h = l >> 5, col = l & 31;
   RowsShare<NKS, NDV> c;
@@ -620,7 +670,7 @@ __global__ __launch_bounds__(64 * NW, 2) void rows_tile_kernel(logkv_rows_args a
   const int t_max = q_first / a.tq == q_last / a.tq ? q_last % a.tq : a.tq - 1;
   const int own_end = r.causal ? min(c.own, t_max + 1) : c.own;
   c.np = (c.n + TR - 1) / TR;
-  const int tiles = c.np + (own_end + TR - 1) / TR, share = (tiles + r.splits - 1) / r.splits;
+  const int tiles = c.np + (own_end + TR - 1) / TR, share = (tiles + splits - 1) / splits;
   c.begin = min(id.split * share, tiles);
   c.end = min(c.begin + share, tiles);
 #pragma unroll
@@ -653,7 +703,7 @@ __global__ __launch_bounds__(64 * NW, 2) void rows_tile_kernel(logkv_rows_args a
         for (int i = 0; i < 16; ++i) c.o[k][nb][i] = 0.f;
     }
   }
-  float* part = r.part + (static_cast<int64_t>(lane) * r.splits + id.split) * nq * (a.dv + kRowsPartTail);
+  float* part = r.part + (static_cast<int64_t>(lane) * r.room + id.split) * nq * (a.dv + kRowsPartTail);
   if constexpr (RW == 1) {
 #pragma unroll
     for (int k = 0; k < kCols; ++k) {

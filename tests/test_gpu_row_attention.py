@@ -361,3 +361,49 @@ def test_17_to_32_queries_over_many_rows(rep, T, dk, dv):
         total[b, :, m:m + T] = column[b, :, cap:cap + T]
         check_close(w[b], total[b], (rel + (rep * T + 4) * 2.0 ** -23) * total[b].abs() + 1e-30)
         assert torch.equal(ck[b, :, m:m + T], k[b]) and torch.equal(cv[b, :, m:m + T], v[b])
+
+
+@pytest.mark.parametrize("rep,T,d,dtype", [(2, 20, 64, BF16), (1, 70, 128, F16), (3, 61, 64, F16), (4, 70, 128, BF16)])
+@pytest.mark.parametrize("lengths", [[4099, 33, 0, 700, 64], [5000, 5000, 4990, 5000, 5000], [1, 5000, 1, 1, 2],
+                                     [-7, 2500, 9999, 1300, 640]])
+def test_shares_by_length(lengths, rep, T, d, dtype):
+    """Sequences of very different lengths in one call, whose rows are dealt out over the batch; the length of one
+    call's sequence alone gives the same result but for the rounding of its shares' sums."""
+    B, G, cap = len(lengths), 2, 5000
+    q, k, v, ck, cv = inputs(B, G, rep, T, cap, d, d, dtype, 91)
+    n, scale = torch.tensor(lengths, dtype=torch.int32, device="cuda"), d ** -0.5
+    visible = torch.stack([tree_mask(T, 70 + b, empty=(T - 1,)) for b in range(B)])
+    pick = [0, T // 2, T - 1]      # the reference's time goes by the queries: three tokens' rows of every head
+    out = log_kv_tree_attention(q, k, v, ck, cv, n, visible.cuda(), scale)
+    again = log_kv_tree_attention(q, k, v, ck, cv, n, visible.cuda(), scale)
+    assert torch.equal(out, again)
+    for b, m in enumerate(lengths):
+        m = min(max(m, 0), cap)
+        for t in pick:
+            see = visible[b, t].nonzero().flatten().cuda()
+            one = [x[b:b + 1] for x in (q[:, :, t:t + 1], torch.cat((ck[:, :, :m], k[:, :, see]), 2), torch.cat((cv[:, :, :m], v[:, :, see]), 2))]
+            if one[1].size(2) == 0:
+                assert bool((out[b, :, t] == 0).all())
+                continue
+            rows_k, rows_v = one[1], one[2]
+            want, _, bound, _ = reference(one[0], rows_k[:, :, -1:], rows_v[:, :, -1:], rows_k[:, :, :-1], rows_v[:, :, :-1],
+                                          [rows_k.size(2) - 1], torch.ones(1, 1, 1, dtype=torch.bool), scale)
+            check_close(out[b:b + 1, :, t:t + 1], want, bound, f"row {b}, token {t}")
+
+
+def test_shares_by_length_of_a_padded_batch_of_weights():
+    B, G, rep, T, cap, d = 4, 2, 2, 40, 3000, 64
+    lengths, counts = [2900, 0, 7, 1200], [T, 0, T - 1, 1]
+    q, k, v, ck, cv = inputs(B, G, rep, T, cap, d, d, BF16, 92)
+    w = torch.rand(B, G, cap, generator=torch.Generator().manual_seed(8)).cuda()
+    total, before = w.cpu().double(), ck.clone()
+    causal = torch.ones(T, T, dtype=torch.bool).tril()[None].expand(B, T, T)
+    want, column, bound, rel = reference(q, k, v, ck, cv, lengths, causal, 0.125, counts=counts)
+    out = log_kv_weight_attention(q, k, v, ck, cv, w, torch.tensor(lengths, device="cuda"), 0.125,
+                                  counts=torch.tensor(counts, device="cuda"))
+    check_close(out, want, bound)
+    for b, (m, c) in enumerate(zip(lengths, counts)):
+        total[b, :, :m] += column[b, :, :m]
+        total[b, :, m:m + c] = column[b, :, cap:cap + c]
+        check_close(w[b], total[b], (rel + (rep * T + 4) * 2.0 ** -23) * total[b].abs() + 1e-30)
+        assert torch.equal(ck[b, :, m:m + c], k[b, :, :c]) and torch.equal(ck[b, :, m + c:], before[b, :, m + c:])
