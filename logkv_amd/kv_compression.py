@@ -10,12 +10,14 @@ so they are not a memory figure.
 The log-structured counts are reductions over device buffers (one host read per
 layer); a dense cache (anything without ``token_count``) is counted from
 ``processed_tokens``, or from its populated positions for a sliding window, as the
-reference does.
+reference does; an ``EvictingKVCache`` by its rows in use.
 """
 
 from __future__ import annotations
 
 from typing import NamedTuple
+
+from .evicting_cache import EvictingKVCache
 
 _TOTAL_FIELDS = (
     "processed_tokens",
@@ -55,7 +57,7 @@ def _count_layer(attn, processed_tokens: int) -> _LayerCount:
     counts its recent window plus a pending tail the attention module holds, the valid exact-pool
     rows of every KV group and the ladder slots of positive mass (device reductions, one host read);
     a dense cache holds ``processed_tokens`` per lane, or its populated positions when it is a
-    sliding window."""
+    sliding window, or its rows in use when it evicts."""
     cache = attn.kv_cache
     if cache is None:
         raise ValueError("every attention layer needs an initialized KV cache to measure compression")
@@ -71,7 +73,9 @@ def _count_layer(attn, processed_tokens: int) -> _LayerCount:
         return _LayerCount(cache.token_count + tail_len, lanes, (cache.recent_count + tail_len) * lanes, exact, live)
     batch, groups = cache.k.shape[:2]
     lanes = batch * groups
-    if getattr(cache, "is_sliding_window", False):
+    if isinstance(cache, EvictingKVCache):
+        held = int(cache.lengths.sum().item()) * groups
+    elif getattr(cache, "is_sliding_window", False):
         held = int((cache.positions >= 0).sum().item()) * groups
     else:
         held = processed_tokens * lanes

@@ -72,3 +72,15 @@ def test_evicting_cache_sizes():
     with pytest.raises((ValueError, RuntimeError)):
         cache(x, x, torch.zeros(1, 2, 1, 16, dtype=torch.bfloat16))
     assert cache.lengths.tolist() == [0]
+
+
+def test_accounting_counts_the_rows_in_use():
+    from types import SimpleNamespace
+
+    from logkv_amd import cache_compression_snapshot
+
+    cache = EvictingKVCache(2, 4, 8, 8, 16, scale=1.0, device="cpu")
+    cache.lengths.copy_(torch.tensor([16, 9], dtype=torch.int32))
+    model = SimpleNamespace(transformer=SimpleNamespace(h=[SimpleNamespace(attn=SimpleNamespace(kv_cache=cache))]))
+    counts = cache_compression_snapshot(model, 100)
+    assert counts["retained_slots"] == 25 * 4 and counts["dense_slots"] == 100 * 8 and counts["layer_group_count"] == 8
