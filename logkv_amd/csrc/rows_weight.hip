@@ -2,7 +2,7 @@
 //   weight_j = sum over queries of 2^(s_j c2 - L),  c2 = scale log2(e).
 // S = Q K^T by 32x32x16 matrix products with the keys as columns, so a lane sums its own key over
 // the queries in registers: a wave holds 32 KB keys' operands for good, and the block's queries pass
-// through LDS, 64 to a tile, two buffers, the next tile's rows on their way in registers. The products
+// through LDS, a tile of 64, two buffers, the next tile's rows on their way in registers. The products
 // of one 32x32 block and the exponentials of the one before are independent and interleaved: both
 // take about as long (16 quarter-rate exponentials a lane against eight products of 32 cycles at 128
 // features). One wave owns a key: no atomics, a fixed order. 8 lanes of 30720 rows and 2048 new ones,
@@ -20,7 +20,6 @@ namespace {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
-constexpr int kQueries = 64;   // per staged tile
 
 template <int DT>
 __device__ __forceinline__ f32x16 mfma32(uint4 x, uint4 y, f32x16 c) {
@@ -39,10 +38,12 @@ __device__ __forceinline__ int swizzle(int r) {
 
 }  // namespace
 
-// NKS 16-wide steps of dk, KB 32-key blocks per wave.
-template <int DT, int NKS, int KB>
+// NKS 16-wide steps of dk, KB 32-key blocks per wave, QG groups of waves that share a tile's queries.
+template <int DT, int NKS, int KB, int QG>
 __global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_args a, RowsLaunch r, int cache_blocks) {
-  constexpr int KU = 2 * NKS, kTasks = kQueries * KU / kThreads, kKeys = 4 * 32 * KB;
+  constexpr int kQueries = NKS > 8 ? 32 : 64;   // per staged tile (64 of 256 features spill: 8 lanes, 4096 rows, 400
+                                                // queries 200 us the call, 149)
+  constexpr int KU = 2 * NKS, kTasks = kQueries * KU / kThreads, kKeyWaves = 4 / QG, kKeys = kKeyWaves * 32 * KB;
   __shared__ __align__(16) uint4 q_s[2][kQueries * KU];
   __shared__ __align__(16) float l_s[2][kQueries];
   __shared__ __align__(16) int t_s[2][kQueries];
@@ -57,7 +58,7 @@ __global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_arg
   const bool of_cache = x < cache_blocks;
   const int rows = of_cache ? n : own, b0 = (of_cache ? x : (x - cache_blocks + lane) % own_blocks) * kKeys;
   if (b0 >= rows || own == 0) return;
-  const int k0 = b0 + w * 32 * KB;
+  const int k0 = b0 + w % kKeyWaves * 32 * KB, q_block = w / kKeyWaves * (kQueries / 32 / QG);   // the wave's first query block of a tile
   const LOGKV_G uint16_t* kr = of_cache ? gp(a.cache_k) + b * a.ck_sb + g * a.ck_sg : gp(a.k) + b * a.k_sb + g * a.k_sg;
   const int64_t kst = of_cache ? a.ck_st : a.k_st;
   uint4 kf[KB][NKS];
@@ -138,10 +139,10 @@ __global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_arg
     };
     auto tile = [&](auto own_tag) {
       constexpr bool OWN = decltype(own_tag)::value;
-      constexpr int kBlocks = 2 * KB, kShare = 16 / NKS;   // 32x32 blocks; exponentials per product
+      constexpr int kBlocks = kQueries / 32 * KB / QG, kShare = 16 / NKS;   // 32x32 blocks; exponentials per product
       uint4 qa[NKS];
 #pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) qa[ks] = frag(0, ks);
+      for (int ks = 0; ks < NKS; ++ks) qa[ks] = frag(q_block, ks);
       f32x16 s, next;
 #pragma unroll
       for (int i = 0; i < 16; ++i) next[i] = 0.f;
@@ -154,8 +155,8 @@ __global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_arg
         if (blk > 0) {
 #pragma unroll
           for (int i4 = 0; i4 < 4; ++i4) {
-            x[i4] = *reinterpret_cast<const f32x4*>(&l_s[bf][32 * ((blk - 1) / KB) + 8 * i4 + 4 * h]);
-            if constexpr (OWN) t[i4] = *reinterpret_cast<const i32x4*>(&t_s[bf][32 * ((blk - 1) / KB) + 8 * i4 + 4 * h]);
+            x[i4] = *reinterpret_cast<const f32x4*>(&l_s[bf][32 * (q_block + (blk - 1) / KB) + 8 * i4 + 4 * h]);
+            if constexpr (OWN) t[i4] = *reinterpret_cast<const i32x4*>(&t_s[bf][32 * (q_block + (blk - 1) / KB) + 8 * i4 + 4 * h]);
           }
         }
 #pragma unroll
@@ -164,10 +165,10 @@ __global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_arg
         for (int ks = 0; ks < NKS; ++ks) {
           if (blk < kBlocks) {
             next = mfma32<DT>(qa[ks], kf[blk % KB][ks], next);
-            if (blk % KB == KB - 1 && blk + 1 < kBlocks) qa[ks] = frag((blk + 1) / KB, ks);
+            if (blk % KB == KB - 1 && blk + 1 < kBlocks) qa[ks] = frag(q_block + (blk + 1) / KB, ks);
           }
           if (blk > 0) {
-            // Element i is query 32 ((blk - 1) / KB) + 8 (i / 4) + 4 h + i % 4 against key 32 ((blk - 1) % KB) + col.
+            // Element i is query 32 (q_block + (blk - 1) / KB) + 8 (i / 4) + 4 h + i % 4 against key 32 ((blk - 1) % KB) + col.
 #pragma unroll
             for (int i = kShare * ks; i < kShare * (ks + 1); ++i) {
               float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c2, -x[i / 4][i % 4]));
@@ -186,10 +187,24 @@ __global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_arg
       if (it + 2 < tiles) load(kQueries * (it + 2));
     }
   }
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) sum[kb] += __shfl_xor(sum[kb], 32, kWave);
+  if constexpr (QG > 1) {
+    // The groups' sums joined in their order.
+    __shared__ float sum_s[4][KB][32];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+      if (h == 0) sum_s[w][kb][col] = sum[kb];
+    __syncthreads();
+    if (w >= kKeyWaves) return;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int k = 1; k < QG; ++k) sum[kb] += sum_s[k * kKeyWaves + w][kb][col];
+  }
   LOGKV_G float* wrow = gp(a.weights) + b * a.w_sb + g * a.w_sg;
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
-    sum[kb] += __shfl_xor(sum[kb], 32, kWave);
     const int j = k0 + 32 * kb + col;
     if (h || j >= rows) continue;
     if (of_cache) wrow[j] += sum[kb];
@@ -199,26 +214,31 @@ __global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_arg
 
 namespace {
 
-template <int DT, int NKS, int KB>
+template <int DT, int NKS, int KB, int QG>
 void launch_one(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
-  constexpr int kKeys = 4 * 32 * KB;
+  constexpr int kKeys = 4 / QG * 32 * KB;
   const int cache_blocks = (a.cap + kKeys - 1) / kKeys;
   const dim3 grid(cache_blocks + (a.tq + kKeys - 1) / kKeys, a.n_batch * a.n_groups);
-  hipLaunchKernelGGL((rows_weight_kernel<DT, NKS, KB>), grid, dim3(kThreads), 0, stream, a, r, cache_blocks);
+  hipLaunchKernelGGL((rows_weight_kernel<DT, NKS, KB, QG>), grid, dim3(kThreads), 0, stream, a, r, cache_blocks);
 }
 
 template <int DT>
 void launch_type(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
-  // 64 keys a wave where that leaves two blocks for every CU.
-  const bool many = (static_cast<int64_t>(a.cap) + a.tq) * a.n_batch * a.n_groups >= 512 * 256;
+  // 64 keys a wave where that leaves two blocks for every CU; two waves to 32 keys, each half of the queries, where
+  // four waves of 32 keys would leave less than two blocks (4 lanes of 2048 rows, 2000 queries: 71.5 us the call, 79.6
+  // without; 8 lanes of 4096, 666: 51.0 and 51.9).
+  const int64_t keys = (static_cast<int64_t>(a.cap) + a.tq) * a.n_batch * a.n_groups;
+  const bool many = keys >= 512 * 256, few = keys < 512 * 128;
   if (a.dk <= 64) {
-    if (many) launch_one<DT, 4, 2>(a, r, stream);
-    else launch_one<DT, 4, 1>(a, r, stream);
+    if (many) launch_one<DT, 4, 2, 1>(a, r, stream);
+    else if (few) launch_one<DT, 4, 1, 2>(a, r, stream);
+    else launch_one<DT, 4, 1, 1>(a, r, stream);
   } else if (a.dk <= 128) {
-    if (many) launch_one<DT, 8, 2>(a, r, stream);
-    else launch_one<DT, 8, 1>(a, r, stream);
+    if (many) launch_one<DT, 8, 2, 1>(a, r, stream);
+    else if (few) launch_one<DT, 8, 1, 2>(a, r, stream);
+    else launch_one<DT, 8, 1, 1>(a, r, stream);
   } else {
-    launch_one<DT, 16, 1>(a, r, stream);
+    launch_one<DT, 16, 1, 1>(a, r, stream);
   }
 }
 
