@@ -268,7 +268,9 @@ RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws) {
     r.shift = kTileShift;
     r.splits = tile_splits(a, lanes * ((nq + 32 * r.q_waves - 1) / (32 * r.q_waves)), r.q_waves);
   } else {
-    r.cols = nq <= 16 ? 1 : 2;
+    // Wide rows' two query blocks spill; read twice instead up to 128 queries: 32 lanes of 16000 rows of 192 and 128
+    // features, 24 queries: 155 us, in blocks of 16 queries 114; 8 lanes of 8000 rows of 256, 256 queries: 117 and 123.
+    r.cols = nq <= 16 || (wide && nq <= 128) ? 1 : 2;
     r.shift = a.dtype == LOGKV_F16 ? Elem<LOGKV_F16>::kShift : Elem<LOGKV_BF16>::kShift;
     const int64_t q_blocks = (nq + 16 * r.cols - 1) / (16 * r.cols);
     // One share per resident block, none shorter than a tile for each of its waves.

@@ -1,5 +1,5 @@
 // Attention over a cache's rows and the call's own rows, streamed: up to 32 query rows of a KV
-// group (16 NC; wider rows take several such blocks of queries) are the columns of the matrix products while the group's rows pass once from memory.
+// group (16 NC; rows wider than 128 take several such blocks of queries) are the columns of the matrix products while the group's rows pass once from memory.
 //
 //   s_j = scale q . k_j + bias_j;  out = sum_j 2^(s'_j - m) v_j / sum_j 2^(s'_j - m),  s' = s log2(e)
 //
