@@ -2,7 +2,8 @@
 
 Host surface mirrors the reference modules (litgpt/log_kv_cache.py,
 litgpt/alpha_log_kv.py, litgpt/beta_log_kv.py, litgpt/log_kv_pack.py);
-compute runs in liblogkv_hip.so through the C ABI in include/logkv_hip.h.
+compute runs in liblogkv_hip.so through the C ABI in include/logkv_hip.h and
+logkv_rows.h (row attention and eviction, which have no counterpart there).
 """
 
 from .log_kv_cache import (CacheAttentionState, LogKVStreamTrainingAttention, LogStructuredKVCache,  # noqa: F401

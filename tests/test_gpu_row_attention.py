@@ -407,3 +407,50 @@ def test_shares_by_length_of_a_padded_batch_of_weights():
         total[b, :, m:m + c] = column[b, :, cap:cap + c]
         check_close(w[b], total[b], (rel + (rep * T + 4) * 2.0 ** -23) * total[b].abs() + 1e-30)
         assert torch.equal(ck[b, :, m:m + c], k[b, :, :c]) and torch.equal(ck[b, :, m + c:], before[b, :, m + c:])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_wide_rows_of_many_queries_with_infinities(dtype):
+    """Blocks of 32 queries of rows wider than 128 features; infinities and NaN reach only who sees them."""
+    G, cap, rep, T, d = 1, 70, 4, 35, 256
+    q, k, v, ck, cv = inputs(1, G, rep, T, cap, d, d, dtype, 21)
+    visible = tree_mask(T, 2)
+    v[0, 0, 1, 3], v[0, 0, 2, 200], v[0, 0, 4, 5] = math.inf, -math.inf, math.nan
+    out = log_kv_tree_attention(q, k, v, ck, cv, 65, visible.cuda(), d ** -0.5)
+    want, _, bound, _ = reference(q, k, v, ck, cv, [65], visible[None], d ** -0.5)
+    assert bool(torch.isinf(want).any()) and bool(torch.isfinite(want[0, 0, 0]).all())
+    check_close(out, want, bound)
+
+
+def test_two_graphs_of_ragged_batches_at_once():
+    """Two captured calls whose shares go by length, replayed on two streams together with an eager call on a third,
+    over lengths that change between the replays."""
+    B, G, rep, T, cap, d = 3, 2, 2, 24, 4000, 64
+    sets = [inputs(B, G, rep, T, cap, d, d, BF16, 95 + i) for i in range(3)]
+    ns = [torch.tensor([100, 4000, 1], dtype=torch.int32, device="cuda") for _ in sets]
+    visible = tree_mask(T, 4).cuda()
+    streams = [torch.cuda.Stream() for _ in sets]
+
+    def call(i):
+        q, k, v, ck, cv = sets[i]
+        return log_kv_tree_attention(q, k, v, ck, cv, ns[i], visible, 0.125)
+
+    call(0)
+    graphs, outs = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            outs.append(call(i))
+    for lengths in ([100, 4000, 1], [4000, 4000, 4000], [3000, 0, 2222], [64, 65, 4000]):
+        for n in ns:
+            n.copy_(torch.tensor(lengths, dtype=torch.int32))
+        want = [call(i) for i in range(3)]
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        with torch.cuda.stream(streams[2]):
+            eager = call(2)
+        torch.cuda.synchronize()
+        for got, w in zip((*outs, eager), want):
+            assert torch.equal(got, w), lengths
