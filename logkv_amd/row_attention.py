@@ -58,17 +58,14 @@ def _no_gradient():
 
 
 def _small_rows(x, dtype):
-    """Rows of the call in the cache's dtype, readable in 16-byte units, and their strides."""
+    """Rows of the call in the cache's dtype, readable in 16-byte units."""
     if x.dtype != dtype:
         check_activation_dtype(x.dtype)
         x = x.to(dtype)
     sb, sh, st, sd = x.stride()
     if sd != 1 or (sb | sh | st) & 7 or x.data_ptr() & 15:
-        x = x.contiguous()
-        if x.data_ptr() & 15:
-            x = x.clone()
-        sb, sh, st, sd = x.stride()
-    return x, sb, sh, st
+        x = x.clone(memory_format=torch.contiguous_format)   # of any strides, also those of size-1 dimensions
+    return x
 
 
 def _lengths(lengths, batch, cap, index, room=0):
@@ -128,7 +125,14 @@ def _attention(q, k, v, cache_k, cache_v, scale, lengths, room, *, bias=None, vi
     if cap and (ck_sd != 1 or cv_sd != 1 or (ck_sb | ck_sg | ck_st | cv_sb | cv_sg | cv_st) & 7 or (ck | cv) & 15):
         raise ValueError("cache rows must be 16-byte aligned with contiguous features")
     out_dtype = q.dtype
-    (q, *q_st), (k, *k_st), (v, *v_st) = _small_rows(q, dtype), _small_rows(k, dtype), _small_rows(v, dtype)
+    q_st, k_st, v_st = q.stride(), k.stride(), v.stride()
+    qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if (q.dtype != dtype or k.dtype != dtype or v.dtype != dtype or not q_st[3] == k_st[3] == v_st[3] == 1
+            or (q_st[0] | q_st[1] | q_st[2] | k_st[0] | k_st[1] | k_st[2] | v_st[0] | v_st[1] | v_st[2]) & 7
+            or (qp | kp | vp) & 15):
+        q, k, v = _small_rows(q, dtype), _small_rows(k, dtype), _small_rows(v, dtype)
+        q_st, k_st, v_st = q.stride(), k.stride(), v.stride()
+        qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
     n2_ptr = 0
     if in_use is None:
         lengths, n_ptr, n_st, len_add = _lengths(lengths, batch, cap, index, room)
@@ -149,7 +153,7 @@ def _attention(q, k, v, cache_k, cache_v, scale, lengths, room, *, bias=None, vi
     workspace = cache_k.new_empty(need // 2)
     o_sh = tq * dv
     args = pack_rows(
-        q.data_ptr(), *q_st, k.data_ptr(), *k_st, v.data_ptr(), *v_st, ck, ck_sb, ck_sg, ck_st, cv, cv_sb, cv_sg, cv_st,
+        qp, *q_st[:3], kp, *k_st[:3], vp, *v_st[:3], ck, ck_sb, ck_sg, ck_st, cv, cv_sb, cv_sg, cv_st,
         b_ptr, *b_st, n_ptr, n2_ptr, vis_ptr, vis_sb, vis_st,
         0 if counts is None else counts.data_ptr(), w_ptr, w_sb, w_sg, out.data_ptr(), heads * o_sh, o_sh, dv,
         batch, heads, groups, tq, cap, dk, dv, code, n_st, len_add, b_half, scale)
@@ -179,8 +183,11 @@ def log_kv_tree_attention(q, k, v, cache_k, cache_v, lengths, visible, scale, *,
 
 def _tree(visible, q, cache_k):
     """The checked mask of a draft, with contiguous rows."""
-    if (not isinstance(visible, torch.Tensor) or visible.dtype not in (torch.bool, torch.uint8) or q.ndim != 4
-            or visible.shape not in ((q.size(2),) * 2, (q.size(0), q.size(2), q.size(2)))
+    if not isinstance(visible, torch.Tensor) or q.ndim != 4:
+        raise ValueError("visible must be a bool tensor [T, T] or [B, T, T], queries [B, n_heads, T, d]")
+    tokens, shape = q.size(2), visible.shape
+    if (visible.dtype not in (torch.bool, torch.uint8)
+            or not (shape == (tokens, tokens) or shape == (q.size(0), tokens, tokens))
             or visible.get_device() != cache_k.get_device()):
         raise ValueError("visible must be a bool tensor [T, T] or [B, T, T] on the cache's device")
     return visible if visible.stride(-1) == 1 else visible.contiguous()

@@ -454,3 +454,20 @@ def test_two_graphs_of_ragged_batches_at_once():
         torch.cuda.synchronize()
         for got, w in zip((*outs, eager), want):
             assert torch.equal(got, w), lengths
+
+
+def test_one_token_of_padded_rows():
+    """A single token cut from rows of an odd width: the strides of its size-1 dimensions are odd too."""
+    G, rep, d, cap = 2, 2, 64, 40
+    wide = [rows((1, 1, h * d + 1), BF16, 50 + i)[..., 1:] for i, h in enumerate((G * rep, G, G))]
+    q, k, v = (x.view(1, 1, h, d).transpose(1, 2) for x, h in zip(wide, (G * rep, G, G)))
+    _, _, _, ck, cv = inputs(1, G, rep, 1, cap, d, d, BF16, 53)
+    see = torch.ones(1, 1, dtype=torch.bool, device="cuda")
+    out = log_kv_tree_attention(q, k, v, ck, cv, 37, see, 0.125)
+    want, _, bound, _ = reference(q, k, v, ck, cv, [37], see.cpu()[None], 0.125)
+    check_close(out, want, bound)
+    dense = [torch.empty(x.shape, dtype=BF16, device="cuda").copy_(x) for x in (q, k, v)]
+    assert torch.equal(out, log_kv_tree_attention(*dense, ck, cv, 37, see, 0.125))
+    # Aligned rows with odd strides of dimensions of one element.
+    odd = [x.as_strided(x.shape, (7, x.stride(1), 5, 1)) for x in dense]
+    assert torch.equal(out, log_kv_tree_attention(*odd, ck, cv, 37, see, 0.125))
