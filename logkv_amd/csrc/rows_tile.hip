@@ -27,12 +27,13 @@
 // the second form is for infinities and NaNs in V, which it adds row by row for the queries that
 // see them. The second launch's blocks read a flag and end: 4.7 us.
 // Rows are stored without padding, their 16-byte units permuted by row so that the operand reads
-// and the transposed reads meet every bank once. Two buffers, one barrier per tile, the following
-// tiles' rows on their way in registers.
+// and the transposed reads meet every bank once. One barrier per tile, the following tiles' rows on
+// their way in registers; two buffers of V and, by RowsSchedule, two or three of K.
 #include <algorithm>
 #include <type_traits>
 
 #include "rows.hpp"
+#include "rows_schedule.hpp"
 
 namespace logkv {
 
@@ -182,12 +183,13 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
   constexpr int kThreads = 64 * NW, RW = NW / QW, TR = 32 * RB * RW;   // row groups, rows per tile
   constexpr int KU = 2 * NKS, VU = 4 * NDV;            // 16-byte units of a staged row
   constexpr int kKTasks = TR * KU / kThreads, kVTasks = TR * VU / kThreads;
-  constexpr int kTileBytes = TR * (KU + VU) * 16;
+  typedef RowsSchedule<RB> Order;
+  constexpr int kKBytes = TR * KU * 16, kVBytes = TR * VU * 16, kVBase = Order::kKBuffers * kKBytes;
   constexpr bool kHalfV = DT == LOGKV_BF16;            // V converted to fp16
   const int tid = threadIdx.x, l = lane_id(), h = l >> 5, col = l & 31, rw = wave_id() / QW;
   const int kunits = a.dk / 8, vunits = a.dv / 8, b = c.b, g = c.g, np = c.np, begin = c.begin, end = c.end;
-  auto k_tile = [&](int bf) { return reinterpret_cast<uint4*>(buf + bf * kTileBytes); };
-  auto v_tile = [&](int bf) { return reinterpret_cast<uint4*>(buf + bf * kTileBytes + TR * KU * 16); };
+  auto k_tile = [&](int bf) { return reinterpret_cast<uint4*>(buf + bf * kKBytes); };
+  auto v_tile = [&](int bf) { return reinterpret_cast<uint4*>(buf + kVBase + bf * kVBytes); };
 
   // Registers of the tiles on their way: K two tiles ahead of the sums, V one. A thread's units are
   // rows tid / KU + kThreads / KU q of a tile. The loads are issued on one path for every tile (values
@@ -288,13 +290,13 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int rv = r0 + 4 * h + (i >> 2) + 8 * half, f = 32 * nb + (l & 16) + 4 * (i & 3);
-        v_at[nb][half] = (ldsb)(buf + TR * KU * 16 + 16 * (rv * VU + ((f >> 3) ^ swizzle<VU>(rv))) + 2 * (f & 7));
+        v_at[nb][half] = (ldsb)(buf + kVBase + 16 * (rv * VU + ((f >> 3) ^ swizzle<VU>(rv))) + 2 * (f & 7));
       }
   }
   // K operand ks of 32-row block kb, V^T operand nb of the 16 rows st (in P's order) of a tile.
-  auto k_frag = [&](int bf, int kb, int ks) { return __builtin_bit_cast(uint4, *(ldsq)(k_at[ks] + bf * kTileBytes + kb * 32 * KU * 16)); };
+  auto k_frag = [&](int bf, int kb, int ks) { return __builtin_bit_cast(uint4, *(ldsq)(k_at[ks] + bf * kKBytes + kb * 32 * KU * 16)); };
   auto v_frag = [&](int bf, int st, int nb) {
-    const int at = bf * kTileBytes + st * 16 * VU * 16;
+    const int at = bf * kVBytes + st * 16 * VU * 16;
     const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(v_at[nb][0] + at)));
     const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(v_at[nb][1] + at)));
     return make_uint4(x.x, x.y, y.x, y.y);
@@ -307,10 +309,10 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
   float mx[kCols], arg0[kCols];
 #pragma unroll
   for (int k = 0; k < kCols; ++k) arg0[k] = kTileShift;
-  // Element i is row r0 + 32 kb + 8 (i / 4) + 4 h + i % 4 of tile ti.
-  auto finish_scores = [&](int ti, int kb) {
+  // Element i is row r0 + 32 kb + 8 (i / 4) + 4 h + i % 4 of tile ti, whose bias is in buffer bf.
+  auto finish_scores = [&](int ti, int kb, int bf) {
     const bool own = ti >= np;
-    const int bf = (ti - begin) & 1, t0 = TR * (own ? ti - np : ti), rows = min(TR, (own ? c.own : c.n) - t0);
+    const int t0 = TR * (own ? ti - np : ti), rows = min(TR, (own ? c.own : c.n) - t0);
     if constexpr (BIAS) {
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
@@ -380,7 +382,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
 #pragma unroll
     for (int k = 0; k < kCols; ++k) next[k] = mfma32<DT>(kf[ks % kHalf], c.qf[k][ks], next[k]);
   }
-  finish_scores(begin, 0);
+  finish_scores(begin, 0, 0);
 #pragma unroll
   for (int k = 0; k < kCols; ++k)
 #pragma unroll
@@ -389,9 +391,12 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
 #pragma unroll
   for (int ks = 0; ks < kHalf; ++ks) kf[ks] = k_frag(RB > 1 ? 0 : 1, RB > 1 ? 1 : 0, ks);
 
+  int k_cur = 0, v_cur = 0;   // the buffers of tile ti
   for (int ti = begin; ti < end; ++ti) {
-    const int it = ti - begin, bf = it & 1;
-    __syncthreads();   // V of tile ti and K of tile ti + 1 are stored, V of tile ti - 1 and K of tile ti have been read
+    const int it = ti - begin, k_next = Order::next_k(k_cur), v_next = Order::next_v(v_cur);
+    // V of tile ti and K of tile ti + 1 are stored; V of tile ti - 1 has been read, and K of the tile whose buffer
+    // tile ti + 2 takes (RB == 1: of tile ti, of which RB > 1 still reads the later blocks: of tile ti - 1).
+    __syncthreads();
     const int flags = flag_s[it % 3];
     if ((flags & 1) || (flags & 6) == 2) return false;
     if (tid == 0) flag_s[(it + 2) % 3] = 0;
@@ -399,7 +404,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
     for (int kb = 0; kb < RB; ++kb) {
       // 32 rows: their exponentials among the score products of the next 32, then their value products
       // among the maxima of those and, behind a tile's last rows, the staging of the next tiles. (Behind
-      // the share's last rows the scores are of what the buffer holds, and unused.)
+      // the share's last rows the scores are of what the buffer holds, if anything, and unused.)
       f32x16 s[kCols];
 #pragma unroll
       for (int k = 0; k < kCols; ++k) {
@@ -407,14 +412,14 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
 #pragma unroll
         for (int i = 0; i < 16; ++i) next[k][i] = 0.f;
       }
-      const int nbf = kb + 1 < RB ? bf : bf ^ 1, nkb = kb + 1 < RB ? kb + 1 : 0;
+      const int nbf = kb + 1 < RB ? k_cur : k_next, nkb = kb + 1 < RB ? kb + 1 : 0;
       uint4 vf[NDV];
       if constexpr (RB == 1) {
 #pragma unroll
         for (int ks = 0; ks < kHalf; ++ks) kf[ks] = k_frag(nbf, nkb, ks);
       }
 #pragma unroll
-      for (int nb = 0; nb < NDV; ++nb) vf[nb] = v_frag(bf, 2 * kb, nb);
+      for (int nb = 0; nb < NDV; ++nb) vf[nb] = v_frag(v_cur, 2 * kb, nb);
       uint32_t hi[kCols][2][4], lo[kCols][2][4];
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -438,7 +443,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
           __builtin_amdgcn_sched_barrier(0);
         }
       const bool last = kb + 1 == RB, stage_k = last && ti + 2 < end, stage_v = last && ti + 1 < end;
-      if (!last || ti + 1 < end) finish_scores(last ? ti + 1 : ti, nkb);
+      if (!last || ti + 1 < end) finish_scores(last ? ti + 1 : ti, nkb, nbf);
       constexpr int kSlots = 2 * NDV * kCols;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -451,7 +456,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
             c.o[k][nb] = mfma32<LOGKV_F16>(vf[nb], make_uint4(hi[k][st][0], hi[k][st][1], hi[k][st][2], hi[k][st][3]), c.o[k][nb]);
             if constexpr (!kHalfV)
               c.o[k][nb] = mfma32<LOGKV_F16>(vf[nb], make_uint4(lo[k][st][0], lo[k][st][1], lo[k][st][2], lo[k][st][3]), c.o[k][nb]);
-            if (k == kCols - 1 && st == 0) vf[nb] = v_frag(bf, 2 * kb + 1, nb);
+            if (k == kCols - 1 && st == 0) vf[nb] = v_frag(v_cur, 2 * kb + 1, nb);
             here(c.o[k][nb]);
 #pragma unroll
             for (int kk = 0; kk < kCols; ++kk) {
@@ -462,24 +467,26 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
             if constexpr (RB > 1) {
               // After (ti, 0) the products were of (ti, 1), the ones to come are of (ti + 1, 0); after (ti, 1),
               // of (ti + 1, 1).
-              if (j < kHalf) kf[j] = k_frag(bf ^ 1, kb, j);
+              if (j < kHalf) kf[j] = k_frag(k_next, kb, j);
             }
             if (stage_v) {
               constexpr int kStores = (kVTasks + kSlots - 1) / kSlots;
 #pragma unroll
-              for (int q = kStores * j; q < min(kStores * (j + 1), kVTasks); ++q) store_v(ti + 1, bf ^ 1, q);
+              for (int q = kStores * j; q < min(kStores * (j + 1), kVTasks); ++q) store_v(ti + 1, v_next, q);
             }
             __builtin_amdgcn_sched_barrier(0);
           }
       if (!last || ti + 1 < end) move_base();
       if (stage_k) {
 #pragma unroll
-        for (int q = 0; q < kKTasks; ++q) store_k(ti + 2, bf, q);
+        for (int q = 0; q < kKTasks; ++q) store_k(ti + Order::kAhead, Order::next_k(k_next), q);
       }
       if (stage_v) store_flags(ti + 1);
     }
     load_k(min(ti + 3, end - 1));
     load_v(min(ti + 2, end - 1));
+    k_cur = k_next;
+    v_cur = v_next;
   }
   return true;
 }
@@ -492,7 +499,7 @@ __device__ __forceinline__ void rows_tile_share2(const logkv_rows_args& a, const
                                                  uint8_t* buf, float (*bias_s)[32 * RB * NW / QW], int* flag_s) {
   typedef __attribute__((address_space(3))) s16x4* lds4;
   constexpr int kThreads = 64 * NW, RW = NW / QW, TR = 32 * RB * RW, KU = 2 * NKS, VU = 4 * NDV;
-  static_assert(NW * 16 * 32 * 4 <= TR * (KU + VU) * 16, "the second buffer holds 16 rows' probabilities of every wave");
+  static_assert(NW * 16 * 32 * 4 <= TR * (KU + VU) * 16, "a second tile's place holds 16 rows' probabilities of every wave");
   const int tid = threadIdx.x, w = wave_id(), l = lane_id(), h = l >> 5, col = l & 31, r0 = 32 * RB * (w / QW);
   uint4* ks_ = reinterpret_cast<uint4*>(buf);
   uint4* vs_ = reinterpret_cast<uint4*>(buf + TR * KU * 16);
@@ -640,10 +647,10 @@ __device__ __forceinline__ void rows_tile_share2(const logkv_rows_args& a, const
 template <int DT, int NKS, int NDV, int NW, int QW, int RB, bool BIAS, bool SECOND>
 __global__ __launch_bounds__(64 * NW, 2) void rows_tile_kernel(logkv_rows_args a, RowsLaunch r) {
   constexpr int kThreads = 64 * NW, RW = NW / QW, TR = 32 * RB * RW, kQueries = 32 * kCols;   // per wave
-  constexpr int kTileBytes = TR * (2 * NKS + 4 * NDV) * 16;
+  constexpr int kTileBytes = TR * 16 * (RowsSchedule<RB>::kKBuffers * 2 * NKS + RowsSchedule<RB>::kVBuffers * 4 * NDV);
   constexpr int kOutBytes = RW > 1 ? NW * kQueries * 32 * NDV * 4 : 0;
-  __shared__ __align__(16) uint8_t buf[2 * kTileBytes > kOutBytes ? 2 * kTileBytes : kOutBytes];
-  __shared__ __align__(16) float bias_s[BIAS ? 2 : 1][TR];
+  __shared__ __align__(16) uint8_t buf[kTileBytes > kOutBytes ? kTileBytes : kOutBytes];
+  __shared__ __align__(16) float bias_s[BIAS ? RowsSchedule<RB>::kKBuffers : 1][TR];
   __shared__ int flag_s[3];
   __shared__ float m_s[NW][kQueries], l_s[NW][kQueries];
   RowsBlock id = rows_block();
