@@ -258,11 +258,11 @@ RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws) {
   RowsLaunch r{};
   r.causal = causal ? 1 : 0;
   const int64_t tiles = (a.cap + kRowTile - 1) / kRowTile + (a.tq + kRowTile - 1) / kRowTile;
-  // More than 32 queries: tiles in LDS. From 17 on too where bf16 rows of more than 64 features are many: the streaming
+  // More than 32 queries: tiles in LDS. From 17 on too where rows of more than 64 features are many: the streaming
   // kernel's two query blocks spill there, and the tiled kernel pays a launch more. Streaming and tiled, 128 features, 8
-  // lanes of 32768 rows, 32 queries: 46.5 and 39.2 us; 64 lanes of 8192, 20: 74 and 58; 8 lanes of 2048, 24: 16 and 21.
-  // fp16's two products a step tip it the other way (74 and 81), as do 64 features (51 and 66).
-  const bool rows_pay = nq > 16 && a.dtype == LOGKV_BF16 && (a.dk > 64 || a.dv > 64) && lanes * a.cap >= 1 << 17;
+  // lanes of 32768 rows, 32 queries: 46.8 and 40.3 us (fp16: 46.4 and 39.8); 64 lanes of 8192, 20: 74.8 and 59.5 (74.4
+  // and 57.1); 8 lanes of 2048, 24: 16.3 and 19.2. At 64 features nothing spills: 64 lanes of 16000 rows, 30: 51 and 67.
+  const bool rows_pay = nq > 16 && (a.dk > 64 || a.dv > 64) && lanes * a.cap >= 1 << 17;
   if (!wide && (nq > 32 || rows_pay)) {
     r.q_waves = nq <= 64 ? 2 : nq <= 128 ? 4 : 8;
     r.shift = kTileShift;

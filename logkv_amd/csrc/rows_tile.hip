@@ -10,22 +10,20 @@
 // Bound by the vector unit beside the matrix cores: two waves a SIMD issue a vector operation every
 // 4.7 cycles (one wave: 8), and the exponentials, maxima and conversions of 32 rows take about as
 // long as their products. So two waves a SIMD, and in each the score products of the next 32 rows
-// are interleaved with the maxima and half of the exponentials of these, the value products with
-// the other half and with the staging of the next tile. 32768 rows of 128 features, 8 lanes of 512
+// are interleaved with the exponentials of these, the value products with half of the conversions,
+// the next maxima and the staging of the next tile. 32768 rows of 128 features, 8 lanes of 512
 // queries: 107 us, 645 TFLOP/s of the 1207 of a large matrix product (one wave a SIMD with 64
 // queries was slower: nothing hid its waits); 30720 rows and 2048 new ones, 8 lanes of 4096
 // queries: 700 us, 760 TFLOP/s.
 // Up to 64 queries: two blocks of four waves a CU (two waves of queries, two of rows): 64 lanes of
 // 8192 rows, 52 queries 80 us, in one block of eight waves 85.
-// bf16 caches: V enters the products as fp16, converted as it is staged (exact from 2^-17 up,
-// below that to 2^-25 absolute), and P as fp16 times 2^7 (11 bits): one product per step, a
-// third less matrix work than two bf16 parts of P, and P's error stays an eighth of the output's
-// rounding. A share with a tile whose largest magnitude is not in [2^-8, 2^16) is done again by a
-// second launch (in one kernel the second form's registers spilled in the first's loop, and a
-// reload there waits for every load ahead) in a second form: V as bf16, P as two parts. fp16
-// caches: P as two fp16 parts in both forms, since one part's rounding would equal the output's;
-// the second form is for infinities and NaNs in V, which it adds row by row for the queries that
-// see them. The second launch's blocks read a flag and end: 4.7 us.
+// P enters the value products as two parts of the cache's type (one part's rounding would equal the
+// output's), V as it is. For bf16, one fp16 part of P against V converted to fp16 was faster (a third
+// less matrix work: 64 tokens x 8 heads over 32768 rows 122 us the call against 139, 2048 tokens over
+// 30720 rows 1067 against 1189) but rounded P to 2^-11 and V below 2^-17 to 2^-25. A share with an infinity or NaN in V is done again by a second
+// launch (in one kernel the second form's registers spilled in the first's loop, and a reload there
+// waits for every load ahead) in a second form that adds such a tile row by row for the queries that
+// see its rows. The second launch's blocks read a flag and end: 4.7 us.
 // Rows are stored without padding, their 16-byte units permuted by row so that the operand reads
 // and the transposed reads meet every bank once. One barrier per tile, the following tiles' rows on
 // their way in registers; two buffers of V and, by RowsSchedule, two or three of K.
@@ -82,12 +80,6 @@ __device__ __forceinline__ int fresh(int x) {
 template <typename T>
 __device__ __forceinline__ void here(T& x) {
   asm volatile("" : "+v"(x));
-}
-
-// Two bf16 values as fp16, exact in the range above.
-__device__ __forceinline__ uint32_t half_of_bf16(uint32_t x) {
-  const f32x2 f = {__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)};
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, f16x2));
 }
 
 }  // namespace
@@ -185,7 +177,6 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
   constexpr int kKTasks = TR * KU / kThreads, kVTasks = TR * VU / kThreads;
   typedef RowsSchedule<RB> Order;
   constexpr int kKBytes = TR * KU * 16, kVBytes = TR * VU * 16, kVBase = Order::kKBuffers * kKBytes;
-  constexpr bool kHalfV = DT == LOGKV_BF16;            // V converted to fp16
   const int tid = threadIdx.x, l = lane_id(), h = l >> 5, col = l & 31, rw = wave_id() / QW;
   const int kunits = a.dk / 8, vunits = a.dv / 8, b = c.b, g = c.g, np = c.np, begin = c.begin, end = c.end;
   auto k_tile = [&](int bf) { return reinterpret_cast<uint4*>(buf + bf * kKBytes); };
@@ -242,21 +233,15 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
   auto store_v = [&](int ti, int bf, int q) {
     const int rr = vr0 + kThreads / VU * q, rows = rows_in(ti);
     if (rows < TR && rr >= rows) vx[q] = make_uint4(0, 0, 0, 0);
-    uint32_t x4[4] = {vx[q].x, vx[q].y, vx[q].z, vx[q].w};
+    const uint32_t x4[4] = {vx[q].x, vx[q].y, vx[q].z, vx[q].w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, x4[j] & 0x7fff7fffu));
-      if constexpr (kHalfV) x4[j] = half_of_bf16(x4[j]);
-    }
-    v_tile(bf)[rr * VU + (tid % VU ^ swizzle<VU>(rr))] = make_uint4(x4[0], x4[1], x4[2], x4[3]);
+    for (int j = 0; j < 4; ++j) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, x4[j] & 0x7fff7fffu));
+    v_tile(bf)[rr * VU + (tid % VU ^ swizzle<VU>(rr))] = vx[q];
   };
-  // Flags of tile ti's V: 1 some magnitude at 2^16 (fp16 caches: not finite) or above, 2 some nonzero,
-  // 4 some at 2^-8 or above.
+  // Whether tile ti's V holds an infinity or NaN.
   auto store_flags = [&](int ti) {
-    const int mag = max(static_cast<int>(top[0]), static_cast<int>(top[1]));
-    constexpr int kMost = kHalfV ? (127 + 16) << 7 : static_cast<int>(Elem<DT>::kInf), kLeast = (127 - 8) << 7;
-    const int bits = (__ballot(mag >= kMost) ? 1 : 0) | (kHalfV ? (__ballot(mag != 0) ? 2 : 0) | (__ballot(mag >= kLeast) ? 4 : 0) : 0);
-    if (bits && l == 0) atomicOr(&flag_s[(ti - begin) % 3], bits);
+    const bool odd = __ballot(top[0] >= Elem<DT>::kInf || top[1] >= Elem<DT>::kInf) != 0;
+    if (odd && l == 0) flag_s[(ti - begin) % 3] = 1;
     top = u16x2{0, 0};
   };
   clear_sums(c);
@@ -278,27 +263,21 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
   load_k(min(begin + 2, end - 1));
   load_v(min(begin + 1, end - 1));
 
-  // LDS addresses of this lane's operands in buffer 0: K of its row (unit 2 ks + h), V of its
-  // transposed reads (features 32 nb + l % 32 of rows 4 h .. and 8 + 4 h ..).
-  ldsb k_at[NKS], v_at[NDV][2];
-  {
-    const int rr = r0 + col, i = l & 15;
-#pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) k_at[ks] = (ldsb)(buf + 16 * (rr * KU + ((2 * ks + h) ^ swizzle<KU>(rr))));
-#pragma unroll
-    for (int nb = 0; nb < NDV; ++nb)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int rv = r0 + 4 * h + (i >> 2) + 8 * half, f = 32 * nb + (l & 16) + 4 * (i & 3);
-        v_at[nb][half] = (ldsb)(buf + kVBase + 16 * (rv * VU + ((f >> 3) ^ swizzle<VU>(rv))) + 2 * (f & 7));
-      }
-  }
+  // LDS addresses of this lane's operands in buffer 0: unit h of K's row r0 + l % 32, and of V's transposed reads
+  // features l & 16 .. of rows 4 h .. (8 + 4 h .. behind). Other units are reached by exclusive or: the permutation is
+  // one, rows begin at multiples of their length, and row + 8 has the permutation's second bit the other way round.
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((ldsb)buf));
+  const int rk = r0 + col, i16 = l & 15, rv = r0 + 4 * h + (i16 >> 2), f = (l & 16) + 4 * (i16 & 3);
+  const uint32_t k_at = lds0 + 16 * (rk * KU + (h ^ swizzle<KU>(rk)));
+  const uint32_t v_at = lds0 + kVBase + 16 * (rv * VU + ((f >> 3) ^ swizzle<VU>(rv))) + 2 * (f & 7);
   // K operand ks of 32-row block kb, V^T operand nb of the 16 rows st (in P's order) of a tile.
-  auto k_frag = [&](int bf, int kb, int ks) { return __builtin_bit_cast(uint4, *(ldsq)(k_at[ks] + bf * kKBytes + kb * 32 * KU * 16)); };
+  auto k_frag = [&](int bf, int kb, int ks) {
+    return __builtin_bit_cast(uint4, *(ldsq)(uintptr_t)(((k_at + bf * kKBytes) ^ (32 * ks)) + kb * 32 * KU * 16));
+  };
   auto v_frag = [&](int bf, int st, int nb) {
-    const int at = bf * kVBytes + st * 16 * VU * 16;
-    const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(v_at[nb][0] + at)));
-    const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(v_at[nb][1] + at)));
+    const uint32_t at = v_at + bf * kVBytes;
+    const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)((at ^ (64 * nb)) + st * 16 * VU * 16)));
+    const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)((at ^ (64 * nb + 32)) + (st * 16 + 8) * VU * 16)));
     return make_uint4(x.x, x.y, y.x, y.y);
   };
   // Scores of the next 32 rows, then with their bias and masks; the first half of their products'
@@ -397,13 +376,13 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
     // V of tile ti and K of tile ti + 1 are stored; V of tile ti - 1 has been read, and K of the tile whose buffer
     // tile ti + 2 takes (RB == 1: of tile ti, of which RB > 1 still reads the later blocks: of tile ti - 1).
     __syncthreads();
-    const int flags = flag_s[it % 3];
-    if ((flags & 1) || (flags & 6) == 2) return false;
+    if (flag_s[it % 3]) return false;
     if (tid == 0) flag_s[(it + 2) % 3] = 0;
 #pragma unroll
     for (int kb = 0; kb < RB; ++kb) {
-      // 32 rows: their exponentials among the score products of the next 32, then their value products
-      // among the maxima of those and, behind a tile's last rows, the staging of the next tiles. (Behind
+      // 32 rows: their exponentials and the first 16 rows' parts among the score products of the next 32,
+      // then their value products among the other parts, the maxima of those and, behind a tile's last
+      // rows, the staging of the next tiles. (Behind
       // the share's last rows the scores are of what the buffer holds, if anything, and unused.)
       f32x16 s[kCols];
 #pragma unroll
@@ -420,7 +399,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
       }
 #pragma unroll
       for (int nb = 0; nb < NDV; ++nb) vf[nb] = v_frag(v_cur, 2 * kb, nb);
-      uint32_t hi[kCols][2][4], lo[kCols][2][4];
+      uint32_t hi[kCols][4], lo[kCols][4], hi1[kCols][4], lo1[kCols][4];   // P of the first and the second 16 rows
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int ks = 0; ks < NKS; ++ks)
@@ -435,9 +414,13 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
             const float p1 = __builtin_amdgcn_exp2f(BIAS ? s[k][i + 1] + arg0[k] : __builtin_fmaf(s[k][i + 1], c2, arg0[k]));
             c.lsum[k] += p0;
             c.lsum[k] += p1;
-            if constexpr (kHalfV) hi[k][i / 8][i / 2 % 4] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{p0, p1}, f16x2));
-            else Elem<DT>::parts(p0, p1, hi[k][i / 8][i / 2 % 4], lo[k][i / 8][i / 2 % 4]);
-            here(hi[k][i / 8][i / 2 % 4]);
+            if (i < 8) {
+              Elem<DT>::parts(p0, p1, hi[k][i / 2], lo[k][i / 2]);
+              here(hi[k][i / 2]);
+            } else {
+              s[k][i] = p0;
+              s[k][i + 1] = p1;
+            }
             here(c.lsum[k]);
           }
           __builtin_amdgcn_sched_barrier(0);
@@ -453,9 +436,18 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
 #pragma unroll
           for (int k = 0; k < kCols; ++k) {
             const int j = (st * NDV + nb) * kCols + k;
-            c.o[k][nb] = mfma32<LOGKV_F16>(vf[nb], make_uint4(hi[k][st][0], hi[k][st][1], hi[k][st][2], hi[k][st][3]), c.o[k][nb]);
-            if constexpr (!kHalfV)
-              c.o[k][nb] = mfma32<LOGKV_F16>(vf[nb], make_uint4(lo[k][st][0], lo[k][st][1], lo[k][st][2], lo[k][st][3]), c.o[k][nb]);
+            c.o[k][nb] = mfma32<DT>(vf[nb], st ? make_uint4(hi1[k][0], hi1[k][1], hi1[k][2], hi1[k][3]) : make_uint4(hi[k][0], hi[k][1], hi[k][2], hi[k][3]), c.o[k][nb]);
+            if (st == 0) {
+              // The second 16 rows' parts among the first ones' products.
+#pragma unroll
+              for (int i = 4 / NDV * nb; i < 4 / NDV * (nb + 1); ++i) {
+                Elem<DT>::parts(s[k][8 + 2 * i], s[k][9 + 2 * i], hi1[k][i], lo1[k][i]);
+                here(hi1[k][i]);
+                here(lo1[k][i]);
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+            c.o[k][nb] = mfma32<DT>(vf[nb], st ? make_uint4(lo1[k][0], lo1[k][1], lo1[k][2], lo1[k][3]) : make_uint4(lo[k][0], lo[k][1], lo[k][2], lo[k][3]), c.o[k][nb]);
             if (k == kCols - 1 && st == 0) vf[nb] = v_frag(v_cur, 2 * kb + 1, nb);
             here(c.o[k][nb]);
 #pragma unroll
@@ -491,9 +483,8 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
   return true;
 }
 
-// The same in the second form: V in its own type, P as two parts of that type, and a tile that is not
-// finite row by row in float32, each row for the queries that see it. Plain steps (one buffer, nothing
-// ahead): shares that need it are rare.
+// The same in the second form: a tile that is not finite row by row in float32, each row for the
+// queries that see it. Plain steps (one buffer, nothing ahead): shares that need it are rare.
 template <int DT, int NKS, int NDV, int NW, int QW, int RB, bool BIAS>
 __device__ __forceinline__ void rows_tile_share2(const logkv_rows_args& a, const RowsLaunch& r, RowsShare<NKS, NDV>& c,
                                                  uint8_t* buf, float (*bias_s)[32 * RB * NW / QW], int* flag_s) {
@@ -649,7 +640,7 @@ __global__ __launch_bounds__(64 * NW, 2) void rows_tile_kernel(logkv_rows_args a
   constexpr int kThreads = 64 * NW, RW = NW / QW, TR = 32 * RB * RW, kQueries = 32 * kCols;   // per wave
   constexpr int kTileBytes = TR * 16 * (RowsSchedule<RB>::kKBuffers * 2 * NKS + RowsSchedule<RB>::kVBuffers * 4 * NDV);
   constexpr int kOutBytes = RW > 1 ? NW * kQueries * 32 * NDV * 4 : 0;
-  __shared__ __align__(16) uint8_t buf[kTileBytes > kOutBytes ? kTileBytes : kOutBytes];
+  __shared__ __align__(256) uint8_t buf[kTileBytes > kOutBytes ? kTileBytes : kOutBytes];
   __shared__ __align__(16) float bias_s[BIAS ? RowsSchedule<RB>::kKBuffers : 1][TR];
   __shared__ int flag_s[3];
   __shared__ float m_s[NW][kQueries], l_s[NW][kQueries];
