@@ -60,6 +60,7 @@ __device__ __forceinline__ float bias_base2(float x) {
   return __builtin_isinf(y) && !__builtin_isinf(x) ? __builtin_copysignf(3.402823466e38f, x) : y;
 }
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -81,12 +82,11 @@ struct Elem<LOGKV_BF16> {
   }
   static __device__ __forceinline__ uint16_t from_f32(float f) { return f32_to_bf16(f); }
   static __device__ __forceinline__ float to_f32(uint16_t u) { return bf16_to_f32(u); }
-  // x0, x1 (not negative) as two packed parts: the leading 8 bits and the next 8, both cut.
+  // Two packed parts, each rounded to nearest: 8 and 8 bits. (Cut ones would bias the sums against the divisor's.)
   static __device__ __forceinline__ void parts(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-    const uint32_t u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
-    hi = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
-    const float r0 = x0 - __uint_as_float(u0 & 0xffff0000u), r1 = x1 - __uint_as_float(u1 & 0xffff0000u);
-    lo = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302u);
+    hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x0, x1}, bf16x2));
+    const f32x2 r = {x0 - __uint_as_float(hi << 16), x1 - __uint_as_float(hi & 0xffff0000u)};
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
   }
 };
 template <>
