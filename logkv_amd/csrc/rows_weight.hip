@@ -84,10 +84,13 @@ __global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_arg
     qp[k] = gp(a.q) + b * a.q_sb + (g * rep + qq / a.tq) * a.q_sh + pos[k] * a.q_st + 8 * unit;
   }
   int my_t = tid % a.tq;   // of query tid of the tile (tid < kQueries)
+  // A key's position for the masks: the cache's rows are before every query.
+  const int key0 = of_cache ? 0 : k0 + col, key_step = of_cache ? 0 : 32;
   uint4 qx[kTasks];
   float lx = 0.f;
   int tx = 0;
-  // Queries past the row's tokens see nothing (L = +inf, probabilities 2^-inf) and are stored as zeros.
+  // Queries past nq or the row's tokens are stored as zeros before every key (position -1): L = +inf alone would not
+  // do, since a key's infinity times zero is NaN.
   auto load = [&](int q0) {
 #pragma unroll
     for (int k = 0; k < kTasks; ++k) {
@@ -101,7 +104,7 @@ __global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_arg
       }
     }
     if (tid < kQueries) lx = q0 + tid < nq ? lse[q0 + tid] : __builtin_inff();
-    tx = my_t;
+    tx = q0 + tid < nq && my_t < own ? my_t : -1;
     my_t += step_t;
     if (my_t >= a.tq) my_t -= a.tq;
   };
@@ -137,8 +140,8 @@ __global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_arg
       const int qq = 32 * qb + col;
       return q_s[bf][qq * KU + ((2 * ks + h) ^ swizzle<KU>(qq))];
     };
-    auto tile = [&](auto own_tag) {
-      constexpr bool OWN = decltype(own_tag)::value;
+    auto tile = [&](auto mask_tag) {
+      constexpr bool MASK = decltype(mask_tag)::value;
       constexpr int kBlocks = kQueries / 32 * KB / QG, kShare = 16 / NKS;   // 32x32 blocks; exponentials per product
       uint4 qa[NKS];
 #pragma unroll
@@ -156,7 +159,7 @@ __global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_arg
 #pragma unroll
           for (int i4 = 0; i4 < 4; ++i4) {
             x[i4] = *reinterpret_cast<const f32x4*>(&l_s[bf][32 * (q_block + (blk - 1) / KB) + 8 * i4 + 4 * h]);
-            if constexpr (OWN) t[i4] = *reinterpret_cast<const i32x4*>(&t_s[bf][32 * (q_block + (blk - 1) / KB) + 8 * i4 + 4 * h]);
+            if constexpr (MASK) t[i4] = *reinterpret_cast<const i32x4*>(&t_s[bf][32 * (q_block + (blk - 1) / KB) + 8 * i4 + 4 * h]);
           }
         }
 #pragma unroll
@@ -172,7 +175,7 @@ __global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_arg
 #pragma unroll
             for (int i = kShare * ks; i < kShare * (ks + 1); ++i) {
               float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c2, -x[i / 4][i % 4]));
-              if (OWN && k0 + 32 * ((blk - 1) % KB) + col > t[i / 4][i % 4]) p = 0.f;
+              if (MASK && key0 + key_step * ((blk - 1) % KB) > t[i / 4][i % 4]) p = 0.f;
               sum[(blk - 1) % KB] += p;
             }
           }
@@ -180,7 +183,8 @@ __global__ __launch_bounds__(kThreads, 2) void rows_weight_kernel(logkv_rows_arg
         }
       }
     };
-    if (of_cache) tile(std::false_type{});
+    // Against the cache's rows only padding is masked: past the last query, or in a padded batch.
+    if (of_cache && own == a.tq && kQueries * (it + 1) <= nq) tile(std::false_type{});
     else if (!none) tile(std::true_type{});
     if (it + 1 < tiles) {
       store(bf ^ 1);
