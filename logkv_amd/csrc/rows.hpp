@@ -60,6 +60,20 @@ __device__ __forceinline__ float bias_base2(float x) {
   return __builtin_isinf(y) && !__builtin_isinf(x) ? __builtin_copysignf(3.402823466e38f, x) : y;
 }
 
+// What is added to a base-2 logit so that the largest of them, y(mx), has the exponent `shift`: shift - m, for m the
+// rounded maximum. Where m is beyond 2^22 that sum rounds, and so did m: fp16 probabilities would pass their range (a
+// bias of -1e8 leaves spacings of 16, and 15 + 1e8 rounds up to 2^16), so the offset goes down as far.
+template <bool BIAS>
+__device__ __forceinline__ float exponent_offset(float shift, float m, float mx, float c2) {
+  float off = shift - m;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {   // a step of off is at least half of both roundings
+    if ((BIAS ? mx + off : __builtin_fmaf(mx, c2, off)) > shift + 0.5f)
+      off = __uint_as_float(__float_as_uint(off) + (off > 0.f ? -1 : 1));
+  }
+  return off;
+}
+
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));

@@ -238,7 +238,7 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
         seen[c] |= __shfl_xor(seen[c], 16, kWave);
         seen[c] |= __shfl_xor(seen[c], 32, kWave);
       }
-      const float arg0 = E::kShift - mb;
+      const float arg0 = exponent_offset<BIAS>(E::kShift, mb, mx, c2);
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {

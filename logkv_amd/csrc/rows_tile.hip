@@ -329,13 +329,14 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
   // The sums' base moves when a maximum passes it by more than 2^8 (P stays below 2^(8 + kTileShift)):
   // a few times a share instead of at every new maximum.
   auto move_base = [&]() {
-    float y[kCols];
+    float x[kCols], y[kCols];
     bool past = false;
 #pragma unroll
     for (int k = 0; k < kCols; ++k) {
-      const float x = pair_max32(mx[k]);
-      y[k] = BIAS ? x : x * c2;
-      past |= y[k] > c.m[k] + 8.f;
+      x[k] = pair_max32(mx[k]);
+      y[k] = BIAS ? x[k] : x[k] * c2;
+      // The difference, since a sum rounds beside a large maximum; and the exponent as it will be formed.
+      past |= y[k] - c.m[k] > 8.f || (BIAS ? x[k] + arg0[k] : __builtin_fmaf(x[k], c2, arg0[k])) > kTileShift + 8.5f;
     }
     if (!__ballot(past)) return;
 #pragma unroll
@@ -343,7 +344,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
       const float m_new = fmaxf(c.m[k], y[k]), mb = m_new == -__builtin_inff() ? 0.f : m_new;
       const float corr = __builtin_amdgcn_exp2f(c.m[k] - mb);
       c.m[k] = m_new;
-      arg0[k] = kTileShift - mb;
+      arg0[k] = exponent_offset<BIAS>(kTileShift, mb, x[k], c2);
       c.lsum[k] *= corr;
 #pragma unroll
       for (int nb = 0; nb < NDV; ++nb)
@@ -573,6 +574,7 @@ __device__ __forceinline__ void rows_tile_share2(const logkv_rows_args& a, const
         mx = pair_max32(mx);
         const float m_new = fmaxf(c.m[k], BIAS ? mx : mx * c2);
         const float mb = m_new == -__builtin_inff() ? 0.f : m_new, corr = __builtin_amdgcn_exp2f(c.m[k] - mb);
+        const float arg0 = exponent_offset<BIAS>(kTileShift, mb, mx, c2);
         c.m[k] = m_new;
         c.lsum[k] *= corr;
 #pragma unroll
@@ -581,7 +583,7 @@ __device__ __forceinline__ void rows_tile_share2(const logkv_rows_args& a, const
           for (int i = 0; i < 16; ++i) c.o[k][nb][i] *= corr;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          s[i] = __builtin_amdgcn_exp2f(BIAS ? s[i] + (kTileShift - mb) : __builtin_fmaf(s[i], c2, kTileShift - mb));
+          s[i] = __builtin_amdgcn_exp2f(BIAS ? s[i] + arg0 : __builtin_fmaf(s[i], c2, arg0));
           c.lsum[k] += s[i];
         }
 #pragma unroll
