@@ -26,9 +26,9 @@ enum { LOGKV_BF16 = 0, LOGKV_F16 = 1 };
  * [n_batch, n_groups, tq, dk / dv] (one per query position), head h reading KV group
  * h / (n_heads / n_groups):
  *
- *   s_j = scale q . cache_k_j + bias_j          for j < n_b
- *   s_r = scale q . k_r                         for the own rows r that the query sees
- *   out = softmax(s) [cache_v; v]               (zeros where a query sees no row)
+ *   s_j = scale q . cache_k_j + bias_scale bias_j   for j < n_b
+ *   s_r = scale q . k_r                             for the own rows r that the query sees
+ *   out = softmax(s) [cache_v; v]                   (zeros where a query sees no row)
  *
  * n_b = lengths[b * len_stride] + *lengths2 + len_add (absent pointers count as 0), held to
  * [0, cap]. A NaN or infinity in a row that a query does not see does not reach its output.
@@ -36,7 +36,8 @@ enum { LOGKV_BF16 = 0, LOGKV_F16 = 1 };
  * probabilities enter the value products as two parts of 8 (bf16) or 11 (fp16) bits each.
  * dk, dv: multiples of 8 up to 256; every row 16-byte aligned (strides multiples of 8); features
  * contiguous. bias (tree attention): float32, or dtype with bias_half, strided; NULL for none;
- * -inf hides a row.
+ * -inf hides a row. bias_scale: a positive factor, 0 for 1. Where float32 holds the logits in steps
+ * of 1 or more (beyond 2^22), an output is still a mean of values, but weights are not kept to it.
  * visible (tree attention): uint8 [tq, tq] per batch row (vis_sb 0: one for all), rows vis_st
  * apart: own row r is seen by query t where visible[t, r] is not 0.
  * counts (weight attention, optional): int32 [n_batch]; only the first counts[b] queries and own
@@ -66,7 +67,7 @@ typedef struct logkv_rows_args {
   int64_t o_sb, o_sh, o_st;
   int32_t n_batch, n_heads, n_groups, tq, cap, dk, dv, dtype;
   int32_t len_stride, len_add, bias_half;
-  float scale;
+  float scale, bias_scale;
 } logkv_rows_args;
 
 /* Scratch of one call of either attention below. */

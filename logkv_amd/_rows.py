@@ -25,7 +25,7 @@ class RowsArgs(C.Structure):
         ("out", _p), ("o_sb", _i64), ("o_sh", _i64), ("o_st", _i64),
         ("n_batch", _i32), ("n_heads", _i32), ("n_groups", _i32), ("tq", _i32), ("cap", _i32), ("dk", _i32),
         ("dv", _i32), ("dtype", _i32), ("len_stride", _i32), ("len_add", _i32), ("bias_half", _i32),
-        ("scale", C.c_float),
+        ("scale", C.c_float), ("bias_scale", C.c_float),
     ]
 
 

@@ -856,6 +856,8 @@ int check_rows(const logkv_rows_args* a, const void* ws, int64_t ws_bytes, bool 
   if (reinterpret_cast<uintptr_t>(a->out) % 8 || a->o_sb % 4 || a->o_sh % 4 || a->o_st % 4)
     return fail(LOGKV_EINVAL, "row attention output rows must be 8-byte aligned");
   if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return fail(LOGKV_EINVAL, "attention scale must be positive");
+  if (!(a->bias_scale >= 0.f) || !std::isfinite(a->bias_scale))
+    return fail(LOGKV_EINVAL, "attention bias_scale must be positive, or 0 for 1");
   if (weights ? !a->weights || a->visible || a->bias : !a->visible || a->weights || a->counts)
     return fail(LOGKV_EINVAL, weights ? "weight attention takes weights, no bias and no mask"
                                       : "tree attention takes a mask of the own rows, no weights and no counts");

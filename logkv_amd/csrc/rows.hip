@@ -257,6 +257,7 @@ RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws) {
   const bool wide = a.dk > 128 || a.dv > 128;
   RowsLaunch r{};
   r.causal = causal ? 1 : 0;
+  r.bias2 = (a.bias_scale == 0.f ? 1.f : a.bias_scale) * kLog2e;
   const int64_t tiles = (a.cap + kRowTile - 1) / kRowTile + (a.tq + kRowTile - 1) / kRowTile;
   // More than 32 queries: tiles in LDS. From 17 on too where rows of more than 64 features are many: the streaming
   // kernel's two query blocks spill there, and the tiled kernel pays a launch more. Streaming and tiled, 128 features, 8

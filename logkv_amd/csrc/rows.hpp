@@ -32,6 +32,7 @@ struct RowsLaunch {
   int cols;       // streamed kernel: 16-query column blocks per wave
   int q_waves;    // tiled kernel: waves with 32 queries each (0: the streamed kernel)
   float shift;    // the partials' sums carry 2^shift
+  float bias2;    // bias to base-2 logits: bias_scale log2(e)
   int causal;     // weight attention; otherwise the visible mask
 };
 
@@ -55,8 +56,8 @@ __device__ __forceinline__ int own_rows(const logkv_rows_args& a, int b) {
 
 // A bias in base 2. A finite one stays finite (a mask of the type's lowest value hides a row only
 // beside larger logits).
-__device__ __forceinline__ float bias_base2(float x) {
-  const float y = x * kLog2e;
+__device__ __forceinline__ float bias_base2(float x, float bias2) {
+  const float y = x * bias2;
   return __builtin_isinf(y) && !__builtin_isinf(x) ? __builtin_copysignf(3.402823466e38f, x) : y;
 }
 

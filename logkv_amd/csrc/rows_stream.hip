@@ -112,7 +112,7 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
           const int64_t at = b * a.b_sb + g * a.b_sg + (t0 + rr) * a.b_st;
           const float x = a.bias_half ? E::to_f32(gp(static_cast<const uint16_t*>(a.bias))[at])
                                       : gp(static_cast<const float*>(a.bias))[at];
-          bx[j] = bias_base2(x);
+          bx[j] = bias_base2(x, r.bias2);
         }
       }
     }

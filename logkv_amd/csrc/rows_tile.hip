@@ -224,7 +224,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
     if constexpr (BIAS) {
       if (q == 0 && tid < TR) {
         const float x = a.bias_half ? Elem<DT>::to_f32(bx[0]) : __uint_as_float(bx[0] | static_cast<uint32_t>(bx[1]) << 16);
-        bias_s[bf][tid] = ti < np ? bias_base2(x) : 0.f;
+        bias_s[bf][tid] = ti < np ? bias_base2(x, r.bias2) : 0.f;
       }
     }
   };
@@ -533,7 +533,7 @@ __device__ __forceinline__ void rows_tile_share2(const logkv_rows_args& a, const
         if (!own) {
           const int64_t at = c.b * a.b_sb + c.g * a.b_sg + (t0 + min(tid, rows - 1)) * a.b_st;
           x = bias_base2(a.bias_half ? Elem<DT>::to_f32(gp(static_cast<const uint16_t*>(a.bias))[at])
-                                     : gp(static_cast<const float*>(a.bias))[at]);
+                                     : gp(static_cast<const float*>(a.bias))[at], r.bias2);
         }
         bias_s[0][tid] = x;
       }

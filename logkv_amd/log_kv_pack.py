@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from functools import lru_cache
 
 import torch
 
@@ -196,6 +197,7 @@ class _PackMidKV(torch.autograd.Function):
         return gk, gv, None, None, None
 
 
+@lru_cache(maxsize=64)
 def _inv_scale_bf16(scale: float) -> float:
     return torch.tensor(1.0 / scale, dtype=torch.float32).to(torch.bfloat16).item()
 
@@ -214,7 +216,7 @@ def packed_attention(q, ka, va, plan, tail, scale, causal_tail, v_dim, n_groups,
         raise ValueError("packed K/V must be contiguous and of one shape")
     out = q.new_empty(bt, hq, tq, v_dim)
     args = AttentionArgs(ptr(q), *q.stride()[:3], bt, hq, n_groups, tq, dk, v_dim, ka.size(3), ptr(ka), ptr(va),
-                         ka.size(2), tail, causal_tail, float(scale), _inv_scale_bf16(scale), ptr(out),
+                         ka.size(2), tail, causal_tail, float(scale), _inv_scale_bf16(float(scale)), ptr(out),
                          *out.stride()[:3], ptr(alpha_count_dev))
     if (hq // n_groups) * tq > 16:
         # Many query rows per KV group: the matrix-core chunk kernel.
@@ -250,7 +252,7 @@ def packed_attention_backward(q, ka, va, out, dout, plan, tail, scale, causal_ta
     gk = q.new_empty(bt, n_groups, grad_rows, dk)
     gv = q.new_empty(bt, n_groups, grad_rows, v_dim)
     args = AttentionArgs(ptr(q), *q.stride()[:3], bt, hq, n_groups, tq, dk, v_dim, ka.size(3), ptr(ka), ptr(va),
-                         ka.size(2), tail, causal_tail, float(scale), _inv_scale_bf16(scale), ptr(out),
+                         ka.size(2), tail, causal_tail, float(scale), _inv_scale_bf16(float(scale)), ptr(out),
                          *out.stride()[:3], ptr(alpha_count_dev))
     grads = AttentionGradArgs(ptr(dout), *dout.stride()[:3], ptr(dq), *dq.stride()[:3], ptr(gk), ptr(gv), grad_rows)
     need = int(lib().logkv_chunk_backward_workspace_bytes(C.byref(args)))
@@ -375,8 +377,9 @@ def log_kv_draft_attention(cache, q, k, v, visible, scale, *, pending=None):
 
     ``q [B, n_heads, T, k_dim]``, ``k / v [B, G, T, .]`` post-RoPE at the tokens' depths; ``visible`` (bool, ``[T, T]``
     or ``[B, T, T]``) gives the drafted rows that each token sees, its ancestors and itself; ``pending`` is an optional
-    ``(k, v)`` of one attended but uncommitted row, which every token sees. A slot's logit is ``scale * q.k + log w``
-    with its log-mass as packed. The packed prefix is shared with ``log_kv_chunk_attention(reuse_prefix=True)``."""
+    ``(k, v)`` of one attended but uncommitted row, which every token sees. A slot's logit is a call's,
+    ``scale * (q.k + bf16(1 / scale) * log w)`` with its log-mass as packed, and the packed prefix is shared with
+    ``log_kv_chunk_attention(reuse_prefix=True)``."""
     if not cache.semantic_clusters or cache.semantic_anchor_mode != "mid":
         raise NotImplementedError("logkv_amd reads out the first-order mid-anchor path (second_order_scale=0)")
     _check_backend(cache.semantic_pack_backend)
@@ -390,7 +393,9 @@ def log_kv_draft_attention(cache, q, k, v, visible, scale, *, pending=None):
         raise ValueError("at most one token can be pending")
     if q.ndim != 4 or q.size(0) != cache.batch_size or q.device != k.device:
         raise ValueError("queries must be [B, n_heads, T, k_dim] on the cache's device")
-    visible = _tree(visible, q, k)
+    visible, scale = _tree(visible, q, k), float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError("attention scale must be positive")
     dim = packed_dim(cache.k_dim, cache.v_dim)
     with torch.no_grad():
         key, plan, (ka, va), workspace = _pack_prefix(cache, readout_view(cache), pk, pv, dim, True)
@@ -399,8 +404,9 @@ def log_kv_draft_attention(cache, q, k, v, visible, scale, *, pending=None):
         # The plan's width and the exact pool's rows are read on the device.
         in_use = (plan.table[-1:].data_ptr(), 0, cache.alpha_count_dev.data_ptr() if cache.alpha_exact_tokens else 0,
                   recent + pk.size(2))
-        return _attention(q, k, v, ka[..., :cache.k_dim], va[..., :cache.v_dim], float(scale), None, 0,
-                          bias=ka[..., cache.k_dim], visible=visible, in_use=in_use)
+        return _attention(q, k, v, ka[..., :cache.k_dim], va[..., :cache.v_dim], scale, None, 0,
+                          bias=ka[..., cache.k_dim], visible=visible, in_use=in_use,
+                          bias_scale=scale * _inv_scale_bf16(scale))
 
 
 def attention_state(cache, plan):

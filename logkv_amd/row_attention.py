@@ -94,9 +94,9 @@ def _workspace_bytes(weights, batch, heads, groups, tq, cap, dk, dv, dtype):
 
 
 def _attention(q, k, v, cache_k, cache_v, scale, lengths, room, *, bias=None, visible=None, counts=None, weights=None,
-               in_use=None):
+               in_use=None, bias_scale=1.0):
     """Checks and launch of both attentions. ``in_use`` in place of ``lengths``: (address, stride) of device counts
-    per batch row, a second count's address (0: none) and rows to add to both."""
+    per batch row, a second count's address (0: none) and rows to add to both. ``bias_scale``: a factor of the bias."""
     if not q.ndim == k.ndim == v.ndim == cache_k.ndim == cache_v.ndim == 4:
         raise ValueError("queries, rows and cache must be 4-dimensional")
     batch, heads, tq, dk = q.shape
@@ -156,7 +156,7 @@ def _attention(q, k, v, cache_k, cache_v, scale, lengths, room, *, bias=None, vi
         qp, *q_st[:3], kp, *k_st[:3], vp, *v_st[:3], ck, ck_sb, ck_sg, ck_st, cv, cv_sb, cv_sg, cv_st,
         b_ptr, *b_st, n_ptr, n2_ptr, vis_ptr, vis_sb, vis_st,
         0 if counts is None else counts.data_ptr(), w_ptr, w_sb, w_sg, out.data_ptr(), heads * o_sh, o_sh, dv,
-        batch, heads, groups, tq, cap, dk, dv, code, n_st, len_add, b_half, scale)
+        batch, heads, groups, tq, cap, dk, dv, code, n_st, len_add, b_half, scale, bias_scale)
     handle = rows_lib()
     if weights is None:
         _launch(handle.logkv_tree_attention, "logkv_tree_attention", index, args, workspace.data_ptr(), need)
