@@ -6,9 +6,13 @@ counterpart in the reference, whose dense cache grows with the sequence.
 
 from __future__ import annotations
 
+import math
+
 import torch
 
-from .row_attention import EvictedRows, log_kv_evict, log_kv_tree_attention, log_kv_weight_attention
+from ._lib import check_activation_dtype
+from .row_attention import (_ROW_DTYPES, EvictedRows, _workspace_bytes, log_kv_evict, log_kv_tree_attention,
+                            log_kv_weight_attention)
 
 
 class EvictingKVCache:
@@ -19,12 +23,12 @@ class EvictingKVCache:
     to its last ``recent`` rows and, up to ``budget`` in all, its others of largest weight. ``cache.draft(q, k, v,
     visible)`` attends a tree of drafted tokens without a change: commit the accepted ones with a call.
 
-    Calls longer than ``block`` tokens run in blocks (an eviction may fall between them). ``lengths`` (int32 ``[batch]``,
-    on the device) are the rows in use; the host keeps only an upper bound of them and never waits. Eviction copies into
-    a second set of buffers, which swaps with the first. Keys are kept as given, post-RoPE at the tokens' own positions;
-    with ``track_positions`` the ordinal of each row's token stands in ``positions`` (int64 ``[batch, n_groups,
-    capacity]``). Its calls cannot be captured into a HIP graph: the host's bound decides when to evict, and eviction
-    swaps the buffers."""
+    Calls longer than ``block`` tokens run in blocks (an eviction may fall between them); a refused call leaves the
+    cache as it was. ``lengths`` (int32 ``[batch]``, on the device) are the rows in use; the host keeps only an upper
+    bound of them and never waits. Eviction copies into a second set of buffers, which swaps with the first. Keys are
+    kept as given, post-RoPE at the tokens' own positions; with ``track_positions`` the ordinal of each row's token
+    stands in ``positions`` (int64 ``[batch, n_groups, capacity]``). Its calls cannot be captured into a HIP graph: the
+    host's bound decides when to evict, and eviction swaps the buffers."""
 
     def __init__(self, batch_size: int, n_groups: int, k_dim: int, v_dim: int, budget: int, *, scale: float,
                  recent: int | None = None, block: int | None = None, dtype=torch.bfloat16, device="cuda",
@@ -33,8 +37,11 @@ class EvictingKVCache:
         block = max(1, budget // 4) if block is None else block
         if min(batch_size, n_groups, k_dim, v_dim, budget, block) < 1 or not 0 <= recent <= budget:
             raise ValueError("sizes, budget and block must be positive, recent between 0 and the budget")
-        if dtype not in (torch.bfloat16, torch.float16):
+        if dtype not in _ROW_DTYPES:
             raise ValueError("the cache must be bfloat16 or float16")
+        if not 0.0 < scale < math.inf:
+            raise ValueError("attention scale must be positive")
+        _workspace_bytes(True, batch_size, n_groups, n_groups, 1, budget + block, k_dim, v_dim, _ROW_DTYPES[dtype])
         self.batch_size, self.n_groups, self.budget, self.recent, self.block = batch_size, n_groups, budget, recent, block
         self.scale, self.capacity = float(scale), budget + block
         shape = (batch_size, n_groups, self.capacity)
@@ -103,17 +110,30 @@ class EvictingKVCache:
         """Attention ``[batch, n_heads, T, v_dim]`` of T new tokens, which join the cache. ``counts`` (int32
         ``[batch]`` on the device) gives the tokens that exist per row of a padded batch."""
         self._refuse_capture()
-        tokens = q.size(2)
-        if tokens < 1 or k.ndim != 4 or k.shape[:3] != (self.batch_size, self.n_groups, tokens) or (
-                counts is not None and (counts.shape != (self.batch_size,) or counts.dtype not in (torch.int32, torch.int64)
-                                        or counts.device != self.lengths.device)):
-            raise ValueError("a call takes at least one token: q [B, n_heads, T, d], k and v [B, G, T, d], counts [B]")
+        tokens = self._check_call(q, k, v, counts)
         outputs = []
         for start in range(0, tokens, self.block):
             end = min(tokens, start + self.block)
             part = None if counts is None else (counts - start).clamp(0, end - start).to(torch.int32)
             outputs.append(self._step(q[:, :, start:end], k[:, :, start:end], v[:, :, start:end], part))
         return outputs[0] if len(outputs) == 1 else torch.cat(outputs, dim=2)
+
+    def _check_call(self, q, k, v, counts):
+        """The call's tokens; refuses what any of its blocks would, before a row is dropped or stored."""
+        batch, groups, device, tokens = self.batch_size, self.n_groups, self.k.device, q.size(2) if q.ndim == 4 else 0
+        heads, dk, dv = q.size(1), self.k.size(3), self.v.size(3)
+        if (tokens < 1 or q.shape != (batch, heads, tokens, dk) or heads < 1 or heads % groups
+                or k.shape != (batch, groups, tokens, dk) or v.shape != (batch, groups, tokens, dv)
+                or not q.device == k.device == v.device == device
+                or counts is not None and (counts.shape != (batch,) or counts.dtype not in (torch.int32, torch.int64)
+                                           or counts.device != device)):
+            raise ValueError("a call takes at least one token: q [B, n_heads, T, d], k and v [B, G, T, d], counts [B], "
+                             "all on the cache's device")
+        for x in (q, k, v):
+            check_activation_dtype(x.dtype)
+        # The sizes that an attention refuses.
+        _workspace_bytes(True, batch, heads, groups, min(tokens, self.block), self.capacity, dk, dv, _ROW_DTYPES[self.k.dtype])
+        return tokens
 
     def _step(self, q, k, v, counts):
         n = q.size(2)
