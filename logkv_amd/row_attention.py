@@ -68,6 +68,15 @@ def _small_rows(x, dtype):
     return x
 
 
+def _row_strides(x):
+    """Strides of the first three dimensions, 0 for those of one element (theirs are never taken)."""
+    return tuple(0 if n == 1 else s for n, s in zip(x.shape[:3], x.stride()))
+
+
+def _contiguous_rows(x):
+    return x.stride(2) == 1 or x.size(2) == 1
+
+
 def _lengths(lengths, batch, cap, index, room=0):
     """(int32 tensor or None, its address, its stride, added rows) of an int or an int tensor ``[B]``."""
     if isinstance(lengths, torch.Tensor):
@@ -123,7 +132,10 @@ def _attention(q, k, v, cache_k, cache_v, scale, lengths, room, *, bias=None, vi
     ck_sb, ck_sg, ck_st, ck_sd = cache_k.stride()
     cv_sb, cv_sg, cv_st, cv_sd = cache_v.stride()
     if cap and (ck_sd != 1 or cv_sd != 1 or (ck_sb | ck_sg | ck_st | cv_sb | cv_sg | cv_st) & 7 or (ck | cv) & 15):
-        raise ValueError("cache rows must be 16-byte aligned with contiguous features")
+        ck_sb, ck_sg, ck_st = _row_strides(cache_k)
+        cv_sb, cv_sg, cv_st = _row_strides(cache_v)
+        if ck_sd != 1 or cv_sd != 1 or (ck_sb | ck_sg | ck_st | cv_sb | cv_sg | cv_st) & 7 or (ck | cv) & 15:
+            raise ValueError("cache rows must be 16-byte aligned with contiguous features")
     out_dtype = q.dtype
     q_st, k_st, v_st = q.stride(), k.stride(), v.stride()
     qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
@@ -205,7 +217,7 @@ def log_kv_weight_attention(q, k, v, cache_k, cache_v, weights, lengths, scale, 
     they add no weight and are not stored. ``weights`` is float32 ``[B, G, capacity]`` with contiguous rows."""
     batch, _, cap = shape = cache_k.shape[:3]
     if (weights.shape != shape or weights.dtype != torch.float32 or weights.get_device() != cache_k.get_device()
-            or weights.stride(2) != 1 or cap < 1):
+            or not _contiguous_rows(weights) or cap < 1):
         raise ValueError("weights must be float32 [B, G, capacity] on the cache's device with contiguous rows")
     if _repeats(weights) or _repeats(cache_k) or _repeats(cache_v):
         raise ValueError("weights and cache are written: their rows must not share memory (expanded tensors)")
@@ -230,9 +242,13 @@ def _span(t):
     return t.data_ptr(), t.data_ptr() + last * t.element_size()
 
 
-def _evict_rows_ok(t):
+def _unit_strides(t):
+    """Strides of rows that are read in 16-byte units, None where they cannot be."""
     sb, sg, st, sd = t.stride()
-    return sd == 1 and ((sb | sg | st) * t.element_size() | t.data_ptr()) & 15 == 0
+    size, at = t.element_size(), t.data_ptr()
+    if ((sb | sg | st) * size | at) & 15:
+        sb, sg, st = _row_strides(t)
+    return (sb, sg, st) if sd == 1 and not ((sb | sg | st) * size | at) & 15 else None
 
 
 def log_kv_evict(cache_k, cache_v, weights, lengths, keep, *, recent=0, positions=None, out=None):
@@ -256,15 +272,16 @@ def log_kv_evict(cache_k, cache_v, weights, lengths, keep, *, recent=0, position
     require_device(cache_k, "cache_k")
     if cache_v.dtype != dtype or not cache_v.get_device() == weights.get_device() == index:
         raise ValueError("all tensors must be on the cache's device, keys and values of one dtype")
-    if weights.shape != (batch, groups, cap) or weights.dtype != torch.float32 or weights.stride(2) != 1:
+    if weights.shape != (batch, groups, cap) or weights.dtype != torch.float32 or not _contiguous_rows(weights):
         raise ValueError("weights must be float32 [B, G, capacity] with contiguous rows")
     p_in = p_out = _NO_STRIDES
     if positions is not None:
         p_in = (positions.data_ptr(), *positions.stride()[:2])
-        if (positions.shape != (batch, groups, cap) or positions.dtype != torch.int64 or positions.stride(2) != 1
+        if (positions.shape != (batch, groups, cap) or positions.dtype != torch.int64 or not _contiguous_rows(positions)
                 or positions.get_device() != index):
             raise ValueError("positions must be int64 [B, G, capacity] with contiguous rows")
-    if not (_evict_rows_ok(cache_k) and _evict_rows_ok(cache_v)):
+    ck_st, cv_st = _unit_strides(cache_k), _unit_strides(cache_v)
+    if ck_st is None or cv_st is None:
         raise ValueError("cache rows must be 16-byte aligned with contiguous features")
     if torch.is_grad_enabled() and (cache_k.requires_grad or cache_v.requires_grad or weights.requires_grad):
         raise _no_gradient()
@@ -275,14 +292,17 @@ def log_kv_evict(cache_k, cache_v, weights, lengths, keep, *, recent=0, position
             cache_k.new_empty((batch, groups, keep, dk)), cache_v.new_empty((batch, groups, keep, dv)),
             weights.new_empty((batch, groups, keep)),
             None if positions is None else positions.new_empty((batch, groups, keep)), kept, kept.new_empty(batch))
+        k, v, w, p, kept, n = out
+        k_st, v_st = k.stride()[:3], v.stride()[:3]
     else:
         _check_evict_out(out, cache_k, cache_v, weights, positions, lengths, keep)
-    k, v, w, p, kept, n = out
+        k, v, w, p, kept, n = out
+        k_st, v_st = _unit_strides(k), _unit_strides(v)
     if p is not None:
         p_out = (p.data_ptr(), *p.stride()[:2])
     args = pack_evict(
-        cache_k.data_ptr(), *cache_k.stride()[:3], cache_v.data_ptr(), *cache_v.stride()[:3], weights.data_ptr(),
-        *weights.stride()[:2], *p_in, n_ptr, k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], w.data_ptr(),
+        cache_k.data_ptr(), *ck_st, cache_v.data_ptr(), *cv_st, weights.data_ptr(),
+        *weights.stride()[:2], *p_in, n_ptr, k.data_ptr(), *k_st, v.data_ptr(), *v_st, w.data_ptr(),
         *w.stride()[:2], *p_out, kept.data_ptr(), n.data_ptr(), batch, groups, cap, dk, dv, cache_k.element_size(),
         len_add, keep, recent)
     _launch(rows_lib().logkv_evict_rows, "logkv_evict_rows", index, args)
@@ -296,10 +316,10 @@ def _check_evict_out(out, cache_k, cache_v, weights, positions, lengths, keep):
 
     def rows(t, dtype, *rest):
         return (t.ndim == 3 + len(rest) and t.shape[:2] == (batch, groups) and t.size(2) >= keep and t.shape[3:] == rest
-                and t.dtype == dtype and t.device == device and t.stride(2 if not rest else 3) == 1)
+                and t.dtype == dtype and t.device == device and (t.stride(3) == 1 if rest else _contiguous_rows(t)))
 
     if not (rows(k, cache_k.dtype, dk) and rows(v, cache_k.dtype, dv) and rows(w, torch.float32)
-            and _evict_rows_ok(k) and _evict_rows_ok(v) and (p is None) == (positions is None)
+            and _unit_strides(k) and _unit_strides(v) and (p is None) == (positions is None)
             and (p is None or rows(p, torch.int64)) and kept.shape == (batch, groups, keep) and kept.is_contiguous()
             and kept.dtype == torch.int32 and kept.device == device and n.shape == (batch,) and n.is_contiguous()
             and n.dtype == torch.int32 and n.device == device and not any(_repeats(t) for t in (k, v, w))
