@@ -11,6 +11,8 @@ is the cache's ``add_recent`` (the flush kernels).
 
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from .log_kv_pack import log_kv_chunk_attention, log_kv_draft_attention
@@ -46,12 +48,19 @@ def _join_pos(a, b):
 
 def _check_path(path, tokens, batch):
     """The accepted tokens as one list of indices per batch row (or one for all), each in the draft's order."""
-    if isinstance(path, torch.Tensor):
-        path = path.tolist() if path.dim() else [path.item()]
+    if hasattr(path, "tolist"):
+        path = path.tolist() if path.ndim else [path.item()]
     path = list(path)
     if not path:
         return [[]]
-    rows = [list(row) for row in path] if isinstance(path[0], (list, tuple)) else [path]
+    try:
+        rows = [list(row) for row in path] if isinstance(path[0], (list, tuple)) else [path]
+        rows = [[i.item() if hasattr(i, "item") else i for i in row] for row in rows]
+        if any(isinstance(i, bool) for row in rows for i in row):
+            raise TypeError("a mask")
+        rows = [[operator.index(i) for i in row] for row in rows]
+    except TypeError as e:
+        raise ValueError("path must hold indices of drafted tokens") from e
     if len(rows) not in (1, batch) or len({len(row) for row in rows}) != 1:
         raise ValueError("path must be [n] or [B, n] indices of drafted tokens, as many in every batch row")
     for row in rows:
