@@ -120,8 +120,8 @@ class EvictingKVCache:
 
     def _check_call(self, q, k, v, counts):
         """The call's tokens; refuses what any of its blocks would, before a row is dropped or stored."""
-        batch, groups, device, tokens = self.batch_size, self.n_groups, self.k.device, q.size(2) if q.ndim == 4 else 0
-        heads, dk, dv = q.size(1), self.k.size(3), self.v.size(3)
+        batch, groups, dk, dv, device = self.batch_size, self.n_groups, self.k.size(3), self.v.size(3), self.k.device
+        heads, tokens = q.shape[1:3] if q.ndim == 4 else (0, 0)
         if (tokens < 1 or q.shape != (batch, heads, tokens, dk) or heads < 1 or heads % groups
                 or k.shape != (batch, groups, tokens, dk) or v.shape != (batch, groups, tokens, dv)
                 or not q.device == k.device == v.device == device

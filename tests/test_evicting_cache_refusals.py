@@ -42,6 +42,7 @@ BAD = {
     "more keys": lambda T: (rows(4, T, D), rows(G, T + 1, D), rows(G, T, DV)),
     "batch": lambda T: (rows(4, T, D)[:1], rows(G, T, D), rows(G, T, DV)),
     "3-dimensional": lambda T: (rows(4, T, D)[0], rows(G, T, D), rows(G, T, DV)),
+    "1-dimensional": lambda T: (rows(4, T, D).flatten(), rows(G, T, D), rows(G, T, DV)),
     "device": lambda T: (rows(4, T, D), rows(G, T, D), rows(G, T, DV, device="meta")),
     "counts' shape": lambda T: (rows(4, T, D), rows(G, T, D), rows(G, T, DV), torch.ones(3, dtype=torch.int32)),
     "counts' dtype": lambda T: (rows(4, T, D), rows(G, T, D), rows(G, T, DV), torch.ones(B)),
