@@ -33,7 +33,8 @@ enum { LOGKV_BF16 = 0, LOGKV_F16 = 1 };
  * n_b = lengths[b * len_stride] + *lengths2 + len_add (absent pointers count as 0), held to
  * [0, cap]. A NaN or infinity in a row that a query does not see does not reach its output.
  * dtype: LOGKV_BF16 or LOGKV_F16 for q, k, v, the cache and out; arithmetic in float32, the
- * probabilities enter the value products as two parts of 8 (bf16) or 11 (fp16) bits each.
+ * probabilities enter the value products as two parts of 8 (bf16) or 11 (fp16) bits each, rounded,
+ * whatever the queries' number and the values' size.
  * dk, dv: multiples of 8 up to 256; every row 16-byte aligned (strides multiples of 8); features
  * contiguous. bias (tree attention): float32, or dtype with bias_half, strided; NULL for none;
  * -inf hides a row. bias_scale: a positive factor, 0 for 1. Where float32 holds the logits in steps

@@ -221,7 +221,7 @@ void launch_finish_cols(const logkv_rows_args& a, const RowsLaunch& r, hipStream
 template <int DT>
 void launch_finish_type(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
   // Groups of splits share a query where eight queries a block would not fill the CUs: 1 x 32768 rows of 8 heads and
-  // 512 queries without them 120 us, with them 123; 4096 rows and 666 queries 54.6 and 60.9 us.
+  // 512 queries without them 145 us, with them 145 - 152; 4096 rows and 666 queries 55 and 62 us.
   const bool many = r.splits > 8 && static_cast<int64_t>(a.n_batch) * a.n_heads * a.tq < 8 * 256;
   if (a.dv <= 128) {
     if (many) launch_finish_cols<DT, 32, 8>(a, r, stream);

@@ -8,10 +8,10 @@
 //   S^T = K Q^T by 16x16x32 matrix products (keys x queries: a lane holds 8 keys of its query
 //   l % 16 in each of the NC column blocks), K loaded from memory in operand layout;
 //   O^T += V^T P^T, V staged row-major in the wave's own LDS and read transposed
-//   (ds_read_b64_tr_b16), P as two parts (16 bits for bf16, 22 for fp16).
+//   (ds_read_b64_tr_b16), P as two rounded parts (16 bits for bf16, 22 for fp16).
 // The next tile's K and V are on their way while one is computed.
-// Bound by HBM: one query over 64 lanes of 32768 rows of 2 x 128 bf16 in 213 us, 5.04 TB/s with the
-// stored products, the rate of a large copy; loads past the caches took 230 us in the whole call
+// Bound by HBM: two queries (heads) of one token over 64 lanes of 32768 rows of 2 x 128 bf16 in 213 us,
+// 5.04 TB/s with the stored products, the rate of a large copy; loads past the caches took 230 us in the whole call
 // against 237 there but 40 against 34 where the rows fit the last cache, and are not used.
 // Rows that no query sees (past the rows in use) have V = 0; a tile with an infinity or NaN in V
 // takes a form of its own in which an element reaches only the queries that see its row.

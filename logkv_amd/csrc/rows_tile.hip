@@ -12,18 +12,19 @@
 // long as their products. So two waves a SIMD, and in each the score products of the next 32 rows
 // are interleaved with the exponentials of these, the value products with half of the conversions,
 // the next maxima and the staging of the next tile. 32768 rows of 128 features, 8 lanes of 512
-// queries: 107 us, 645 TFLOP/s of the 1207 of a large matrix product (one wave a SIMD with 64
+// queries: 124 us, 555 TFLOP/s of the 1207 of a large matrix product (one wave a SIMD with 64
 // queries was slower: nothing hid its waits); 30720 rows and 2048 new ones, 8 lanes of 4096
-// queries: 700 us, 760 TFLOP/s.
+// queries: 824 - 876 us, 610 - 650 TFLOP/s, the two units busy 50% and 46% of the cycles, in turn.
 // Up to 64 queries: two blocks of four waves a CU (two waves of queries, two of rows): 64 lanes of
-// 8192 rows, 52 queries 80 us, in one block of eight waves 85.
+// 8192 rows, 52 queries 64 us the call, in one block of eight waves 86.
 // P enters the value products as two parts of the cache's type (one part's rounding would equal the
 // output's), V as it is. For bf16, one fp16 part of P against V converted to fp16 was faster (a third
-// less matrix work: 64 tokens x 8 heads over 32768 rows 122 us the call against 139, 2048 tokens over
-// 30720 rows 1067 against 1189) but rounded P to 2^-11 and V below 2^-17 to 2^-25. A share with an infinity or NaN in V is done again by a second
-// launch (in one kernel the second form's registers spilled in the first's loop, and a reload there
-// waits for every load ahead) in a second form that adds such a tile row by row for the queries that
-// see its rows. The second launch's blocks read a flag and end: 4.7 us.
+// less matrix work and five conversions a pair fewer: 64 tokens x 8 heads over 32768 rows 104 us the
+// call against 125, 2048 tokens over 30720 rows 975 - 1030 against 1150) but rounded P to 2^-11 and V
+// below 2^-17 to 2^-25. A share with an infinity or NaN in V is done again by a second launch (in one
+// kernel the second form's registers spilled in the first's loop, and a reload there waits for every
+// load ahead) in a second form that adds such a tile row by row for the queries that see its rows. The
+// second launch's blocks read a flag and end: 4.7 us.
 // Rows are stored without padding, their 16-byte units permuted by row so that the operand reads
 // and the transposed reads meet every bank once. One barrier per tile, the following tiles' rows on
 // their way in registers; two buffers of V and, by RowsSchedule, two or three of K.

@@ -6,8 +6,8 @@
 // of one 32x32 block and the exponentials of the one before are independent and interleaved: both
 // take about as long (16 quarter-rate exponentials a lane against eight products of 32 cycles at 128
 // features). One wave owns a key: no atomics, a fixed order. 8 lanes of 30720 rows and 2048 new ones,
-// 4096 queries of 128 features: 366 us, 730 TFLOP/s; the vector unit and the matrix cores are busy 47%
-// and 31% of the cycles. 32 keys a wave (twice the reads of Q): 50 us more.
+// 4096 queries of 128 features: 374 - 393 us, 680 - 710 TFLOP/s; the vector unit and the matrix cores are
+// busy 49% and 32% of the cycles. 32 keys a wave (twice the reads of Q): 50 us more.
 #include <algorithm>
 #include <type_traits>
 
@@ -229,8 +229,8 @@ void launch_one(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t strea
 template <int DT>
 void launch_type(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
   // 64 keys a wave where that leaves two blocks for every CU; two waves to 32 keys, each half of the queries, where
-  // four waves of 32 keys would leave less than two blocks (4 lanes of 2048 rows, 2000 queries: 71.5 us the call, 79.6
-  // without; 8 lanes of 4096, 666: 51.0 and 51.9).
+  // four waves of 32 keys would leave less than two blocks (4 lanes of 2048 rows, 2000 queries of 128 features: 78.5 us
+  // the call, 85.1 without; 8 lanes of 4096, 666: 66.0 and 66.7).
   const int64_t keys = (static_cast<int64_t>(a.cap) + a.tq) * a.n_batch * a.n_groups;
   const bool many = keys >= 512 * 256, few = keys < 512 * 128;
   if (a.dk <= 64) {
