@@ -16,3 +16,5 @@ from .streaming import LogKVStreamingAttention  # noqa: F401
 from .flush_group import flush_grouping, set_flush_grouping  # noqa: F401
 from .row_attention import EvictedRows, log_kv_evict, log_kv_tree_attention, log_kv_weight_attention  # noqa: F401
 from .evicting_cache import EvictingKVCache  # noqa: F401
+from .rotary import log_kv_rotary, rotary_frequencies, rotary_tables  # noqa: F401
+from .paged_attention import SharedPrefix, log_kv_paged_append, log_kv_paged_attention  # noqa: F401

@@ -10,6 +10,7 @@
 
 #include "route.hpp"
 #include "rows.hpp"
+#include "paged.hpp"
 #include "unified.hpp"
 
 thread_local const char* logkv::g_refusal = nullptr;
@@ -910,6 +911,110 @@ int logkv_evict_rows(const logkv_evict_args* a, void* stream) {
     if (s * a->size % 16) return fail(LOGKV_EINVAL, "evicted rows must be 16-byte aligned (strides)");
   const int rc = logkv::launch_evict(*a, static_cast<hipStream_t>(stream));
   if (rc) return launch_failed(rc, "eviction");
+  return LOGKV_OK;
+}
+
+namespace {
+
+int check_rotary(const logkv_rotary_args* a, bool append) {
+  if (!a) return fail(LOGKV_EINVAL, "rotary args are NULL");
+  if (a->n_batch < 1 || a->tokens < 1 || (a->q && a->n_heads < 1) || ((a->k || append) && a->n_groups < 1) || (!a->q && !a->k))
+    return fail(LOGKV_EINVAL, "rotary shape: batch %d, heads %d and %d, tokens %d", a->n_batch, a->n_heads, a->n_groups, a->tokens);
+  if (a->dim < 1 || a->dim > 512 || a->rotated < 0 || a->rotated > a->dim || a->rotated % 2)
+    return fail(LOGKV_EINVAL, "rotary widths: an even part of up to 512 features, got %d of %d", a->rotated, a->dim);
+  if (a->dtype != LOGKV_BF16 && a->dtype != LOGKV_F16 && a->dtype != LOGKV_F32)
+    return fail(LOGKV_EINVAL, "rotary takes bf16, fp16 or float32");
+  if ((a->q && !a->q_out) || (!append && a->k && !a->k_out) || (a->rotated && !a->frequencies))
+    return fail(LOGKV_EINVAL, "rotary buffer is NULL");
+  if (!std::isfinite(a->amplitude) || (a->sign != 1.f && a->sign != -1.f))
+    return fail(LOGKV_EINVAL, "rotary amplitude must be finite, sign 1 or -1");
+  if (!append) return a->v ? fail(LOGKV_EINVAL, "a rotation takes no values") : LOGKV_OK;
+  if (a->page < 16 || (a->page & (a->page - 1)) || a->table_len < 0 || a->n_pages < 0 || a->dim_v < 1 || a->dim_v > 512 ||
+      int64_t(a->table_len) * a->page > INT32_MAX)
+    return fail(LOGKV_EINVAL, "append: pages of %d rows (a power of two from 16 on), %d a sequence, %d in all, values of %d",
+                a->page, a->table_len, a->n_pages, a->dim_v);
+  if (a->cache_dtype != LOGKV_BF16 && a->cache_dtype != LOGKV_F16) return fail(LOGKV_EINVAL, "a paged cache is bf16 or fp16");
+  if (!a->k || !a->v || (a->table_len && !a->table) || (a->n_pages && (!a->k_pages || !a->v_pages)))
+    return fail(LOGKV_EINVAL, "append buffer is NULL");
+  return LOGKV_OK;
+}
+
+}  // namespace
+
+int logkv_rotary(const logkv_rotary_args* a, void* stream) {
+  int rc = check_rotary(a, false);
+  if (rc) return rc;
+  rc = logkv::launch_rotary(*a, false, static_cast<hipStream_t>(stream));
+  if (rc) return launch_failed(rc, "rotary");
+  return LOGKV_OK;
+}
+
+int logkv_paged_append(const logkv_rotary_args* a, void* stream) {
+  int rc = check_rotary(a, true);
+  if (rc) return rc;
+  rc = logkv::launch_rotary(*a, true, static_cast<hipStream_t>(stream));
+  if (rc) return launch_failed(rc, "append");
+  return LOGKV_OK;
+}
+
+namespace {
+
+int check_paged_shape(const logkv_paged_args* a) {
+  if (!a) return fail(LOGKV_EINVAL, "paged attention args are NULL");
+  if (a->n_batch < 1 || a->n_groups < 1 || a->n_heads < 1 || a->n_heads % a->n_groups || a->tq < 1)
+    return fail(LOGKV_EINVAL, "paged attention shape: batch %d, heads %d, groups %d, queries %d", a->n_batch, a->n_heads,
+                a->n_groups, a->tq);
+  if (a->n_prefixes < 0 || (a->n_prefixes && a->n_batch % a->n_prefixes))
+    return fail(LOGKV_EINVAL, "%d prefixes do not divide %d sequences", a->n_prefixes, a->n_batch);
+  const int64_t queries = int64_t(a->n_heads / a->n_groups) * a->tq * (a->n_prefixes ? a->n_batch / a->n_prefixes : 1);
+  if (int64_t(a->n_batch) * a->n_groups > 65535 || queries > 1 << 19)
+    return fail(LOGKV_EINVAL, "paged attention takes at most 65535 lanes and 2^19 query rows per prefix and KV group");
+  if (a->dk < 8 || a->dv < 8 || a->dk % 8 || a->dv % 8 || a->dk > 256 || a->dv > 256)
+    return fail(LOGKV_EINVAL, "paged attention widths must be multiples of 8 in [8, 256], got %d/%d", a->dk, a->dv);
+  if (a->page < 16 || (a->page & (a->page - 1)) || a->table_len < 0 || a->n_pages < 0 || a->prefix_len < 0 ||
+      int64_t(a->table_len) * a->page > 1 << 30 || int64_t(a->prefix_len) * (a->prefix_table ? a->page : 1) > 1 << 30)
+    return fail(LOGKV_EINVAL, "paged attention: pages of %d rows (a power of two from 16 on), %d a sequence, a prefix of %d",
+                a->page, a->table_len, a->prefix_len);
+  if (a->dtype != LOGKV_BF16 && a->dtype != LOGKV_F16) return fail(LOGKV_EINVAL, "paged attention takes bf16 or fp16");
+  return LOGKV_OK;
+}
+
+int check_paged(const logkv_paged_args* a, const void* ws, int64_t ws_bytes) {
+  int rc = check_paged_shape(a);
+  if (rc) return rc;
+  if (!a->q || !a->k || !a->v || !a->out || (a->table_len && !a->table) || (a->n_pages && (!a->k_pages || !a->v_pages)))
+    return fail(LOGKV_EINVAL, "paged attention buffer is NULL");
+  if (a->n_prefixes && a->prefix_len && !a->prefix_table && (!a->prefix_k || !a->prefix_v))
+    return fail(LOGKV_EINVAL, "paged attention prefix is NULL");
+  if (a->bias && (a->prefix_table || !a->n_prefixes)) return fail(LOGKV_EINVAL, "a bias is of a prefix's contiguous rows");
+  if (!unit_rows(a->q, a->q_sb, a->q_sh, a->q_st) || !unit_rows(a->k, a->k_sb, a->k_sg, a->k_st) ||
+      !unit_rows(a->v, a->v_sb, a->v_sg, a->v_st) || !unit_rows(a->k_pages, a->kp_sp, a->kp_sg, a->kp_st) ||
+      !unit_rows(a->v_pages, a->vp_sp, a->vp_sg, a->vp_st) || !unit_rows(a->prefix_k, a->pk_sb, a->pk_sg, a->pk_st) ||
+      !unit_rows(a->prefix_v, a->pv_sb, a->pv_sg, a->pv_st))
+    return fail(LOGKV_EINVAL, "paged attention rows must be 16-byte aligned (strides multiples of 8 elements)");
+  if (reinterpret_cast<uintptr_t>(a->out) % 8 || a->o_sb % 4 || a->o_sh % 4 || a->o_st % 4)
+    return fail(LOGKV_EINVAL, "paged attention output rows must be 8-byte aligned");
+  if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return fail(LOGKV_EINVAL, "attention scale must be positive");
+  if (!(a->bias_scale >= 0.f) || !std::isfinite(a->bias_scale))
+    return fail(LOGKV_EINVAL, "attention bias_scale must be positive, or 0 for 1");
+  if (a->visible && a->counts) return fail(LOGKV_EINVAL, "paged attention takes a mask of the call's rows or their counts");
+  if (!aligned16(ws) || !ws || ws_bytes < logkv::paged_launch(*a, nullptr).bytes)
+    return fail(LOGKV_EINVAL, "paged attention workspace too small");
+  return LOGKV_OK;
+}
+
+}  // namespace
+
+int64_t logkv_paged_workspace_bytes(const logkv_paged_args* a) {
+  if (check_paged_shape(a)) return -1;
+  return logkv::paged_launch(*a, nullptr).bytes;
+}
+
+int logkv_paged_attention(const logkv_paged_args* a, void* ws, int64_t ws_bytes, void* stream) {
+  int rc = check_paged(a, ws, ws_bytes);
+  if (rc) return rc;
+  rc = logkv::launch_paged_attention(*a, logkv::paged_launch(*a, ws), static_cast<hipStream_t>(stream));
+  if (rc) return launch_failed(rc, "paged attention");
   return LOGKV_OK;
 }
 

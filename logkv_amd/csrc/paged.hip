@@ -1,0 +1,217 @@
+// Attention of a batch over a paged cache, with prefixes that several sequences share.
+//
+// Softmax over [prefix | own pages | the call's rows] splits by rows: each part gives a query an
+// unnormalised sum, a maximum and a sum of exponentials, which join under the largest maximum. So a
+// prefix's rows are read once for all of its sequences: their queries (sequences x heads of the KV group
+// x tokens) are the columns of one product, in the kernel that so many columns take (rows_plan), and a
+// sequence's own rows are read in a second pass of few columns. Both passes are the row attention
+// kernels over a page table; this file joins their partials.
+#include <algorithm>
+
+#include "paged.hpp"
+
+namespace logkv {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+int64_t align256(int64_t x) { return (x + 255) & ~int64_t(255); }
+
+}  // namespace
+
+// TQ threads per query, four features each; the block's other factor is shared by queries and by groups of
+// partials (QPB queries x SG groups), joined in group order.
+template <int DT, int TQ, int SG>
+__global__ __launch_bounds__(kThreads) void paged_finish_kernel(logkv_rows_args a, RowsLaunch own, RowsLaunch shared) {
+  typedef Elem<DT> E;
+  constexpr int QPB = kThreads / (TQ * SG);
+  __shared__ __align__(16) float acc_s[QPB][SG][4 * TQ];
+  __shared__ float m_s[QPB][SG], l_s[QPB][SG];
+  const int G = a.n_groups, b = static_cast<int>(blockIdx.y) / G, g = static_cast<int>(blockIdx.y) % G;
+  const int rep = a.n_heads / G, nq = rep * a.tq, tid = threadIdx.x, stride = a.dv + kRowsPartTail;
+  const int qs = tid / (TQ * SG), sg = tid / TQ % SG, d = 4 * (tid % TQ);
+  const int qi = static_cast<int>(blockIdx.x) * QPB + qs;
+  const bool there = qi < nq && d < a.dv;
+  const bool live = min(qi, nq - 1) % a.tq < own_rows(a, b);   // a query past its sequence's count sees nothing
+  float m = -__builtin_inff(), lsum = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int set = 0; set < 2; ++set) {
+    const RowsLaunch& r = set ? shared : own;
+    if (set && !r.seqs) continue;
+    const int lane = (set ? b / r.seqs : b) * G + g, splits = r.shares ? r.shares[lane] : r.splits;
+    const int64_t step = static_cast<int64_t>(set ? r.seqs * nq : nq) * stride;
+    const float* base = r.part + static_cast<int64_t>(lane) * r.room * step +
+                        static_cast<int64_t>((set ? b % r.seqs * nq : 0) + min(qi, nq - 1)) * stride;
+    const float unit = __builtin_amdgcn_exp2f(-r.shift);
+    // Eight partials' loads at a time, joined under the running maximum.
+    for (int s0 = sg; s0 < splits; s0 += 8 * SG) {
+      float2 ml[8];
+      f32x4 x[8];
+      float mx = m;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int sp = s0 + k * SG;
+        ml[k] = make_float2(-__builtin_inff(), 0.f);
+        x[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (there && live && sp < splits) {
+          ml[k] = *reinterpret_cast<const float2*>(base + sp * step + a.dv);
+          x[k] = *reinterpret_cast<const f32x4*>(base + sp * step + d);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mx = fmaxf(mx, ml[k].x);
+      const float top = mx == -__builtin_inff() ? 0.f : mx;
+      const float corr = __builtin_amdgcn_exp2f(m - top);
+      lsum *= corr;
+      acc *= corr;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float f = unit * __builtin_amdgcn_exp2f(ml[k].x - top);
+        lsum += ml[k].y * f;
+        acc += x[k] * f;
+      }
+      m = mx;
+    }
+  }
+  if constexpr (SG > 1) {
+    *reinterpret_cast<f32x4*>(&acc_s[qs][sg][d]) = acc;
+    if (d == 0) {
+      m_s[qs][sg] = m;
+      l_s[qs][sg] = lsum;
+    }
+    __syncthreads();
+    if (sg) return;
+    float mx = m;
+#pragma unroll
+    for (int k = 1; k < SG; ++k) mx = fmaxf(mx, m_s[qs][k]);
+    const float top = mx == -__builtin_inff() ? 0.f : mx;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    float total = 0.f;
+#pragma unroll
+    for (int k = 0; k < SG; ++k) {
+      const float f = __builtin_amdgcn_exp2f(m_s[qs][k] - top);
+      total += l_s[qs][k] * f;
+      sum += *reinterpret_cast<const f32x4*>(&acc_s[qs][k][d]) * f;
+    }
+    lsum = total;
+    acc = sum;
+  }
+  if (!there) return;
+  uint16_t y[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) y[k] = lsum == 0.f ? uint16_t(0) : E::from_f32(acc[k] / lsum);
+  LOGKV_G uint16_t* o = gp(a.out) + b * a.o_sb + (g * rep + qi / a.tq) * a.o_sh + qi % a.tq * a.o_st + d;
+  *reinterpret_cast<LOGKV_G uint2*>(o) =
+      make_uint2(y[0] | static_cast<uint32_t>(y[1]) << 16, y[2] | static_cast<uint32_t>(y[3]) << 16);
+}
+
+namespace {
+
+template <int DT, int TQ, int SG>
+void launch_finish(const PagedLaunch& p, hipStream_t stream) {
+  const logkv_rows_args& a = p.own.args;
+  const int nq = a.n_heads / a.n_groups * a.tq, qpb = kThreads / (TQ * SG);
+  hipLaunchKernelGGL((paged_finish_kernel<DT, TQ, SG>), dim3((nq + qpb - 1) / qpb, a.n_batch * a.n_groups), dim3(kThreads),
+                     0, stream, a, p.own.launch, p.shared.launch);
+}
+
+template <int DT>
+void launch_finish_type(const PagedLaunch& p, hipStream_t stream) {
+  const logkv_rows_args& a = p.own.args;
+  // Groups of partials share a query where eight queries a block would not fill the CUs.
+  const bool many = std::max(p.own.launch.splits, p.shared.launch.splits) > 8 &&
+                    static_cast<int64_t>(a.n_batch) * a.n_heads * a.tq < 8 * 256;
+  if (a.dv <= 128) {
+    if (many) launch_finish<DT, 32, 8>(p, stream);
+    else launch_finish<DT, 32, 1>(p, stream);
+  } else {
+    if (many) launch_finish<DT, 64, 4>(p, stream);
+    else launch_finish<DT, 64, 1>(p, stream);
+  }
+}
+
+int launch_pass(const PagedPass& p, hipStream_t stream) {
+  return p.launch.q_waves ? launch_paged_tile(p, stream) : launch_paged_stream(p, stream);
+}
+
+}  // namespace
+
+PagedLaunch paged_launch(const logkv_paged_args& a, void* ws) {
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  int64_t off = 0;
+  auto take = [&](int64_t words) {
+    float* p = base ? reinterpret_cast<float*>(base + off) : nullptr;
+    off += align256(4 * words);
+    return p;
+  };
+  auto plan = [&](PagedPass& pass) {
+    RowsLaunch& r = pass.launch;
+    const logkv_rows_args& x = pass.args;
+    const int64_t lanes = static_cast<int64_t>(x.n_batch) * x.n_groups;
+    const int64_t nq = static_cast<int64_t>(x.n_heads / x.n_groups) * x.tq * r.seqs;
+    r.bias2 = (x.bias_scale == 0.f ? 1.f : x.bias_scale) * kLog2e;
+    r.causal = x.visible ? 0 : 1;
+    rows_plan(x, lanes, nq, r);
+    // Shares by length (rows_tile.hpp), as of contiguous rows.
+    const bool by_length = r.q_waves && r.splits > 1 && x.n_batch > 1 && x.n_batch <= kWave;
+    r.room = by_length ? 2 * r.splits : r.splits;
+    r.part = take(lanes * r.room * nq * (x.dv + kRowsPartTail));
+    if (r.q_waves) r.redo = reinterpret_cast<int*>(take(lanes * r.splits * ((nq + 32 * r.q_waves - 1) / (32 * r.q_waves))));
+    if (by_length) {
+      r.shares = reinterpret_cast<int*>(take(lanes));
+      if (!x.lengths || !x.len_stride) r.shares = nullptr;   // rows of one length
+    }
+  };
+  PagedLaunch p{};
+  logkv_rows_args& x = p.own.args;
+  x.q = a.q, x.q_sb = a.q_sb, x.q_sh = a.q_sh, x.q_st = a.q_st;
+  x.k = a.k, x.k_sb = a.k_sb, x.k_sg = a.k_sg, x.k_st = a.k_st;
+  x.v = a.v, x.v_sb = a.v_sb, x.v_sg = a.v_sg, x.v_st = a.v_st;
+  x.cache_k = a.k_pages, x.ck_sb = a.kp_sp, x.ck_sg = a.kp_sg, x.ck_st = a.kp_st;
+  x.cache_v = a.v_pages, x.cv_sb = a.vp_sp, x.cv_sg = a.vp_sg, x.cv_st = a.vp_st;
+  x.lengths = a.lengths, x.len_stride = a.len_stride, x.len_add = a.len_add;
+  x.visible = a.visible, x.vis_sb = a.vis_sb, x.vis_st = a.vis_st, x.counts = a.counts;
+  x.out = a.out, x.o_sb = a.o_sb, x.o_sh = a.o_sh, x.o_st = a.o_st;
+  x.n_batch = a.n_batch, x.n_heads = a.n_heads, x.n_groups = a.n_groups, x.tq = a.tq, x.dk = a.dk, x.dv = a.dv;
+  x.dtype = a.dtype, x.scale = a.scale, x.cap = a.table_len * a.page;
+  p.shared.args = x;
+  p.own.launch.seqs = 1;
+  p.own.launch.table = a.table, p.own.launch.table_sb = a.table_sb;
+  p.own.launch.page_shift = __builtin_ctz(a.page), p.own.launch.pages = a.n_pages;
+  plan(p.own);
+  if (a.n_prefixes) {
+    logkv_rows_args& y = p.shared.args;
+    RowsLaunch& r = p.shared.launch;
+    y.n_batch = a.n_prefixes;
+    y.lengths = a.prefix_lengths, y.lengths2 = a.prefix_lengths2, y.len_stride = a.prefix_stride, y.len_add = a.prefix_add;
+    y.counts = nullptr, y.visible = nullptr;
+    r.seqs = a.n_batch / a.n_prefixes, r.prefix = 1, r.pages = a.n_pages;
+    if (a.prefix_table) {
+      r.table = a.prefix_table, r.table_sb = a.prefix_sb, r.page_shift = p.own.launch.page_shift;
+      y.cap = a.prefix_len * a.page;
+    } else {
+      r.page_shift = 30;
+      y.cache_k = a.prefix_k, y.ck_sb = a.pk_sb, y.ck_sg = a.pk_sg, y.ck_st = a.pk_st;
+      y.cache_v = a.prefix_v, y.cv_sb = a.pv_sb, y.cv_sg = a.pv_sg, y.cv_st = a.pv_st;
+      y.bias = a.bias, y.b_sb = a.b_sb, y.b_sg = a.b_sg, y.b_st = a.b_st, y.bias_half = a.bias_half;
+      y.bias_scale = a.bias_scale;
+      y.cap = a.prefix_len;
+    }
+    plan(p.shared);
+  }
+  p.bytes = off;
+  return p;
+}
+
+int launch_paged_attention(const logkv_paged_args& a, const PagedLaunch& p, hipStream_t stream) {
+  int rc = a.n_prefixes ? launch_pass(p.shared, stream) : LOGKV_OK;
+  if (!rc) rc = launch_pass(p.own, stream);
+  if (rc) return rc;
+  if (a.dtype == LOGKV_BF16) launch_finish_type<LOGKV_BF16>(p, stream);
+  else launch_finish_type<LOGKV_F16>(p, stream);
+  return hipGetLastError() == hipSuccess ? LOGKV_OK : LOGKV_ERUNTIME;
+}
+
+}  // namespace logkv

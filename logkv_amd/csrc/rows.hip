@@ -252,12 +252,9 @@ int tile_splits(const logkv_rows_args& a, int64_t blocks, int q_waves) {
 
 }  // namespace
 
-RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws) {
-  const int64_t lanes = static_cast<int64_t>(a.n_batch) * a.n_groups, nq = static_cast<int64_t>(a.n_heads / a.n_groups) * a.tq;
+// Which kernel a lane's queries take, with how many shares of its rows.
+void rows_plan(const logkv_rows_args& a, int64_t lanes, int64_t nq, RowsLaunch& r) {
   const bool wide = a.dk > 128 || a.dv > 128;
-  RowsLaunch r{};
-  r.causal = causal ? 1 : 0;
-  r.bias2 = (a.bias_scale == 0.f ? 1.f : a.bias_scale) * kLog2e;
   const int64_t tiles = (a.cap + kRowTile - 1) / kRowTile + (a.tq + kRowTile - 1) / kRowTile;
   // More than 32 queries: tiles in LDS. From 17 on too where rows of more than 64 features are many: the streaming
   // kernel's two query blocks spill there, and the tiled kernel pays a launch more. Streaming and tiled, 128 features, 8
@@ -279,6 +276,15 @@ RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws) {
     r.splits = static_cast<int>(std::max<int64_t>(
         1, std::min<int64_t>({kMaxRowSplits, (tiles + 3) / 4, resident / std::max<int64_t>(1, lanes * q_blocks)})));
   }
+}
+
+RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws) {
+  const int64_t lanes = static_cast<int64_t>(a.n_batch) * a.n_groups, nq = static_cast<int64_t>(a.n_heads / a.n_groups) * a.tq;
+  const int64_t tiles = (a.cap + kRowTile - 1) / kRowTile + (a.tq + kRowTile - 1) / kRowTile;
+  RowsLaunch r{};
+  r.causal = causal ? 1 : 0;
+  r.bias2 = (a.bias_scale == 0.f ? 1.f : a.bias_scale) * kLog2e;
+  rows_plan(a, lanes, nq, r);
   uint8_t* base = static_cast<uint8_t*>(ws);
   int64_t off = 0;
   auto take = [&](int64_t floats) {

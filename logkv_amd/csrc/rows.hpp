@@ -34,8 +34,17 @@ struct RowsLaunch {
   float shift;    // the partials' sums carry 2^shift
   float bias2;    // bias to base-2 logits: bias_scale log2(e)
   int causal;     // weight attention; otherwise the visible mask
+  // Kernels over pages (template PAGED): cache_k / cache_v are pages [pages, G, 1 << page_shift, d] with
+  // strides ck_sb of a page, ck_sg, ck_st, and row i of lane row b is slot i % (1 << page_shift) of page
+  // table[b table_sb + (i >> page_shift)]; without a table, of page b (rows of an ordinary cache, page_shift 30).
+  const int32_t* table;
+  int64_t table_sb;
+  int page_shift, pages;
+  int seqs;       // sequences whose queries a lane takes
+  int prefix;     // rows that several sequences share: no own rows, every query sees all
 };
 
+void rows_plan(const logkv_rows_args& a, int64_t lanes, int64_t nq, RowsLaunch& r);
 RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws);
 int launch_rows_stream(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream);
 int launch_rows_tile(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream);
@@ -52,6 +61,54 @@ __device__ __forceinline__ int rows_in_use(const logkv_rows_args& a, int b) {
 }
 __device__ __forceinline__ int own_rows(const logkv_rows_args& a, int b) {
   return a.counts ? max(0, min(a.counts[b], a.tq)) : a.tq;
+}
+
+// Queries of a lane, and query qi of lane row b, group g: its row and its token.
+template <bool PAGED>
+__device__ __forceinline__ int lane_queries(const logkv_rows_args& a, const RowsLaunch& r) {
+  const int nq = a.n_heads / a.n_groups * a.tq;
+  return PAGED ? nq * r.seqs : nq;
+}
+template <bool PAGED>
+__device__ __forceinline__ const LOGKV_G uint16_t* query_row(const logkv_rows_args& a, const RowsLaunch& r, int b, int g,
+                                                             int qi, int& t) {
+  const int rep = a.n_heads / a.n_groups;
+  if constexpr (PAGED) {
+    const int s = qi / (rep * a.tq);
+    b = b * r.seqs + s;
+    qi -= s * (rep * a.tq);
+  }
+  t = qi % a.tq;
+  return gp(a.q) + b * a.q_sb + (g * rep + qi / a.tq) * a.q_sh + t * a.q_st;
+}
+template <bool PAGED>
+__device__ __forceinline__ int lane_own_rows(const logkv_rows_args& a, const RowsLaunch& r, int b) {
+  return PAGED && r.prefix ? 0 : own_rows(a, b);
+}
+
+// Rows of a page that is not there: of zeros.
+inline constexpr int kMostFeatures = 256;
+static __device__ const uint4 kZeroRow[kMostFeatures / 8] = {};
+
+#if defined(__HIP_DEVICE_COMPILE__)
+#define LOGKV_C __attribute__((address_space(4)))
+#else
+#define LOGKV_C
+#endif
+
+// The page of row `row` of lane row b, -1 for none. For an index that is the same in all lanes: a scalar load (the table
+// is not written while a kernel reads it).
+__device__ __forceinline__ int page_of(const RowsLaunch& r, int b, int row) {
+  if (!r.table) return b;
+  const int page = ((const LOGKV_C int32_t*)r.table)[b * r.table_sb + (row >> r.page_shift)];
+  return static_cast<uint32_t>(page) < static_cast<uint32_t>(r.pages) ? page : -1;
+}
+// Row `row` of the cache rows `base` (group g's, page 0's) that lie on `page`, and the step to the next rows of the page.
+__device__ __forceinline__ const LOGKV_G uint16_t* page_row(const RowsLaunch& r, const LOGKV_G uint16_t* base, int64_t sb,
+                                                            int64_t st, int page, int row, int64_t& step) {
+  step = page < 0 ? 0 : st;
+  const LOGKV_G uint16_t* zero = (const LOGKV_G uint16_t*)gp(kZeroRow);
+  return page < 0 ? zero : base + page * sb + (row & ((1 << r.page_shift) - 1)) * st;
 }
 
 // A bias in base 2. A finite one stays finite (a mask of the type's lowest value hides a row only

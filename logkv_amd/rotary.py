@@ -1,0 +1,212 @@
+"""Rotary positions: queries and keys turned by their tokens' positions, for training and inference.
+
+A model rotates before it calls this package's caches (they take post-RoPE queries and keys beside the pre-RoPE
+keys that routing uses); ``log_kv_rotary`` is that step in one launch, with angles formed in 64 bits instead of read
+from a table, and ``rotary_tables`` gives the tables of the same frequencies that ``LogStructuredKVCache`` takes
+(``cos_cache``, ``sin_cache``; half layout). The reference rotates in torch (litgpt/model.py:918-925).
+"""
+
+from __future__ import annotations
+
+import math
+import operator
+
+import torch
+
+from ._lib import check_activation_dtype, require_device
+from ._paged import F32, pack_rotary, paged_lib
+from ._rows import BF16, F16
+from .row_attention import _launch
+
+_TYPES = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
+_NO_ROWS = (0, 0, 0, 0)
+MAX_WIDTH = 512
+
+
+def rotary_frequencies(dim, base=10000.0, *, scaling=None, device="cuda"):
+    """(frequencies, amplitude) of ``dim`` rotated features: radians per position, float64 ``[dim / 2]`` on ``device``,
+    and the factor of the rotated values.
+
+    ``scaling`` fits them to contexts longer than a model was trained on: a dict with ``kind`` and ``factor``;
+
+    * ``"linear"``: every frequency divided by the factor;
+    * ``"wavelength"``: with ``original_max_seq_len`` n, ``low_freq_factor`` l and ``high_freq_factor`` h: wavelengths
+      above n / l divided by the factor, below n / h kept, interpolated between;
+    * ``"yarn"``: with ``original_max_seq_len`` and optionally ``beta_fast`` (32), ``beta_slow`` (1): pairs that turn
+      more than beta_fast times over that length kept, fewer than beta_slow times divided, a ramp over the pairs
+      between; amplitude ``0.1 ln(factor) + 1`` or ``attention_factor``."""
+    if dim < 2 or dim % 2 or dim > MAX_WIDTH:
+        raise ValueError(f"rotated features must be an even number up to {MAX_WIDTH}")
+    if not (math.isfinite(base) and base > 1.0):
+        raise ValueError("the rotary base must be finite and above 1")
+    freq = base ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    amplitude = 1.0
+    if scaling is not None:
+        given = dict(scaling)
+        kind, factor = given.pop("kind", None), float(given.pop("factor", 0.0))
+        if not (math.isfinite(factor) and factor > 0.0):
+            raise ValueError("scaling needs a positive factor")
+        try:
+            if kind == "linear":
+                freq = freq / factor
+            elif kind == "wavelength":
+                low, high = float(given.pop("low_freq_factor")), float(given.pop("high_freq_factor"))
+                turns = _length(given) * freq / (2 * math.pi)
+                if not 0.0 < low < high < math.inf:
+                    raise ValueError("low_freq_factor must be positive and below high_freq_factor")
+                keep = ((turns - low) / (high - low)).clamp(0, 1)
+                freq = freq * (keep + (1 - keep) / factor)
+            elif kind == "yarn":
+                n, fast, slow = _length(given), float(given.pop("beta_fast", 32.0)), float(given.pop("beta_slow", 1.0))
+                if not 0.0 < slow < fast < math.inf:
+                    raise ValueError("beta_slow must be positive and below beta_fast")
+
+                def pair(turns):   # the pair that turns so often over the original length
+                    return dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+                lo, hi = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), dim - 1)
+                ramp = ((torch.arange(dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+                freq = freq * (1 - ramp + ramp / factor)
+                amplitude = float(given.pop("attention_factor", 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0))
+                if not math.isfinite(amplitude):
+                    raise ValueError("attention_factor must be finite")
+            else:
+                raise ValueError(f"unknown scaling {kind!r}: 'linear', 'wavelength' or 'yarn'")
+        except KeyError as e:
+            raise ValueError(f"scaling {kind!r} needs {e.args[0]}") from None
+        if given:
+            raise ValueError(f"scaling {kind!r} takes no {', '.join(sorted(given))}")
+    return freq.to(device), amplitude
+
+
+def _length(given):
+    n = float(given.pop("original_max_seq_len"))
+    if not (math.isfinite(n) and n >= 1.0):
+        raise ValueError("original_max_seq_len must be at least 1")
+    return n
+
+
+def rotary_tables(frequencies, n, *, amplitude=1.0, dtype=torch.float32):
+    """(cos, sin) ``[n, dim]`` of positions 0 .. n - 1 in the half layout, as ``LogStructuredKVCache`` takes them: each
+    the 64-bit value rounded once."""
+    angles = torch.outer(torch.arange(n, dtype=torch.float64, device=frequencies.device), frequencies.double())
+    angles = torch.cat((angles, angles), dim=-1)
+    return (amplitude * torch.cos(angles)).to(dtype), (amplitude * torch.sin(angles)).to(dtype)
+
+
+def _rows(x):
+    """``x [B, H, T, d]`` with contiguous features."""
+    return x if x.stride(3) == 1 or x.size(3) == 1 else x.contiguous()
+
+
+def _like(x):
+    """New rows in ``x``'s dimension order, features contiguous."""
+    y = torch.empty_like(x)
+    return y if y.stride(3) == 1 or y.size(3) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def _check_frequencies(frequencies, dim, index):
+    """(address, rotated features, whether float32)."""
+    if (frequencies.ndim != 1 or frequencies.dtype not in (torch.float64, torch.float32)
+            or frequencies.get_device() != index or 2 * frequencies.size(0) > dim):
+        raise ValueError("frequencies must be float64 or float32 [rotated features / 2] on the rows' device, "
+                         f"for up to {dim} features")
+    if frequencies.requires_grad:
+        raise NotImplementedError("frequencies have no gradient")
+    return 2 * frequencies.size(0), int(frequencies.dtype == torch.float32)
+
+
+def _check_positions(positions, batch, tokens, index):
+    """(tensor or None, address, strides, whether int32, first position)."""
+    if not isinstance(positions, torch.Tensor):
+        return None, 0, 0, 0, 0, operator.index(positions)
+    shape = positions.shape
+    if (not (shape == (tokens,) or shape == (batch, tokens)) or positions.get_device() != index
+            or positions.dtype not in (torch.int64, torch.int32)):
+        raise ValueError("positions must be an int, or int64 or int32 [T] or [B, T] on the rows' device")
+    sb, st = (0, positions.stride(0)) if len(shape) == 1 else positions.stride()
+    return positions, positions.data_ptr(), sb, st, int(positions.dtype == torch.int32), 0
+
+
+def _rotate(q, k, frequencies, positions, interleaved, amplitude, sign):
+    """The launch on checked tensors; k or q may be None."""
+    x = k if q is None else q
+    batch, _, tokens, dim = x.shape
+    index = x.get_device()
+    rotated, freq_float = _check_frequencies(frequencies, dim, index)
+    frequencies = frequencies.contiguous()
+    positions, p_ptr, p_sb, p_st, p_int, first = _check_positions(positions, batch, tokens, index)
+    heads = groups = 0
+    q_in = q_to = k_in = k_to = _NO_ROWS
+    q_out = k_out = None
+    if q is not None:
+        q = _rows(q)
+        q_out, heads = _like(q), q.size(1)
+        if q.numel():
+            q_in, q_to = (q.data_ptr(), *q.stride()[:3]), (q_out.data_ptr(), *q_out.stride()[:3])
+    if k is not None:
+        k = _rows(k)
+        k_out, groups = _like(k), k.size(1)
+        if k.numel():
+            k_in, k_to = (k.data_ptr(), *k.stride()[:3]), (k_out.data_ptr(), *k_out.stride()[:3])
+    if not q_in[0] and not k_in[0]:
+        return q_out, k_out
+    args = pack_rotary(*q_in, *q_to, *k_in, *k_to, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0, 0, 0, 0,
+                       frequencies.data_ptr(), p_ptr, p_sb, p_st, 0, first, batch, heads, groups, tokens, dim, 0,
+                       rotated, _TYPES[x.dtype], 0, int(interleaved), freq_float, p_int, 0, 0, 0, 0, amplitude, sign)
+    _launch(paged_lib().logkv_rotary, "logkv_rotary", index, args)
+    return q_out, k_out
+
+
+class _Rotary(torch.autograd.Function):
+    """The rotation as a function of the rows; its gradient is the rotation back."""
+
+    @staticmethod
+    def forward(ctx, q, k, frequencies, positions, interleaved, amplitude, sign):
+        ctx.set_materialize_grads(False)
+        at = positions if isinstance(positions, torch.Tensor) else None
+        ctx.save_for_backward(frequencies, *(() if at is None else (at,)))
+        ctx.rest = (None if at is not None else positions, interleaved, amplitude, sign)
+        out = _rotate(q, k, frequencies, positions, interleaved, amplitude, sign)
+        ctx.mark_non_differentiable(*(y for y, need in zip(out, ctx.needs_input_grad) if y is not None and not need))
+        return out
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        frequencies, *at = ctx.saved_tensors
+        positions, interleaved, amplitude, sign = ctx.rest
+        dq, dk = (g if need else None for g, need in zip((dq, dk), ctx.needs_input_grad))
+        if dq is None and dk is None:
+            return (None,) * 7
+        dq, dk = _Rotary.apply(dq, dk, frequencies, at[0] if at else positions, interleaved, amplitude, -sign)
+        return dq, dk, None, None, None, None, None
+
+
+def log_kv_rotary(q, k, frequencies, positions=0, *, interleaved=False, amplitude=1.0):
+    """(q, k) rotated by their tokens' positions: pair i of a head's first ``2 n`` features turned by ``position *
+    frequencies[i]`` and scaled by ``amplitude``, its other features as they are.
+
+    ``q [B, n_heads, T, d]`` and ``k [B, G, T, d]`` (or None) in one of bfloat16, float16 or float32, of any strides;
+    ``frequencies [n]`` in radians per position, float64 or float32 (``rotary_frequencies``); ``positions`` the first
+    token's (an int), or int64 or int32 ``[T]`` or ``[B, T]``. Pairs are features ``(i, i + n)``, or ``(2 i, 2 i + 1)``
+    with ``interleaved``. Angles are formed in 64 bits, products in float32, rounded once. New tensors in the inputs'
+    dimension order; differentiable in q and k any number of times."""
+    if k is None:
+        x, others = q, ()
+    else:
+        x, others = q, (k,)
+    if x.ndim != 4 or any(y.ndim != 4 or y.size(0) != x.size(0) or y.shape[2:] != x.shape[2:] for y in others):
+        raise ValueError("q and k must be [B, heads, T, d] of one batch, length and width")
+    check_activation_dtype(x.dtype)
+    require_device(x, "q")
+    if any(y.dtype != x.dtype or y.device != x.device for y in others):
+        raise ValueError("q and k must be of one dtype on one device")
+    if not 1 <= x.size(3) <= MAX_WIDTH:
+        raise ValueError(f"head widths must be in [1, {MAX_WIDTH}]")
+    amplitude = float(amplitude)
+    if not math.isfinite(amplitude):
+        raise ValueError("amplitude must be finite")
+    if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
+        _check_frequencies(frequencies, x.size(3), x.get_device())
+        return _Rotary.apply(q, k, frequencies, positions, bool(interleaved), amplitude, 1.0)
+    return _rotate(q, k, frequencies, positions, interleaved, amplitude, 1.0)
