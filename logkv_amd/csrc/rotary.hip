@@ -2,14 +2,16 @@
 //
 //   (a, b) -> amplitude (a cos t - b sin t, b cos t + a sin t),  t = sign pos f_i
 //
-// for the pairs i of a head's rotated part; the rest passes through. A block takes TPB tokens with all
-// of their heads, so that an angle is formed once for every head: as turns, pos (f / 2 pi) in 64 bits
-// with the product's rounding error added back, reduced to [-1/2, 1/2] before it is rounded to float32
-// (a float32 product would be off by 2^-8 of a turn at position 65536). Sine and cosine of the block's
-// angles wait in LDS. An item is VEC pairs, VEC features that pass through, or VEC features of a value;
-// threads load a batch of items before they form angles.
+// for the pairs i of a head's rotated part; the rest passes through. A block takes TPB tokens of a batch
+// row with all of their heads, so that an angle is formed once for every head: as turns, pos (f / 2 pi) in
+// 64 bits with the product's rounding error added back, reduced to [-1/2, 1/2] before it is rounded to
+// float32 (a float32 product would be off by 2^-8 of a turn at position 65536). Sine and cosine of the
+// block's angles wait in LDS behind the block's only barrier. An item is VEC pairs, VEC features that pass
+// through, or VEC features of a value; a thread loads its first query's, key's and value's item before it
+// forms angles, and then one ahead.
 // Bound by HBM for many tokens, by the chain length -> table entry -> store for one.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.hpp"
 
@@ -18,36 +20,22 @@ namespace logkv {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxAngles = 1024;   // of a block: 4 tokens of 512 rotated features
-constexpr int kBatch = 4;          // items of a thread on their way at once
+constexpr int kMaxTokens = 8;      // of a block
+constexpr int kMaxAngles = 1024;   // of a block
+constexpr int64_t kMostItems = 1024, kLeastBlocks = 1024;   // of a block beyond one token, and of a launch
 
 // What the launch derives from the arguments. Quotients by multiplication: n / d = high32(n * magic),
 // exact for n * d < 2^32 (checked by the launch).
 struct RotaryPlan {
-  int tpb;                      // tokens of a block
-  int turned, items;            // items of a head: pairs, and in all
-  int q_items, k_items, v_items, token_items;   // of a token
-  int v_units;                  // items of a value
-  uint32_t by_token, by_head, by_value, by_half;
-  int half;
+  int tpb, tiles;         // tokens of a block, blocks of a batch row
+  int half, turned;       // pairs of a head, and items of pairs
+  int items[3], heads[3]; // of q, k and v: items of a head, heads
+  uint32_t by_item[3], by_head[3], by_half;
 };
 
 __device__ __forceinline__ int quotient(int n, uint32_t magic, int d) {
   return d == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), magic));
 }
-
-template <int DT>
-struct Type {
-  typedef uint16_t raw;
-  static __device__ __forceinline__ float get(raw x) { return Elem<DT>::to_f32(x); }
-  static __device__ __forceinline__ raw put(float x) { return Elem<DT>::from_f32(x); }
-};
-template <>
-struct Type<LOGKV_F32> {
-  typedef float raw;
-  static __device__ __forceinline__ float get(raw x) { return x; }
-  static __device__ __forceinline__ raw put(float x) { return x; }
-};
 
 template <typename T, int N>
 struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) Pack {
@@ -63,82 +51,106 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& x) {
   *(LOGKV_G Pack<T, N>*)gp(p) = x;
 }
 
+template <int DT>
+struct Type {
+  typedef uint16_t raw;
+  static __device__ __forceinline__ float get(raw x) { return Elem<DT>::to_f32(x); }
+  // Rounded to nearest, two at a time by the hardware's conversions.
+  template <int N>
+  static __device__ __forceinline__ Pack<raw, N> put(const float (&y)[N]) {
+    Pack<raw, N> z;
+    if constexpr (N == 1) {
+      z.x[0] = Elem<DT>::from_f32(y[0]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; k += 2) {
+        uint32_t two;
+        if constexpr (DT == LOGKV_BF16) two = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{y[k], y[k + 1]}, bf16x2));
+        else two = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{y[k], y[k + 1]}, f16x2));
+        z.x[k] = static_cast<raw>(two), z.x[k + 1] = static_cast<raw>(two >> 16);
+      }
+    }
+    return z;
+  }
+};
+template <>
+struct Type<LOGKV_F32> {
+  typedef float raw;
+  static __device__ __forceinline__ float get(raw x) { return x; }
+  template <int N>
+  static __device__ __forceinline__ Pack<raw, N> put(const float (&y)[N]) {
+    Pack<raw, N> z;
+#pragma unroll
+    for (int k = 0; k < N; ++k) z.x[k] = y[k];
+    return z;
+  }
+};
+
 }  // namespace
 
 template <int DT, int CT, int VEC, bool APPEND>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(logkv_rotary_args a, RotaryPlan p) {
   typedef Type<DT> In;
-  typedef Type<CT> Out;
   typedef typename In::raw raw;
-  typedef typename Out::raw cached;
+  typedef Type<APPEND ? CT : LOGKV_BF16> Out;   // of an append's pages
+  typedef uint16_t cached;
   __shared__ __align__(16) float2 turn_s[kMaxAngles];
-  __shared__ int64_t pos_s[16], k_at[16], v_at[16];
+  __shared__ int64_t k_at[kMaxTokens], v_at[kMaxTokens];   // rows in the pages, below 0 for none
   const int tid = threadIdx.x;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * p.tpb, all = static_cast<int64_t>(a.n_batch) * a.tokens;
-  const int here = static_cast<int>(imin64(p.tpb, all - first)), total = here * p.token_items;
+  const int b = static_cast<int>(blockIdx.x) / p.tiles, t0 = (static_cast<int>(blockIdx.x) - b * p.tiles) * p.tpb;
+  const int here = min(p.tpb, a.tokens - t0);
 
-  // An item: its token, whose features they are (0: q, 1: k, 2: v), its head and its place there.
+  // Item e of the block's queries (OF 0), keys (1) or values (2): its token, head, first feature and that of its second
+  // vector (-1: it passes through).
   struct Item {
-    int token, of, head, j;
+    int token, head, f, second;
   };
-  auto item = [&](int e) {
+  auto item = [&](auto of, int e) {
+    constexpr int OF = decltype(of)::value;
+    const int row = quotient(e, p.by_item[OF], p.items[OF]), j = e - row * p.items[OF];
     Item x;
-    x.token = quotient(e, p.by_token, p.token_items);
-    int r = e - x.token * p.token_items;
-    x.of = r < p.q_items ? 0 : r < p.q_items + p.k_items ? 1 : 2;
-    r -= x.of == 0 ? 0 : x.of == 1 ? p.q_items : p.q_items + p.k_items;
-    const int d = x.of == 2 ? p.v_units : p.items;
-    x.head = quotient(r, x.of == 2 ? p.by_value : p.by_head, d);
-    x.j = r - x.head * d;
+    x.token = quotient(row, p.by_head[OF], p.heads[OF]);
+    x.head = row - x.token * p.heads[OF];
+    x.second = -1;
+    if (OF == 2) {
+      x.f = VEC * j;
+    } else if (j < p.turned) {
+      x.f = a.interleaved ? 2 * VEC * j : VEC * j;
+      x.second = a.interleaved ? x.f + VEC : x.f + p.half;
+    } else {
+      x.f = a.rotated + VEC * (j - p.turned);
+    }
     return x;
   };
-  auto feature = [&](const Item& x, int& second) {
-    // The item's first feature, and that of its second vector.
-    if (x.of < 2 && x.j < p.turned) {
-      const int f = a.interleaved ? 2 * VEC * x.j : VEC * x.j;
-      second = a.interleaved ? f + VEC : f + p.half;
-      return f;
-    }
-    second = -1;
-    return x.of < 2 ? a.rotated + VEC * (x.j - p.turned) : VEC * x.j;
+  typedef Pack<raw, VEC> vec;
+  // An item's vectors on their way (of an item past the last: nothing).
+  auto load = [&](auto of, int e, int n, vec& x0, vec& x1) {
+    constexpr int OF = decltype(of)::value;
+    if (e >= n) return;
+    const Item x = item(of, e);
+    const raw* row = OF == 0   ? static_cast<const raw*>(a.q) + b * a.q_sb + x.head * a.q_sh + (t0 + x.token) * a.q_st
+                     : OF == 1 ? static_cast<const raw*>(a.k) + b * a.k_sb + x.head * a.k_sh + (t0 + x.token) * a.k_st
+                               : static_cast<const raw*>(a.v) + b * a.v_sb + x.head * a.v_sh + (t0 + x.token) * a.v_st;
+    x0 = load_pack<raw, VEC>(row + x.f);
+    if (OF < 2) x1 = load_pack<raw, VEC>(row + (x.second < 0 ? x.f : x.second));
   };
-  auto batch_row = [&](int token, int& t) {
-    const int64_t at = first + token;
-    const int b = static_cast<int>(at / a.tokens);
-    t = static_cast<int>(at - static_cast<int64_t>(b) * a.tokens);
-    return b;
-  };
-  auto source = [&](const Item& x) {
-    int t;
-    const int b = batch_row(x.token, t);
-    if (x.of == 0) return static_cast<const raw*>(a.q) + b * a.q_sb + x.head * a.q_sh + t * a.q_st;
-    if (x.of == 1) return static_cast<const raw*>(a.k) + b * a.k_sb + x.head * a.k_sh + t * a.k_st;
-    return static_cast<const raw*>(a.v) + b * a.v_sb + x.head * a.v_sh + t * a.v_st;
-  };
+  std::integral_constant<int, 0> of_q;
+  std::integral_constant<int, 1> of_k;
+  std::integral_constant<int, 2> of_v;
+  const int nq = here * p.heads[0] * p.items[0], nk = here * p.heads[1] * p.items[1];
+  const int nv = APPEND ? here * p.heads[2] * p.items[2] : 0;
+  // The first item of each kind is loaded before the angles are formed.
+  vec q0, q1, k0, k1, v0, v1;
+  load(of_q, tid, nq, q0, q1);
+  load(of_k, tid, nk, k0, k1);
+  if constexpr (APPEND) load(of_v, tid, nv, v0, v1);
 
-  Pack<raw, VEC> x0[kBatch], x1[kBatch];
-  auto load = [&](int e0) {
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int e = min(e0 + kThreads * i, total - 1);
-      const Item it = item(e);
-      int second;
-      const int f = feature(it, second);
-      const raw* row = source(it);
-      x0[i] = load_pack<raw, VEC>(row + f);
-      x1[i] = load_pack<raw, VEC>(row + (second < 0 ? f : second));
-    }
-  };
-  load(tid);
-
-  // Positions, and where the tokens' rows are stored.
-  if (tid < here) {
-    int t;
-    const int b = batch_row(tid, t);
-    int64_t pos = a.first + t, row = 0;
-    if constexpr (APPEND) {
-      row = static_cast<int64_t>(a.len_add) + (a.lengths ? gp(a.lengths)[b] : 0) + t;
-      pos = a.first + row;
+  int64_t row0 = 0;   // the row of the batch row's first token
+  if constexpr (APPEND) {
+    row0 = static_cast<int64_t>(a.len_add) + (a.lengths ? gp(a.lengths)[b] : 0);
+    if (tid < here) {
+      const int t = t0 + tid;
+      const int64_t row = row0 + t;
       int64_t ko = -1, vo = -1;
       if (row >= 0 && row < static_cast<int64_t>(a.table_len) * a.page && (!a.counts || t < gp(a.counts)[b])) {
         const int shift = __builtin_ctz(a.page), slot = static_cast<int>(row) & (a.page - 1);
@@ -151,20 +163,20 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(logkv_rotary_args a, R
       k_at[tid] = ko;
       v_at[tid] = vo;
     }
-    if (a.first_dev) pos += gp(a.first_dev)[b];
+  }
+  for (int e = tid; e < here * p.half; e += kThreads) {
+    const int token = quotient(e, p.by_half, p.half), i = e - token * p.half, t = t0 + token;
+    int64_t pos;
     if (a.positions) {
       const int64_t at = b * a.pos_sb + t * a.pos_st;
       pos = a.pos_int ? gp(static_cast<const int32_t*>(a.positions))[at] : gp(static_cast<const int64_t*>(a.positions))[at];
+    } else {
+      pos = a.first + (a.first_dev ? gp(a.first_dev)[b] : 0) + row0 + t;
     }
-    pos_s[tid] = pos;
-  }
-  __syncthreads();
-  for (int e = tid; e < here * p.half; e += kThreads) {
-    const int token = quotient(e, p.by_half, p.half), i = e - token * p.half;
     const double f = a.freq_float ? static_cast<double>(gp(static_cast<const float*>(a.frequencies))[i])
                                   : gp(static_cast<const double*>(a.frequencies))[i];
-    const double turns = f * 0.15915494309189533577, n = static_cast<double>(pos_s[token]);
-    const double u = n * turns, lost = __builtin_fma(n, turns, -u);
+    const double turns = f * 0.15915494309189533577, at = static_cast<double>(pos);
+    const double u = at * turns, lost = __builtin_fma(at, turns, -u);
     const float x = static_cast<float>((u - __builtin_rint(u)) + lost);
     float sn, cs;
     sincospif(2.f * x, &sn, &cs);
@@ -172,69 +184,64 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(logkv_rotary_args a, R
   }
   __syncthreads();
 
-  for (int e0 = tid; e0 < total; e0 += kBatch * kThreads) {
+  auto turn = [&](const Item& x, float (&y0)[VEC], float (&y1)[VEC]) {
+    if (x.second < 0) return;
+    const float2* at = turn_s + x.token * p.half + (a.interleaved ? x.f / 2 : x.f);
+    auto pair = [](float& u, float& v, float2 c) {
+      const float r = __builtin_fmaf(u, c.x, -(v * c.y));
+      v = __builtin_fmaf(v, c.x, u * c.y);
+      u = r;
+    };
+    if (VEC > 1 && a.interleaved) {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int e = e0 + kThreads * i;
-      if (e >= total) break;
-      const Item it = item(e);
-      int second, t;
-      const int f = feature(it, second), b = batch_row(it.token, t);
-      float y0[VEC], y1[VEC];
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) y0[k] = In::get(x0[i].x[k]), y1[k] = In::get(x1[i].x[k]);
-      if (second >= 0) {
-        const float2* turn = turn_s + it.token * p.half + VEC * it.j;
-        auto turned = [&](float& u, float& w, float2 c) {
-          const float r = __builtin_fmaf(u, c.x, -(w * c.y));
-          w = __builtin_fmaf(w, c.x, u * c.y);
-          u = r;
-        };
-        if (VEC > 1 && a.interleaved) {
-#pragma unroll
-          for (int k = 0; k + 1 < VEC; k += 2) {
-            turned(y0[k], y0[k + 1], turn[k / 2]);
-            turned(y1[k], y1[k + 1], turn[(VEC + k) / 2]);
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) turned(y0[k], y1[k], turn[k]);
-        }
+      for (int k = 0; k + 1 < VEC; k += 2) {
+        pair(y0[k], y0[k + 1], at[k / 2]);
+        pair(y1[k], y1[k + 1], at[(VEC + k) / 2]);
       }
-      if (it.of == 0 || (!APPEND && it.of == 1)) {
-        raw* o = it.of == 0 ? static_cast<raw*>(a.q_out) + b * a.qo_sb + it.head * a.qo_sh + t * a.qo_st
-                            : static_cast<raw*>(a.k_out) + b * a.ko_sb + it.head * a.ko_sh + t * a.ko_st;
-        Pack<raw, VEC> z;
+    } else {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) z.x[k] = In::put(y0[k]);
-        store_pack(o + f, z);
-        if (second >= 0) {
+      for (int k = 0; k < VEC; ++k) pair(y0[k], y1[k], at[k]);
+    }
+  };
+  auto spread = [](const vec& x, float (&y)[VEC]) {
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) z.x[k] = In::put(y1[k]);
-          store_pack(o + second, z);
-        }
-      } else if constexpr (APPEND) {
-        Pack<cached, VEC> z0, z1;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) z0.x[k] = Out::put(y0[k]), z1.x[k] = Out::put(y1[k]);
-        if (it.of == 1) {
-          if (a.k_out) {
-            cached* o = static_cast<cached*>(a.k_out) + b * a.ko_sb + it.head * a.ko_sh + t * a.ko_st;
-            store_pack(o + f, z0);
-            if (second >= 0) store_pack(o + second, z1);
-          }
-          if (k_at[it.token] >= 0) {
-            cached* o = reinterpret_cast<cached*>(a.k_pages) + k_at[it.token] + it.head * a.kp_sg;
-            store_pack(o + f, z0);
-            if (second >= 0) store_pack(o + second, z1);
-          }
-        } else if (v_at[it.token] >= 0) {
-          store_pack(reinterpret_cast<cached*>(a.v_pages) + v_at[it.token] + it.head * a.vp_sg + f, z0);
+    for (int k = 0; k < VEC; ++k) y[k] = In::get(x.x[k]);
+  };
+  // All items of one kind; the next one's loads are issued before one is finished.
+  auto finish = [&](auto of, int n, vec& x0, vec& x1) {
+    constexpr int OF = decltype(of)::value;
+#pragma unroll 1
+    for (int e = tid; e < n; e += kThreads) {
+      const vec c0 = x0, c1 = x1;
+      load(of, e + kThreads, n, x0, x1);
+      const Item x = item(of, e);
+      float y0[VEC], y1[VEC];
+      spread(c0, y0);
+      if constexpr (OF == 2) {
+        if (v_at[x.token] >= 0) store_pack(a.v_pages + v_at[x.token] + x.head * a.vp_sg + x.f, Out::put(y0));
+      } else {
+        spread(c1, y1);
+        turn(x, y0, y1);
+        auto store = [&](auto* row, auto as) {
+          typedef decltype(as) T;
+          store_pack(row + x.f, T::put(y0));
+          if (x.second >= 0) store_pack(row + x.second, T::put(y1));
+        };
+        const int t = t0 + x.token;
+        if constexpr (OF == 0) {
+          store(static_cast<raw*>(a.q_out) + b * a.qo_sb + x.head * a.qo_sh + t * a.qo_st, In());
+        } else if constexpr (!APPEND) {
+          store(static_cast<raw*>(a.k_out) + b * a.ko_sb + x.head * a.ko_sh + t * a.ko_st, In());
+        } else {
+          if (a.k_out) store(static_cast<cached*>(a.k_out) + b * a.ko_sb + x.head * a.ko_sh + t * a.ko_st, Out());
+          if (k_at[x.token] >= 0) store(a.k_pages + k_at[x.token] + x.head * a.kp_sg, Out());
         }
       }
     }
-    if (e0 + kBatch * kThreads < total) load(e0 + kBatch * kThreads);
-  }
+  };
+  finish(of_q, nq, q0, q1);
+  finish(of_k, nk, k0, k1);
+  if constexpr (APPEND) finish(of_v, nv, v0, v1);
 }
 
 namespace {
@@ -262,22 +269,26 @@ int launch_vec(const logkv_rotary_args& a, hipStream_t stream) {
   RotaryPlan p{};
   p.half = a.rotated / 2;
   p.turned = p.half / vec;
-  p.items = p.turned + (a.dim - a.rotated) / vec;
-  p.q_items = a.q ? a.n_heads * p.items : 0;
-  p.k_items = a.k ? a.n_groups * p.items : 0;
-  p.v_units = APPEND ? a.dim_v / vec : 0;
-  p.v_items = a.n_groups * p.v_units;
-  p.token_items = p.q_items + p.k_items + p.v_items;
-  const int64_t all = static_cast<int64_t>(a.n_batch) * a.tokens;
-  // Four tokens a block where that leaves every CU blocks to overlap.
-  p.tpb = all >= 4 * 1024 ? 4 : 1;
-  const int64_t most = static_cast<int64_t>(p.tpb) * p.token_items, widest = std::max({p.token_items, p.items, p.v_units, p.half});
-  if (most * widest >= int64_t(1) << 32) return refuse("too many heads for one rotation");
-  p.by_token = magic_of(p.token_items);
-  p.by_head = magic_of(p.items);
-  p.by_value = magic_of(p.v_units);
+  const int row_items = p.turned + (a.dim - a.rotated) / vec;
+  const int items[3] = {row_items, row_items, APPEND ? a.dim_v / vec : 1};
+  const int heads[3] = {a.q ? a.n_heads : 0, a.k ? a.n_groups : 0, APPEND ? a.n_groups : 0};
+  int64_t token_items = 0, widest = p.half;
+  for (int of = 0; of < 3; ++of) {
+    p.items[of] = items[of], p.heads[of] = heads[of];
+    p.by_item[of] = magic_of(items[of]), p.by_head[of] = magic_of(heads[of]);
+    token_items += int64_t(items[of]) * heads[of];
+    widest = std::max<int64_t>({widest, items[of], heads[of]});
+  }
   p.by_half = magic_of(p.half);
-  const int64_t blocks = (all + p.tpb - 1) / p.tpb;
+  // As many tokens a block as its angles have room for, where that leaves every CU blocks to overlap.
+  p.tpb = 1;
+  while (p.tpb < kMaxTokens && p.tpb < a.tokens && 2 * p.tpb * p.half <= kMaxAngles && p.tpb * token_items < kMostItems &&
+         static_cast<int64_t>(a.n_batch) * a.tokens >= 2 * p.tpb * kLeastBlocks)
+    p.tpb *= 2;
+  // A block's items, and their products in quotient().
+  if (p.tpb * token_items * std::max<int64_t>(widest, 1) >= int64_t(1) << 32) return refuse("too many heads for one rotation");
+  p.tiles = (a.tokens + p.tpb - 1) / p.tpb;
+  const int64_t blocks = static_cast<int64_t>(p.tiles) * a.n_batch;
   if (blocks > INT32_MAX) return refuse("too many tokens for one rotation");
   const dim3 grid(static_cast<uint32_t>(blocks));
   if (vec == 8) {

@@ -26,7 +26,7 @@ import torch
 
 from ._lib import check_activation_dtype, require_device
 from ._paged import PagedArgs, pack_paged, pack_rotary, paged_lib
-from .rotary import MAX_WIDTH, _NO_ROWS, _TYPES, _check_frequencies, _check_positions, _like, _rows
+from .rotary import MAX_WIDTH, _NO_ROWS, _TYPES, _check_frequencies, _check_positions, _in_and_out
 from .row_attention import (_LENGTH_DTYPES, _NO_STRIDES, _ROW_DTYPES, _launch, _lengths, _repeats, _small_rows, _tree,
                             _unit_strides)
 
@@ -51,23 +51,26 @@ class SharedPrefix(NamedTuple):
 
 def _check_pages(k_pages, v_pages, groups):
     """(dtype code, page size) of a pool whose rows are read in 16-byte units; its device is checked too."""
-    if k_pages.ndim != 4 or v_pages.ndim != 4 or k_pages.shape[:3] != v_pages.shape[:3] or k_pages.size(1) != groups:
+    shape, dtype = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or v_pages.ndim != 4 or shape[:3] != v_pages.shape[:3] or shape[1] != groups:
         raise ValueError("pages must be [pages, groups, page_size, d], keys and values alike")
-    page = k_pages.size(2)
+    page = shape[2]
     if page < MIN_PAGE or page & (page - 1):
         raise ValueError(f"page_size must be a power of two from {MIN_PAGE} on, got {page}")
-    code = _ROW_DTYPES.get(k_pages.dtype)
-    if code is None or v_pages.dtype != k_pages.dtype:
+    code = _ROW_DTYPES.get(dtype)
+    if code is None or v_pages.dtype != dtype:
         raise ValueError("the pages must be bfloat16 or float16")
-    require_device(k_pages, "k_pages")
+    if not k_pages.is_cuda:
+        require_device(k_pages, "k_pages")
     return code, page
 
 
 def _check_table(table, rows, index):
-    if (table.ndim != 2 or table.size(0) != rows or table.dtype != torch.int32 or table.get_device() != index
-            or table.size(1) > 1 and table.stride(1) != 1):
+    shape = table.shape
+    if (len(shape) != 2 or shape[0] != rows or table.dtype != torch.int32 or table.get_device() != index
+            or shape[1] > 1 and table.stride(1) != 1):
         raise ValueError(f"a page table must be int32 [{rows}, n] on the pages' device with contiguous rows")
-    return table.data_ptr(), table.stride(0), table.size(1)
+    return table.data_ptr(), table.stride(0), shape[1]
 
 
 def _check_counts(counts, batch, index):
@@ -91,21 +94,26 @@ def log_kv_paged_append(k, v, k_pages, v_pages, table, lengths, *, q=None, frequ
     Returned are the rotated queries in their dtype (None without ``q``) and the keys in the pages' dtype, as
     ``log_kv_paged_attention`` takes them beside the rows before the call. Sequences must not share the pages that a
     call writes."""
-    if k.ndim != 4 or v.ndim != 4 or v.shape[:3] != k.shape[:3] or q is not None and (
-            q.ndim != 4 or q.size(0) != k.size(0) or q.shape[2:] != k.shape[2:]):
-        raise ValueError("new rows must be k [B, G, T, dk] and v [B, G, T, dv], queries [B, n_heads, T, dk]")
-    batch, groups, tokens, dk = k.shape
-    dv, index = v.size(3), k_pages.get_device()
+    k_shape, v_shape, dtype, index = k.shape, v.shape, k.dtype, k_pages.get_device()
+    if len(k_shape) != 4 or len(v_shape) != 4 or v_shape[:3] != k_shape[:3]:
+        raise ValueError("new rows must be k [B, G, T, dk] and v [B, G, T, dv]")
+    batch, groups, tokens, dk = k_shape
+    dv = v_shape[3]
     code, page = _check_pages(k_pages, v_pages, groups)
-    given = (k, v) if q is None else (k, v, q)
-    check_activation_dtype(k.dtype)
-    if any(x.dtype != k.dtype or x.get_device() != index for x in given) or v_pages.get_device() != index:
-        raise ValueError("queries and new rows must be of one dtype, on the pages' device")
+    if v.dtype != dtype or not k.get_device() == v.get_device() == v_pages.get_device() == index:
+        raise ValueError("new rows must be of one dtype, on the pages' device")
+    if q is not None and (q.ndim != 4 or q.size(0) != batch or q.size(2) != tokens or q.size(3) != dk or q.dtype != dtype
+                          or q.get_device() != index):
+        raise ValueError("queries must be [B, n_heads, T, dk], in the new rows' dtype on their device")
+    check_activation_dtype(dtype)
+    kp_sp, kp_sg, kp_st, kp_sd = k_pages.stride()
+    vp_sp, vp_sg, vp_st, vp_sd = v_pages.stride()
     if k_pages.size(3) != dk or v_pages.size(3) != dv or not 1 <= dk <= MAX_WIDTH or not 1 <= dv <= MAX_WIDTH:
         raise ValueError(f"the pages' rows must be as wide as the new ones, up to {MAX_WIDTH} features")
-    if torch.is_grad_enabled() and any(x.requires_grad for x in (*given, k_pages, v_pages)):
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad
+                                    or q is not None and q.requires_grad):
         raise NotImplementedError("a paged append is for inference: it has no gradient (run it under torch.no_grad())")
-    if k_pages.stride(3) != 1 and dk > 1 or v_pages.stride(3) != 1 and dv > 1:
+    if kp_sd != 1 and dk > 1 or vp_sd != 1 and dv > 1:
         raise ValueError("the pages' features must be contiguous")
     if _repeats(k_pages) or _repeats(v_pages):
         raise ValueError("pages are written: their rows must not share memory (expanded tensors)")
@@ -116,46 +124,49 @@ def log_kv_paged_append(k, v, k_pages, v_pages, table, lengths, *, q=None, frequ
     if table_len * page > 2 ** 30:
         raise ValueError("a sequence has at most 2^30 rows")
     lengths, n_ptr, _, len_add = _lengths(lengths, batch, table_len * page, index, tokens if counts is None else 0)
+    c_ptr = 0
     if counts is not None:
         counts = _check_counts(counts, batch, index)
+        c_ptr = counts.data_ptr()
+    first_ptr = 0
     if isinstance(first, torch.Tensor):
         if first.shape != (batch,) or first.dtype != torch.int64 or first.get_device() != index:
             raise ValueError("first must be an int or an int64 tensor [batch] on the pages' device")
-        first_dev, first_ptr, first = first.contiguous(), first.data_ptr(), 0
+        first_dev, first = first.contiguous(), 0
         first_ptr = first_dev.data_ptr()
     else:
-        first_ptr, first = 0, operator.index(first)
+        first = operator.index(first)
     rotated = freq_ptr = freq_float = 0
     if frequencies is not None:
         rotated, freq_float = _check_frequencies(frequencies, dk, index)
-        frequencies = frequencies.contiguous()
+        if not frequencies.is_contiguous():
+            frequencies = frequencies.contiguous()
         freq_ptr = frequencies.data_ptr()
     p_ptr = p_sb = p_st = p_int = 0
     if positions is not None:
         if not isinstance(positions, torch.Tensor):
             raise ValueError("positions must be int64 or int32 [T] or [B, T] on the pages' device")
         positions, p_ptr, p_sb, p_st, p_int, _ = _check_positions(positions, batch, tokens, index)
-    k, v = _rows(k), _rows(v)
+    heads, q_out, q_in, q_to = 0, q, _NO_ROWS, _NO_ROWS
+    if q is not None and rotated:
+        heads = q.size(1)
+        q, q_out, q_in, q_to = _in_and_out(q)
+    if dk > 1 and k.stride(3) != 1:
+        k = k.contiguous()
+    if dv > 1 and v.stride(3) != 1:
+        v = v.contiguous()
     # Without a rotation or a rounding the keys are the caller's own.
-    k_out = k if not rotated and k.dtype == k_pages.dtype else k.new_empty(k.shape, dtype=k_pages.dtype)
-    q_out = q_in = q_to = None
-    if q is not None:
-        q = _rows(q)
-        q_out = _like(q) if rotated else q
+    k_out, k_to = k, _NO_ROWS
+    if rotated or dtype != k_pages.dtype:
+        k_out = k_pages.new_empty(k_shape)
+        k_to = k_out.data_ptr(), *k_out.stride()[:3]
     if not k.numel() or not v.numel():
         return q_out, k_out
-    q_in = q_to = k_to = _NO_ROWS
-    heads = 0
-    if q is not None and rotated and q.numel():
-        heads, q_in, q_to = q.size(1), (q.data_ptr(), *q.stride()[:3]), (q_out.data_ptr(), *q_out.stride()[:3])
-    if k_out is not k:
-        k_to = (k_out.data_ptr(), *k_out.stride()[:3])
     args = pack_rotary(*q_in, *q_to, k.data_ptr(), *k.stride()[:3], *k_to, v.data_ptr(), *v.stride()[:3],
-                       k_pages.data_ptr(), *k_pages.stride()[:3], v_pages.data_ptr(), *v_pages.stride()[:3],
-                       table_ptr, table_sb, n_ptr, 0 if counts is None else counts.data_ptr(), freq_ptr,
-                       p_ptr, p_sb, p_st, first_ptr, first, batch, heads, groups, tokens, dk, dv, rotated,
-                       _TYPES[k.dtype], code, int(interleaved), freq_float, p_int, len_add, page, table_len,
-                       k_pages.size(0), amplitude, 1.0)
+                       k_pages.data_ptr(), kp_sp, kp_sg, kp_st, v_pages.data_ptr(), vp_sp, vp_sg, vp_st,
+                       table_ptr, table_sb, n_ptr, c_ptr, freq_ptr, p_ptr, p_sb, p_st, first_ptr, first, batch, heads,
+                       groups, tokens, dk, dv, rotated, _TYPES[dtype], code, int(interleaved), freq_float, p_int,
+                       len_add, page, table_len, k_pages.size(0), amplitude, 1.0)
     _launch(paged_lib().logkv_paged_append, "logkv_paged_append", index, args)
     return q_out, k_out
 

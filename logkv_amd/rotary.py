@@ -94,15 +94,18 @@ def rotary_tables(frequencies, n, *, amplitude=1.0, dtype=torch.float32):
     return (amplitude * torch.cos(angles)).to(dtype), (amplitude * torch.sin(angles)).to(dtype)
 
 
-def _rows(x):
-    """``x [B, H, T, d]`` with contiguous features."""
-    return x if x.stride(3) == 1 or x.size(3) == 1 else x.contiguous()
-
-
-def _like(x):
-    """New rows in ``x``'s dimension order, features contiguous."""
+def _in_and_out(x):
+    """(rows with contiguous features, new ones in their dimension order, addresses and strides of both: 0 of none)."""
     y = torch.empty_like(x)
-    return y if y.stride(3) == 1 or y.size(3) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    sb, sh, st, sd = x.stride()
+    tb, th, tt, td = y.stride()
+    if (sd != 1 or td != 1) and x.size(3) != 1:
+        x = x.contiguous()
+        y = torch.empty_like(x)
+        (sb, sh, st, _), (tb, th, tt, _) = x.stride(), y.stride()
+    if not x.numel():
+        return x, y, _NO_ROWS, _NO_ROWS
+    return x, y, (x.data_ptr(), sb, sh, st), (y.data_ptr(), tb, th, tt)
 
 
 def _check_frequencies(frequencies, dim, index):
@@ -134,21 +137,18 @@ def _rotate(q, k, frequencies, positions, interleaved, amplitude, sign):
     batch, _, tokens, dim = x.shape
     index = x.get_device()
     rotated, freq_float = _check_frequencies(frequencies, dim, index)
-    frequencies = frequencies.contiguous()
+    if not frequencies.is_contiguous():
+        frequencies = frequencies.contiguous()
     positions, p_ptr, p_sb, p_st, p_int, first = _check_positions(positions, batch, tokens, index)
     heads = groups = 0
     q_in = q_to = k_in = k_to = _NO_ROWS
     q_out = k_out = None
     if q is not None:
-        q = _rows(q)
-        q_out, heads = _like(q), q.size(1)
-        if q.numel():
-            q_in, q_to = (q.data_ptr(), *q.stride()[:3]), (q_out.data_ptr(), *q_out.stride()[:3])
+        q, q_out, q_in, q_to = _in_and_out(q)
+        heads = q.size(1)
     if k is not None:
-        k = _rows(k)
-        k_out, groups = _like(k), k.size(1)
-        if k.numel():
-            k_in, k_to = (k.data_ptr(), *k.stride()[:3]), (k_out.data_ptr(), *k_out.stride()[:3])
+        k, k_out, k_in, k_to = _in_and_out(k)
+        groups = k.size(1)
     if not q_in[0] and not k_in[0]:
         return q_out, k_out
     args = pack_rotary(*q_in, *q_to, *k_in, *k_to, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0, 0, 0, 0,
@@ -178,7 +178,8 @@ class _Rotary(torch.autograd.Function):
         dq, dk = (g if need else None for g, need in zip((dq, dk), ctx.needs_input_grad))
         if dq is None and dk is None:
             return (None,) * 7
-        dq, dk = _Rotary.apply(dq, dk, frequencies, at[0] if at else positions, interleaved, amplitude, -sign)
+        back = _Rotary.apply if torch.is_grad_enabled() else _rotate      # a graph of the gradient only where one is built
+        dq, dk = back(dq, dk, frequencies, at[0] if at else positions, interleaved, amplitude, -sign)
         return dq, dk, None, None, None, None, None
 
 
@@ -191,22 +192,24 @@ def log_kv_rotary(q, k, frequencies, positions=0, *, interleaved=False, amplitud
     token's (an int), or int64 or int32 ``[T]`` or ``[B, T]``. Pairs are features ``(i, i + n)``, or ``(2 i, 2 i + 1)``
     with ``interleaved``. Angles are formed in 64 bits, products in float32, rounded once. New tensors in the inputs'
     dimension order; differentiable in q and k any number of times."""
-    if k is None:
-        x, others = q, ()
-    else:
-        x, others = q, (k,)
-    if x.ndim != 4 or any(y.ndim != 4 or y.size(0) != x.size(0) or y.shape[2:] != x.shape[2:] for y in others):
+    shape, dtype, index = q.shape, q.dtype, q.get_device()
+    if len(shape) != 4:
         raise ValueError("q and k must be [B, heads, T, d] of one batch, length and width")
-    check_activation_dtype(x.dtype)
-    require_device(x, "q")
-    if any(y.dtype != x.dtype or y.device != x.device for y in others):
-        raise ValueError("q and k must be of one dtype on one device")
-    if not 1 <= x.size(3) <= MAX_WIDTH:
+    if k is not None:
+        other = k.shape
+        if len(other) != 4 or other[0] != shape[0] or other[2] != shape[2] or other[3] != shape[3]:
+            raise ValueError("q and k must be [B, heads, T, d] of one batch, length and width")
+        if k.dtype != dtype or k.get_device() != index:
+            raise ValueError("q and k must be of one dtype on one device")
+    check_activation_dtype(dtype)
+    if index < 0:
+        require_device(q, "q")
+    if not 1 <= shape[3] <= MAX_WIDTH:
         raise ValueError(f"head widths must be in [1, {MAX_WIDTH}]")
     amplitude = float(amplitude)
     if not math.isfinite(amplitude):
         raise ValueError("amplitude must be finite")
     if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
-        _check_frequencies(frequencies, x.size(3), x.get_device())
+        _check_frequencies(frequencies, shape[3], index)
         return _Rotary.apply(q, k, frequencies, positions, bool(interleaved), amplitude, 1.0)
     return _rotate(q, k, frequencies, positions, interleaved, amplitude, 1.0)
