@@ -4,9 +4,10 @@ from __future__ import annotations
 
 import ctypes as C
 from functools import lru_cache
+from struct import Struct
 
 from ._lib import _i32, _i64, _p, lib
-from ._rows import BF16, F16, _packer
+from ._rows import BF16, F16, _CODES, _packer  # noqa: F401
 
 F32 = 2
 
@@ -52,6 +53,11 @@ class PagedArgs(C.Structure):
 
 
 pack_rotary = _packer(RotaryArgs).pack
+# The rotation's rows (q, q_out, k, k_out) and the rest, whose last field is the sign.
+_ROWS = 16
+pack_rotary_rows = Struct("=" + "Qqqq" * 4).pack
+pack_rotary_rest = Struct("=" + "".join(_CODES[t] for _, t in RotaryArgs._fields_[_ROWS:-1])).pack
+ROTARY_SIGNS = {sign: Struct("=f").pack(sign) for sign in (1.0, -1.0)}
 pack_paged = _packer(PagedArgs).pack
 
 # Exported symbol -> (restype, argtypes); the tests check this table against the header. The structs are passed as

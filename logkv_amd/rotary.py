@@ -14,7 +14,7 @@ import operator
 import torch
 
 from ._lib import check_activation_dtype, require_device
-from ._paged import F32, pack_rotary, paged_lib
+from ._paged import F32, ROTARY_SIGNS, pack_rotary_rest, pack_rotary_rows, paged_lib
 from ._rows import BF16, F16
 from .row_attention import _launch
 
@@ -131,30 +131,31 @@ def _check_positions(positions, batch, tokens, index):
     return positions, positions.data_ptr(), sb, st, int(positions.dtype == torch.int32), 0
 
 
-def _rotate(q, k, frequencies, positions, interleaved, amplitude, sign):
-    """The launch on checked tensors; k or q may be None."""
-    x = k if q is None else q
+def _plan(x, heads, groups, frequencies, positions, interleaved, amplitude):
+    """What a launch needs beside its rows and its sign (for rows like ``x``), with the tensors that it points into."""
     batch, _, tokens, dim = x.shape
     index = x.get_device()
     rotated, freq_float = _check_frequencies(frequencies, dim, index)
     if not frequencies.is_contiguous():
         frequencies = frequencies.contiguous()
     positions, p_ptr, p_sb, p_st, p_int, first = _check_positions(positions, batch, tokens, index)
-    heads = groups = 0
+    rest = pack_rotary_rest(*_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0, 0, 0, 0, frequencies.data_ptr(), p_ptr, p_sb, p_st, 0, first,
+                            batch, heads, groups, tokens, dim, 0, rotated, _TYPES[x.dtype], 0, int(interleaved), freq_float,
+                            p_int, 0, 0, 0, 0, amplitude)
+    return rest, frequencies, positions
+
+
+def _rotate(q, k, rest, sign, index):
+    """The launch; q or k may be None."""
     q_in = q_to = k_in = k_to = _NO_ROWS
     q_out = k_out = None
     if q is not None:
         q, q_out, q_in, q_to = _in_and_out(q)
-        heads = q.size(1)
     if k is not None:
         k, k_out, k_in, k_to = _in_and_out(k)
-        groups = k.size(1)
-    if not q_in[0] and not k_in[0]:
-        return q_out, k_out
-    args = pack_rotary(*q_in, *q_to, *k_in, *k_to, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0, 0, 0, 0,
-                       frequencies.data_ptr(), p_ptr, p_sb, p_st, 0, first, batch, heads, groups, tokens, dim, 0,
-                       rotated, _TYPES[x.dtype], 0, int(interleaved), freq_float, p_int, 0, 0, 0, 0, amplitude, sign)
-    _launch(paged_lib().logkv_rotary, "logkv_rotary", index, args)
+    if q_in[0] or k_in[0]:
+        args = pack_rotary_rows(*q_in, *q_to, *k_in, *k_to) + rest + ROTARY_SIGNS[sign]
+        _launch(paged_lib().logkv_rotary, "logkv_rotary", index, args)
     return q_out, k_out
 
 
@@ -162,25 +163,22 @@ class _Rotary(torch.autograd.Function):
     """The rotation as a function of the rows; its gradient is the rotation back."""
 
     @staticmethod
-    def forward(ctx, q, k, frequencies, positions, interleaved, amplitude, sign):
+    def forward(ctx, q, k, frequencies, positions, rest, sign, index):
         ctx.set_materialize_grads(False)
-        at = positions if isinstance(positions, torch.Tensor) else None
-        ctx.save_for_backward(frequencies, *(() if at is None else (at,)))
-        ctx.rest = (None if at is not None else positions, interleaved, amplitude, sign)
-        out = _rotate(q, k, frequencies, positions, interleaved, amplitude, sign)
-        ctx.mark_non_differentiable(*(y for y, need in zip(out, ctx.needs_input_grad) if y is not None and not need))
+        ctx.save_for_backward(frequencies, positions)
+        ctx.rest = rest, sign, index
+        out = _rotate(q, k, rest, sign, index)
+        if not all(ctx.needs_input_grad[:2]):
+            ctx.mark_non_differentiable(*(y for y, need in zip(out, ctx.needs_input_grad) if y is not None and not need))
         return out
 
     @staticmethod
     def backward(ctx, dq, dk):
-        frequencies, *at = ctx.saved_tensors
-        positions, interleaved, amplitude, sign = ctx.rest
-        dq, dk = (g if need else None for g, need in zip((dq, dk), ctx.needs_input_grad))
-        if dq is None and dk is None:
-            return (None,) * 7
-        back = _Rotary.apply if torch.is_grad_enabled() else _rotate      # a graph of the gradient only where one is built
-        dq, dk = back(dq, dk, frequencies, at[0] if at else positions, interleaved, amplitude, -sign)
-        return dq, dk, None, None, None, None, None
+        frequencies, positions = ctx.saved_tensors      # unchanged since the forward, and kept until here
+        rest, sign, index = ctx.rest
+        if not torch.is_grad_enabled():      # no graph of the gradient
+            return *_rotate(dq, dk, rest, -sign, index), None, None, None, None, None
+        return *_Rotary.apply(dq, dk, frequencies, positions, rest, -sign, index), None, None, None, None, None
 
 
 def log_kv_rotary(q, k, frequencies, positions=0, *, interleaved=False, amplitude=1.0):
@@ -209,7 +207,8 @@ def log_kv_rotary(q, k, frequencies, positions=0, *, interleaved=False, amplitud
     amplitude = float(amplitude)
     if not math.isfinite(amplitude):
         raise ValueError("amplitude must be finite")
+    rest, frequencies, positions = _plan(q, shape[1], 0 if k is None else k.size(1), frequencies, positions, interleaved,
+                                         amplitude)
     if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
-        _check_frequencies(frequencies, shape[3], index)
-        return _Rotary.apply(q, k, frequencies, positions, bool(interleaved), amplitude, 1.0)
-    return _rotate(q, k, frequencies, positions, interleaved, amplitude, 1.0)
+        return _Rotary.apply(q, k, frequencies, positions, rest, 1.0, index)
+    return _rotate(q, k, rest, 1.0, index)

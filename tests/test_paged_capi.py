@@ -50,6 +50,10 @@ def test_ctypes_structs_match_the_header(tmp_path):
         values = [3 * i + 1 for i in range(len(cls._fields_))]
         a = cls.from_buffer_copy(pack(*values))
         assert [getattr(a, f) for f, _ in cls._fields_] == values
+    # The rotation's struct in its three parts.
+    values = [3 * i + 1 for i in range(len(_paged.RotaryArgs._fields_) - 1)] + [1.0]
+    assert _paged.pack_rotary_rows(*values[:16]) + _paged.pack_rotary_rest(*values[16:-1]) + _paged.ROTARY_SIGNS[1.0] \
+        == _paged.pack_rotary(*values)
 
 
 def rotary_args(**over):
