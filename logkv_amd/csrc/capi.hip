@@ -976,6 +976,8 @@ int check_paged_shape(const logkv_paged_args* a) {
     return fail(LOGKV_EINVAL, "paged attention: pages of %d rows (a power of two from 16 on), %d a sequence, a prefix of %d",
                 a->page, a->table_len, a->prefix_len);
   if (a->dtype != LOGKV_BF16 && a->dtype != LOGKV_F16) return fail(LOGKV_EINVAL, "paged attention takes bf16 or fp16");
+  if (logkv::paged_launch(*a, nullptr).blocks > logkv::kMostPagedBlocks)
+    return fail(LOGKV_EINVAL, "paged attention over too many queries and lanes at once");
   return LOGKV_OK;
 }
 

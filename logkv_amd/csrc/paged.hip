@@ -5,7 +5,9 @@
 // prefix's rows are read once for all of its sequences: their queries (sequences x heads of the KV group
 // x tokens) are the columns of one product, in the kernel that so many columns take (rows_plan), and a
 // sequence's own rows are read in a second pass of few columns. Both passes are the row attention
-// kernels over a page table; this file joins their partials.
+// kernels over a page table, in one launch where their kernels go together; this file joins their partials.
+// An infinity or NaN in V is left out of a pass's products, which would spread it to queries that do not
+// see its row, and noted behind the partial's sums; the join then adds those of the rows that a query sees.
 #include <algorithm>
 
 #include "paged.hpp"
@@ -20,14 +22,51 @@ int64_t align256(int64_t x) { return (x + 255) & ~int64_t(255); }
 
 }  // namespace
 
+// Values of row `at` that are infinite or NaN added to the query's features; others are in its sum.
+template <int DT>
+__device__ __forceinline__ void add_odd(const LOGKV_G uint16_t* at, f32x4& y) {
+  const uint2 x = *(const LOGKV_G uint2*)at;
+  const uint32_t v[4] = {x.x & 0xffffu, x.x >> 16, x.y & 0xffffu, x.y >> 16};
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if ((v[k] & 0x7fffu) >= Elem<DT>::kInf) y[k] += Elem<DT>::to_f32(static_cast<uint16_t>(v[k]));
+}
+
+// Those of every row of a lane that query t sees.
+template <int DT>
+__device__ __forceinline__ void add_odd_rows(const logkv_rows_args& a, const RowsLaunch& r, int b, int g, int t, int d, f32x4& y) {
+  const int n = rows_in_use(a, b), own = lane_own_rows<true>(a, r, b);
+  const LOGKV_G uint16_t* base = gp(a.cache_v) + g * a.cv_sg + d;
+#pragma unroll 1
+  for (int i = 0; i < n; ++i) {
+    const int page = page_of(r, b, i);
+    bool see = page >= 0;
+    if (a.bias && see) {
+      const int64_t at = b * a.b_sb + g * a.b_sg + i * a.b_st;
+      const float x = a.bias_half ? Elem<DT>::to_f32(gp(static_cast<const uint16_t*>(a.bias))[at])
+                                  : gp(static_cast<const float*>(a.bias))[at];
+      see = x != -__builtin_inff();
+    }
+    int64_t step;
+    if (see) add_odd<DT>(page_row(r, base, a.cv_sb, a.cv_st, page, i, step), y);
+  }
+#pragma unroll 1
+  for (int i = 0; i < own; ++i) {
+    const bool see = r.causal ? i <= t : gp(a.visible)[b * a.vis_sb + t * a.vis_st + i] != 0;
+    if (see) add_odd<DT>(gp(a.v) + b * a.v_sb + g * a.v_sg + i * a.v_st + d, y);
+  }
+}
+
 // TQ threads per query, four features each; the block's other factor is shared by queries and by groups of
 // partials (QPB queries x SG groups), joined in group order.
 template <int DT, int TQ, int SG>
-__global__ __launch_bounds__(kThreads) void paged_finish_kernel(logkv_rows_args a, RowsLaunch own, RowsLaunch shared) {
+__global__ __launch_bounds__(kThreads) void paged_finish_kernel(PagedPass own, PagedPass shared) {
   typedef Elem<DT> E;
+  const logkv_rows_args& a = own.args;
   constexpr int QPB = kThreads / (TQ * SG);
   __shared__ __align__(16) float acc_s[QPB][SG][4 * TQ];
   __shared__ float m_s[QPB][SG], l_s[QPB][SG];
+  __shared__ float2 odd_s[QPB][SG];
   const int G = a.n_groups, b = static_cast<int>(blockIdx.y) / G, g = static_cast<int>(blockIdx.y) % G;
   const int rep = a.n_heads / G, nq = rep * a.tq, tid = threadIdx.x, stride = a.dv + kRowsPartTail;
   const int qs = tid / (TQ * SG), sg = tid / TQ % SG, d = 4 * (tid % TQ);
@@ -36,9 +75,11 @@ __global__ __launch_bounds__(kThreads) void paged_finish_kernel(logkv_rows_args 
   const bool live = min(qi, nq - 1) % a.tq < own_rows(a, b);   // a query past its sequence's count sees nothing
   float m = -__builtin_inff(), lsum = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  float odd[2] = {0.f, 0.f};   // the partials' notes
 #pragma unroll
   for (int set = 0; set < 2; ++set) {
-    const RowsLaunch& r = set ? shared : own;
+    const PagedPass& pass = set ? shared : own;
+    const RowsLaunch& r = pass.launch;
     if (set && !r.seqs) continue;
     const int lane = (set ? b / r.seqs : b) * G + g, splits = r.shares ? r.shares[lane] : r.splits;
     const int64_t step = static_cast<int64_t>(set ? r.seqs * nq : nq) * stride;
@@ -47,30 +88,30 @@ __global__ __launch_bounds__(kThreads) void paged_finish_kernel(logkv_rows_args 
     const float unit = __builtin_amdgcn_exp2f(-r.shift);
     // Eight partials' loads at a time, joined under the running maximum.
     for (int s0 = sg; s0 < splits; s0 += 8 * SG) {
-      float2 ml[8];
-      f32x4 x[8];
+      f32x4 ml[8], x[8];
       float mx = m;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int sp = s0 + k * SG;
-        ml[k] = make_float2(-__builtin_inff(), 0.f);
+        ml[k] = f32x4{-__builtin_inff(), 0.f, 0.f, 0.f};
         x[k] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (there && live && sp < splits) {
-          ml[k] = *reinterpret_cast<const float2*>(base + sp * step + a.dv);
+          ml[k] = *reinterpret_cast<const f32x4*>(base + sp * step + a.dv);
           x[k] = *reinterpret_cast<const f32x4*>(base + sp * step + d);
         }
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) mx = fmaxf(mx, ml[k].x);
+      for (int k = 0; k < 8; ++k) mx = fmaxf(mx, ml[k][0]);
       const float top = mx == -__builtin_inff() ? 0.f : mx;
       const float corr = __builtin_amdgcn_exp2f(m - top);
       lsum *= corr;
       acc *= corr;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float f = unit * __builtin_amdgcn_exp2f(ml[k].x - top);
-        lsum += ml[k].y * f;
+        const float f = unit * __builtin_amdgcn_exp2f(ml[k][0] - top);
+        lsum += ml[k][1] * f;
         acc += x[k] * f;
+        odd[set] += ml[k][2];
       }
       m = mx;
     }
@@ -80,6 +121,7 @@ __global__ __launch_bounds__(kThreads) void paged_finish_kernel(logkv_rows_args 
     if (d == 0) {
       m_s[qs][sg] = m;
       l_s[qs][sg] = lsum;
+      odd_s[qs][sg] = make_float2(odd[0], odd[1]);
     }
     __syncthreads();
     if (sg) return;
@@ -93,15 +135,23 @@ __global__ __launch_bounds__(kThreads) void paged_finish_kernel(logkv_rows_args 
     for (int k = 0; k < SG; ++k) {
       const float f = __builtin_amdgcn_exp2f(m_s[qs][k] - top);
       total += l_s[qs][k] * f;
+      if (k) odd[0] += odd_s[qs][k].x, odd[1] += odd_s[qs][k].y;
       sum += *reinterpret_cast<const f32x4*>(&acc_s[qs][k][d]) * f;
     }
     lsum = total;
     acc = sum;
   }
   if (!there) return;
+  f32x4 z = {0.f, 0.f, 0.f, 0.f};
+  if (lsum != 0.f) z = acc / lsum;
+  if (__builtin_expect(odd[0] + odd[1] > 0.f, 0)) {
+    const int t = qi % a.tq;
+    if (odd[0] > 0.f) add_odd_rows<DT>(a, own.launch, b, g, t, d, z);
+    if (odd[1] > 0.f) add_odd_rows<DT>(shared.args, shared.launch, b / shared.launch.seqs, g, t, d, z);
+  }
   uint16_t y[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) y[k] = lsum == 0.f ? uint16_t(0) : E::from_f32(acc[k] / lsum);
+  for (int k = 0; k < 4; ++k) y[k] = E::from_f32(z[k]);
   LOGKV_G uint16_t* o = gp(a.out) + b * a.o_sb + (g * rep + qi / a.tq) * a.o_sh + qi % a.tq * a.o_st + d;
   *reinterpret_cast<LOGKV_G uint2*>(o) =
       make_uint2(y[0] | static_cast<uint32_t>(y[1]) << 16, y[2] | static_cast<uint32_t>(y[3]) << 16);
@@ -114,7 +164,7 @@ void launch_finish(const PagedLaunch& p, hipStream_t stream) {
   const logkv_rows_args& a = p.own.args;
   const int nq = a.n_heads / a.n_groups * a.tq, qpb = kThreads / (TQ * SG);
   hipLaunchKernelGGL((paged_finish_kernel<DT, TQ, SG>), dim3((nq + qpb - 1) / qpb, a.n_batch * a.n_groups), dim3(kThreads),
-                     0, stream, a, p.own.launch, p.shared.launch);
+                     0, stream, p.own, p.shared);
 }
 
 template <int DT>
@@ -123,7 +173,10 @@ void launch_finish_type(const PagedLaunch& p, hipStream_t stream) {
   // Groups of partials share a query where eight queries a block would not fill the CUs.
   const bool many = std::max(p.own.launch.splits, p.shared.launch.splits) > 8 &&
                     static_cast<int64_t>(a.n_batch) * a.n_heads * a.tq < 8 * 256;
-  if (a.dv <= 128) {
+  if (a.dv <= 64) {
+    if (many) launch_finish<DT, 16, 8>(p, stream);
+    else launch_finish<DT, 16, 1>(p, stream);
+  } else if (a.dv <= 128) {
     if (many) launch_finish<DT, 32, 8>(p, stream);
     else launch_finish<DT, 32, 1>(p, stream);
   } else {
@@ -132,8 +185,16 @@ void launch_finish_type(const PagedLaunch& p, hipStream_t stream) {
   }
 }
 
-int launch_pass(const PagedPass& p, hipStream_t stream) {
-  return p.launch.q_waves ? launch_paged_tile(p, stream) : launch_paged_stream(p, stream);
+int launch_passes(const PagedPass& shared, const PagedPass& own, hipStream_t stream) {
+  const logkv_rows_args& a = own.args;
+  const int width = std::max(a.dk, a.dv);
+  if (a.dtype == LOGKV_BF16)
+    return width <= 64    ? launch_paged_bf16_64(shared, own, stream)
+           : width <= 128 ? launch_paged_bf16_128(shared, own, stream)
+                          : launch_paged_bf16_256(shared, own, stream);
+  return width <= 64    ? launch_paged_f16_64(shared, own, stream)
+         : width <= 128 ? launch_paged_f16_128(shared, own, stream)
+                        : launch_paged_f16_256(shared, own, stream);
 }
 
 }  // namespace
@@ -146,6 +207,8 @@ PagedLaunch paged_launch(const logkv_paged_args& a, void* ws) {
     off += align256(4 * words);
     return p;
   };
+  const int width = std::max(a.dk, a.dv);
+  PagedLaunch p{};
   auto plan = [&](PagedPass& pass) {
     RowsLaunch& r = pass.launch;
     const logkv_rows_args& x = pass.args;
@@ -154,17 +217,20 @@ PagedLaunch paged_launch(const logkv_paged_args& a, void* ws) {
     r.bias2 = (x.bias_scale == 0.f ? 1.f : x.bias_scale) * kLog2e;
     r.causal = x.visible ? 0 : 1;
     rows_plan(x, lanes, nq, r);
+    if (!r.q_waves && width > 64) r.cols = 1;
+    r.q_blocks = static_cast<int>(r.q_waves ? (nq + 32 * r.q_waves - 1) / (32 * r.q_waves) : (nq + 16 * r.cols - 1) / (16 * r.cols));
     // Shares by length (rows_tile.hpp), as of contiguous rows.
     const bool by_length = r.q_waves && r.splits > 1 && x.n_batch > 1 && x.n_batch <= kWave;
     r.room = by_length ? 2 * r.splits : r.splits;
     r.part = take(lanes * r.room * nq * (x.dv + kRowsPartTail));
-    if (r.q_waves) r.redo = reinterpret_cast<int*>(take(lanes * r.splits * ((nq + 32 * r.q_waves - 1) / (32 * r.q_waves))));
     if (by_length) {
       r.shares = reinterpret_cast<int*>(take(lanes));
       if (!x.lengths || !x.len_stride) r.shares = nullptr;   // rows of one length
     }
+    const int64_t blocks = lanes * r.splits * r.q_blocks;
+    p.blocks += blocks;
+    pass.blocks = static_cast<int>(blocks);
   };
-  PagedLaunch p{};
   logkv_rows_args& x = p.own.args;
   x.q = a.q, x.q_sb = a.q_sb, x.q_sh = a.q_sh, x.q_st = a.q_st;
   x.k = a.k, x.k_sb = a.k_sb, x.k_sg = a.k_sg, x.k_st = a.k_st;
@@ -201,14 +267,26 @@ PagedLaunch paged_launch(const logkv_paged_args& a, void* ws) {
     }
     plan(p.shared);
   }
+  // Passes of one launch have the same threads a block and at most one tiled and one streamed kernel.
+  const RowsLaunch &o = p.own.launch, &h = p.shared.launch;
+  p.together = a.n_prefixes && (o.q_waves && h.q_waves ? o.q_waves == h.q_waves : o.q_waves || h.q_waves || o.cols == h.cols);
   p.bytes = off;
   return p;
 }
 
 int launch_paged_attention(const logkv_paged_args& a, const PagedLaunch& p, hipStream_t stream) {
-  int rc = a.n_prefixes ? launch_pass(p.shared, stream) : LOGKV_OK;
-  if (!rc) rc = launch_pass(p.own, stream);
-  if (rc) return rc;
+  PagedPass none = p.shared;
+  none.blocks = 0;
+  if (p.together) {
+    if (int rc = launch_passes(p.shared, p.own, stream)) return rc;
+  } else {
+    if (a.n_prefixes) {
+      PagedPass alone = p.own;
+      alone.blocks = 0;
+      if (int rc = launch_passes(p.shared, alone, stream)) return rc;
+    }
+    if (int rc = launch_passes(none, p.own, stream)) return rc;
+  }
   if (a.dtype == LOGKV_BF16) launch_finish_type<LOGKV_BF16>(p, stream);
   else launch_finish_type<LOGKV_F16>(p, stream);
   return hipGetLastError() == hipSuccess ? LOGKV_OK : LOGKV_ERUNTIME;

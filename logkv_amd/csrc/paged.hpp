@@ -11,16 +11,29 @@ namespace logkv {
 struct PagedPass {
   logkv_rows_args args;
   RowsLaunch launch;
+  int blocks;   // of the pass in a launch, 0: not in it
 };
 struct PagedLaunch {
   PagedPass own, shared;
-  int64_t bytes;
+  int64_t bytes, blocks;
+  bool together;   // both passes in one launch
 };
 
+// Blocks of a launch: fewer than 2^32 threads.
+constexpr int64_t kMostPagedBlocks = (int64_t(1) << 32) / 512 - 1;
+
 PagedLaunch paged_launch(const logkv_paged_args& a, void* ws);
-int launch_paged_tile(const PagedPass& p, hipStream_t stream);
-int launch_paged_stream(const PagedPass& p, hipStream_t stream);
 int launch_paged_attention(const logkv_paged_args& a, const PagedLaunch& p, hipStream_t stream);
+// One launch of the passes that have blocks, whose kernels may differ only as paged.hip's rule allows.
+int launch_paged_bf16_64(const PagedPass& shared, const PagedPass& own, hipStream_t stream);
+int launch_paged_bf16_128(const PagedPass& shared, const PagedPass& own, hipStream_t stream);
+int launch_paged_bf16_256(const PagedPass& shared, const PagedPass& own, hipStream_t stream);
+int launch_paged_f16_64(const PagedPass& shared, const PagedPass& own, hipStream_t stream);
+int launch_paged_f16_128(const PagedPass& shared, const PagedPass& own, hipStream_t stream);
+int launch_paged_f16_256(const PagedPass& shared, const PagedPass& own, hipStream_t stream);
 int launch_rotary(const logkv_rotary_args& a, bool append, hipStream_t stream);
+
+// Waves of a block: the tiled kernel's of its query waves, four of the streamed kernel alone.
+constexpr int paged_waves(int q_waves) { return q_waves > 2 ? 8 : 4; }
 
 }  // namespace logkv

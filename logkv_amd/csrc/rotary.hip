@@ -97,7 +97,8 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(logkv_rotary_args a, R
   __shared__ __align__(16) float2 turn_s[kMaxAngles];
   __shared__ int64_t k_at[kMaxTokens], v_at[kMaxTokens];   // rows in the pages, below 0 for none
   const int tid = threadIdx.x;
-  const int b = static_cast<int>(blockIdx.x) / p.tiles, t0 = (static_cast<int>(blockIdx.x) - b * p.tiles) * p.tpb;
+  const int blk = static_cast<int>(blockIdx.y * gridDim.x + blockIdx.x), b = blk / p.tiles, t0 = (blk - b * p.tiles) * p.tpb;
+  if (b >= a.n_batch) return;
   const int here = min(p.tpb, a.tokens - t0);
 
   // Item e of the block's queries (OF 0), keys (1) or values (2): its token, head, first feature and that of its second
@@ -289,8 +290,9 @@ int launch_vec(const logkv_rotary_args& a, hipStream_t stream) {
   if (p.tpb * token_items * std::max<int64_t>(widest, 1) >= int64_t(1) << 32) return refuse("too many heads for one rotation");
   p.tiles = (a.tokens + p.tpb - 1) / p.tpb;
   const int64_t blocks = static_cast<int64_t>(p.tiles) * a.n_batch;
-  if (blocks > INT32_MAX) return refuse("too many tokens for one rotation");
-  const dim3 grid(static_cast<uint32_t>(blocks));
+  constexpr int64_t kLine = int64_t(1) << 20;   // of the grid, whose axes hold fewer than 2^32 threads
+  if (blocks > INT32_MAX - kLine) return refuse("too many tokens for one rotation");
+  const dim3 grid(static_cast<uint32_t>(std::min(blocks, kLine)), static_cast<uint32_t>((blocks + kLine - 1) / kLine));
   if (vec == 8) {
     if constexpr (DT != LOGKV_F32) hipLaunchKernelGGL((rotary_kernel<DT, CT, 8, APPEND>), grid, dim3(kThreads), 0, stream, a, p);
   } else if (vec == 4) {

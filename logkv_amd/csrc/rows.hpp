@@ -41,6 +41,7 @@ struct RowsLaunch {
   int64_t table_sb;
   int page_shift, pages;
   int seqs;       // sequences whose queries a lane takes
+  int q_blocks;   // query blocks of a lane
   int prefix;     // rows that several sequences share: no own rows, every query sees all
 };
 
@@ -96,11 +97,10 @@ static __device__ const uint4 kZeroRow[kMostFeatures / 8] = {};
 #define LOGKV_C
 #endif
 
-// The page of row `row` of lane row b, -1 for none. For an index that is the same in all lanes: a scalar load (the table
-// is not written while a kernel reads it).
+// The page of row `row` of lane row b, -1 for none.
 __device__ __forceinline__ int page_of(const RowsLaunch& r, int b, int row) {
   if (!r.table) return b;
-  const int page = ((const LOGKV_C int32_t*)r.table)[b * r.table_sb + (row >> r.page_shift)];
+  const int page = gp(r.table)[b * r.table_sb + (row >> r.page_shift)];
   return static_cast<uint32_t>(page) < static_cast<uint32_t>(r.pages) ? page : -1;
 }
 // Row `row` of the cache rows `base` (group g's, page 0's) that lie on `page`, and the step to the next rows of the page.
@@ -110,6 +110,43 @@ __device__ __forceinline__ const LOGKV_G uint16_t* page_row(const RowsLaunch& r,
   const LOGKV_G uint16_t* zero = (const LOGKV_G uint16_t*)gp(kZeroRow);
   return page < 0 ? zero : base + page * sb + (row & ((1 << r.page_shift) - 1)) * st;
 }
+
+// A value that is the same in all lanes, kept in a scalar register: a launch's arguments would be read again at every
+// use in a loop, and each such read waits.
+template <typename T>
+__device__ __forceinline__ T held(T x) {
+  asm volatile("" : "+s"(x));
+  return x;
+}
+
+// A lane row's pages for the loops of an attention, where the row's index is the same in all lanes: the table's entries
+// by scalar loads (it is not written while a kernel reads it).
+struct PagedRows {
+  const LOGKV_G uint16_t *k, *v;   // the group's rows of page 0
+  int64_t k_sb, k_st, v_sb, v_st;
+  const LOGKV_C int32_t* line;     // null: of page `b` alone
+  int shift, pages, b;
+
+  __device__ __forceinline__ void init(const logkv_rows_args& a, const RowsLaunch& r, int row_b, int g) {
+    k = gp(a.cache_k) + g * a.ck_sg, v = gp(a.cache_v) + g * a.cv_sg;
+    k_sb = held(a.ck_sb), k_st = held(a.ck_st), v_sb = held(a.cv_sb), v_st = held(a.cv_st);
+    b = row_b, shift = held(r.page_shift), pages = held(r.pages);
+    line = r.table ? (const LOGKV_C int32_t*)r.table + b * r.table_sb : nullptr;
+    line = held(line);
+  }
+  __device__ __forceinline__ int page(int row) const {
+    if (!line) return b;
+    const int x = line[row >> shift];
+    return static_cast<uint32_t>(x) < static_cast<uint32_t>(pages) ? x : -1;
+  }
+  // Row `row`, on page p, and the step to its page's next rows: of zeros where there is no page.
+  __device__ __forceinline__ const LOGKV_G uint16_t* at(const LOGKV_G uint16_t* base, int64_t sb, int64_t st, int p, int row,
+                                                        int64_t& step) const {
+    const LOGKV_G uint16_t* there = base + p * sb + (row & ((1 << shift) - 1)) * st;
+    step = p < 0 ? 0 : st;
+    return p < 0 ? (const LOGKV_G uint16_t*)gp(kZeroRow) : there;
+  }
+};
 
 // A bias in base 2. A finite one stays finite (a mask of the type's lowest value hides a row only
 // beside larger logits).
@@ -183,5 +220,17 @@ struct Elem<LOGKV_F16> {
     lo = __builtin_bit_cast(uint32_t, r);
   }
 };
+
+// Eight elements with zeros in place of infinities and NaNs.
+template <int DT>
+__device__ __forceinline__ uint4 finite_only(uint4 x) {
+  uint32_t* x4[4] = {&x.x, &x.y, &x.z, &x.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t lo = *x4[j] & 0x7fffu, hi = *x4[j] >> 16 & 0x7fffu;
+    *x4[j] &= (lo >= Elem<DT>::kInf ? 0u : 0xffffu) | (hi >= Elem<DT>::kInf ? 0u : 0xffff0000u);
+  }
+  return x;
+}
 
 }  // namespace logkv

@@ -28,37 +28,49 @@ namespace {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 4;   // of a block over contiguous rows
 
 // LDS row stride of a V tile: 8 dwords modulo 32, so the four rows of a transposed read fall into
 // distinct banks.
 constexpr int v_stride(int blocks) { return 16 * blocks + 16; }
 
+// A block's LDS: per wave a V tile, then its sums; the waves' maxima and sums; per wave and feature, where a tile is not
+// finite, the rows (bits) with +infinity, -infinity and NaN (over pages: whether it met one).
+template <int NB, int NWV, bool PAGED>
+struct StreamLds {
+  static constexpr int kTileBytes = kRowTile * v_stride(NB) * 2, kOutBytes = 16 * 16 * NB * 4;
+  alignas(16) uint8_t buf[NWV][kTileBytes > kOutBytes ? kTileBytes : kOutBytes];
+  float m[NWV][16], l[NWV][16];
+  uint32_t odd[NWV][PAGED ? 1 : 3][PAGED ? 1 : 16 * NB];
+};
+
 }  // namespace
 
-// NS 32-wide steps of dk, NB 16-wide blocks of dv, NC 16-query column blocks. Units past dk and dv
-// are zero.
-template <int DT, int NS, int NB, int NC, bool BIAS, bool PAGED>
-__global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void rows_stream_kernel(logkv_rows_args a, RowsLaunch r) {
+// A block's share `split` of lane `lane` for its 16 NC queries from q0 on. NS 32-wide steps of dk, NB 16-wide blocks of
+// dv, NC 16-query column blocks, NWV waves. Units past dk and dv are zero. PAGED: rows in pages; infinities and NaNs of V
+// are left out and noted behind the partials' sums, for the launch that joins them.
+template <int DT, int NS, int NB, int NC, bool BIAS, bool PAGED, int NWV>
+__device__ __forceinline__ void rows_stream_block(const logkv_rows_args& a, const RowsLaunch& r, int split, int lane, int q0,
+                                                  StreamLds<NB, NWV, PAGED>& lds) {
   typedef Elem<DT> E;
   typedef typename E::vec8 vec8;
   typedef __attribute__((address_space(3))) s16x4* lds4;
   constexpr int kLd = v_stride(NB), kVLoads = kRowTile * 2 * NB / 64;
-  constexpr int kTileBytes = kRowTile * kLd * 2, kOutBytes = 16 * 16 * NB * 4;
-  __shared__ __align__(16) uint8_t buf[kWaves][kTileBytes > kOutBytes ? kTileBytes : kOutBytes];
-  __shared__ float m_s[kWaves][16], l_s[kWaves][16];
-  // Where a tile is not finite: per feature the rows (bits) with +infinity, -infinity and NaN.
-  __shared__ uint32_t odd_s[kWaves][3][16 * NB];
-  const int lane = blockIdx.y, G = a.n_groups, b = lane / G, g = lane % G;
-  const int nq = lane_queries<PAGED>(a, r), q0 = 16 * NC * static_cast<int>(blockIdx.z);
+  auto& buf = lds.buf;
+  auto& m_s = lds.m;
+  auto& l_s = lds.l;
+  auto& odd_s = lds.odd;
+  const int G = a.n_groups, b = lane / G, g = lane % G;
+  const int nq = lane_queries<PAGED>(a, r);
   const int units = a.dk / 8, vunits = a.dv / 8;
-  const int w = wave_id(), l = lane_id(), col = l & 15, hq = l >> 4;
-  const int n = rows_in_use(a, b), own = lane_own_rows<PAGED>(a, r, b);
+  const int w = PAGED ? __builtin_amdgcn_readfirstlane(wave_id()) : wave_id(), l = lane_id(), col = l & 15, hq = l >> 4;
+  int n = rows_in_use(a, b), own = lane_own_rows<PAGED>(a, r, b);
+  if constexpr (PAGED) n = __builtin_amdgcn_readfirstlane(n), own = __builtin_amdgcn_readfirstlane(own);
   const int np = (n + kRowTile - 1) / kRowTile, tiles = np + (own + kRowTile - 1) / kRowTile;
-  // The lane's tiles in gridDim.x equal shares, multiples of the block's waves; shares past the
+  // The lane's tiles in r.splits equal shares, multiples of the block's waves; shares past the
   // tiles write empty partials.
-  const int share = (tiles + kWaves * r.splits - 1) / (kWaves * r.splits) * kWaves;
-  const int begin = min(static_cast<int>(blockIdx.x) * share, tiles), end = min(begin + share, tiles);
+  const int share = (tiles + NWV * r.splits - 1) / (NWV * r.splits) * NWV;
+  const int begin = min(split * share, tiles), end = min(begin + share, tiles);
 
   // Query columns as B fragments; columns past nq are zero.
   int tq[NC];
@@ -84,16 +96,20 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
   float bx[8];
   // Paged: the two 16-row halves of a tile lie on one page each; read a tile ahead of its rows.
   int page[2] = {0, 0};
+  PagedRows in_pages;
+  if constexpr (PAGED) in_pages.init(a, r, b, g);
   auto pages = [&](int ti) {
-    if (!PAGED || ti >= np) return;
+    if constexpr (PAGED) {
+      if (ti >= np) return;
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) page[kb] = page_of(r, b, __builtin_amdgcn_readfirstlane(min(kRowTile * ti + 16 * kb, n - 1)));
+      for (int kb = 0; kb < 2; ++kb) page[kb] = in_pages.page(__builtin_amdgcn_readfirstlane(min(kRowTile * ti + 16 * kb, n - 1)));
+    }
   };
   // Rows past the tile's: K repeats its last row (masked in the scores), V is zero.
   auto load = [&](int ti) {
     const bool of_cache = ti < np;
     const int t0 = kRowTile * (of_cache ? ti : ti - np), rows = min(kRowTile, (of_cache ? n : own) - t0);
-    const int64_t kst = of_cache ? a.ck_st : a.k_st, vst = of_cache ? a.cv_st : a.v_st;
+    const int64_t kst = of_cache ? (PAGED ? in_pages.k_st : a.ck_st) : a.k_st, vst = of_cache ? (PAGED ? in_pages.v_st : a.cv_st) : a.v_st;
     const LOGKV_G uint16_t* kr = (of_cache ? kc : ko) + t0 * kst;
     const LOGKV_G uint16_t* vr = (of_cache ? vc : vo) + t0 * vst;
     const LOGKV_G uint16_t* vh[2] = {vr, vr + 16 * vst};   // V's halves, and the steps of their rows
@@ -106,8 +122,8 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
         int64_t step = kst;
         const LOGKV_G uint16_t* half = kr + first * kst;
         if (of_cache) {
-          half = page_row(r, kc, a.ck_sb, kst, page[kb], t0 + first, step);
-          vh[kb] = page_row(r, vc, a.cv_sb, vst, page[kb], t0 + first, vstep[kb]);
+          half = in_pages.at(in_pages.k, in_pages.k_sb, kst, page[kb], t0 + first, step);
+          vh[kb] = in_pages.at(in_pages.v, in_pages.v_sb, vst, page[kb], t0 + first, vstep[kb]);
         }
         row = half + (min(16 * kb + col, rows - 1) - first) * step;
       }
@@ -133,7 +149,7 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
       for (int j = 0; j < 8; ++j) {
         const int rr = min(16 * (j / 4) + 4 * hq + j % 4, rows - 1);
         bx[j] = 0.f;
-        if (of_cache) {
+        if (of_cache && (!PAGED || a.bias)) {
           const int64_t at = b * a.b_sb + g * a.b_sg + (t0 + rr) * a.b_st;
           const float x = a.bias_half ? E::to_f32(gp(static_cast<const uint16_t*>(a.bias))[at])
                                       : gp(static_cast<const float*>(a.bias))[at];
@@ -152,12 +168,13 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
     for (int nb = 0; nb < NB; ++nb) o[c][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   const float c2 = a.scale * kLog2e;
+  bool odd = false;   // paged: whether this wave left something out of V
   if (begin + w < end) {
     pages(begin + w);
     load(begin + w);
-    pages(min(begin + w + kWaves, end - 1));
+    pages(min(begin + w + NWV, end - 1));
   }
-  for (int ti = begin + w; ti < end; ti += kWaves) {
+  for (int ti = begin + w; ti < end; ti += NWV) {
     const bool of_cache = ti < np;
     const int t0 = kRowTile * (of_cache ? ti : ti - np), rows = min(kRowTile, (of_cache ? n : own) - t0);
     f32x4 s[NC][2];
@@ -178,11 +195,18 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
 #pragma unroll
       for (int j = 0; j < 4; ++j) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, x4[j] & 0x7fff7fffu));
     }
-    const bool finite = __ballot(top[0] >= E::kInf || top[1] >= E::kInf) == 0;
+    bool finite = __ballot(top[0] >= E::kInf || top[1] >= E::kInf) == 0;
+    if constexpr (PAGED) {
+      if (__builtin_expect(!finite, 0)) {
+#pragma unroll
+        for (int i = 0; i < kVLoads; ++i) vx[i] = finite_only<DT>(vx[i]);
+        odd = finite = true;
+      }
+    }
     // The wave's own V tile: written and read by this wave only (LDS accesses of a wave complete
     // in order; the fences keep the compiler's order).
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (__builtin_expect(!finite, 0)) {
+    if (!PAGED && __builtin_expect(!finite, 0)) {
       for (int e = l; e < 3 * 16 * NB; e += 64) (&odd_s[w][0][0])[e] = 0;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
@@ -212,9 +236,9 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
         for (int j = 0; j < 8; ++j)   // a row hidden by -inf stays hidden whatever its key holds
           s[c][j / 4][j % 4] = bx[j] == -__builtin_inff() ? bx[j] : __builtin_fmaf(s[c][j / 4][j % 4], c2, bx[j]);
     }
-    if (ti + kWaves < end) {
-      load(ti + kWaves);
-      pages(min(ti + 2 * kWaves, end - 1));
+    if (ti + NWV < end) {
+      load(ti + NWV);
+      pages(min(ti + 2 * NWV, end - 1));
     }
     // Masks: element i of block kb is row t0 + 16 kb + 4 hq + i of its region.
     if (!of_cache || rows < kRowTile) {
@@ -262,7 +286,7 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
         for (int nb = 0; nb < NB; ++nb) o[c][nb] *= corr;
       }
       m[c] = m_new;
-      if (__builtin_expect(!finite, 0)) {
+      if (!PAGED && __builtin_expect(!finite, 0)) {
         seen[c] = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -295,7 +319,7 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
 #pragma unroll
         for (int c = 0; c < NC; ++c) o[c][nb] = E::mfma16(vf, pf[c][q], o[c][nb]);
     }
-    if (__builtin_expect(!finite, 0)) {
+    if (!PAGED && __builtin_expect(!finite, 0)) {
       // The infinities and NaNs left out of the products, for the queries that see their rows.
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
@@ -332,19 +356,26 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
       m_s[w][col] = m[c];
       l_s[w][col] = lsum[c];
     }
+    if (PAGED && c == 0 && l == 0) odd_s[w][0][0] = odd;
     __syncthreads();
     const int qb = q0 + 16 * c, queries = min(16, nq - qb);
-    float* out = r.part + ((static_cast<int64_t>(lane) * r.room + blockIdx.x) * nq + qb) * (a.dv + kRowsPartTail);
+    float* out = r.part + ((static_cast<int64_t>(lane) * r.room + split) * nq + qb) * (a.dv + kRowsPartTail);
+    if (PAGED && static_cast<int>(threadIdx.x) < queries) {
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < NWV; ++i) any |= odd_s[i][0][0];
+      out[static_cast<int64_t>(threadIdx.x) * (a.dv + kRowsPartTail) + a.dv + 2] = any ? 1.f : 0.f;
+    }
     for (int e = threadIdx.x; e < queries * (a.dv + 2); e += blockDim.x) {
       const int q = e / (a.dv + 2), d = e % (a.dv + 2);
       float mx = -__builtin_inff();
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i) mx = fmaxf(mx, m_s[i][q]);
+      for (int i = 0; i < NWV; ++i) mx = fmaxf(mx, m_s[i][q]);
       // An empty share has zero sums; a share of NaN logits alone has no maximum but a NaN sum.
       const float base = mx == -__builtin_inff() ? 0.f : mx;
       float val = 0.f;
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i) {
+      for (int i = 0; i < NWV; ++i) {
         const float x = d < a.dv ? reinterpret_cast<const float*>(buf[i])[q * (16 * NB) + d] : l_s[i][q];
         val += x * __builtin_amdgcn_exp2f(m_s[i][q] - base);
       }
@@ -353,31 +384,5 @@ __global__ __launch_bounds__(64 * kWaves, NB <= 8 && NC * NB <= 16 ? 2 : 1) void
     }
   }
 }
-
-namespace {
-
-template <int DT, int NS, int NB, int NC, bool PAGED>
-void launch_stream_one(const logkv_rows_args& a, const RowsLaunch& r, dim3 grid, hipStream_t stream) {
-  if (a.bias) hipLaunchKernelGGL((rows_stream_kernel<DT, NS, NB, NC, true, PAGED>), grid, dim3(64 * kWaves), 0, stream, a, r);
-  else hipLaunchKernelGGL((rows_stream_kernel<DT, NS, NB, NC, false, PAGED>), grid, dim3(64 * kWaves), 0, stream, a, r);
-}
-
-template <int DT, bool PAGED>
-void launch_stream_type(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
-  const int nq = a.n_heads / a.n_groups * a.tq * (PAGED ? r.seqs : 1);
-  const dim3 grid(r.splits, a.n_batch * a.n_groups, (nq + 16 * r.cols - 1) / (16 * r.cols));
-  if (a.dk <= 64 && a.dv <= 64) {
-    if (r.cols == 1) launch_stream_one<DT, 2, 4, 1, PAGED>(a, r, grid, stream);
-    else launch_stream_one<DT, 2, 4, 2, PAGED>(a, r, grid, stream);
-  } else if (a.dk <= 128 && a.dv <= 128) {
-    if (r.cols == 1) launch_stream_one<DT, 4, 8, 1, PAGED>(a, r, grid, stream);
-    else launch_stream_one<DT, 4, 8, 2, PAGED>(a, r, grid, stream);
-  } else {
-    if (r.cols == 1) launch_stream_one<DT, 8, 16, 1, PAGED>(a, r, grid, stream);
-    else launch_stream_one<DT, 8, 16, 2, PAGED>(a, r, grid, stream);
-  }
-}
-
-}  // namespace
 
 }  // namespace logkv

@@ -94,9 +94,8 @@ __device__ __forceinline__ void here(T& x) {
 struct RowsBlock {
   int qb, split, lane;
 };
-__device__ __forceinline__ RowsBlock rows_block() {
-  const int nx = static_cast<int>(gridDim.x), ny = static_cast<int>(gridDim.y), n = nx * ny * static_cast<int>(gridDim.z);
-  int lin = static_cast<int>(blockIdx.x) + nx * (static_cast<int>(blockIdx.y) + ny * static_cast<int>(blockIdx.z));
+__device__ __forceinline__ RowsBlock rows_block(int lin, int nx, int ny, int nz) {
+  const int n = nx * ny * nz;
   if (n % 8 == 0) lin = lin % 8 * (n / 8) + lin / 8;
   return RowsBlock{lin % nx, lin / nx % ny, lin / (nx * ny)};
 }
@@ -198,24 +197,26 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
   const LOGKV_G uint16_t* vc = gp(a.cache_v) + (PAGED ? 0 : b * a.cv_sb) + g * a.cv_sg;
   const LOGKV_G uint16_t* ko = gp(a.k) + b * a.k_sb + g * a.k_sg;
   const LOGKV_G uint16_t* vo = gp(a.v) + b * a.v_sb + g * a.v_sg;
-  // Paged: a wave's rows of a task lie in 16 rows that begin at a multiple of 16, and so on one page. The pages of a
-  // load's tasks are read a tile ahead.
-  const int kw0 = __builtin_amdgcn_readfirstlane(kr0), vw0 = __builtin_amdgcn_readfirstlane(vr0);
-  int k_page[PAGED ? kKTasks : 1], v_page[PAGED ? kVTasks : 1];
+  // Paged: a wave's rows of a task lie in 16 rows that begin at a multiple of 16, and so on one page. The pages of K's
+  // next load are read a tile ahead; V's, a tile behind, are then K's last ones.
+  static_assert(!PAGED || KU == VU, "tasks of K and V have the same rows");
+  const int kw0 = __builtin_amdgcn_readfirstlane(kr0);
+  int k_page[PAGED ? kKTasks : 1] = {}, v_page[PAGED ? kVTasks : 1];
+  PagedRows in_pages;
+  if constexpr (PAGED) in_pages.init(a, r, b, g);
   auto rows_in = [&](int ti) { return ti < np ? min(TR, c.n - TR * ti) : min(TR, c.own - TR * (ti - np)); };
-  auto page_k = [&](int ti) {
-    if (!PAGED || ti >= np) return;
+  auto next_pages = [&](int ti) {
+    if constexpr (PAGED) {
 #pragma unroll
-    for (int q = 0; q < kKTasks; ++q) k_page[q] = page_of(r, b, TR * ti + min(kw0 + kThreads / KU * q, rows_in(ti) - 1));
-  };
-  auto page_v = [&](int ti) {
-    if (!PAGED || ti >= np) return;
-#pragma unroll
-    for (int q = 0; q < kVTasks; ++q) v_page[q] = page_of(r, b, TR * ti + min(vw0 + kThreads / VU * q, rows_in(ti) - 1));
+      for (int q = 0; q < kKTasks; ++q) {
+        v_page[q] = k_page[q];
+        if (ti < np) k_page[q] = in_pages.page(TR * ti + min(kw0 + kThreads / KU * q, rows_in(ti) - 1));
+      }
+    }
   };
   auto load_k = [&](int ti) {
     const int t0 = TR * (ti < np ? ti : ti - np), last = rows_in(ti) - 1;
-    const int64_t st = ti < np ? a.ck_st : a.k_st;
+    const int64_t st = ti < np ? (PAGED ? in_pages.k_st : a.ck_st) : a.k_st;
     const LOGKV_G uint16_t* base = (ti < np ? kc : ko) + t0 * st;
 #pragma unroll
     for (int q = 0; q < kKTasks; ++q) {
@@ -223,7 +224,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
       if constexpr (PAGED) {
         const int first = min(kw0 + kThreads / KU * q, last);
         int64_t step = st;
-        const LOGKV_G uint16_t* at = ti < np ? page_row(r, kc, a.ck_sb, st, k_page[q], t0 + first, step) : base + first * st;
+        const LOGKV_G uint16_t* at = ti < np ? in_pages.at(in_pages.k, in_pages.k_sb, st, k_page[q], t0 + first, step) : base + first * st;
         kx[q] = *(const LOGKV_G uint4*)(at + (row - first) * step + ku8);
       } else {
         kx[q] = *(const LOGKV_G uint4*)(base + row * st + ku8);
@@ -232,22 +233,22 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
     if constexpr (BIAS) {
       // A bias as its 16-bit halves (behind the cache's rows: any 4 bytes, not used).
       const LOGKV_G uint16_t* at = gp(a.q);
-      if (ti < np) at = gp(static_cast<const uint16_t*>(a.bias)) + (a.bias_half ? 1 : 2) * (b * a.b_sb + g * a.b_sg + (t0 + min(tid % TR, last)) * a.b_st);
+      if (ti < np && (!PAGED || a.bias)) at = gp(static_cast<const uint16_t*>(a.bias)) + (a.bias_half ? 1 : 2) * (b * a.b_sb + g * a.b_sg + (t0 + min(tid % TR, last)) * a.b_st);
       bx[0] = at[0];
       bx[1] = at[a.bias_half ? 0 : 1];
     }
   };
   auto load_v = [&](int ti) {
     const int t0 = TR * (ti < np ? ti : ti - np), last = rows_in(ti) - 1;
-    const int64_t st = ti < np ? a.cv_st : a.v_st;
+    const int64_t st = ti < np ? (PAGED ? in_pages.v_st : a.cv_st) : a.v_st;
     const LOGKV_G uint16_t* base = (ti < np ? vc : vo) + t0 * st;
 #pragma unroll
     for (int q = 0; q < kVTasks; ++q) {
       const int row = min(vr0 + kThreads / VU * q, last);
       if constexpr (PAGED) {
-        const int first = min(vw0 + kThreads / VU * q, last);
+        const int first = min(kw0 + kThreads / VU * q, last);
         int64_t step = st;
-        const LOGKV_G uint16_t* at = ti < np ? page_row(r, vc, a.cv_sb, st, v_page[q], t0 + first, step) : base + first * st;
+        const LOGKV_G uint16_t* at = ti < np ? in_pages.at(in_pages.v, in_pages.v_sb, st, v_page[q], t0 + first, step) : base + first * st;
         vx[q] = *(const LOGKV_G uint4*)(at + (row - first) * step + vu8);
       } else {
         vx[q] = *(const LOGKV_G uint4*)(base + row * st + vu8);
@@ -261,7 +262,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
     if constexpr (BIAS) {
       if (q == 0 && tid < TR) {
         const float x = a.bias_half ? Elem<DT>::to_f32(bx[0]) : __uint_as_float(bx[0] | static_cast<uint32_t>(bx[1]) << 16);
-        bias_s[bf][tid] = ti < np ? bias_base2(x, r.bias2) : 0.f;
+        bias_s[bf][tid] = ti < np && (!PAGED || a.bias) ? bias_base2(x, r.bias2) : 0.f;
       }
     }
   };
@@ -273,29 +274,35 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
     const uint32_t x4[4] = {vx[q].x, vx[q].y, vx[q].z, vx[q].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, x4[j] & 0x7fff7fffu));
+    if constexpr (PAGED) {   // infinities and NaNs are left out and noted
+      if (__builtin_expect(__ballot(top[0] >= Elem<DT>::kInf || top[1] >= Elem<DT>::kInf) != 0, 0)) {
+        vx[q] = finite_only<DT>(vx[q]);
+        flag_s[0] = 1;
+        top = u16x2{0, 0};
+      }
+    }
     v_tile(bf)[rr * VU + (tid % VU ^ swizzle<VU>(rr))] = vx[q];
   };
   // Whether tile ti's V holds an infinity or NaN.
   auto store_flags = [&](int ti) {
+    if constexpr (PAGED) return;
     const bool odd = __ballot(top[0] >= Elem<DT>::kInf || top[1] >= Elem<DT>::kInf) != 0;
     if (odd && l == 0) flag_s[(ti - begin) % 3] = 1;
     top = u16x2{0, 0};
   };
   clear_sums(c);
+  if (tid < 3) flag_s[tid] = 0;
   if (begin >= end) return true;
   const float c2 = a.scale * kLog2e;
   const int r0 = 32 * RB * rw;   // this wave's rows of a tile
-  if (tid < 3) flag_s[tid] = 0;
-  page_k(begin);
-  page_v(begin);
+  next_pages(begin);
   load_k(begin);
+  next_pages(min(begin + 1, end - 1));
   load_v(begin);
-  page_k(min(begin + 1, end - 1));
 #pragma unroll
   for (int q = 0; q < kKTasks; ++q) store_k(begin, 0, q);
   load_k(min(begin + 1, end - 1));
-  page_k(min(begin + 2, end - 1));
-  page_v(min(begin + 1, end - 1));
+  next_pages(min(begin + 2, end - 1));
 #pragma unroll
   for (int q = 0; q < kKTasks; ++q) store_k(min(begin + 1, end - 1), 1, q);
   __syncthreads();   // the flags are clear, K of the first tiles is stored
@@ -304,8 +311,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
   store_flags(begin);
   load_k(min(begin + 2, end - 1));
   load_v(min(begin + 1, end - 1));
-  page_k(min(begin + 3, end - 1));
-  page_v(min(begin + 2, end - 1));
+  next_pages(min(begin + 3, end - 1));
 
   // LDS addresses of this lane's operands in buffer 0: unit h of K's row r0 + l % 32, and of V's transposed reads
   // features l & 16 .. of rows 4 h .. (8 + 4 h .. behind). Other units are reached by exclusive or: the permutation is
@@ -333,6 +339,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
 #pragma unroll
   for (int k = 0; k < kCols; ++k) arg0[k] = kTileShift;
   // Element i is row r0 + 32 kb + 8 (i / 4) + 4 h + i % 4 of tile ti, whose bias is in buffer bf.
+  const int causal = PAGED ? held(r.causal) : r.causal;
   auto finish_scores = [&](int ti, int kb, int bf) {
     const bool own = ti >= np;
     const int t0 = TR * (own ? ti - np : ti), rows = min(TR, (own ? c.own : c.n) - t0);
@@ -350,11 +357,11 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
     if (own || rows < TR) {
 #pragma unroll
       for (int k = 0; k < kCols; ++k) {
-        const int lim = (own && r.causal ? min(rows, fresh(c.t[k]) + 1 - t0) : rows) - r0 - 32 * kb - 4 * h;
+        const int lim = (own && causal ? min(rows, fresh(c.t[k]) + 1 - t0) : rows) - r0 - 32 * kb - 4 * h;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (8 * (i / 4) + i % 4 >= lim) next[k][i] = -__builtin_inff();
-        if (own && !r.causal) {
+        if (own && !causal) {
           // All flags loaded at once, those past the line's end its last one.
           const LOGKV_G uint8_t* line = gp(a.visible) + b * a.vis_sb + fresh(c.t[k]) * a.vis_st;
           const int first = t0 + r0 + 32 * kb + 4 * h;
@@ -421,8 +428,10 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
     // V of tile ti and K of tile ti + 1 are stored; V of tile ti - 1 has been read, and K of the tile whose buffer
     // tile ti + 2 takes (RB == 1: of tile ti, of which RB > 1 still reads the later blocks: of tile ti - 1).
     __syncthreads();
-    if (flag_s[it % 3]) return false;
-    if (tid == 0) flag_s[(it + 2) % 3] = 0;
+    if constexpr (!PAGED) {
+      if (flag_s[it % 3]) return false;
+      if (tid == 0) flag_s[(it + 2) % 3] = 0;
+    }
 #pragma unroll
     for (int kb = 0; kb < RB; ++kb) {
       // 32 rows: their exponentials and the first 16 rows' parts among the score products of the next 32,
@@ -522,8 +531,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
     }
     load_k(min(ti + 3, end - 1));
     load_v(min(ti + 2, end - 1));
-    page_k(min(ti + 4, end - 1));
-    page_v(min(ti + 3, end - 1));
+    next_pages(min(ti + 4, end - 1));
     k_cur = k_next;
     v_cur = v_next;
   }
@@ -532,7 +540,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
 
 // The same in the second form: a tile that is not finite row by row in float32, each row for the
 // queries that see it. Plain steps (one buffer, nothing ahead): shares that need it are rare.
-template <int DT, int NKS, int NDV, int NW, int QW, int RB, bool BIAS, bool PAGED>
+template <int DT, int NKS, int NDV, int NW, int QW, int RB, bool BIAS>
 __device__ __forceinline__ void rows_tile_share2(const logkv_rows_args& a, const RowsLaunch& r, RowsShare<NKS, NDV>& c,
                                                  uint8_t* buf, float (*bias_s)[32 * RB * NW / QW], int* flag_s) {
   typedef __attribute__((address_space(3))) s16x4* lds4;
@@ -549,13 +557,8 @@ __device__ __forceinline__ void rows_tile_share2(const logkv_rows_args& a, const
     const bool own = ti >= c.np;
     const int t0 = TR * (own ? ti - c.np : ti), rows = min(TR, (own ? c.own : c.n) - t0);
     const int64_t kst = own ? a.k_st : a.ck_st, vst = own ? a.v_st : a.cv_st;
-    const LOGKV_G uint16_t* kr = own ? gp(a.k) + c.b * a.k_sb + c.g * a.k_sg + t0 * kst : gp(a.cache_k) + (PAGED ? 0 : c.b * a.ck_sb + t0 * kst) + c.g * a.ck_sg;
-    const LOGKV_G uint16_t* vr = own ? gp(a.v) + c.b * a.v_sb + c.g * a.v_sg + t0 * vst : gp(a.cache_v) + (PAGED ? 0 : c.b * a.cv_sb + t0 * vst) + c.g * a.cv_sg;
-    auto row_at = [&](const LOGKV_G uint16_t* base, int64_t sb, int64_t st, int rr) {
-      int64_t step;
-      if (PAGED && !own) return page_row(r, base, sb, st, page_of(r, c.b, t0 + rr), t0 + rr, step);
-      return base + rr * st;
-    };
+    const LOGKV_G uint16_t* kr = (own ? gp(a.k) + c.b * a.k_sb + c.g * a.k_sg : gp(a.cache_k) + c.b * a.ck_sb + c.g * a.ck_sg) + t0 * kst;
+    const LOGKV_G uint16_t* vr = (own ? gp(a.v) + c.b * a.v_sb + c.g * a.v_sg : gp(a.cache_v) + c.b * a.cv_sb + c.g * a.cv_sg) + t0 * vst;
     __syncthreads();   // the last tile has been read
     if (tid == 0) flag_s[0] = 0;
     __syncthreads();
@@ -563,14 +566,14 @@ __device__ __forceinline__ void rows_tile_share2(const logkv_rows_args& a, const
     for (int i = tid; i < TR * KU; i += kThreads) {
       const int rr = i / KU, u = i % KU;
       uint4 x = make_uint4(0, 0, 0, 0);
-      if (8 * u < a.dk) x = *(const LOGKV_G uint4*)(row_at(kr, a.ck_sb, kst, min(rr, rows - 1)) + 8 * u);
+      if (8 * u < a.dk) x = *(const LOGKV_G uint4*)(kr + min(rr, rows - 1) * kst + 8 * u);
       ks_[rr * KU + (u ^ swizzle<KU>(rr))] = x;
     }
 #pragma unroll 1
     for (int i = tid; i < TR * VU; i += kThreads) {
       const int rr = i / VU, u = i % VU;
       uint4 x = make_uint4(0, 0, 0, 0);
-      if (8 * u < a.dv && rr < rows) x = *(const LOGKV_G uint4*)(row_at(vr, a.cv_sb, vst, rr) + 8 * u);
+      if (8 * u < a.dv && rr < rows) x = *(const LOGKV_G uint4*)(vr + rr * vst + 8 * u);
       const uint32_t x4[4] = {x.x, x.y, x.z, x.w};
       uint32_t most = 0;
 #pragma unroll
@@ -687,23 +690,35 @@ __device__ __forceinline__ void rows_tile_share2(const logkv_rows_args& a, const
   }
 }
 
-// SECOND: the launch that follows, whose blocks do again what the first left (r.redo, one flag a block).
+// A block's LDS: staged tiles, then (RW > 1) the waves' sums; the bias of the staged rows; notes of V that is not finite;
+// the waves' maxima and sums.
+template <int NKS, int NDV, int NW, int QW, int RB, bool BIAS>
+struct TileLds {
+  static constexpr int RW = NW / QW, TR = 32 * RB * RW;
+  static constexpr int kTileBytes = TR * 16 * (RowsSchedule<RB>::kKBuffers * 2 * NKS + RowsSchedule<RB>::kVBuffers * 4 * NDV);
+  static constexpr int kOutBytes = RW > 1 ? NW * 32 * kCols * 32 * NDV * 4 : 0;
+  alignas(256) uint8_t buf[kTileBytes > kOutBytes ? kTileBytes : kOutBytes];
+  alignas(16) float bias[BIAS ? RowsSchedule<RB>::kKBuffers : 1][TR];
+  int flag[3];
+  float m[NW][32 * kCols], l[NW][32 * kCols];
+};
+
+// The block `id` of `q_blocks` query blocks a lane. SECOND: of the launch that follows, whose blocks do again what the
+// first left (r.redo, one flag a block). PAGED: rows in pages; infinities and NaNs of V are left out and noted behind the
+// partials' sums, for the launch that joins them.
 template <int DT, int NKS, int NDV, int NW, int QW, int RB, bool BIAS, bool SECOND, bool PAGED>
-__global__ __launch_bounds__(64 * NW, 2) void rows_tile_kernel(logkv_rows_args a, RowsLaunch r) {
+__device__ __forceinline__ void rows_tile_block(const logkv_rows_args& a, const RowsLaunch& r, RowsBlock id, int q_blocks,
+                                                TileLds<NKS, NDV, NW, QW, RB, BIAS>& lds) {
   constexpr int kThreads = 64 * NW, RW = NW / QW, TR = 32 * RB * RW, kQueries = 32 * kCols;   // per wave
-  constexpr int kTileBytes = TR * 16 * (RowsSchedule<RB>::kKBuffers * 2 * NKS + RowsSchedule<RB>::kVBuffers * 4 * NDV);
-  constexpr int kOutBytes = RW > 1 ? NW * kQueries * 32 * NDV * 4 : 0;
-  __shared__ __align__(256) uint8_t buf[kTileBytes > kOutBytes ? kTileBytes : kOutBytes];
-  __shared__ __align__(16) float bias_s[BIAS ? RowsSchedule<RB>::kKBuffers : 1][TR];
-  __shared__ int flag_s[3];
-  __shared__ float m_s[NW][kQueries], l_s[NW][kQueries];
-  RowsBlock id = rows_block();
-  int* redo = r.redo + (static_cast<int64_t>(id.lane) * gridDim.y + id.split) * gridDim.x + id.qb;
+  auto& buf = lds.buf;
+  auto& m_s = lds.m;
+  auto& l_s = lds.l;
+  int* redo = PAGED ? nullptr : r.redo + (static_cast<int64_t>(id.lane) * r.splits + id.split) * q_blocks + id.qb;
   if (SECOND && *redo == 0) return;
   int splits = r.splits;
   if (r.shares) {
     if (!share_by_length<TR, PAGED>(a, r, id, splits)) {
-      if (threadIdx.x == 0) *redo = 0;
+      if (!PAGED && threadIdx.x == 0) *redo = 0;
       return;
     }
     if (id.split == 0 && id.qb == 0 && threadIdx.x == 0) r.shares[id.lane] = splits;
@@ -724,6 +739,9 @@ __global__ __launch_bounds__(64 * NW, 2) void rows_tile_kernel(logkv_rows_args a
   const int tiles = c.np + (own_end + TR - 1) / TR, share = (tiles + splits - 1) / splits;
   c.begin = min(id.split * share, tiles);
   c.end = min(c.begin + share, tiles);
+  if constexpr (PAGED) {   // the same in every lane, which the compiler does not see through the length's load
+    for (int* x : {&c.b, &c.g, &c.n, &c.own, &c.np, &c.begin, &c.end}) *x = __builtin_amdgcn_readfirstlane(*x);
+  }
 #pragma unroll
   for (int k = 0; k < kCols; ++k) {
     const LOGKV_G uint16_t* qrow = query_row<PAGED>(a, r, c.b, c.g, min(q0 + 32 * k, nq - 1), c.t[k]);
@@ -734,11 +752,15 @@ __global__ __launch_bounds__(64 * NW, 2) void rows_tile_kernel(logkv_rows_args a
     }
   }
   if constexpr (SECOND) {
-    rows_tile_share2<DT, NKS, NDV, NW, QW, RB, BIAS, PAGED>(a, r, c, buf, bias_s, flag_s);
+    rows_tile_share2<DT, NKS, NDV, NW, QW, RB, BIAS>(a, r, c, buf, lds.bias, lds.flag);
   } else {
-    const bool done = rows_tile_share<DT, NKS, NDV, NW, QW, RB, BIAS, PAGED>(a, r, c, buf, bias_s, flag_s);
-    if (tid == 0) *redo = done ? 0 : 1;
-    if (!done) return;
+    const bool done = rows_tile_share<DT, NKS, NDV, NW, QW, RB, BIAS, PAGED>(a, r, c, buf, lds.bias, lds.flag);
+    if constexpr (PAGED) {
+      __syncthreads();   // every wave's note
+    } else {
+      if (tid == 0) *redo = done ? 0 : 1;
+      if (!done) return;
+    }
   }
 #pragma unroll
   for (int k = 0; k < kCols; ++k) {
@@ -752,6 +774,7 @@ __global__ __launch_bounds__(64 * NW, 2) void rows_tile_kernel(logkv_rows_args a
         for (int i = 0; i < 16; ++i) c.o[k][nb][i] = 0.f;
     }
   }
+  const float note = PAGED && lds.flag[0] ? 1.f : 0.f;
   float* part = r.part + (static_cast<int64_t>(lane) * r.room + id.split) * nq * (a.dv + kRowsPartTail);
   if constexpr (RW == 1) {
 #pragma unroll
@@ -759,7 +782,10 @@ __global__ __launch_bounds__(64 * NW, 2) void rows_tile_kernel(logkv_rows_args a
       const int qi = q0 + 32 * k;
       if (qi >= nq) continue;
       float* out = part + static_cast<int64_t>(qi) * (a.dv + kRowsPartTail);
-      if (h == 0) *reinterpret_cast<float2*>(out + a.dv) = make_float2(c.m[k], c.lsum[k]);
+      if (h == 0) {
+        if constexpr (PAGED) *reinterpret_cast<f32x4*>(out + a.dv) = f32x4{c.m[k], c.lsum[k], note, 0.f};
+        else *reinterpret_cast<float2*>(out + a.dv) = make_float2(c.m[k], c.lsum[k]);
+      }
 #pragma unroll
       for (int nb = 0; nb < NDV; ++nb)
 #pragma unroll
@@ -805,39 +831,10 @@ __global__ __launch_bounds__(64 * NW, 2) void rows_tile_kernel(logkv_rows_args a
         else sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(buf) + (ww * kQueries + cc) * kLd + 4 * (u ^ (cc & 7))) * f;
       }
       if (u == units - 1) sum[0] = mx;
+      if (PAGED && u == units - 1) sum[2] = note;
       *reinterpret_cast<f32x4*>(part + static_cast<int64_t>(q_first + q) * (a.dv + kRowsPartTail) + 4 * u) = sum;
     }
   }
 }
-
-namespace {
-
-template <int DT, int NKS, int NDV, int NW, int QW, int RB, bool PAGED>
-void launch_tile_one(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
-  const int nq = a.n_heads / a.n_groups * a.tq * (PAGED ? r.seqs : 1), queries = 32 * kCols * QW;
-  const dim3 grid((nq + queries - 1) / queries, r.splits, a.n_batch * a.n_groups);
-  if (a.bias) {
-    hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, NW, QW, RB, true, false, PAGED>), grid, dim3(64 * NW), 0, stream, a, r);
-    hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, NW, QW, RB, true, true, PAGED>), grid, dim3(64 * NW), 0, stream, a, r);
-  } else {
-    hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, NW, QW, RB, false, false, PAGED>), grid, dim3(64 * NW), 0, stream, a, r);
-    hipLaunchKernelGGL((rows_tile_kernel<DT, NKS, NDV, NW, QW, RB, false, true, PAGED>), grid, dim3(64 * NW), 0, stream, a, r);
-  }
-}
-
-template <int DT, int NKS, int NDV, bool PAGED>
-void launch_tile_width(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
-  if (r.q_waves == 2) launch_tile_one<DT, NKS, NDV, 4, 2, 1, PAGED>(a, r, stream);
-  else if (r.q_waves == 4) launch_tile_one<DT, NKS, NDV, 8, 4, 1, PAGED>(a, r, stream);
-  else launch_tile_one<DT, NKS, NDV, 8, 8, 2, PAGED>(a, r, stream);
-}
-
-template <int DT, bool PAGED>
-void launch_tile_type(const logkv_rows_args& a, const RowsLaunch& r, hipStream_t stream) {
-  if (a.dk <= 64 && a.dv <= 64) launch_tile_width<DT, 4, 2, PAGED>(a, r, stream);
-  else launch_tile_width<DT, 8, 4, PAGED>(a, r, stream);
-}
-
-}  // namespace
 
 }  // namespace logkv
