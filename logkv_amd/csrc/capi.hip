@@ -976,12 +976,12 @@ int check_paged_shape(const logkv_paged_args* a) {
     return fail(LOGKV_EINVAL, "paged attention: pages of %d rows (a power of two from 16 on), %d a sequence, a prefix of %d",
                 a->page, a->table_len, a->prefix_len);
   if (a->dtype != LOGKV_BF16 && a->dtype != LOGKV_F16) return fail(LOGKV_EINVAL, "paged attention takes bf16 or fp16");
-  if (logkv::paged_launch(*a, nullptr).blocks > logkv::kMostPagedBlocks)
-    return fail(LOGKV_EINVAL, "paged attention over too many queries and lanes at once");
   return LOGKV_OK;
 }
 
-int check_paged(const logkv_paged_args* a, const void* ws, int64_t ws_bytes) {
+int too_many_blocks() { return fail(LOGKV_EINVAL, "paged attention over too many queries and lanes at once"); }
+
+int check_paged(const logkv_paged_args* a) {
   int rc = check_paged_shape(a);
   if (rc) return rc;
   if (!a->q || !a->k || !a->v || !a->out || (a->table_len && !a->table) || (a->n_pages && (!a->k_pages || !a->v_pages)))
@@ -1000,8 +1000,6 @@ int check_paged(const logkv_paged_args* a, const void* ws, int64_t ws_bytes) {
   if (!(a->bias_scale >= 0.f) || !std::isfinite(a->bias_scale))
     return fail(LOGKV_EINVAL, "attention bias_scale must be positive, or 0 for 1");
   if (a->visible && a->counts) return fail(LOGKV_EINVAL, "paged attention takes a mask of the call's rows or their counts");
-  if (!aligned16(ws) || !ws || ws_bytes < logkv::paged_launch(*a, nullptr).bytes)
-    return fail(LOGKV_EINVAL, "paged attention workspace too small");
   return LOGKV_OK;
 }
 
@@ -1009,13 +1007,18 @@ int check_paged(const logkv_paged_args* a, const void* ws, int64_t ws_bytes) {
 
 int64_t logkv_paged_workspace_bytes(const logkv_paged_args* a) {
   if (check_paged_shape(a)) return -1;
-  return logkv::paged_launch(*a, nullptr).bytes;
+  const logkv::PagedLaunch p = logkv::paged_launch(*a, nullptr);
+  if (p.blocks > logkv::kMostPagedBlocks) return too_many_blocks(), -1;
+  return p.bytes;
 }
 
 int logkv_paged_attention(const logkv_paged_args* a, void* ws, int64_t ws_bytes, void* stream) {
-  int rc = check_paged(a, ws, ws_bytes);
+  int rc = check_paged(a);
   if (rc) return rc;
-  rc = logkv::launch_paged_attention(*a, logkv::paged_launch(*a, ws), static_cast<hipStream_t>(stream));
+  const logkv::PagedLaunch p = logkv::paged_launch(*a, ws);
+  if (p.blocks > logkv::kMostPagedBlocks) return too_many_blocks();
+  if (!aligned16(ws) || !ws || ws_bytes < p.bytes) return fail(LOGKV_EINVAL, "paged attention workspace too small");
+  rc = logkv::launch_paged_attention(*a, p, static_cast<hipStream_t>(stream));
   if (rc) return launch_failed(rc, "paged attention");
   return LOGKV_OK;
 }

@@ -199,37 +199,70 @@ int launch_passes(const PagedPass& shared, const PagedPass& own, hipStream_t str
 
 }  // namespace
 
+// A pass's lanes, query blocks, rows at most, and a step of one of its blocks: the rows that it takes, in microseconds.
+struct PassShape {
+  int64_t lanes;
+  int q_blocks, queries, rows, step_rows;
+  float step_us;
+  // Blocks of s shares a lane, and a block's time: its steps, and kBlockUs to begin and to end.
+  int64_t blocks(int s) const { return lanes * q_blocks * s; }
+  float time(int s) const { return kBlockUs + ((rows + step_rows - 1) / step_rows + s - 1) / s * step_us; }
+  static constexpr float kBlockUs = 4.f;
+};
+
+PassShape shape_of(const PagedPass& p, int waves) {
+  const logkv_rows_args& a = p.args;
+  const RowsLaunch& r = p.launch;
+  const int width = std::max(a.dk, a.dv);
+  PassShape x;
+  x.lanes = static_cast<int64_t>(a.n_batch) * a.n_groups;
+  x.q_blocks = r.q_blocks;
+  x.queries = a.n_heads / a.n_groups * a.tq * r.seqs;
+  x.rows = a.cap + (r.prefix ? 0 : a.tq);
+  x.step_rows = r.q_waves ? 64 : 32 * waves;
+  x.step_us = r.q_waves ? (r.q_waves == 8 ? 3.6f : 2.f) : 1.5f;
+  if (width <= 64) x.step_us *= 0.6f;
+  if (width > 128) x.step_us *= 2.f;
+  return x;
+}
+
+// Shares of the lanes of two passes in one launch: the ones of least time by what the blocks take side by side, the
+// steps of both over the chip, and the partials' way out and in.
+void share_out(PagedPass& shared, PagedPass& own, int slots, int waves) {
+  const PassShape x = shape_of(shared, waves), y = shape_of(own, waves);
+  static constexpr int kShares[] = {1, 2, 3, 4, 6, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 56, 64};
+  const float partial_us = 8.f * (own.args.dv + kRowsPartTail) / 5e6f;
+  float best = 3e38f;
+  for (int i : kShares) {
+    if (i > 1 && (i - 1) * x.step_rows >= x.rows) break;
+    for (int j : kShares) {
+      if (j > 1 && (j - 1) * y.step_rows >= y.rows) break;
+      const float tx = x.time(i), ty = y.time(j);
+      const int64_t n = x.blocks(i) + y.blocks(j);
+      float t = std::max(tx, ty);
+      if (n > slots) t = std::max(t, (x.blocks(i) * tx + y.blocks(j) * ty) / slots + std::min(tx, ty) / 2);
+      t += partial_us * (static_cast<float>(x.lanes) * x.queries * i + static_cast<float>(y.lanes) * y.queries * j);
+      if (t < best) {
+        best = t;
+        shared.launch.splits = i;
+        own.launch.splits = j;
+      }
+    }
+  }
+}
+
 PagedLaunch paged_launch(const logkv_paged_args& a, void* ws) {
-  uint8_t* base = static_cast<uint8_t*>(ws);
-  int64_t off = 0;
-  auto take = [&](int64_t words) {
-    float* p = base ? reinterpret_cast<float*>(base + off) : nullptr;
-    off += align256(4 * words);
-    return p;
-  };
   const int width = std::max(a.dk, a.dv);
   PagedLaunch p{};
   auto plan = [&](PagedPass& pass) {
     RowsLaunch& r = pass.launch;
     const logkv_rows_args& x = pass.args;
-    const int64_t lanes = static_cast<int64_t>(x.n_batch) * x.n_groups;
     const int64_t nq = static_cast<int64_t>(x.n_heads / x.n_groups) * x.tq * r.seqs;
     r.bias2 = (x.bias_scale == 0.f ? 1.f : x.bias_scale) * kLog2e;
     r.causal = x.visible ? 0 : 1;
-    rows_plan(x, lanes, nq, r);
-    if (!r.q_waves && width > 64) r.cols = 1;
+    rows_plan(x, static_cast<int64_t>(x.n_batch) * x.n_groups, nq, r);
+    if (!r.q_waves && width > 64) r.cols = 1;   // two column blocks of wider rows spill
     r.q_blocks = static_cast<int>(r.q_waves ? (nq + 32 * r.q_waves - 1) / (32 * r.q_waves) : (nq + 16 * r.cols - 1) / (16 * r.cols));
-    // Shares by length (rows_tile.hpp), as of contiguous rows.
-    const bool by_length = r.q_waves && r.splits > 1 && x.n_batch > 1 && x.n_batch <= kWave;
-    r.room = by_length ? 2 * r.splits : r.splits;
-    r.part = take(lanes * r.room * nq * (x.dv + kRowsPartTail));
-    if (by_length) {
-      r.shares = reinterpret_cast<int*>(take(lanes));
-      if (!x.lengths || !x.len_stride) r.shares = nullptr;   // rows of one length
-    }
-    const int64_t blocks = lanes * r.splits * r.q_blocks;
-    p.blocks += blocks;
-    pass.blocks = static_cast<int>(blocks);
   };
   logkv_rows_args& x = p.own.args;
   x.q = a.q, x.q_sb = a.q_sb, x.q_sh = a.q_sh, x.q_st = a.q_st;
@@ -266,11 +299,38 @@ PagedLaunch paged_launch(const logkv_paged_args& a, void* ws) {
       y.cap = a.prefix_len;
     }
     plan(p.shared);
+    // Passes of one launch have the same threads a block and at most one tiled and one streamed kernel.
+    const RowsLaunch &o = p.own.launch, &h = p.shared.launch;
+    p.together = o.q_waves && h.q_waves ? o.q_waves == h.q_waves : o.q_waves || h.q_waves || o.cols == h.cols;
+    if (p.together) {
+      const int q_waves = std::max(o.q_waves, h.q_waves), waves = paged_waves(q_waves);
+      share_out(p.shared, p.own, waves == 8 || width > 128 ? 256 : 512, waves);
+    }
   }
-  // Passes of one launch have the same threads a block and at most one tiled and one streamed kernel.
-  const RowsLaunch &o = p.own.launch, &h = p.shared.launch;
-  p.together = a.n_prefixes && (o.q_waves && h.q_waves ? o.q_waves == h.q_waves : o.q_waves || h.q_waves || o.cols == h.cols);
-  p.bytes = off;
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  auto take = [&](int64_t words) {
+    float* at = base ? reinterpret_cast<float*>(base + p.bytes) : nullptr;
+    p.bytes += align256(4 * words);
+    return at;
+  };
+  for (PagedPass* pass : {&p.own, &p.shared}) {
+    RowsLaunch& r = pass->launch;
+    const logkv_rows_args& y = pass->args;
+    if (!r.seqs) continue;
+    const int64_t lanes = static_cast<int64_t>(y.n_batch) * y.n_groups;
+    const int64_t nq = static_cast<int64_t>(y.n_heads / y.n_groups) * y.tq * r.seqs;
+    // Shares by length (rows_tile.hpp), as of contiguous rows.
+    const bool by_length = r.q_waves && r.splits > 1 && y.n_batch > 1 && y.n_batch <= kWave;
+    r.room = by_length ? 2 * r.splits : r.splits;
+    r.part = take(lanes * r.room * nq * (y.dv + kRowsPartTail));
+    if (by_length) {
+      r.shares = reinterpret_cast<int*>(take(lanes));
+      if (!y.lengths || !y.len_stride) r.shares = nullptr;   // rows of one length
+    }
+    const int64_t blocks = lanes * r.splits * r.q_blocks;
+    p.blocks += blocks;
+    pass->blocks = static_cast<int>(blocks);
+  }
   return p;
 }
 
