@@ -9,6 +9,7 @@
 // An infinity or NaN in V is left out of a pass's products, which would spread it to queries that do not
 // see its row, and noted behind the partial's sums; the join then adds those of the rows that a query sees.
 #include <algorithm>
+#include <cmath>
 
 #include "paged.hpp"
 
@@ -57,64 +58,89 @@ __device__ __forceinline__ void add_odd_rows(const logkv_rows_args& a, const Row
   }
 }
 
+// What the join reads of a pass: the partials of a lane, [room][queries][dv + kRowsPartTail] each.
+struct FinishPass {
+  const float* part;
+  const int* shares;   // partials of a lane, null: `splits` of each
+  int splits, room;
+  int seqs;            // sequences of a lane, 0: no such pass
+  float unit;          // the sums' scale
+};
+// What every block reads comes first; the passes themselves are for the rows of notes.
+struct FinishArgs {
+  FinishPass own, shared;
+  uint16_t* out;
+  int64_t o_sb, o_sh, o_st;
+  const int32_t* counts;
+  int n_groups, rep, tq, dv;
+  PagedPass passes[2];
+};
+
 // TQ threads per query, four features each; the block's other factor is shared by queries and by groups of
-// partials (QPB queries x SG groups), joined in group order.
+// partials (QPB queries x SG groups), joined in group order. A query's partials are its own ones, then its prefix's.
 template <int DT, int TQ, int SG>
-__global__ __launch_bounds__(kThreads) void paged_finish_kernel(PagedPass own, PagedPass shared) {
+__global__ __launch_bounds__(kThreads) void paged_finish_kernel(FinishArgs a) {
   typedef Elem<DT> E;
-  const logkv_rows_args& a = own.args;
   constexpr int QPB = kThreads / (TQ * SG);
   __shared__ __align__(16) float acc_s[QPB][SG][4 * TQ];
   __shared__ float m_s[QPB][SG], l_s[QPB][SG];
   __shared__ float2 odd_s[QPB][SG];
-  const int G = a.n_groups, b = static_cast<int>(blockIdx.y) / G, g = static_cast<int>(blockIdx.y) % G;
-  const int rep = a.n_heads / G, nq = rep * a.tq, tid = threadIdx.x, stride = a.dv + kRowsPartTail;
+  const int G = a.n_groups, b = static_cast<int>(blockIdx.y) / G, g = static_cast<int>(blockIdx.y) - b * G;
+  const int nq = a.rep * a.tq, tid = threadIdx.x, stride = a.dv + kRowsPartTail;
   const int qs = tid / (TQ * SG), sg = tid / TQ % SG, d = 4 * (tid % TQ);
-  const int qi = static_cast<int>(blockIdx.x) * QPB + qs;
+  const int qi = static_cast<int>(blockIdx.x) * QPB + qs, qc = min(qi, nq - 1), head = qc / a.tq, t = qc - head * a.tq;
   const bool there = qi < nq && d < a.dv;
-  const bool live = min(qi, nq - 1) % a.tq < own_rows(a, b);   // a query past its sequence's count sees nothing
+  const bool live = !a.counts || t < gp(a.counts)[b];   // a query past its sequence's count sees nothing
+  // The two passes' partials of this query, and how far the next ones are.
+  const int lane = static_cast<int>(blockIdx.y);
+  int n_own = a.own.splits, n_shared = 0;
+  if (a.own.shares) n_own = gp(a.own.shares)[lane];
+  const int64_t own_step = static_cast<int64_t>(nq) * stride;
+  const LOGKV_G float* own = gp(a.own.part) + lane * (a.own.room * own_step) + static_cast<int64_t>(qc) * stride;
+  const LOGKV_G float* shared = own;
+  int64_t shared_step = 0;
+  if (a.shared.seqs) {
+    const int run = b / a.shared.seqs, run_lane = run * G + g, s = b - run * a.shared.seqs;
+    n_shared = a.shared.splits;
+    if (a.shared.shares) n_shared = gp(a.shared.shares)[run_lane];
+    shared_step = a.shared.seqs * own_step;
+    shared = gp(a.shared.part) + run_lane * (a.shared.room * shared_step) + static_cast<int64_t>(s * nq + qc) * stride;
+  }
+  const int all = live ? n_own + n_shared : 0;
   float m = -__builtin_inff(), lsum = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   float odd[2] = {0.f, 0.f};   // the partials' notes
+  // Eight partials' loads at a time, joined under the running maximum.
+  for (int s0 = sg; s0 < all; s0 += 8 * SG) {
+    f32x4 ml[8], x[8];
+    float mx = m;
 #pragma unroll
-  for (int set = 0; set < 2; ++set) {
-    const PagedPass& pass = set ? shared : own;
-    const RowsLaunch& r = pass.launch;
-    if (set && !r.seqs) continue;
-    const int lane = (set ? b / r.seqs : b) * G + g, splits = r.shares ? r.shares[lane] : r.splits;
-    const int64_t step = static_cast<int64_t>(set ? r.seqs * nq : nq) * stride;
-    const float* base = r.part + static_cast<int64_t>(lane) * r.room * step +
-                        static_cast<int64_t>((set ? b % r.seqs * nq : 0) + min(qi, nq - 1)) * stride;
-    const float unit = __builtin_amdgcn_exp2f(-r.shift);
-    // Eight partials' loads at a time, joined under the running maximum.
-    for (int s0 = sg; s0 < splits; s0 += 8 * SG) {
-      f32x4 ml[8], x[8];
-      float mx = m;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int sp = s0 + k * SG;
-        ml[k] = f32x4{-__builtin_inff(), 0.f, 0.f, 0.f};
-        x[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (there && live && sp < splits) {
-          ml[k] = *reinterpret_cast<const f32x4*>(base + sp * step + a.dv);
-          x[k] = *reinterpret_cast<const f32x4*>(base + sp * step + d);
-        }
+    for (int k = 0; k < 8; ++k) {
+      const int sp = s0 + k * SG;
+      ml[k] = f32x4{-__builtin_inff(), 0.f, 0.f, 0.f};
+      x[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (there && sp < all) {
+        const LOGKV_G float* at = sp < n_own ? own + sp * own_step : shared + (sp - n_own) * shared_step;
+        ml[k] = *reinterpret_cast<const LOGKV_G f32x4*>(at + a.dv);
+        x[k] = *reinterpret_cast<const LOGKV_G f32x4*>(at + d);
       }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) mx = fmaxf(mx, ml[k][0]);
-      const float top = mx == -__builtin_inff() ? 0.f : mx;
-      const float corr = __builtin_amdgcn_exp2f(m - top);
-      lsum *= corr;
-      acc *= corr;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float f = unit * __builtin_amdgcn_exp2f(ml[k][0] - top);
-        lsum += ml[k][1] * f;
-        acc += x[k] * f;
-        odd[set] += ml[k][2];
-      }
-      m = mx;
     }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mx = fmaxf(mx, ml[k][0]);
+    const float top = mx == -__builtin_inff() ? 0.f : mx;
+    const float corr = __builtin_amdgcn_exp2f(m - top);
+    lsum *= corr;
+    acc *= corr;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const bool of_own = s0 + k * SG < n_own;
+      const float f = (of_own ? a.own.unit : a.shared.unit) * __builtin_amdgcn_exp2f(ml[k][0] - top);
+      lsum += ml[k][1] * f;
+      acc += x[k] * f;
+      odd[0] += of_own ? ml[k][2] : 0.f;
+      odd[1] += of_own ? 0.f : ml[k][2];
+    }
+    m = mx;
   }
   if constexpr (SG > 1) {
     *reinterpret_cast<f32x4*>(&acc_s[qs][sg][d]) = acc;
@@ -145,14 +171,14 @@ __global__ __launch_bounds__(kThreads) void paged_finish_kernel(PagedPass own, P
   f32x4 z = {0.f, 0.f, 0.f, 0.f};
   if (lsum != 0.f) z = acc / lsum;
   if (__builtin_expect(odd[0] + odd[1] > 0.f, 0)) {
-    const int t = qi % a.tq;
-    if (odd[0] > 0.f) add_odd_rows<DT>(a, own.launch, b, g, t, d, z);
-    if (odd[1] > 0.f) add_odd_rows<DT>(shared.args, shared.launch, b / shared.launch.seqs, g, t, d, z);
+    const PagedPass &p0 = a.passes[0], &p1 = a.passes[1];
+    if (odd[0] > 0.f) add_odd_rows<DT>(p0.args, p0.launch, b, g, t, d, z);
+    if (odd[1] > 0.f) add_odd_rows<DT>(p1.args, p1.launch, b / a.shared.seqs, g, t, d, z);
   }
   uint16_t y[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) y[k] = E::from_f32(z[k]);
-  LOGKV_G uint16_t* o = gp(a.out) + b * a.o_sb + (g * rep + qi / a.tq) * a.o_sh + qi % a.tq * a.o_st + d;
+  LOGKV_G uint16_t* o = gp(a.out) + b * a.o_sb + (g * a.rep + head) * a.o_sh + t * a.o_st + d;
   *reinterpret_cast<LOGKV_G uint2*>(o) =
       make_uint2(y[0] | static_cast<uint32_t>(y[1]) << 16, y[2] | static_cast<uint32_t>(y[3]) << 16);
 }
@@ -162,9 +188,12 @@ namespace {
 template <int DT, int TQ, int SG>
 void launch_finish(const PagedLaunch& p, hipStream_t stream) {
   const logkv_rows_args& a = p.own.args;
-  const int nq = a.n_heads / a.n_groups * a.tq, qpb = kThreads / (TQ * SG);
+  const int rep = a.n_heads / a.n_groups, nq = rep * a.tq, qpb = kThreads / (TQ * SG);
+  auto pass = [](const RowsLaunch& r) { return FinishPass{r.part, r.shares, r.splits, r.room, r.seqs, exp2f(-r.shift)}; };
+  const FinishArgs args = {pass(p.own.launch), pass(p.shared.launch), a.out, a.o_sb, a.o_sh, a.o_st, a.counts,
+                           a.n_groups, rep, a.tq, a.dv, {p.own, p.shared}};
   hipLaunchKernelGGL((paged_finish_kernel<DT, TQ, SG>), dim3((nq + qpb - 1) / qpb, a.n_batch * a.n_groups), dim3(kThreads),
-                     0, stream, p.own, p.shared);
+                     0, stream, args);
 }
 
 template <int DT>
@@ -234,9 +263,9 @@ void share_out(PagedPass& shared, PagedPass& own, int slots, int waves) {
   const float partial_us = 8.f * (own.args.dv + kRowsPartTail) / 5e6f;
   float best = 3e38f;
   for (int i : kShares) {
-    if (i > 1 && (i - 1) * x.step_rows >= x.rows) break;
+    if (i > 1 && ((i - 1) * x.step_rows >= x.rows || x.blocks(i) > 4 * slots)) break;
     for (int j : kShares) {
-      if (j > 1 && (j - 1) * y.step_rows >= y.rows) break;
+      if (j > 1 && ((j - 1) * y.step_rows >= y.rows || y.blocks(j) > 4 * slots)) break;
       const float tx = x.time(i), ty = y.time(j);
       const int64_t n = x.blocks(i) + y.blocks(j);
       float t = std::max(tx, ty);

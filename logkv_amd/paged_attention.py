@@ -102,12 +102,15 @@ def log_kv_paged_append(k, v, k_pages, v_pages, table, lengths, *, q=None, frequ
     code, page = _check_pages(k_pages, v_pages, groups)
     if v.dtype != dtype or not k.get_device() == v.get_device() == v_pages.get_device() == index:
         raise ValueError("new rows must be of one dtype, on the pages' device")
-    if q is not None and (q.ndim != 4 or q.size(0) != batch or q.size(2) != tokens or q.size(3) != dk or q.dtype != dtype
-                          or q.get_device() != index):
-        raise ValueError("queries must be [B, n_heads, T, dk], in the new rows' dtype on their device")
+    if q is not None:
+        q_shape = q.shape
+        if (len(q_shape) != 4 or q_shape[0] != batch or q_shape[2] != tokens or q_shape[3] != dk or q.dtype != dtype
+                or q.get_device() != index):
+            raise ValueError("queries must be [B, n_heads, T, dk], in the new rows' dtype on their device")
     check_activation_dtype(dtype)
-    kp_sp, kp_sg, kp_st, kp_sd = k_pages.stride()
-    vp_sp, vp_sg, vp_st, vp_sd = v_pages.stride()
+    kp_strides, vp_strides = k_pages.stride(), v_pages.stride()
+    kp_sp, kp_sg, kp_st, kp_sd = kp_strides
+    vp_sp, vp_sg, vp_st, vp_sd = vp_strides
     if k_pages.size(3) != dk or v_pages.size(3) != dv or not 1 <= dk <= MAX_WIDTH or not 1 <= dv <= MAX_WIDTH:
         raise ValueError(f"the pages' rows must be as wide as the new ones, up to {MAX_WIDTH} features")
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad
@@ -115,7 +118,7 @@ def log_kv_paged_append(k, v, k_pages, v_pages, table, lengths, *, q=None, frequ
         raise NotImplementedError("a paged append is for inference: it has no gradient (run it under torch.no_grad())")
     if kp_sd != 1 and dk > 1 or vp_sd != 1 and dv > 1:
         raise ValueError("the pages' features must be contiguous")
-    if _repeats(k_pages) or _repeats(v_pages):
+    if 0 in kp_strides and _repeats(k_pages) or 0 in vp_strides and _repeats(v_pages):
         raise ValueError("pages are written: their rows must not share memory (expanded tensors)")
     amplitude = float(amplitude)
     if not math.isfinite(amplitude):
@@ -149,20 +152,24 @@ def log_kv_paged_append(k, v, k_pages, v_pages, table, lengths, *, q=None, frequ
         positions, p_ptr, p_sb, p_st, p_int, _ = _check_positions(positions, batch, tokens, index)
     heads, q_out, q_in, q_to = 0, q, _NO_ROWS, _NO_ROWS
     if q is not None and rotated:
-        heads = q.size(1)
+        heads = q_shape[1]
         q, q_out, q_in, q_to = _in_and_out(q)
-    if dk > 1 and k.stride(3) != 1:
+    k_sb, k_sh, k_st, k_sd = k.stride()
+    v_sb, v_sh, v_st, v_sd = v.stride()
+    if k_sd != 1 and dk > 1:
         k = k.contiguous()
-    if dv > 1 and v.stride(3) != 1:
+        k_sb, k_sh, k_st, _ = k.stride()
+    if v_sd != 1 and dv > 1:
         v = v.contiguous()
+        v_sb, v_sh, v_st, _ = v.stride()
     # Without a rotation or a rounding the keys are the caller's own.
     k_out, k_to = k, _NO_ROWS
     if rotated or dtype != k_pages.dtype:
         k_out = k_pages.new_empty(k_shape)
-        k_to = k_out.data_ptr(), *k_out.stride()[:3]
-    if not k.numel() or not v.numel():
+        k_to = k_out.data_ptr(), groups * tokens * dk, tokens * dk, dk
+    if batch < 1 or groups < 1 or tokens < 1:
         return q_out, k_out
-    args = pack_rotary(*q_in, *q_to, k.data_ptr(), *k.stride()[:3], *k_to, v.data_ptr(), *v.stride()[:3],
+    args = pack_rotary(*q_in, *q_to, k.data_ptr(), k_sb, k_sh, k_st, *k_to, v.data_ptr(), v_sb, v_sh, v_st,
                        k_pages.data_ptr(), kp_sp, kp_sg, kp_st, v_pages.data_ptr(), vp_sp, vp_sg, vp_st,
                        table_ptr, table_sb, n_ptr, c_ptr, freq_ptr, p_ptr, p_sb, p_st, first_ptr, first, batch, heads,
                        groups, tokens, dk, dv, rotated, _TYPES[dtype], code, int(interleaved), freq_float, p_int,
@@ -183,10 +190,14 @@ def _workspace_bytes(batch, heads, groups, tq, dk, dv, dtype, page, table_len, p
     return need
 
 
+def _needs_gradient(prefix):
+    return any(x is not None and x.requires_grad for x in (prefix.k, prefix.v, prefix.bias))
+
+
 def _check_prefix(prefix, batch, groups, dk, dv, dtype, page, index):
     """(prefixes, rows or pages each, table address and stride, K and V address and strides, bias address and strides,
     its half flag, capacity in rows)."""
-    table, pk, pv, bias = prefix.table, prefix.k, prefix.v, prefix.bias
+    _, table, pk, pv, bias, _ = prefix
     if (table is None) == (pk is None) or (pk is None) != (pv is None) or table is not None and bias is not None:
         raise ValueError("a prefix has a table of pages, or k and v rows with an optional bias")
     if table is not None:
@@ -233,36 +244,47 @@ def log_kv_paged_attention(q, k, v, k_pages, v_pages, table, lengths, scale, *, 
 
 def _paged_attention(q, k, v, k_pages, v_pages, table, lengths, scale, prefix, visible, counts, prefix_in_use):
     """``prefix_in_use`` in place of the prefix's lengths: as ``_attention``'s ``in_use``."""
-    if not q.ndim == k.ndim == v.ndim == 4:
+    q_shape, k_shape, v_shape = q.shape, k.shape, v.shape
+    if not len(q_shape) == len(k_shape) == len(v_shape) == 4:
         raise ValueError("queries and rows must be 4-dimensional")
-    batch, heads, tq, dk = q.shape
-    groups, dv = k.size(1), v.size(3)
+    batch, heads, tq, dk = q_shape
+    groups, dv = k_shape[1], v_shape[3]
     code, page = _check_pages(k_pages, v_pages, groups)
-    dtype, index = k_pages.dtype, k_pages.get_device()
-    if k_pages.size(3) != dk or v_pages.size(3) != dv or groups < 1 or heads % groups or min(heads, tq, batch) < 1:
+    dtype, index, n_pages = k_pages.dtype, k_pages.get_device(), k_pages.size(0)
+    if k_pages.size(3) != dk or v_pages.size(3) != dv or groups < 1 or heads % groups or heads < 1 or tq < 1 or batch < 1:
         raise ValueError("pages must be [pages, G, page_size, d] with G dividing the query heads")
-    if k.shape != (batch, groups, tq, dk) or v.shape != (batch, groups, tq, dv):
+    if k_shape != (batch, groups, tq, dk) or v_shape != (batch, groups, tq, dv):
         raise ValueError("the call's rows must be [B, G, T, d], one per query position")
     if not v_pages.get_device() == q.get_device() == k.get_device() == v.get_device() == index:
         raise ValueError("all tensors must be on the pages' device")
     if not (0.0 < scale < math.inf):
         raise ValueError("attention scale must be positive")
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (
-            q, k, v, k_pages, v_pages, *(() if prefix is None else (prefix.k, prefix.v, prefix.bias)))):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or k_pages.requires_grad
+                                    or v_pages.requires_grad or prefix is not None and _needs_gradient(prefix)):
         raise NotImplementedError("paged attention is for inference: it has no gradient (run it under torch.no_grad())")
-    kp_st, vp_st = (_unit_strides(x) if x.numel() else _NO_STRIDES for x in (k_pages, v_pages))
+    kp_st, vp_st = (_unit_strides(k_pages), _unit_strides(v_pages)) if n_pages else (_NO_STRIDES, _NO_STRIDES)
     if kp_st is None or vp_st is None:
         raise ValueError("the pages' rows must be 16-byte aligned with contiguous features")
     table_ptr, table_sb, table_len = _check_table(table, batch, index)
+    vis_ptr = vis_sb = vis_st = c_ptr = 0
     if visible is not None:
         if counts is not None:
             raise ValueError("paged attention takes a mask of the call's rows or their counts")
         visible = _tree(visible, q, k_pages)
+        vis_ptr, vis_sb, vis_st = visible.data_ptr(), visible.stride(0) if visible.ndim == 3 else 0, visible.stride(-2)
     elif counts is not None:
         counts = _check_counts(counts, batch, index)
+        c_ptr = counts.data_ptr()
     lengths, n_ptr, n_st, len_add = _lengths(lengths, batch, table_len * page, index)
     out_dtype = q.dtype
-    q, k, v = _small_rows(q, dtype), _small_rows(k, dtype), _small_rows(v, dtype)
+    q_st, k_st, v_st = q.stride(), k.stride(), v.stride()
+    qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if (out_dtype != dtype or k.dtype != dtype or v.dtype != dtype or not q_st[3] == k_st[3] == v_st[3] == 1
+            or (q_st[0] | q_st[1] | q_st[2] | k_st[0] | k_st[1] | k_st[2] | v_st[0] | v_st[1] | v_st[2]) & 7
+            or (qp | kp | vp) & 15):
+        q, k, v = _small_rows(q, dtype), _small_rows(k, dtype), _small_rows(v, dtype)
+        q_st, k_st, v_st = q.stride(), k.stride(), v.stride()
+        qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
     prefixes = prefix_len = pt_ptr = pt_sb = b_ptr = b_half = pn_ptr = pn2_ptr = pn_st = pn_add = 0
     pk = pv = _NO_ROWS
     b_st, bias_scale = _NO_STRIDES, 0.0
@@ -280,14 +302,11 @@ def _paged_attention(q, k, v, k_pages, v_pages, table, lengths, scale, prefix, v
     need = _workspace_bytes(batch, heads, groups, tq, dk, dv, code, page, table_len, prefixes, prefix_len, pt_ptr != 0)
     workspace = k_pages.new_empty(need // 2)
     o_sh = tq * dv
-    vis_ptr = vis_sb = vis_st = 0
-    if visible is not None:
-        vis_ptr, vis_sb, vis_st = visible.data_ptr(), visible.stride(0) if visible.ndim == 3 else 0, visible.stride(-2)
     args = pack_paged(
-        q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
+        qp, q_st[0], q_st[1], q_st[2], kp, k_st[0], k_st[1], k_st[2], vp, v_st[0], v_st[1], v_st[2],
         k_pages.data_ptr(), *kp_st, v_pages.data_ptr(), *vp_st, table_ptr, table_sb, n_ptr,
-        0 if counts is None else counts.data_ptr(), vis_ptr, vis_sb, vis_st, pt_ptr, pt_sb, *pk, *pv, b_ptr, *b_st,
+        c_ptr, vis_ptr, vis_sb, vis_st, pt_ptr, pt_sb, *pk, *pv, b_ptr, *b_st,
         pn_ptr, pn2_ptr, out.data_ptr(), heads * o_sh, o_sh, dv, batch, heads, groups, tq, dk, dv, code, page, table_len,
-        k_pages.size(0), prefixes, prefix_len, n_st, len_add, pn_st, pn_add, b_half, scale, bias_scale)
+        n_pages, prefixes, prefix_len, n_st, len_add, pn_st, pn_add, b_half, scale, bias_scale)
     _launch(paged_lib().logkv_paged_attention, "logkv_paged_attention", index, args, workspace.data_ptr(), need)
     return out if out_dtype == dtype else out.to(out_dtype)
