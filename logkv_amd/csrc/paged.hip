@@ -9,6 +9,7 @@
 // An infinity or NaN in V is left out of a pass's products, which would spread it to queries that do not
 // see its row, and noted behind the partial's sums; the join then adds those of the rows that a query sees.
 #include <algorithm>
+#include <array>
 #include <cmath>
 
 #include "paged.hpp"
@@ -228,71 +229,121 @@ int launch_passes(const PagedPass& shared, const PagedPass& own, hipStream_t str
 
 }  // namespace
 
-// A pass's lanes, query blocks, rows at most, and a step of one of its blocks: the rows that it takes, in microseconds.
-struct PassShape {
-  int64_t lanes;
-  int q_blocks, queries, rows, step_rows;
-  float step_us;
-  // Blocks of s shares a lane, and a block's time: its steps, and kBlockUs to begin and to end.
-  int64_t blocks(int s) const { return lanes * q_blocks * s; }
-  float time(int s) const { return kBlockUs + ((rows + step_rows - 1) / step_rows + s - 1) / s * step_us; }
-  static constexpr float kBlockUs = 4.f;
+// How a call is run: per pass the tiled kernel's query waves (0: the streamed kernel's columns) and the shares of a lane.
+struct PagedPlan {
+  int own_waves, own_cols, own_splits;
+  int shared_waves, shared_cols, shared_splits;
 };
 
-PassShape shape_of(const PagedPass& p, int waves) {
-  const logkv_rows_args& a = p.args;
-  const RowsLaunch& r = p.launch;
-  const int width = std::max(a.dk, a.dv);
-  PassShape x;
-  x.lanes = static_cast<int64_t>(a.n_batch) * a.n_groups;
-  x.q_blocks = r.q_blocks;
-  x.queries = a.n_heads / a.n_groups * a.tq * r.seqs;
-  x.rows = a.cap + (r.prefix ? 0 : a.tq);
-  x.step_rows = r.q_waves ? 64 : 32 * waves;
-  x.step_us = r.q_waves ? (r.q_waves == 8 ? 3.6f : 2.f) : 1.5f;
-  if (width <= 64) x.step_us *= 0.6f;
-  if (width > 128) x.step_us *= 2.f;
-  return x;
+// A pass by one of the kernels. A block takes steps of some rows, `us` microseconds each, and block_us to begin and end; a
+// step keeps a CU busy for cu_us (the rest overlaps with another block's). Measured on passes alone and together, 128
+// features (64: 0.62 of a step): the tiled kernel's 64 rows 2.2 us for 64 queries, 2.1 for 128 and 3.1 for 256; the
+// streamed kernel's 32 rows a wave 1.7 us for 16 queries, 2.6 for 32.
+struct PassCost {
+  int64_t lanes;
+  int q_blocks, queries, steps;
+  float us, cu_us, block_us, bytes_us;
+
+  PassCost(const PagedPass& p, int q_waves, int cols, int waves) {
+    const logkv_rows_args& a = p.args;
+    const int width = std::max(a.dk, a.dv);
+    lanes = static_cast<int64_t>(a.n_batch) * a.n_groups;
+    queries = a.n_heads / a.n_groups * a.tq * p.launch.seqs;
+    const int block_queries = q_waves ? 32 * q_waves : 16 * cols, step_rows = q_waves ? 64 : 32 * waves;
+    q_blocks = (queries + block_queries - 1) / block_queries;
+    const int rows = a.cap + (p.launch.prefix ? 0 : a.tq);
+    steps = std::max(1, (rows + step_rows - 1) / step_rows);
+    const float wide = width <= 64 ? 0.62f : width <= 128 ? 1.f : 2.f, more = q_waves == 0 && cols == 2 ? 1.55f : 1.f;
+    us = wide * more * (q_waves == 8 ? 3.1f : q_waves == 4 ? 2.1f : q_waves == 2 ? 2.2f : 1.7f);
+    cu_us = wide * more * (q_waves == 8 ? 3.1f : q_waves == 4 ? 1.8f : q_waves == 2 ? 2.2f : waves == 8 ? 1.7f : 0.85f);
+    block_us = q_waves ? 9.f : 4.f;
+    // Own rows come from memory, a prefix's for every block of queries after the first mostly from the caches.
+    bytes_us = 2.f * (a.dk + a.dv) * lanes * rows * (p.launch.prefix ? q_blocks / 8e6f : 1 / 5e6f);
+  }
+  int64_t blocks(int s) const { return lanes * q_blocks * s; }
+  int steps_of(int s) const { return (steps + s - 1) / s; }
+};
+
+// When `slots` places have run n blocks of tn each and then m of tm, each taken by the first place that is free.
+float finished(int64_t n, float tn, int64_t m, float tm, int slots) {
+  const int64_t late = n % slots, early = slots - late;
+  const float start = n / slots * tn, start_late = start + tn;
+  float end = late ? start_late : start;
+  auto done = [&](float t) {
+    return late * std::max(0.f, std::floor((t - start_late) / tm + 1e-4f)) + early * std::max(0.f, std::floor((t - start) / tm + 1e-4f));
+  };
+  if (done(end) >= m) return end;
+  float best = 3e38f;
+  const float least = (n * tn + m * tm) / slots;
+  for (const float base : {start, start_late}) {
+    float k = std::max(1.f, std::floor((least - base) / tm));
+    while (done(base + k * tm) < m) k += 1.f;
+    best = std::min(best, base + k * tm);
+  }
+  return std::max(end, best);
 }
 
-// Shares of the lanes of two passes in one launch: the ones of least time by what the blocks take side by side, the
-// steps of both over the chip, and the partials' way out and in.
-void share_out(PagedPass& shared, PagedPass& own, int slots, int waves) {
-  const PassShape x = shape_of(shared, waves), y = shape_of(own, waves);
-  static constexpr int kShares[] = {1, 2, 3, 4, 6, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 56, 64};
+// The plan of least time for two passes in one launch, whose blocks run side by side: when the last one ends, the CUs'
+// work, memory's time (a tenth of the less of the two beside the other), and the partials' way out and in. 16 shapes of
+// 24 to 256 queries over 1024 to 30000 rows ran within 4% (mean) of their best kernels and shares so.
+PagedPlan plan_passes(const PagedPass& own, const PagedPass& shared) {
+  static constexpr int kShares[] = {1, 2, 3, 4, 6, 8, 10, 12, 14, 16, 18, 20, 22, 24, 28, 32, 40, 48, 56, 64};
+  static constexpr int kWaves[] = {0, 2, 4, 8};
+  const int width = std::max(own.args.dk, own.args.dv);
+  const int nq = own.args.n_heads / own.args.n_groups * own.args.tq, nq_shared = nq * shared.launch.seqs;
+  // Two column blocks of wider rows than 64 spill.
+  const int cols = width <= 64 && nq_shared > 16 ? 2 : 1;
   const float partial_us = 8.f * (own.args.dv + kRowsPartTail) / 5e6f;
+  PagedPlan plan{};
   float best = 3e38f;
-  for (int i : kShares) {
-    if (i > 1 && ((i - 1) * x.step_rows >= x.rows || x.blocks(i) > 4 * slots)) break;
-    for (int j : kShares) {
-      if (j > 1 && ((j - 1) * y.step_rows >= y.rows || y.blocks(j) > 4 * slots)) break;
-      const float tx = x.time(i), ty = y.time(j);
-      const int64_t n = x.blocks(i) + y.blocks(j);
-      float t = std::max(tx, ty);
-      if (n > slots) t = std::max(t, (x.blocks(i) * tx + y.blocks(j) * ty) / slots + std::min(tx, ty) / 2);
-      t += partial_us * (static_cast<float>(x.lanes) * x.queries * i + static_cast<float>(y.lanes) * y.queries * j);
-      if (t < best) {
-        best = t;
-        shared.launch.splits = i;
-        own.launch.splits = j;
+  for (int qw : kWaves) {
+    if (qw && (width > 128 || nq_shared <= 16)) continue;
+    for (int own_qw : {0, qw}) {
+      // The streamed kernel reads rows again for every 16 (64 features: 32) queries: up to 16 times where there is a choice.
+      if (own_qw ? nq <= 16 : width <= 128 && nq > 16 * 16 * cols) continue;
+      const int waves = paged_waves(qw), slots = waves == 8 || width > 128 ? 256 : 512;
+      const PassCost x(shared, qw, cols, waves), y(own, own_qw, cols, waves);
+      if (!qw && width <= 128 && x.q_blocks > 16) break;
+      const float memory = x.bytes_us + y.bytes_us;
+      for (int i : kShares) {
+        if (i > 1 && (i > x.steps || x.blocks(i) > 4 * slots)) break;
+        for (int j : kShares) {
+          if (j > 1 && (j > y.steps || y.blocks(j) > 4 * slots)) break;
+          const int sx = x.steps_of(i), sy = y.steps_of(j);
+          const float blocks = finished(x.blocks(i), x.block_us + sx * x.us, y.blocks(j), y.block_us + sy * y.us, slots);
+          const float work = (x.blocks(i) * sx * x.cu_us + y.blocks(j) * sy * y.cu_us) / 256 + 4.f;
+          const float t = std::max({blocks, work, memory}) + 0.1f * std::min(blocks, memory) +
+                          partial_us * (static_cast<float>(x.lanes) * x.queries * i + static_cast<float>(y.lanes) * y.queries * j);
+          if (t < best) {
+            best = t;
+            plan = PagedPlan{own_qw, cols, j, qw, cols, i};
+          }
+        }
       }
+      if (!qw) break;   // both choices are one
     }
   }
+  return plan;
+}
+
+// Plans by a call's sizes, kept per thread: a search takes about 10 us, a kernel's launch 2.
+PagedPlan plan_of(const logkv_paged_args& a, const PagedPass& own, const PagedPass& shared) {
+  const std::array<int, 9> key = {a.n_batch, a.n_heads, a.n_groups, a.tq, a.dk, a.dv, a.n_prefixes, own.args.cap, shared.args.cap};
+  struct Entry {
+    std::array<int, 9> key;
+    PagedPlan plan;
+  };
+  static thread_local std::array<Entry, 64> entries{};
+  uint32_t hash = 0;
+  for (int x : key) hash = hash * 31 + static_cast<uint32_t>(x);
+  Entry& e = entries[(hash ^ hash >> 15) % entries.size()];
+  if (e.key != key) e = Entry{key, plan_passes(own, shared)};
+  return e.plan;
 }
 
 PagedLaunch paged_launch(const logkv_paged_args& a, void* ws) {
   const int width = std::max(a.dk, a.dv);
   PagedLaunch p{};
-  auto plan = [&](PagedPass& pass) {
-    RowsLaunch& r = pass.launch;
-    const logkv_rows_args& x = pass.args;
-    const int64_t nq = static_cast<int64_t>(x.n_heads / x.n_groups) * x.tq * r.seqs;
-    r.bias2 = (x.bias_scale == 0.f ? 1.f : x.bias_scale) * kLog2e;
-    r.causal = x.visible ? 0 : 1;
-    rows_plan(x, static_cast<int64_t>(x.n_batch) * x.n_groups, nq, r);
-    if (!r.q_waves && width > 64) r.cols = 1;   // two column blocks of wider rows spill
-    r.q_blocks = static_cast<int>(r.q_waves ? (nq + 32 * r.q_waves - 1) / (32 * r.q_waves) : (nq + 16 * r.cols - 1) / (16 * r.cols));
-  };
   logkv_rows_args& x = p.own.args;
   x.q = a.q, x.q_sb = a.q_sb, x.q_sh = a.q_sh, x.q_st = a.q_st;
   x.k = a.k, x.k_sb = a.k_sb, x.k_sg = a.k_sg, x.k_st = a.k_st;
@@ -305,36 +356,32 @@ PagedLaunch paged_launch(const logkv_paged_args& a, void* ws) {
   x.n_batch = a.n_batch, x.n_heads = a.n_heads, x.n_groups = a.n_groups, x.tq = a.tq, x.dk = a.dk, x.dv = a.dv;
   x.dtype = a.dtype, x.scale = a.scale, x.cap = a.table_len * a.page;
   p.shared.args = x;
-  p.own.launch.seqs = 1;
-  p.own.launch.table = a.table, p.own.launch.table_sb = a.table_sb;
-  p.own.launch.page_shift = __builtin_ctz(a.page), p.own.launch.pages = a.n_pages;
-  plan(p.own);
-  if (a.n_prefixes) {
+  RowsLaunch &o = p.own.launch, &h = p.shared.launch;
+  o.seqs = 1;
+  o.table = a.table, o.table_sb = a.table_sb, o.page_shift = __builtin_ctz(a.page), o.pages = a.n_pages;
+  if (!a.n_prefixes) {
+    rows_plan(x, static_cast<int64_t>(x.n_batch) * x.n_groups, static_cast<int64_t>(x.n_heads / x.n_groups) * x.tq, o);
+    if (!o.q_waves && width > 64) o.cols = 1;
+  } else {
     logkv_rows_args& y = p.shared.args;
-    RowsLaunch& r = p.shared.launch;
     y.n_batch = a.n_prefixes;
     y.lengths = a.prefix_lengths, y.lengths2 = a.prefix_lengths2, y.len_stride = a.prefix_stride, y.len_add = a.prefix_add;
     y.counts = nullptr, y.visible = nullptr;
-    r.seqs = a.n_batch / a.n_prefixes, r.prefix = 1, r.pages = a.n_pages;
+    h.seqs = a.n_batch / a.n_prefixes, h.prefix = 1, h.pages = a.n_pages;
     if (a.prefix_table) {
-      r.table = a.prefix_table, r.table_sb = a.prefix_sb, r.page_shift = p.own.launch.page_shift;
+      h.table = a.prefix_table, h.table_sb = a.prefix_sb, h.page_shift = o.page_shift;
       y.cap = a.prefix_len * a.page;
     } else {
-      r.page_shift = 30;
+      h.page_shift = 30;
       y.cache_k = a.prefix_k, y.ck_sb = a.pk_sb, y.ck_sg = a.pk_sg, y.ck_st = a.pk_st;
       y.cache_v = a.prefix_v, y.cv_sb = a.pv_sb, y.cv_sg = a.pv_sg, y.cv_st = a.pv_st;
       y.bias = a.bias, y.b_sb = a.b_sb, y.b_sg = a.b_sg, y.b_st = a.b_st, y.bias_half = a.bias_half;
       y.bias_scale = a.bias_scale;
       y.cap = a.prefix_len;
     }
-    plan(p.shared);
-    // Passes of one launch have the same threads a block and at most one tiled and one streamed kernel.
-    const RowsLaunch &o = p.own.launch, &h = p.shared.launch;
-    p.together = o.q_waves && h.q_waves ? o.q_waves == h.q_waves : o.q_waves || h.q_waves || o.cols == h.cols;
-    if (p.together) {
-      const int q_waves = std::max(o.q_waves, h.q_waves), waves = paged_waves(q_waves);
-      share_out(p.shared, p.own, waves == 8 || width > 128 ? 256 : 512, waves);
-    }
+    const PagedPlan plan = plan_of(a, p.own, p.shared);
+    o.q_waves = plan.own_waves, o.cols = plan.own_cols, o.splits = plan.own_splits;
+    h.q_waves = plan.shared_waves, h.cols = plan.shared_cols, h.splits = plan.shared_splits;
   }
   uint8_t* base = static_cast<uint8_t*>(ws);
   auto take = [&](int64_t words) {
@@ -348,6 +395,10 @@ PagedLaunch paged_launch(const logkv_paged_args& a, void* ws) {
     if (!r.seqs) continue;
     const int64_t lanes = static_cast<int64_t>(y.n_batch) * y.n_groups;
     const int64_t nq = static_cast<int64_t>(y.n_heads / y.n_groups) * y.tq * r.seqs;
+    r.bias2 = (y.bias_scale == 0.f ? 1.f : y.bias_scale) * kLog2e;
+    r.causal = y.visible ? 0 : 1;
+    r.shift = r.q_waves ? kTileShift : y.dtype == LOGKV_F16 ? Elem<LOGKV_F16>::kShift : Elem<LOGKV_BF16>::kShift;
+    r.q_blocks = static_cast<int>(r.q_waves ? (nq + 32 * r.q_waves - 1) / (32 * r.q_waves) : (nq + 16 * r.cols - 1) / (16 * r.cols));
     // Shares by length (rows_tile.hpp), as of contiguous rows.
     const bool by_length = r.q_waves && r.splits > 1 && y.n_batch > 1 && y.n_batch <= kWave;
     r.room = by_length ? 2 * r.splits : r.splits;
@@ -364,18 +415,7 @@ PagedLaunch paged_launch(const logkv_paged_args& a, void* ws) {
 }
 
 int launch_paged_attention(const logkv_paged_args& a, const PagedLaunch& p, hipStream_t stream) {
-  PagedPass none = p.shared;
-  none.blocks = 0;
-  if (p.together) {
-    if (int rc = launch_passes(p.shared, p.own, stream)) return rc;
-  } else {
-    if (a.n_prefixes) {
-      PagedPass alone = p.own;
-      alone.blocks = 0;
-      if (int rc = launch_passes(p.shared, alone, stream)) return rc;
-    }
-    if (int rc = launch_passes(none, p.own, stream)) return rc;
-  }
+  if (int rc = launch_passes(p.shared, p.own, stream)) return rc;
   if (a.dtype == LOGKV_BF16) launch_finish_type<LOGKV_BF16>(p, stream);
   else launch_finish_type<LOGKV_F16>(p, stream);
   return hipGetLastError() == hipSuccess ? LOGKV_OK : LOGKV_ERUNTIME;

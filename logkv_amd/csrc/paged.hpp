@@ -16,7 +16,6 @@ struct PagedPass {
 struct PagedLaunch {
   PagedPass own, shared;
   int64_t bytes, blocks;
-  bool together;   // both passes in one launch
 };
 
 // Blocks of a launch: fewer than 2^32 threads.
@@ -24,7 +23,7 @@ constexpr int64_t kMostPagedBlocks = (int64_t(1) << 32) / 512 - 1;
 
 PagedLaunch paged_launch(const logkv_paged_args& a, void* ws);
 int launch_paged_attention(const logkv_paged_args& a, const PagedLaunch& p, hipStream_t stream);
-// One launch of the passes that have blocks, whose kernels may differ only as paged.hip's rule allows.
+// One launch of both passes: of the same threads a block, by at most one form of the tiled and of the streamed kernel.
 int launch_paged_bf16_64(const PagedPass& shared, const PagedPass& own, hipStream_t stream);
 int launch_paged_bf16_128(const PagedPass& shared, const PagedPass& own, hipStream_t stream);
 int launch_paged_bf16_256(const PagedPass& shared, const PagedPass& own, hipStream_t stream);
