@@ -238,7 +238,7 @@ struct PagedPlan {
 // A pass by one of the kernels. A block takes steps of some rows, `us` microseconds each, and block_us to begin and end; a
 // step keeps a CU busy for cu_us (the rest overlaps with another block's). Measured on passes alone and together, 128
 // features (64: 0.62 of a step): the tiled kernel's 64 rows 2.2 us for 64 queries, 2.1 for 128 and 3.1 for 256; the
-// streamed kernel's 32 rows a wave 1.7 us for 16 queries, 2.6 for 32.
+// streamed kernel's 32 rows a wave 1.7 us for 16 queries, 3.1 for 32.
 struct PassCost {
   int64_t lanes;
   int q_blocks, queries, steps;
@@ -253,12 +253,12 @@ struct PassCost {
     q_blocks = (queries + block_queries - 1) / block_queries;
     const int rows = a.cap + (p.launch.prefix ? 0 : a.tq);
     steps = std::max(1, (rows + step_rows - 1) / step_rows);
-    const float wide = width <= 64 ? 0.62f : width <= 128 ? 1.f : 2.f, more = q_waves == 0 && cols == 2 ? 1.55f : 1.f;
+    const float wide = width <= 64 ? 0.62f : width <= 128 ? 1.f : 2.f, more = q_waves == 0 && cols == 2 ? 1.8f : 1.f;
     us = wide * more * (q_waves == 8 ? 3.1f : q_waves == 4 ? 2.1f : q_waves == 2 ? 2.2f : 1.7f);
     cu_us = wide * more * (q_waves == 8 ? 3.1f : q_waves == 4 ? 1.8f : q_waves == 2 ? 2.2f : waves == 8 ? 1.7f : 0.85f);
-    block_us = q_waves ? 9.f : 4.f;
+    block_us = q_waves ? 9.f : 5.f;
     // Own rows come from memory, a prefix's for every block of queries after the first mostly from the caches.
-    bytes_us = 2.f * (a.dk + a.dv) * lanes * rows * (p.launch.prefix ? q_blocks / 8e6f : 1 / 5e6f);
+    bytes_us = 2.f * (a.dk + a.dv) * lanes * rows * (p.launch.prefix ? q_blocks / 6e6f : 1 / 5e6f);
   }
   int64_t blocks(int s) const { return lanes * q_blocks * s; }
   int steps_of(int s) const { return (steps + s - 1) / s; }
@@ -285,7 +285,7 @@ float finished(int64_t n, float tn, int64_t m, float tm, int slots) {
 
 // The plan of least time for two passes in one launch, whose blocks run side by side: when the last one ends, the CUs'
 // work, memory's time (a tenth of the less of the two beside the other), and the partials' way out and in. 16 shapes of
-// 24 to 256 queries over 1024 to 30000 rows ran within 4% (mean) of their best kernels and shares so.
+// 24 to 256 queries over 1024 to 30000 rows ran within 5% (mean) of their best kernels and shares so.
 PagedPlan plan_passes(const PagedPass& own, const PagedPass& shared) {
   static constexpr int kShares[] = {1, 2, 3, 4, 6, 8, 10, 12, 14, 16, 18, 20, 22, 24, 28, 32, 40, 48, 56, 64};
   static constexpr int kWaves[] = {0, 2, 4, 8};

@@ -10,7 +10,8 @@ so they are not a memory figure.
 The log-structured counts are reductions over device buffers (one host read per
 layer); a dense cache (anything without ``token_count``) is counted from
 ``processed_tokens``, or from its populated positions for a sliding window, as the
-reference does; an ``EvictingKVCache`` by its rows in use.
+reference does; an ``EvictingKVCache`` by its rows in use, a ``PagedKVCache`` too, with a prefix in
+its pages counted once (a compressed document that it shares is its own cache's).
 """
 
 from __future__ import annotations
@@ -18,6 +19,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 from .evicting_cache import EvictingKVCache
+from .paged_cache import PagedKVCache
 
 _TOTAL_FIELDS = (
     "processed_tokens",
@@ -71,6 +73,9 @@ def _count_layer(attn, processed_tokens: int) -> _LayerCount:
         exact = int(cache.alpha_valid.sum().item()) * cache.n_groups if cache.alpha_exact_tokens else 0
         live = int((cache.level_w > 0).sum().item())
         return _LayerCount(cache.token_count + tail_len, lanes, (cache.recent_count + tail_len) * lanes, exact, live)
+    if isinstance(cache, PagedKVCache):
+        rows = int(cache.lengths.sum().item()) + cache.prefix_rows
+        return _LayerCount(processed_tokens, cache.batch_size * cache.n_groups, rows * cache.n_groups, 0, 0)
     batch, groups = cache.k.shape[:2]
     lanes = batch * groups
     if isinstance(cache, EvictingKVCache):

@@ -29,6 +29,7 @@ import torch
 
 from ._lib import (AttentionArgs, AttentionGradArgs, PackArgs, ReadoutView, SlotPackArgs, as_storage, check, lib, ptr,
                    require_device, stream_of)
+from .paged_attention import SharedPrefix, _paged_attention
 from .row_attention import _attention, _tree
 
 _BACKENDS = ("auto", "triton", "hip")
@@ -407,6 +408,46 @@ def log_kv_draft_attention(cache, q, k, v, visible, scale, *, pending=None):
         return _attention(q, k, v, ka[..., :cache.k_dim], va[..., :cache.v_dim], scale, None, 0,
                           bias=ka[..., cache.k_dim], visible=visible, in_use=in_use,
                           bias_scale=scale * _inv_scale_bf16(scale))
+
+
+def log_kv_prefix_attention(cache, q, k, v, k_pages, v_pages, table, lengths, scale, *, pending=None, visible=None,
+                            counts=None):
+    """Attention of a batch of sequences behind compressed documents, ``[B, n_heads, T, v_dim]``: ``log_kv_paged_attention``
+    whose shared prefixes are the states of ``cache`` (batch N, a divisor of B; document i belongs to the i-th of N equal
+    runs of sequences). The packed slots are read once for all sequences of a document.
+
+    A slot's logit is a draft's, ``scale * (q.k + bf16(1 / scale) * log w)``; ``pending`` is an optional ``(k, v)`` of one
+    attended but uncommitted row of each document. The pages are bfloat16, and the documents are only read: the packed rows
+    are shared with ``log_kv_chunk_attention(reuse_prefix=True)``. For inference: it has no gradient."""
+    if not cache.semantic_clusters or cache.semantic_anchor_mode != "mid":
+        raise NotImplementedError("logkv_amd reads out the first-order mid-anchor path (second_order_scale=0)")
+    _check_backend(cache.semantic_pack_backend)
+    if torch.is_grad_enabled() and pending is not None and any(t.requires_grad for t in pending):
+        raise NotImplementedError("prefix attention is for inference: it has no gradient (run it under torch.no_grad())")
+    if k_pages.ndim != 4 or k_pages.dtype != torch.bfloat16 or k_pages.device != cache.recent_k.device:
+        raise ValueError("pages beside a compressed document must be bfloat16 on its device")
+    batch, groups = cache.batch_size, cache.n_groups
+    if pending is None:
+        pk, pv = (k_pages.new_empty((batch, groups, 0, d)) for d in (cache.k_dim, cache.v_dim))
+    else:
+        pk, pv = (as_storage(x) for x in pending)
+    _check_kv(cache, pk, pv)
+    if pk.size(2) > 1:
+        raise ValueError("at most one token can be pending")
+    scale = float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError("attention scale must be positive")
+    with torch.no_grad():
+        dim = packed_dim(cache.k_dim, cache.v_dim)
+        key, plan, (ka, va), workspace = _pack_prefix(cache, readout_view(cache), pk, pv, dim, True)
+        recent = cache.recent_count
+        cache._mid_decode_state = (key, plan, (ka, va), recent, workspace)
+        prefix = SharedPrefix(None, k=ka[..., :cache.k_dim], v=va[..., :cache.v_dim], bias=ka[..., cache.k_dim],
+                              bias_scale=scale * _inv_scale_bf16(scale))
+    # The plan's width and the exact pool's rows are read on the device.
+    in_use = (plan.table[-1:].data_ptr(), 0, cache.alpha_count_dev.data_ptr() if cache.alpha_exact_tokens else 0,
+              recent + pk.size(2))
+    return _paged_attention(q, k, v, k_pages, v_pages, table, lengths, scale, prefix, visible, counts, in_use)
 
 
 def attention_state(cache, plan):
