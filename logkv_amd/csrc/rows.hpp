@@ -87,15 +87,28 @@ __device__ __forceinline__ int lane_own_rows(const logkv_rows_args& a, const Row
   return PAGED && r.prefix ? 0 : own_rows(a, b);
 }
 
-// Rows of a page that is not there: of zeros.
-inline constexpr int kMostFeatures = 256;
-static __device__ const uint4 kZeroRow[kMostFeatures / 8] = {};
-
 #if defined(__HIP_DEVICE_COMPILE__)
 #define LOGKV_C __attribute__((address_space(4)))
 #else
 #define LOGKV_C
 #endif
+
+// Over pages: a lane's rows and tokens by scalar loads (lane row b is the same in all lanes, and what they read is not
+// written while a kernel runs).
+__device__ __forceinline__ int lane_rows(const logkv_rows_args& a, int b) {
+  int64_t n = a.len_add;
+  if (a.lengths) n += ((const LOGKV_C int32_t*)a.lengths)[static_cast<int64_t>(b) * a.len_stride];
+  if (a.lengths2) n += *(const LOGKV_C int32_t*)a.lengths2;
+  return static_cast<int>(imax64(0, imin64(n, a.cap)));
+}
+__device__ __forceinline__ int lane_tokens(const logkv_rows_args& a, const RowsLaunch& r, int b) {
+  if (r.prefix) return 0;
+  return a.counts ? max(0, min(((const LOGKV_C int32_t*)a.counts)[b], a.tq)) : a.tq;
+}
+
+// Rows of a page that is not there: of zeros.
+inline constexpr int kMostFeatures = 256;
+static __device__ const uint4 kZeroRow[kMostFeatures / 8] = {};
 
 // The page of row `row` of lane row b, -1 for none.
 __device__ __forceinline__ int page_of(const RowsLaunch& r, int b, int row) {

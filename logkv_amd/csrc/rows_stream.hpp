@@ -64,8 +64,7 @@ __device__ __forceinline__ void rows_stream_block(const logkv_rows_args& a, cons
   const int nq = lane_queries<PAGED>(a, r);
   const int units = a.dk / 8, vunits = a.dv / 8;
   const int w = PAGED ? __builtin_amdgcn_readfirstlane(wave_id()) : wave_id(), l = lane_id(), col = l & 15, hq = l >> 4;
-  int n = rows_in_use(a, b), own = lane_own_rows<PAGED>(a, r, b);
-  if constexpr (PAGED) n = __builtin_amdgcn_readfirstlane(n), own = __builtin_amdgcn_readfirstlane(own);
+  const int n = PAGED ? lane_rows(a, b) : rows_in_use(a, b), own = PAGED ? lane_tokens(a, r, b) : own_rows(a, b);
   const int np = (n + kRowTile - 1) / kRowTile, tiles = np + (own + kRowTile - 1) / kRowTile;
   // The lane's tiles in r.splits equal shares, multiples of the block's waves; shares past the
   // tiles write empty partials.
@@ -350,8 +349,8 @@ __device__ __forceinline__ void rows_stream_block(const logkv_rows_args& a, cons
     __syncthreads();   // the waves' V tiles (c = 0) or the last block's sums are read
     float* acc_w = reinterpret_cast<float*>(buf[w]);
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-      *reinterpret_cast<f32x4*>(acc_w + col * (16 * NB) + 16 * nb + 4 * hq) = o[c][nb];
+    for (int nb = 0; nb < NB; ++nb)   // four features a unit, permuted by query: distinct banks
+      *reinterpret_cast<f32x4*>(acc_w + col * (16 * NB) + 4 * ((4 * nb + hq) ^ (col & 7))) = o[c][nb];
     if (hq == 0) {
       m_s[w][col] = m[c];
       l_s[w][col] = lsum[c];
@@ -360,27 +359,41 @@ __device__ __forceinline__ void rows_stream_block(const logkv_rows_args& a, cons
     __syncthreads();
     const int qb = q0 + 16 * c, queries = min(16, nq - qb);
     float* out = r.part + ((static_cast<int64_t>(lane) * r.room + split) * nq + qb) * (a.dv + kRowsPartTail);
-    if (PAGED && static_cast<int>(threadIdx.x) < queries) {
-      uint32_t any = 0;
-#pragma unroll
-      for (int i = 0; i < NWV; ++i) any |= odd_s[i][0][0];
-      out[static_cast<int64_t>(threadIdx.x) * (a.dv + kRowsPartTail) + a.dv + 2] = any ? 1.f : 0.f;
-    }
-    for (int e = threadIdx.x; e < queries * (a.dv + 2); e += blockDim.x) {
-      const int q = e / (a.dv + 2), d = e % (a.dv + 2);
-      float mx = -__builtin_inff();
+    const int tid = threadIdx.x;
+    // An empty share has zero sums; a share of NaN logits alone has no maximum but a NaN sum.
+    float mx, f[NWV];
+    auto factors = [&](int q) {
+      mx = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < NWV; ++i) mx = fmaxf(mx, m_s[i][q]);
-      // An empty share has zero sums; a share of NaN logits alone has no maximum but a NaN sum.
       const float base = mx == -__builtin_inff() ? 0.f : mx;
-      float val = 0.f;
 #pragma unroll
-      for (int i = 0; i < NWV; ++i) {
-        const float x = d < a.dv ? reinterpret_cast<const float*>(buf[i])[q * (16 * NB) + d] : l_s[i][q];
-        val += x * __builtin_amdgcn_exp2f(m_s[i][q] - base);
+      for (int i = 0; i < NWV; ++i) f[i] = __builtin_amdgcn_exp2f(m_s[i][q] - base);
+    };
+    for (int e = tid; e < queries * 4 * NB; e += 64 * NWV) {
+      const int q = e / (4 * NB), u = e % (4 * NB);
+      if (4 * u >= a.dv) continue;
+      factors(q);
+      f32x4 val = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NWV; ++i)
+        val += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(buf[i]) + q * (16 * NB) + 4 * (u ^ (q & 7))) * f[i];
+      *reinterpret_cast<f32x4*>(out + static_cast<int64_t>(q) * (a.dv + kRowsPartTail) + 4 * u) = val;
+    }
+    if (tid < queries) {
+      factors(tid);
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < NWV; ++i) sum += l_s[i][tid] * f[i];
+      float* tail = out + static_cast<int64_t>(tid) * (a.dv + kRowsPartTail) + a.dv;
+      if constexpr (PAGED) {
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < NWV; ++i) any |= odd_s[i][0][0];
+        *reinterpret_cast<f32x4*>(tail) = f32x4{mx, sum, any ? 1.f : 0.f, 0.f};
+      } else {
+        *reinterpret_cast<float2*>(tail) = make_float2(mx, sum);
       }
-      out[static_cast<int64_t>(q) * (a.dv + kRowsPartTail) + (d < a.dv ? d : d == a.dv ? a.dv + 1 : a.dv)] =
-          d == a.dv + 1 ? mx : val;
     }
   }
 }

@@ -295,14 +295,34 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
   if (begin >= end) return true;
   const float c2 = a.scale * kLog2e;
   const int r0 = 32 * RB * rw;   // this wave's rows of a tile
-  next_pages(begin);
-  load_k(begin);
-  next_pages(min(begin + 1, end - 1));
-  load_v(begin);
+  if constexpr (PAGED) {   // the first tiles' loads all under way before the first is waited for
+    next_pages(begin);
+    load_k(begin);
+    uint4 k0[kKTasks];
+    const uint16_t b0[2] = {bx[0], bx[1]};
 #pragma unroll
-  for (int q = 0; q < kKTasks; ++q) store_k(begin, 0, q);
-  load_k(min(begin + 1, end - 1));
-  next_pages(min(begin + 2, end - 1));
+    for (int q = 0; q < kKTasks; ++q) k0[q] = kx[q];
+    next_pages(min(begin + 1, end - 1));
+    load_v(begin);
+    load_k(min(begin + 1, end - 1));
+    next_pages(min(begin + 2, end - 1));
+    const uint16_t b1[2] = {bx[0], bx[1]};
+    bx[0] = b0[0], bx[1] = b0[1];
+#pragma unroll
+    for (int q = 0; q < kKTasks; ++q) {
+      const uint4 k1 = kx[q];
+      kx[q] = k0[q];
+      store_k(begin, 0, q);
+      kx[q] = k1;
+    }
+    bx[0] = b1[0], bx[1] = b1[1];
+  } else {
+    load_k(begin);
+    load_v(begin);
+#pragma unroll
+    for (int q = 0; q < kKTasks; ++q) store_k(begin, 0, q);
+    load_k(min(begin + 1, end - 1));
+  }
 #pragma unroll
   for (int q = 0; q < kKTasks; ++q) store_k(min(begin + 1, end - 1), 1, q);
   __syncthreads();   // the flags are clear, K of the first tiles is stored
@@ -728,8 +748,12 @@ __device__ __forceinline__ void rows_tile_block(const logkv_rows_args& a, const 
   RowsShare<NKS, NDV> c;
   c.b = lane / G;
   c.g = lane % G;
-  c.n = rows_in_use(a, c.b);
-  c.own = lane_own_rows<PAGED>(a, r, c.b);
+  if constexpr (PAGED) {   // scalar loads: the lane is the same in all of the wave, which the compiler does not see
+    c.b = __builtin_amdgcn_readfirstlane(c.b);
+    c.g = __builtin_amdgcn_readfirstlane(c.g);
+  }
+  c.n = PAGED ? lane_rows(a, c.b) : rows_in_use(a, c.b);
+  c.own = PAGED ? lane_tokens(a, r, c.b) : own_rows(a, c.b);
   const int q_first = id.qb * kQueries * QW, q_last = min(q_first + kQueries * QW, nq) - 1;
   const int q0 = q_first + kQueries * (w % QW) + col;   // the first column block's query
   // Own rows that some query of the block may see.
@@ -739,8 +763,8 @@ __device__ __forceinline__ void rows_tile_block(const logkv_rows_args& a, const 
   const int tiles = c.np + (own_end + TR - 1) / TR, share = (tiles + splits - 1) / splits;
   c.begin = min(id.split * share, tiles);
   c.end = min(c.begin + share, tiles);
-  if constexpr (PAGED) {   // the same in every lane, which the compiler does not see through the length's load
-    for (int* x : {&c.b, &c.g, &c.n, &c.own, &c.np, &c.begin, &c.end}) *x = __builtin_amdgcn_readfirstlane(*x);
+  if constexpr (PAGED) {
+    for (int* x : {&c.n, &c.own, &c.np, &c.begin, &c.end}) *x = __builtin_amdgcn_readfirstlane(*x);
   }
 #pragma unroll
   for (int k = 0; k < kCols; ++k) {
@@ -815,24 +839,33 @@ __device__ __forceinline__ void rows_tile_block(const logkv_rows_args& a, const 
       }
     }
     __syncthreads();
-    const int queries = min(kQueries * QW, nq - q_first), units = a.dv / 4 + 1;
-    for (int e = tid; e < queries * units; e += kThreads) {
-      const int q = e / units, u = e % units, qq = q / kQueries, cc = q % kQueries;
-      float mx = -__builtin_inff();
+    const int queries = min(kQueries * QW, nq - q_first);
+    float mx, f[RW];
+    auto factors = [&](int q) {
+      const int qq = q / kQueries, cc = q % kQueries;
+      mx = -__builtin_inff();
 #pragma unroll
       for (int k = 0; k < RW; ++k) mx = fmaxf(mx, m_s[k * QW + qq][cc]);
       const float top = mx == -__builtin_inff() ? 0.f : mx;
+#pragma unroll
+      for (int k = 0; k < RW; ++k) f[k] = __builtin_amdgcn_exp2f(m_s[k * QW + qq][cc] - top);
+    };
+    for (int e = tid; e < queries * 8 * NDV; e += kThreads) {
+      const int q = e / (8 * NDV), u = e % (8 * NDV), qq = q / kQueries, cc = q % kQueries;
+      if (4 * u >= a.dv) continue;
+      factors(q);
       f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < RW; ++k) {
-        const int ww = k * QW + qq;
-        const float f = __builtin_amdgcn_exp2f(m_s[ww][cc] - top);
-        if (u == units - 1) sum[1] += l_s[ww][cc] * f;
-        else sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(buf) + (ww * kQueries + cc) * kLd + 4 * (u ^ (cc & 7))) * f;
-      }
-      if (u == units - 1) sum[0] = mx;
-      if (PAGED && u == units - 1) sum[2] = note;
+      for (int k = 0; k < RW; ++k)
+        sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(buf) + ((k * QW + qq) * kQueries + cc) * kLd + 4 * (u ^ (cc & 7))) * f[k];
       *reinterpret_cast<f32x4*>(part + static_cast<int64_t>(q_first + q) * (a.dv + kRowsPartTail) + 4 * u) = sum;
+    }
+    if (tid < queries) {
+      factors(tid);
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < RW; ++k) sum += l_s[k * QW + tid / kQueries][tid % kQueries] * f[k];
+      *reinterpret_cast<f32x4*>(part + static_cast<int64_t>(q_first + tid) * (a.dv + kRowsPartTail) + a.dv) = f32x4{mx, sum, note, 0.f};
     }
   }
 }
