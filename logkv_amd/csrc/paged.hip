@@ -265,20 +265,22 @@ struct PassCost {
 };
 
 // When `slots` places have run n blocks of tn each and then m of tm, each taken by the first place that is free.
-float finished(int64_t n, float tn, int64_t m, float tm, int slots) {
-  const int64_t late = n % slots, early = slots - late;
-  const float start = n / slots * tn, start_late = start + tn;
-  float end = late ? start_late : start;
-  auto done = [&](float t) {
-    return late * std::max(0.f, std::floor((t - start_late) / tm + 1e-4f)) + early * std::max(0.f, std::floor((t - start) / tm + 1e-4f));
+double finished(double n, double tn, double m, double tm, int slots) {
+  const double rounds = std::floor(n / slots), late = n - rounds * slots, early = slots - late;
+  const double start = rounds * tn, start_late = start + tn, end = late > 0 ? start_late : start;
+  auto done = [&](double t) {
+    return late * std::max(0.0, std::floor((t - start_late) / tm + 1e-6)) + early * std::max(0.0, std::floor((t - start) / tm + 1e-6));
   };
   if (done(end) >= m) return end;
-  float best = 3e38f;
-  const float least = (n * tn + m * tm) / slots;
-  for (const float base : {start, start_late}) {
-    float k = std::max(1.f, std::floor((least - base) / tm));
-    while (done(base + k * tm) < m) k += 1.f;
-    best = std::min(best, base + k * tm);
+  // The last one ends a number of tm after either start: the first such time that will do.
+  const double even = (m * tm + late * start_late + early * start) / slots;
+  double best = even + 2 * tm;
+  for (const double base : {start, start_late}) {
+    const double k0 = std::max(1.0, std::floor((even - base) / tm) - 1);
+    for (int i = 0; i < 4; ++i) {
+      const double t = base + (k0 + i) * tm;
+      if (t < best && done(t) >= m) best = t;
+    }
   }
   return std::max(end, best);
 }
@@ -310,7 +312,8 @@ PagedPlan plan_passes(const PagedPass& own, const PagedPass& shared) {
         for (int j : kShares) {
           if (j > 1 && (j > y.steps || y.blocks(j) > 4 * slots)) break;
           const int sx = x.steps_of(i), sy = y.steps_of(j);
-          const float blocks = finished(x.blocks(i), x.block_us + sx * x.us, y.blocks(j), y.block_us + sy * y.us, slots);
+          const float blocks = static_cast<float>(finished(static_cast<double>(x.blocks(i)), x.block_us + sx * x.us,
+                                                           static_cast<double>(y.blocks(j)), y.block_us + sy * y.us, slots));
           const float work = (x.blocks(i) * sx * x.cu_us + y.blocks(j) * sy * y.cu_us) / 256 + 4.f;
           const float t = std::max({blocks, work, memory}) + 0.1f * std::min(blocks, memory) +
                           partial_us * (static_cast<float>(x.lanes) * x.queries * i + static_cast<float>(y.lanes) * y.queries * j);

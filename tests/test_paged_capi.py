@@ -147,3 +147,22 @@ def test_workspace_is_checked():
     assert lib.logkv_paged_workspace_bytes(C.byref(paged_args(dk=4))) == -1
     assert lib.logkv_paged_workspace_bytes(None) == -1
     assert lib.logkv_paged_attention(None, FAKE, need, None) == _lib.LOGKV_EINVAL
+
+
+def test_every_size_has_a_plan():
+    """Workspaces of calls of any size that the entry point takes, in bounded time."""
+    import random
+
+    lib, r, planned = _paged.paged_lib(), random.Random(5), 0
+    for _ in range(2000):
+        n = r.choice((1, 1, 2, 3, 8))
+        groups = r.choice((1, 2, 8, 16))
+        a = _paged.PagedArgs(
+            n_batch=n * r.choice((1, 1, 2, 7, 64, 500)), n_groups=groups, n_heads=groups * r.choice((1, 1, 2, 3, 8, 64)),
+            tq=r.choice((1, 1, 2, 7, 33, 300, 4000)), dk=8 * r.randint(1, 32), dv=8 * r.randint(1, 32), dtype=r.choice((0, 1)),
+            page=r.choice((16, 64, 1 << 20)), table_len=r.choice((0, 1, 5, 100, 1024)), n_prefixes=n,
+            prefix_len=r.choice((0, 1, 3, 50, 1000)), prefix_table=r.choice((0, 1)))
+        need = lib.logkv_paged_workspace_bytes(C.byref(a))
+        planned += need > 0
+        assert need > 0 or any(x in lib.logkv_last_error().decode() for x in ("2^19", "65535", "too many"))
+    assert planned > 1500
