@@ -232,6 +232,75 @@ def test_captured_twice_and_on_side_streams():
         c.check(step)
 
 
+def test_two_calls_at_once():
+    """Calls on two streams, each with its own scratch, give what they give alone."""
+    cases = [Case(16, 8, 2, 1, 128, 128, 16, [200 + 7 * b for b in range(16)], [3000], seed=1),
+             Case(6, 4, 1, 12, 128, 128, 16, [900, 3, 40, 0, 700, 64], [2000, 100], seed=2)]
+    want = [c() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (c, st) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(c())
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_rows_beyond_2_31_elements():
+    """Pages and rows of a shared cache whose offsets pass 32 bits."""
+    from logkv_amd import SharedPrefix, log_kv_paged_attention
+
+    G, d, page, pages = 8, 128, 256, 8300                       # 2.18e9 elements
+    kp = torch.zeros(pages, G, page, d, dtype=torch.bfloat16, device="cuda")
+    vp = torch.zeros(pages, G, page, 8, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator("cuda").manual_seed(1)
+    for p in (pages - 1, pages - 2, 3):
+        kp[p].normal_(generator=g), vp[p].normal_(generator=g)
+    q, k, v = make(2, G, 1, d, torch.bfloat16, 1, 2.0), make(2, G, 1, d, torch.bfloat16, 2), make(2, G, 1, 8, torch.bfloat16, 3)
+    table = torch.tensor([[pages - 1], [3]], dtype=torch.int32, device="cuda")
+    pre = torch.tensor([[pages - 2]], dtype=torch.int32, device="cuda")
+    out = log_kv_paged_attention(q, k, v, kp, vp, table, 200, d ** -0.5, prefix=SharedPrefix(250, table=pre))
+    few = [x[[pages - 1, 3, pages - 2]].clone() for x in (kp, vp)]
+    small = torch.tensor([[0], [1]], dtype=torch.int32, device="cuda")
+    want = log_kv_paged_attention(q, k, v, *few, small, 200, d ** -0.5, prefix=SharedPrefix(250, table=small[:1] + 2))
+    assert torch.equal(out, want)
+    # Rows far behind the first of a contiguous prefix: one group's of a cache with 17 million rows between groups.
+    far = kp.view(-1, d)[: 2 * 8_400_000].view(1, 2, 8_400_000, d)
+    far_v = vp.view(-1, 8)[: 2 * 8_400_000].view(1, 2, 8_400_000, 8)
+    near = [x[:, :, :300].clone() for x in (far, far_v)]
+    q, k, v = (x[:, :2] for x in (q, k, v))
+    out, want = (log_kv_paged_attention(q, k, v, few[0][:, :2], few[1][:, :2], small, 5, d ** -0.5, prefix=SharedPrefix(300, k=a, v=b))
+                 for a, b in ((far, far_v), near))
+    assert out.shape == want.shape and torch.isfinite(out).all()
+    # A longer cache has more shares: equal within the rounding of their sums and of the output.
+    assert ((out.double() - want.double()).abs() <= 2 * 2.0 ** -8 * want.double().abs() + 1e-4).all()
+
+
+def test_masks_of_the_lowest_value():
+    """A finite bias of the type's lowest value beside ordinary rows leaves them all the weight."""
+    from logkv_amd import SharedPrefix
+
+    for T, H in ((1, 2), (5, 4), (40, 2)):
+        c = Case(4, H, 1, T, 64, 64, 16, [9, 0, 20, 16], dtype=torch.bfloat16)
+        pk, pv = make(2, 1, 70, 64, torch.bfloat16, 5), make(2, 1, 70, 64, torch.bfloat16, 6)
+        bias = torch.full((2, 1, 70), torch.finfo(torch.float32).min, device="cuda")
+        hidden = c(prefix=SharedPrefix(70, k=pk, v=pv, bias=bias))
+        c.shared = None
+        out, bound = c.want()
+        check_close(hidden, out, bound, T)
+        bias[0, 0, 3] = 0.5
+        hidden = c(prefix=SharedPrefix(70, k=pk, v=pv, bias=bias))
+        rows = (pk[:, :, 3:4].cpu(), [1, 0]), (pv[:, :, 3:4].cpu(), [1, 0])
+        own = [(dense(p, c.table, c.lengths, 20), c.lengths) for p in (c.kp, c.vp)]
+        (ck, total), (cv, _) = (joined(a, b, 4) for a, b in zip(own, rows))
+        add = joined_bias(torch.full((2, 1, 1), 0.5), [1, 0], c.lengths, ck.size(2))
+        out, _, bound, _ = reference(c.q, c.k, c.v, ck, cv, total, causal(4, T), c.scale, bias=add)
+        check_close(hidden, out, bound, T)
+
+
 def test_append_then_attend():
     """Steps of a batch behind a shared prefix, as they are used: the new tokens stored and attended, the lengths
     advanced; against one causal attention over everything."""

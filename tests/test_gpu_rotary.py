@@ -202,6 +202,49 @@ def test_streams_devices_and_graphs():
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_captured_training_step():
+    """Forward and gradient in one graph, replayed with the program's own work between."""
+    from logkv_amd import log_kv_rotary
+
+    f = inverse(10000.0, 32).cuda()
+    q0, k0 = (make(2, n, 16, 64, torch.bfloat16, n) for n in (4, 2))
+    wq, wk = (make(2, n, 16, 64, torch.bfloat16, 9 + n) for n in (4, 2))
+
+    def step():
+        q, k = (x.detach().requires_grad_() for x in (q0, k0))      # leaves that no earlier graph knows
+        out = log_kv_rotary(q, k, f, 11)
+        return (*out, *torch.autograd.grad(out, (q, k), (wq, wk)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        q0.normal_(generator=torch.Generator("cuda").manual_seed(i))
+        wk.mul_(0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+def test_more_blocks_than_a_line_of_the_grid():
+    from logkv_amd import log_kv_rotary
+
+    T = (1 << 20) * 8 + 77      # 8 tokens a block
+    f = torch.ones(1, dtype=torch.float64, device="cuda")
+    q = torch.ones(2, 1, T, 2, dtype=torch.bfloat16, device="cuda")
+    out, _ = log_kv_rotary(q, None, f)
+    pos = torch.arange(T, device="cuda", dtype=torch.float64)
+    want = torch.stack((pos.cos() - pos.sin(), pos.cos() + pos.sin()), dim=-1)
+    bound = 2.0 ** -8 * want.abs() + 2.0 ** -20
+    for b in range(2):
+        assert ((out[b, 0].double() - want).abs() <= bound).all()
+
+
 def test_refusals():
     from logkv_amd import log_kv_rotary
 
