@@ -131,8 +131,9 @@ class PagedKVCache:
         at = self._upload(torch.tensor([list(x) for x in zip(*new)] + [given], dtype=torch.int64))
         table.index_put_((at[0], at[1]), at[2].to(torch.int32))
 
-    def _check(self, q, k, v, batch):
-        """A call's tokens; refuses what an append or an attention would, before a page is handed out."""
+    def _check(self, q, k, v, batch, sharing):
+        """A call's tokens; refuses what an append or an attention would, before a page is handed out. ``sharing``: the
+        sequences whose queries read the same rows."""
         shape = q.shape
         if len(shape) != 4 or shape[0] != batch or shape[2] < 1 or shape[1] < 1 or shape[1] % self.n_groups:
             raise ValueError("queries must be [batch, n_heads, T, k_dim] with n_groups dividing the heads")
@@ -144,18 +145,17 @@ class PagedKVCache:
         check_activation_dtype(q.dtype)
         if not q.device == k.device == v.device == self.k_pages.device:
             raise ValueError("queries and new rows must be on the cache's device")
-        run = batch // self._runs() if batch == self.batch_size else 1
-        if shape[1] // self.n_groups * tokens * run > 2 ** 19:
+        if shape[1] // self.n_groups * tokens * sharing > 2 ** 19:
             raise ValueError("too many queries a KV group at once: split the call")
         if self.k_pages.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a PagedKVCache's calls cannot be captured: capture log_kv_paged_append and "
                                "log_kv_paged_attention on its tensors instead")
         return tokens
 
-    def _runs(self):
-        if self._compressed is not None:
-            return self._compressed[0].batch_size
-        return max(1, len(self._prefix_pages))
+    def _sharing(self):
+        """Sequences behind one prefix, 1 without one."""
+        prefixes = len(self._prefix_pages) if self._compressed is None else self._compressed[0].batch_size
+        return self.batch_size // prefixes if prefixes else 1
 
     def _append(self, q, k, v, table, lengths, **position):
         return log_kv_paged_append(k, v, self.k_pages, self.v_pages, table, lengths, q=q, frequencies=self.frequencies,
@@ -179,7 +179,7 @@ class PagedKVCache:
             raise RuntimeError("a prefix comes before the sequences' rows and beside no other one: reset() the cache first")
         if runs < 1 or self.batch_size % runs:
             raise ValueError(f"{runs} prefixes do not divide a batch of {self.batch_size}")
-        tokens = self._check(q, k, v, runs)
+        tokens = self._check(q, k, v, runs, 1)
         if self._prefix_rows + tokens > 2 ** 30:
             raise ValueError("at most 2^30 rows a prefix")
         lines = [list(line) for line in self._prefix_pages] or [[] for _ in range(runs)]
@@ -215,7 +215,7 @@ class PagedKVCache:
         """Attention of T drafted tokens of every sequence over its prefix, its rows and the drafted rows that ``visible``
         (bool, ``[T, T]`` or ``[B, T, T]``) shows each; nothing is stored. With ``frequencies``, ``positions`` (``[T]`` or
         ``[B, T]``) are the tokens' own, those of their depths in the tree."""
-        self._check(q, k, v, self.batch_size)
+        self._check(q, k, v, self.batch_size, self._sharing())
         if self.frequencies is not None:
             if positions is None:
                 raise ValueError("drafted tokens that are rotated need their positions")
@@ -226,7 +226,7 @@ class PagedKVCache:
     def __call__(self, q, k, v, counts=None):
         """Attention ``[batch, n_heads, T, v_dim]`` of T new tokens, which join the cache. ``counts`` (int32 ``[batch]`` on
         the device) gives the tokens that exist per sequence of a padded batch."""
-        tokens = self._check(q, k, v, self.batch_size)
+        tokens = self._check(q, k, v, self.batch_size, self._sharing())
         if counts is not None:
             if (counts.shape != (self.batch_size,) or counts.dtype not in (torch.int32, torch.int64)
                     or counts.device != self.k_pages.device):

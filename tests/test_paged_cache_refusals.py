@@ -130,3 +130,26 @@ def test_construction_widths():
     for widths in ((60, 64), (64, 264), (0, 64), (64, 4)):
         with pytest.raises(ValueError):
             PagedKVCache(1, 1, *widths, 4, scale=1.0, max_rows=16, device="cpu")
+
+
+def test_the_limit_of_queries_is_of_sequences_that_share_rows():
+    """2^19 query rows a KV group for the sequences behind one prefix; each sequence has its own without one."""
+    T = 1 << 15      # 8 heads a group: half of the limit a sequence, twice the limit all four
+
+    def large(batch):
+        one = torch.zeros((), dtype=torch.bfloat16)
+        return one.expand(batch, 8 * G, T, D), one.expand(batch, G, T, D), one.expand(batch, G, T, DV)
+
+    cache = new(max_rows=T)
+    for call in (cache, cache.prefix):
+        with pytest.raises(RuntimeError, match="pages left"):      # not refused before
+            call(*large(B))
+    cache._prefix_pages = [[], []]
+    with pytest.raises(RuntimeError, match="pages left"):
+        cache(*large(B))
+    cache._prefix_pages = [[]]
+    with pytest.raises(ValueError, match="split the call"):
+        cache(*large(B))
+    cache._prefix_pages = []
+    with pytest.raises(ValueError, match="split the call"):
+        cache(*(x.expand(B, -1, 4 * T, -1) for x in (y[:, :, :1] for y in large(B))))
