@@ -238,24 +238,30 @@ struct PagedPlan {
 // A pass by one of the kernels. A block takes steps of some rows, `us` microseconds each, and block_us to begin and end; a
 // step keeps a CU busy for cu_us (the rest overlaps with another block's). Measured on passes alone and together, 128
 // features (64: 0.62 of a step): the tiled kernel's 64 rows 2.2 us for 64 queries, 2.1 for 128 and 3.1 for 256; the
-// streamed kernel's 32 rows a wave 1.7 us for 16 queries, 3.1 for 32.
+// streamed kernel's 32 rows a wave 1.7 us for 16 queries, 3.1 for 32. 256 features: the tiled kernel's 32 rows 2.9 us for
+// 128 queries, the streamed kernel's 3.4 us for 16.
 struct PassCost {
-  int64_t lanes;
+  int64_t lanes;   // 0: no such pass
   int q_blocks, queries, steps;
   float us, cu_us, block_us, bytes_us;
 
   PassCost(const PagedPass& p, int q_waves, int cols, int waves) {
     const logkv_rows_args& a = p.args;
     const int width = std::max(a.dk, a.dv);
-    lanes = static_cast<int64_t>(a.n_batch) * a.n_groups;
+    const bool wide = width > 128;
+    lanes = p.launch.seqs ? static_cast<int64_t>(a.n_batch) * a.n_groups : 0;
     queries = a.n_heads / a.n_groups * a.tq * p.launch.seqs;
-    const int block_queries = q_waves ? 32 * q_waves : 16 * cols, step_rows = q_waves ? 64 : 32 * waves;
+    const int block_queries = q_waves ? 32 * q_waves : 16 * cols, step_rows = !q_waves ? 32 * waves : wide ? 32 : 64;
     q_blocks = (queries + block_queries - 1) / block_queries;
     const int rows = a.cap + (p.launch.prefix ? 0 : a.tq);
     steps = std::max(1, (rows + step_rows - 1) / step_rows);
-    const float wide = width <= 64 ? 0.62f : width <= 128 ? 1.f : 2.f, more = q_waves == 0 && cols == 2 ? 1.8f : 1.f;
-    us = wide * more * (q_waves == 8 ? 3.1f : q_waves == 4 ? 2.1f : q_waves == 2 ? 2.2f : 1.7f);
-    cu_us = wide * more * (q_waves == 8 ? 3.1f : q_waves == 4 ? 1.8f : q_waves == 2 ? 2.2f : waves == 8 ? 1.7f : 0.85f);
+    if (q_waves && wide) {
+      us = cu_us = 2.9f;
+    } else {
+      const float factor = (width <= 64 ? 0.62f : wide ? 2.f : 1.f) * (q_waves == 0 && cols == 2 ? 1.8f : 1.f);
+      us = factor * (q_waves == 8 ? 3.1f : q_waves == 4 ? 2.1f : q_waves == 2 ? 2.2f : 1.7f);
+      cu_us = factor * (q_waves == 8 ? 3.1f : q_waves == 4 ? 1.8f : q_waves == 2 ? 2.2f : waves == 8 ? 1.7f : 0.85f);
+    }
     block_us = q_waves ? 9.f : 5.f;
     // Own rows come from memory, a prefix's for every block of queries after the first mostly from the caches.
     bytes_us = 2.f * (a.dk + a.dv) * lanes * rows * (p.launch.prefix ? q_blocks / 6e6f : 1 / 5e6f);
@@ -299,16 +305,16 @@ PagedPlan plan_passes(const PagedPass& own, const PagedPass& shared) {
   PagedPlan plan{};
   float best = 3e38f;
   for (int qw : kWaves) {
-    if (qw && (width > 128 || nq_shared <= 16)) continue;
+    if (qw && ((width > 128 && qw != 4) || std::max(nq, nq_shared) <= 16)) continue;
     for (int own_qw : {0, qw}) {
       // The streamed kernel reads rows again for every 16 (64 features: 32) queries: up to 16 times where there is a choice.
-      if (own_qw ? nq <= 16 : width <= 128 && nq > 16 * 16 * cols) continue;
+      if (width > 128 ? own_qw != qw : own_qw ? nq <= 16 : nq > 16 * 16 * cols) continue;
       const int waves = paged_waves(qw), slots = waves == 8 || width > 128 ? 256 : 512;
       const PassCost x(shared, qw, cols, waves), y(own, own_qw, cols, waves);
       if (!qw && width <= 128 && x.q_blocks > 16) break;
       const float memory = x.bytes_us + y.bytes_us;
       for (int i : kShares) {
-        if (i > 1 && (i > x.steps || x.blocks(i) > 4 * slots)) break;
+        if (i > 1 && (!x.lanes || i > x.steps || x.blocks(i) > 4 * slots)) break;
         for (int j : kShares) {
           if (j > 1 && (j > y.steps || y.blocks(j) > 4 * slots)) break;
           const int sx = x.steps_of(i), sy = y.steps_of(j);
@@ -362,10 +368,7 @@ PagedLaunch paged_launch(const logkv_paged_args& a, void* ws) {
   RowsLaunch &o = p.own.launch, &h = p.shared.launch;
   o.seqs = 1;
   o.table = a.table, o.table_sb = a.table_sb, o.page_shift = __builtin_ctz(a.page), o.pages = a.n_pages;
-  if (!a.n_prefixes) {
-    rows_plan(x, static_cast<int64_t>(x.n_batch) * x.n_groups, static_cast<int64_t>(x.n_heads / x.n_groups) * x.tq, o);
-    if (!o.q_waves && width > 64) o.cols = 1;
-  } else {
+  if (a.n_prefixes) {
     logkv_rows_args& y = p.shared.args;
     y.n_batch = a.n_prefixes;
     y.lengths = a.prefix_lengths, y.lengths2 = a.prefix_lengths2, y.len_stride = a.prefix_stride, y.len_add = a.prefix_add;
@@ -382,9 +385,14 @@ PagedLaunch paged_launch(const logkv_paged_args& a, void* ws) {
       y.bias_scale = a.bias_scale;
       y.cap = a.prefix_len;
     }
+  }
+  if (a.n_prefixes || width > 128) {
     const PagedPlan plan = plan_of(a, p.own, p.shared);
     o.q_waves = plan.own_waves, o.cols = plan.own_cols, o.splits = plan.own_splits;
-    h.q_waves = plan.shared_waves, h.cols = plan.shared_cols, h.splits = plan.shared_splits;
+    if (a.n_prefixes) h.q_waves = plan.shared_waves, h.cols = plan.shared_cols, h.splits = plan.shared_splits;
+  } else {   // as of contiguous rows
+    rows_plan(x, static_cast<int64_t>(x.n_batch) * x.n_groups, static_cast<int64_t>(x.n_heads / x.n_groups) * x.tq, o);
+    if (!o.q_waves && width > 64) o.cols = 1;
   }
   uint8_t* base = static_cast<uint8_t*>(ws);
   auto take = [&](int64_t words) {

@@ -21,11 +21,11 @@ struct PagedPasses {
 // NKS 16-wide steps of dk and NDV 32-wide blocks of dv; QW query waves of the tiled kernel (0: none), NC column blocks of
 // the streamed one (0: none). A block takes the pass that its index falls into, by the kernel of that pass.
 template <int DT, int NKS, int NDV, int QW, int NC, bool BIAS>
-__global__ __launch_bounds__(64 * paged_waves(QW), NDV <= 4 ? 2 : 1) void paged_pass_kernel(PagedPasses both) {
+__global__ __launch_bounds__(64 * paged_waves(QW), NDV <= 4 || QW ? 2 : 1) void paged_pass_kernel(PagedPasses both) {
   constexpr int NW = paged_waves(QW), NB = 2 * NDV, RB = QW == 8 ? 2 : 1;
   typedef TileLds<NKS, NDV, NW, QW ? QW : 1, RB, BIAS> Tile;
   typedef StreamLds<NB, NW, true> Stream;
-  __shared__ __align__(256) uint8_t lds[most(QW ? sizeof(Tile) : 0, NC ? sizeof(Stream) : 0)];
+  __shared__ __align__(most(alignof(Tile), alignof(Stream))) uint8_t lds[most(QW ? sizeof(Tile) : 0, NC ? sizeof(Stream) : 0)];
   int lin = blockIdx.x;
   const bool own = lin >= both.pass[0].blocks;
   if (own) lin -= both.pass[0].blocks;
@@ -84,6 +84,8 @@ int launch_paged_width(const PagedPass& shared, const PagedPass& own, hipStream_
       if (qw == 4) return launch_passes<DT, NKS, NDV, 4, 0>(shared, own, stream);
       if (qw == 8) return launch_passes<DT, NKS, NDV, 8, 0>(shared, own, stream);
     }
+  } else if (qw) {   // of both passes (the streamed kernel takes more registers)
+    return launch_passes<DT, NKS, NDV, 4, 0>(shared, own, stream);
   }
   return launch_passes<DT, NKS, NDV, 0, 1>(shared, own, stream);
 }

@@ -1,5 +1,5 @@
 // Attention over a cache's rows and the call's own rows: what follows the streamed products
-// (rows_stream.hip), and the sizes of a launch.
+// (rows_stream.hpp), and the sizes of a launch.
 #include <algorithm>
 #include <type_traits>
 
@@ -292,7 +292,7 @@ RowsLaunch rows_launch(const logkv_rows_args& a, bool causal, void* ws) {
     off += align256(4 * floats);
     return p;
   };
-  // Shares by length (rows_tile.hip): a lane may take up to twice the equal number.
+  // Shares by length (rows_tile.hpp): a lane may take up to twice the equal number.
   const bool by_length = r.q_waves && r.splits > 1 && a.n_batch > 1 && a.n_batch <= kWave;
   r.room = by_length ? 2 * r.splits : r.splits;
   r.part = take(lanes * r.room * nq * (a.dv + kRowsPartTail));

@@ -1,4 +1,4 @@
-// Shared pieces of the row attention kernels (rows_stream.hip, rows.hip): element types, row
+// Shared pieces of the row attention kernels (rows_stream.hpp, rows_tile.hpp, rows.hip): element types, row
 // counts, launch parameters.
 #pragma once
 

@@ -1,4 +1,4 @@
-// Which LDS buffer of the tiled row attention kernel (rows_tile.hip) holds which staged rows, and when
+// Which LDS buffer of the tiled row attention kernel (rows_tile.hpp) holds which staged rows, and when
 // they are touched. Host code too: the order is checked on the CPU by walking a share's iterations.
 #pragma once
 

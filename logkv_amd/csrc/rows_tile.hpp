@@ -1,7 +1,7 @@
 // Attention over a cache's rows and the call's own rows for many queries per KV group (rows.hip's rule):
 // tiles of K and V in LDS, shared by a block's NW waves.
 //
-// Same mathematics as rows_stream.hip (one pass with a running maximum). QW waves hold 32 queries
+// Same mathematics as rows_stream.hpp (one pass with a running maximum). QW waves hold 32 queries
 // each, in registers for the whole range, and NW / QW groups of them take 32 RB rows each of a
 // tile. Per 32 rows:
 //   S^T = K Q^T by 32x32x16 matrix products (a lane holds 16 rows of its own query);
@@ -28,6 +28,9 @@
 // Rows are stored without padding, their 16-byte units permuted by row so that the operand reads
 // and the transposed reads meet every bank once. One barrier per tile, the following tiles' rows on
 // their way in registers; two buffers of V and, by RowsSchedule, two or three of K.
+// Over pages also for rows of up to 256 features: 128 queries a block, two waves to 32 of them, each with half of V's
+// features (one wave with all of them left one a SIMD: 3.1 us a tile of 32 rows against 2.9). 30 sequences x 224 queries
+// x 4 groups over 1936 shared rows of 256 features: 213 us, by the streamed kernel 489.
 #pragma once
 
 #include <algorithm>
@@ -46,12 +49,12 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kCols = 1;                 // 32-query column blocks per wave
 
-// Where 16-byte unit u of row r is stored: u ^ swizzle. 16 units a row: four consecutive rows fall
+// Where 16-byte unit u of row r is stored: u ^ swizzle. 16 or 32 units a row: four consecutive rows fall
 // into distinct 64-byte quarters of the 256-byte bank row, sixteen into distinct units. 8 units a
 // row (two rows to the bank row): the same over row pairs.
 template <int UNITS>
 __device__ __forceinline__ int swizzle(int r) {
-  return UNITS == 16 ? (r & 3) << 2 | (r >> 2 & 3) : (r >> 1 & 1) << 2 | (r >> 2 & 3);
+  return UNITS >= 16 ? (r & 3) << 2 | (r >> 2 & 3) : (r >> 1 & 1) << 2 | (r >> 2 & 3);
 }
 
 __device__ __forceinline__ float pair_max32(float x) {
@@ -142,6 +145,10 @@ __device__ __forceinline__ bool share_by_length(const logkv_rows_args& a, const 
   return true;
 }
 
+// Waves that share queries and rows, each with a part of V's features: two where rows are wider than 128 (sums and queries
+// of one would leave no second wave a SIMD; both form the scores).
+constexpr int feature_waves(int ndv) { return ndv > 4 ? 2 : 1; }
+
 // What a block's share needs beside its tiles, and what it leaves: per column block a lane's query
 // with 16 features of each 32 per register block.
 template <int NKS, int NDV>
@@ -169,17 +176,19 @@ __device__ __forceinline__ void clear_sums(RowsShare<NKS, NDV>& c) {
 // A share's tiles in the first form; false where it meets one that it cannot take. NKS 16-wide steps
 // of dk, NDV 32-wide blocks of dv.
 template <int DT, int NKS, int NDV, int NW, int QW, int RB, bool BIAS, bool PAGED>
-__device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const RowsLaunch& r, RowsShare<NKS, NDV>& c,
-                                                uint8_t* buf, float (*bias_s)[32 * RB * NW / QW], int* flag_s) {
+__device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const RowsLaunch& r,
+                                                RowsShare<NKS, NDV / feature_waves(NDV)>& c, uint8_t* buf,
+                                                float (*bias_s)[32 * RB * NW / QW / feature_waves(NDV)], int* flag_s) {
   typedef __attribute__((address_space(3))) s16x4* lds4;
   typedef __attribute__((address_space(3))) const uint8_t* ldsb;
   typedef __attribute__((address_space(3))) const u32x4* ldsq;
-  constexpr int kThreads = 64 * NW, RW = NW / QW, TR = 32 * RB * RW;   // row groups, rows per tile
+  constexpr int FW = feature_waves(NDV), NV = NDV / FW;   // a wave's blocks of V's features
+  constexpr int kThreads = 64 * NW, RW = NW / QW / FW, TR = 32 * RB * RW;   // row groups, rows per tile
   constexpr int KU = 2 * NKS, VU = 4 * NDV;            // 16-byte units of a staged row
   constexpr int kKTasks = TR * KU / kThreads, kVTasks = TR * VU / kThreads;
   typedef RowsSchedule<RB> Order;
   constexpr int kKBytes = TR * KU * 16, kVBytes = TR * VU * 16, kVBase = Order::kKBuffers * kKBytes;
-  const int tid = threadIdx.x, l = lane_id(), h = l >> 5, col = l & 31, rw = wave_id() / QW;
+  const int tid = threadIdx.x, l = lane_id(), h = l >> 5, col = l & 31, rw = wave_id() / QW % RW, fw = wave_id() / (QW * RW);
   const int kunits = a.dk / 8, vunits = a.dv / 8, b = c.b, g = c.g, np = c.np, begin = c.begin, end = c.end;
   auto k_tile = [&](int bf) { return reinterpret_cast<uint4*>(buf + bf * kKBytes); };
   auto v_tile = [&](int bf) { return reinterpret_cast<uint4*>(buf + kVBase + bf * kVBytes); };
@@ -339,7 +348,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((ldsb)buf));
   const int rk = r0 + col, i16 = l & 15, rv = r0 + 4 * h + (i16 >> 2), f = (l & 16) + 4 * (i16 & 3);
   const uint32_t k_at = lds0 + 16 * (rk * KU + (h ^ swizzle<KU>(rk)));
-  const uint32_t v_at = lds0 + kVBase + 16 * (rv * VU + ((f >> 3) ^ swizzle<VU>(rv))) + 2 * (f & 7);
+  const uint32_t v_at = (lds0 + kVBase + 16 * (rv * VU + ((f >> 3) ^ swizzle<VU>(rv))) + 2 * (f & 7)) ^ (FW > 1 ? 64 * NV * fw : 0);
   // K operand ks of 32-row block kb, V^T operand nb of the 16 rows st (in P's order) of a tile.
   auto k_frag = [&](int bf, int kb, int ks) {
     return __builtin_bit_cast(uint4, *(ldsq)(uintptr_t)(((k_at + bf * kKBytes) ^ (32 * ks)) + kb * 32 * KU * 16));
@@ -350,11 +359,10 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
     const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)((at ^ (64 * nb + 32)) + (st * 16 + 8) * VU * 16)));
     return make_uint4(x.x, x.y, y.x, y.y);
   };
-  // Scores of the next 32 rows, then with their bias and masks; the first half of their products'
-  // operands is read ahead.
-  constexpr int kHalf = NKS / 2;
+  // Scores of the next 32 rows, then with their bias and masks; the first of their products' operands are read ahead.
+  constexpr int kFrags = NKS < 8 ? NKS / 2 : 4;   // (more leave no registers)
   f32x16 next[kCols];
-  uint4 kf[kHalf];
+  uint4 kf[kFrags];
   float mx[kCols], arg0[kCols];
 #pragma unroll
   for (int k = 0; k < kCols; ++k) arg0[k] = kTileShift;
@@ -418,7 +426,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
       arg0[k] = exponent_offset<BIAS>(kTileShift, mb, x[k], c2);
       c.lsum[k] *= corr;
 #pragma unroll
-      for (int nb = 0; nb < NDV; ++nb)
+      for (int nb = 0; nb < NV; ++nb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) c.o[k][nb][i] *= corr;
     }
@@ -429,9 +437,9 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
     for (int i = 0; i < 16; ++i) next[k][i] = 0.f;
 #pragma unroll
   for (int ks = 0; ks < NKS; ++ks) {
-    kf[ks % kHalf] = k_frag(0, 0, ks);
+    kf[ks % kFrags] = k_frag(0, 0, ks);
 #pragma unroll
-    for (int k = 0; k < kCols; ++k) next[k] = mfma32<DT>(kf[ks % kHalf], c.qf[k][ks], next[k]);
+    for (int k = 0; k < kCols; ++k) next[k] = mfma32<DT>(kf[ks % kFrags], c.qf[k][ks], next[k]);
   }
   finish_scores(begin, 0, 0);
 #pragma unroll
@@ -440,7 +448,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
     for (int i = 0; i < 16; ++i) mx[k] = fmaxf(mx[k], next[k][i]);
   move_base();
 #pragma unroll
-  for (int ks = 0; ks < kHalf; ++ks) kf[ks] = k_frag(RB > 1 ? 0 : 1, RB > 1 ? 1 : 0, ks);
+  for (int ks = 0; ks < kFrags; ++ks) kf[ks] = k_frag(RB > 1 ? 0 : 1, RB > 1 ? 1 : 0, ks);
 
   int k_cur = 0, v_cur = 0;   // the buffers of tile ti
   for (int ti = begin; ti < end; ++ti) {
@@ -466,24 +474,24 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
         for (int i = 0; i < 16; ++i) next[k][i] = 0.f;
       }
       const int nbf = kb + 1 < RB ? k_cur : k_next, nkb = kb + 1 < RB ? kb + 1 : 0;
-      uint4 vf[NDV];
+      uint4 vf[NV];
       if constexpr (RB == 1) {
 #pragma unroll
-        for (int ks = 0; ks < kHalf; ++ks) kf[ks] = k_frag(nbf, nkb, ks);
+        for (int ks = 0; ks < kFrags; ++ks) kf[ks] = k_frag(nbf, nkb, ks);
       }
 #pragma unroll
-      for (int nb = 0; nb < NDV; ++nb) vf[nb] = v_frag(v_cur, 2 * kb, nb);
+      for (int nb = 0; nb < NV; ++nb) vf[nb] = v_frag(v_cur, 2 * kb, nb);
       uint32_t hi[kCols][4], lo[kCols][4], hi1[kCols][4], lo1[kCols][4];   // P of the first and the second 16 rows
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int ks = 0; ks < NKS; ++ks)
 #pragma unroll
         for (int k = 0; k < kCols; ++k) {
-          next[k] = mfma32<DT>(kf[ks % kHalf], c.qf[k][ks], next[k]);
-          if (k == kCols - 1 && ks < kHalf) kf[ks] = k_frag(nbf, nkb, ks + kHalf);
+          next[k] = mfma32<DT>(kf[ks % kFrags], c.qf[k][ks], next[k]);
+          if (k == kCols - 1 && ks + kFrags < NKS) kf[ks % kFrags] = k_frag(nbf, nkb, ks + kFrags);
           here(next[k]);
 #pragma unroll
-          for (int i = 16 / NKS * ks; i < 16 / NKS * (ks + 1); i += 2) {
+          for (int i = 8 * ks / NKS * 2; i < 8 * (ks + 1) / NKS * 2; i += 2) {
             const float p0 = __builtin_amdgcn_exp2f(BIAS ? s[k][i] + arg0[k] : __builtin_fmaf(s[k][i], c2, arg0[k]));
             const float p1 = __builtin_amdgcn_exp2f(BIAS ? s[k][i + 1] + arg0[k] : __builtin_fmaf(s[k][i + 1], c2, arg0[k]));
             c.lsum[k] += p0;
@@ -501,20 +509,20 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
         }
       const bool last = kb + 1 == RB, stage_k = last && ti + 2 < end, stage_v = last && ti + 1 < end;
       if (!last || ti + 1 < end) finish_scores(last ? ti + 1 : ti, nkb, nbf);
-      constexpr int kSlots = 2 * NDV * kCols;
+      constexpr int kSlots = 2 * NV * kCols;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
-        for (int nb = 0; nb < NDV; ++nb)
+        for (int nb = 0; nb < NV; ++nb)
 #pragma unroll
           for (int k = 0; k < kCols; ++k) {
-            const int j = (st * NDV + nb) * kCols + k;
+            const int j = (st * NV + nb) * kCols + k;
             c.o[k][nb] = mfma32<DT>(vf[nb], st ? make_uint4(hi1[k][0], hi1[k][1], hi1[k][2], hi1[k][3]) : make_uint4(hi[k][0], hi[k][1], hi[k][2], hi[k][3]), c.o[k][nb]);
             if (st == 0) {
               // The second 16 rows' parts among the first ones' products.
 #pragma unroll
-              for (int i = 4 / NDV * nb; i < 4 / NDV * (nb + 1); ++i) {
+              for (int i = 4 * nb / NV; i < 4 * (nb + 1) / NV; ++i) {
                 Elem<DT>::parts(s[k][8 + 2 * i], s[k][9 + 2 * i], hi1[k][i], lo1[k][i]);
                 here(hi1[k][i]);
                 here(lo1[k][i]);
@@ -533,7 +541,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
             if constexpr (RB > 1) {
               // After (ti, 0) the products were of (ti, 1), the ones to come are of (ti + 1, 0); after (ti, 1),
               // of (ti + 1, 1).
-              if (j < kHalf) kf[j] = k_frag(k_next, kb, j);
+              if (j < kFrags) kf[j] = k_frag(k_next, kb, j);
             }
             if (stage_v) {
               constexpr int kStores = (kVTasks + kSlots - 1) / kSlots;
@@ -714,10 +722,11 @@ __device__ __forceinline__ void rows_tile_share2(const logkv_rows_args& a, const
 // the waves' maxima and sums.
 template <int NKS, int NDV, int NW, int QW, int RB, bool BIAS>
 struct TileLds {
-  static constexpr int RW = NW / QW, TR = 32 * RB * RW;
+  static constexpr int RW = NW / QW / feature_waves(NDV), TR = 32 * RB * RW;
   static constexpr int kTileBytes = TR * 16 * (RowsSchedule<RB>::kKBuffers * 2 * NKS + RowsSchedule<RB>::kVBuffers * 4 * NDV);
   static constexpr int kOutBytes = RW > 1 ? NW * 32 * kCols * 32 * NDV * 4 : 0;
-  alignas(256) uint8_t buf[kTileBytes > kOutBytes ? kTileBytes : kOutBytes];
+  static constexpr int kRowBytes = 32 * (NKS > 2 * NDV ? NKS : 2 * NDV);   // a multiple of every row's length
+  alignas(kRowBytes > 256 ? kRowBytes : 256) uint8_t buf[kTileBytes > kOutBytes ? kTileBytes : kOutBytes];
   alignas(16) float bias[BIAS ? RowsSchedule<RB>::kKBuffers : 1][TR];
   int flag[3];
   float m[NW][32 * kCols], l[NW][32 * kCols];
@@ -729,7 +738,8 @@ struct TileLds {
 template <int DT, int NKS, int NDV, int NW, int QW, int RB, bool BIAS, bool SECOND, bool PAGED>
 __device__ __forceinline__ void rows_tile_block(const logkv_rows_args& a, const RowsLaunch& r, RowsBlock id, int q_blocks,
                                                 TileLds<NKS, NDV, NW, QW, RB, BIAS>& lds) {
-  constexpr int kThreads = 64 * NW, RW = NW / QW, TR = 32 * RB * RW, kQueries = 32 * kCols;   // per wave
+  constexpr int FW = feature_waves(NDV), NV = NDV / FW, kThreads = 64 * NW, RW = NW / QW / FW, TR = 32 * RB * RW;
+  constexpr int kQueries = 32 * kCols;   // per wave
   auto& buf = lds.buf;
   auto& m_s = lds.m;
   auto& l_s = lds.l;
@@ -745,7 +755,7 @@ __device__ __forceinline__ void rows_tile_block(const logkv_rows_args& a, const 
   }
   const int lane = id.lane, G = a.n_groups, tid = threadIdx.x;
   const int nq = lane_queries<PAGED>(a, r), w = wave_id(), l = lane_id(), h = l >> 5, col = l & 31;
-  RowsShare<NKS, NDV> c;
+  RowsShare<NKS, NV> c;
   c.b = lane / G;
   c.g = lane % G;
   if constexpr (PAGED) {   // scalar loads: the lane is the same in all of the wave, which the compiler does not see
@@ -793,7 +803,7 @@ __device__ __forceinline__ void rows_tile_block(const logkv_rows_args& a, const 
       c.m[k] = -__builtin_inff();
       c.lsum[k] = 0.f;
 #pragma unroll
-      for (int nb = 0; nb < NDV; ++nb)
+      for (int nb = 0; nb < NV; ++nb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) c.o[k][nb][i] = 0.f;
     }
@@ -801,26 +811,28 @@ __device__ __forceinline__ void rows_tile_block(const logkv_rows_args& a, const 
   const float note = PAGED && lds.flag[0] ? 1.f : 0.f;
   float* part = r.part + (static_cast<int64_t>(lane) * r.room + id.split) * nq * (a.dv + kRowsPartTail);
   if constexpr (RW == 1) {
+    const int fw = FW > 1 ? w / QW : 0;
 #pragma unroll
     for (int k = 0; k < kCols; ++k) {
       const int qi = q0 + 32 * k;
       if (qi >= nq) continue;
       float* out = part + static_cast<int64_t>(qi) * (a.dv + kRowsPartTail);
-      if (h == 0) {
+      if (h == 0 && fw == 0) {
         if constexpr (PAGED) *reinterpret_cast<f32x4*>(out + a.dv) = f32x4{c.m[k], c.lsum[k], note, 0.f};
         else *reinterpret_cast<float2*>(out + a.dv) = make_float2(c.m[k], c.lsum[k]);
       }
 #pragma unroll
-      for (int nb = 0; nb < NDV; ++nb)
+      for (int nb = 0; nb < NV; ++nb)
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4) {
-          const int d = 32 * nb + 8 * i4 + 4 * h;
+          const int d = 32 * (nb + NV * fw) + 8 * i4 + 4 * h;
           const f32x4 y = {c.o[k][nb][4 * i4], c.o[k][nb][4 * i4 + 1], c.o[k][nb][4 * i4 + 2], c.o[k][nb][4 * i4 + 3]};
           if (d < a.dv) *reinterpret_cast<f32x4*>(out + d) = y;
         }
     }
   } else {
     // The row groups joined in their order.
+    static_assert(FW == 1, "row groups of whole rows");
     constexpr int kLd = 32 * NDV;
     __syncthreads();
 #pragma unroll
