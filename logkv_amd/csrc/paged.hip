@@ -3,11 +3,15 @@
 // Softmax over [prefix | own pages | the call's rows] splits by rows: each part gives a query an
 // unnormalised sum, a maximum and a sum of exponentials, which join under the largest maximum. So a
 // prefix's rows are read once for all of its sequences: their queries (sequences x heads of the KV group
-// x tokens) are the columns of one product, in the kernel that so many columns take (rows_plan), and a
+// x tokens) are the columns of one product, in the kernel that so many columns take (plan_passes), and a
 // sequence's own rows are read in a second pass of few columns. Both passes are the row attention
 // kernels over a page table, in one launch where their kernels go together; this file joins their partials.
 // An infinity or NaN in V is left out of a pass's products, which would spread it to queries that do not
 // see its row, and noted behind the partial's sums; the join then adds those of the rows that a query sees.
+//
+// 64 sequences of 32 heads over 16384 shared rows and 2000 of their own (8 KV groups, 128 features): 112 us, 4.1 TB/s. 8
+// sequences of 256 tokens x 16 heads over 32768 shared rows: 876 us, 630 TFLOP/s. Bound by what bounds the passes; few
+// queries by the launches, 8 us of the first and 6 of the join for 4 sequences over 2048 rows.
 #include <algorithm>
 #include <array>
 #include <cmath>
@@ -200,7 +204,9 @@ void launch_finish(const PagedLaunch& p, hipStream_t stream) {
 template <int DT>
 void launch_finish_type(const PagedLaunch& p, hipStream_t stream) {
   const logkv_rows_args& a = p.own.args;
-  // Groups of partials share a query where eight queries a block would not fill the CUs.
+  // Groups of partials share a query where eight queries a block would not fill the CUs. The whole call without, by this
+  // rule and with them always: 8 heads x 4 sequences over 2000 rows 12.9, 11.6 and 11.8 us, one sequence of 16 heads over
+  // 30000 32.0, 27.5 and 27.3; 64 sequences of 32 heads over 4000 36.3, 36.5 and 38.8, 128 of 16 heads 51.8, 51.8 and 54.4.
   const bool many = std::max(p.own.launch.splits, p.shared.launch.splits) > 8 &&
                     static_cast<int64_t>(a.n_batch) * a.n_heads * a.tq < 8 * 256;
   if (a.dv <= 64) {
@@ -293,7 +299,8 @@ double finished(double n, double tn, double m, double tm, int slots) {
 
 // The plan of least time for two passes in one launch, whose blocks run side by side: when the last one ends, the CUs'
 // work, memory's time (a tenth of the less of the two beside the other), and the partials' way out and in. 16 shapes of
-// 24 to 256 queries over 1024 to 30000 rows ran within 5% (mean) of their best kernels and shares so.
+// 24 to 256 queries over 1024 to 30000 rows ran within 5% (mean) of their best kernels and shares so. Rows wider than 128
+// features: both passes by one kernel (the two side by side take more registers than two waves a SIMD have).
 PagedPlan plan_passes(const PagedPass& own, const PagedPass& shared) {
   static constexpr int kShares[] = {1, 2, 3, 4, 6, 8, 10, 12, 14, 16, 18, 20, 22, 24, 28, 32, 40, 48, 56, 64};
   static constexpr int kWaves[] = {0, 2, 4, 8};
