@@ -418,7 +418,9 @@ def log_kv_prefix_attention(cache, q, k, v, k_pages, v_pages, table, lengths, sc
 
     A slot's logit is a draft's, ``scale * (q.k + bf16(1 / scale) * log w)``; ``pending`` is an optional ``(k, v)`` of one
     attended but uncommitted row of each document. The pages are bfloat16, and the documents are only read: the packed rows
-    are shared with ``log_kv_chunk_attention(reuse_prefix=True)``. For inference: it has no gradient."""
+    are shared with ``log_kv_chunk_attention(reuse_prefix=True)``, and so a document's calls run on one stream or are
+    ordered by the caller. In a HIP graph they are the graph's own, packed at each replay; the documents stay as they were at
+    its capture. For inference: it has no gradient."""
     if not cache.semantic_clusters or cache.semantic_anchor_mode != "mid":
         raise NotImplementedError("logkv_amd reads out the first-order mid-anchor path (second_order_scale=0)")
     _check_backend(cache.semantic_pack_backend)
@@ -439,9 +441,12 @@ def log_kv_prefix_attention(cache, q, k, v, k_pages, v_pages, table, lengths, sc
         raise ValueError("attention scale must be positive")
     with torch.no_grad():
         dim = packed_dim(cache.k_dim, cache.v_dim)
-        key, plan, (ka, va), workspace = _pack_prefix(cache, readout_view(cache), pk, pv, dim, True)
+        # What a capture records has not run, and what it allocates is the graph's: neither is left on the cache.
+        captured = torch.cuda.is_current_stream_capturing()
+        key, plan, (ka, va), workspace = _pack_prefix(cache, readout_view(cache), pk, pv, dim, not captured)
         recent = cache.recent_count
-        cache._mid_decode_state = (key, plan, (ka, va), recent, workspace)
+        if not captured:
+            cache._mid_decode_state = (key, plan, (ka, va), recent, workspace)
         prefix = SharedPrefix(None, k=ka[..., :cache.k_dim], v=va[..., :cache.v_dim], bias=ka[..., cache.k_dim],
                               bias_scale=scale * _inv_scale_bf16(scale))
     # The plan's width and the exact pool's rows are read on the device.

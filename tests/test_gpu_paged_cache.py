@@ -213,6 +213,42 @@ def test_captures_are_refused():
     assert torch.equal(cache.lengths, before) and cache._bound == [1, 1]
 
 
+def test_prefix_attention_in_a_graph():
+    """Over a compressed document that nobody has read yet: the capture, which runs nothing, leaves nothing behind; replays
+    between the program's own calls equal them."""
+    from logkv_amd import log_kv_prefix_attention
+
+    engine, _ = new_engine(2, 64, False)
+    q, k, v = rows(2, 4, 2, 150, 64, 64, torch.bfloat16, 5)
+    engine(q, k, v, k, input_pos=torch.arange(150, device="cuda"), span_ends=None)
+    cache = engine.cache
+    pending = None if engine._log_kv_pending is None else engine._log_kv_pending[:2]
+    q, k, v = rows(4, 4, 2, 1, 64, 64, torch.bfloat16, 9)
+    pages = make(4, 2, 16, 64, torch.bfloat16, 12), make(4, 2, 16, 64, torch.bfloat16, 13)
+    table = torch.arange(4, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    n = torch.tensor([3, 0, 16, 7], dtype=torch.int32, device="cuda")
+
+    def call():
+        with torch.no_grad():
+            return log_kv_prefix_attention(cache, q, k, v, *pages, table, n, 0.125, pending=pending)
+
+    cache._mid_decode_state = None
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = call()
+    assert cache._mid_decode_state is None
+    first = call()      # packs for itself
+    for i in range(3):
+        q.normal_(generator=torch.Generator("cuda").manual_seed(i))
+        n.add_(1).clamp_(max=16)
+        graph.replay()
+        want = call()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and not torch.equal(got, first)
+
+
 def test_compression_accounting():
     from types import SimpleNamespace as S
 
