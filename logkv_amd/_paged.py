@@ -7,7 +7,7 @@ from functools import lru_cache
 from struct import Struct
 
 from ._lib import _i32, _i64, _p, lib
-from ._rows import BF16, F16, _CODES, _packer  # noqa: F401
+from ._rows import _CODES, _packer
 
 F32 = 2
 

@@ -160,25 +160,33 @@ def _rotate(q, k, rest, sign, index):
 
 
 class _Rotary(torch.autograd.Function):
-    """The rotation as a function of the rows; its gradient is the rotation back."""
+    """The rotation as a function of the rows; its gradient is the rotation back. ``state`` is what a launch needs beside
+    them: (arguments, device, frequencies, positions, their versions). The tensors are held here, not saved through
+    autograd, whose way there and back takes as long as a launch."""
 
     @staticmethod
-    def forward(ctx, q, k, frequencies, positions, rest, sign, index):
+    def forward(ctx, q, k, state, sign):
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(frequencies, positions)
-        ctx.rest = rest, sign, index
-        out = _rotate(q, k, rest, sign, index)
-        if not all(ctx.needs_input_grad[:2]):
-            ctx.mark_non_differentiable(*(y for y, need in zip(out, ctx.needs_input_grad) if y is not None and not need))
+        ctx.state, ctx.sign = state, sign
+        out = _rotate(q, k, state[0], sign, state[1])
+        need_q, need_k, _, _ = ctx.needs_input_grad
+        if not (need_q and need_k):
+            ctx.mark_non_differentiable(*(y for y, need in zip(out, (need_q, need_k)) if y is not None and not need))
         return out
 
     @staticmethod
     def backward(ctx, dq, dk):
-        frequencies, positions = ctx.saved_tensors      # unchanged since the forward, and kept until here
-        rest, sign, index = ctx.rest
-        if not torch.is_grad_enabled():      # no graph of the gradient
-            return *_rotate(dq, dk, rest, -sign, index), None, None, None, None, None
-        return *_Rotary.apply(dq, dk, frequencies, positions, rest, -sign, index), None, None, None, None, None
+        state, sign = ctx.state, -ctx.sign
+        rest, index, frequencies, positions, versions = state
+        if versions != _versions(frequencies, positions):
+            raise RuntimeError("the frequencies or positions of a rotation have been modified in place before its gradient")
+        if torch.is_grad_enabled():      # the gradient has a graph of its own
+            return *_Rotary.apply(dq, dk, state, sign), None, None
+        return *_rotate(dq, dk, rest, sign, index), None, None
+
+
+def _versions(frequencies, positions):
+    return frequencies._version, 0 if positions is None else positions._version
 
 
 def log_kv_rotary(q, k, frequencies, positions=0, *, interleaved=False, amplitude=1.0):
@@ -210,5 +218,6 @@ def log_kv_rotary(q, k, frequencies, positions=0, *, interleaved=False, amplitud
     rest, frequencies, positions = _plan(q, shape[1], 0 if k is None else k.size(1), frequencies, positions, interleaved,
                                          amplitude)
     if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
-        return _Rotary.apply(q, k, frequencies, positions, rest, 1.0, index)
+        state = rest, index, frequencies, positions, _versions(frequencies, positions)
+        return _Rotary.apply(q, k, state, 1.0)
     return _rotate(q, k, rest, 1.0, index)

@@ -231,6 +231,19 @@ def test_captured_training_step():
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
 
 
+def test_gradient_of_changed_positions_is_refused():
+    from logkv_amd import log_kv_rotary
+
+    f, pos = inverse(10000.0, 16).cuda(), torch.arange(5, device="cuda")
+    q = make(1, 2, 5, 32, torch.float32, 1).requires_grad_()
+    for change in (lambda: pos.add_(1), lambda: f.mul_(2.0)):
+        out, _ = log_kv_rotary(q, None, f, pos)
+        out.sum().backward(retain_graph=True)
+        change()
+        with pytest.raises(RuntimeError, match="modified"):
+            out.sum().backward()
+
+
 def test_more_blocks_than_a_line_of_the_grid():
     from logkv_amd import log_kv_rotary
 
