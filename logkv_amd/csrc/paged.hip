@@ -416,7 +416,7 @@ PagedLaunch paged_launch(const logkv_paged_args& a, void* ws) {
     r.bias2 = (y.bias_scale == 0.f ? 1.f : y.bias_scale) * kLog2e;
     r.causal = y.visible ? 0 : 1;
     r.shift = r.q_waves ? kTileShift : y.dtype == LOGKV_F16 ? Elem<LOGKV_F16>::kShift : Elem<LOGKV_BF16>::kShift;
-    r.q_blocks = static_cast<int>(r.q_waves ? (nq + 32 * r.q_waves - 1) / (32 * r.q_waves) : (nq + 16 * r.cols - 1) / (16 * r.cols));
+    const int block_queries = r.q_waves ? 32 * r.q_waves : 16 * r.cols;
     // Shares by length (rows_tile.hpp), as of contiguous rows.
     const bool by_length = r.q_waves && r.splits > 1 && y.n_batch > 1 && y.n_batch <= kWave;
     r.room = by_length ? 2 * r.splits : r.splits;
@@ -425,7 +425,7 @@ PagedLaunch paged_launch(const logkv_paged_args& a, void* ws) {
       r.shares = reinterpret_cast<int*>(take(lanes));
       if (!y.lengths || !y.len_stride) r.shares = nullptr;   // rows of one length
     }
-    const int64_t blocks = lanes * r.splits * r.q_blocks;
+    const int64_t blocks = lanes * r.splits * ((nq + block_queries - 1) / block_queries);
     p.blocks += blocks;
     pass->blocks = static_cast<int>(blocks);
   }

@@ -41,7 +41,6 @@ struct RowsLaunch {
   int64_t table_sb;
   int page_shift, pages;
   int seqs;       // sequences whose queries a lane takes
-  int q_blocks;   // query blocks of a lane
   int prefix;     // rows that several sequences share: no own rows, every query sees all
 };
 

@@ -12,7 +12,7 @@
 // long as their products. So two waves a SIMD, and in each the score products of the next 32 rows
 // are interleaved with the exponentials of these, the value products with half of the conversions,
 // the next maxima and the staging of the next tile. 32768 rows of 128 features, 8 lanes of 512
-// queries: 124 us, 555 TFLOP/s of the 1207 of a large matrix product (one wave a SIMD with 64
+// queries: 121 us, 565 TFLOP/s of the 1207 of a large matrix product (one wave a SIMD with 64
 // queries was slower: nothing hid its waits); 30720 rows and 2048 new ones, 8 lanes of 4096
 // queries: 824 - 876 us, 610 - 650 TFLOP/s, the two units busy 50% and 46% of the cycles, in turn.
 // The score products go before the other wave's value products, and those before what is between (the waves' priorities):
