@@ -362,7 +362,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
     return make_uint4(x.x, x.y, y.x, y.y);
   };
   // Scores of the next 32 rows, then with their bias and masks; the first of their products' operands are read ahead.
-  constexpr int kFrags = NKS < 8 ? NKS / 2 : 4;   // (more leave no registers)
+  constexpr int kFrags = NKS < 8 ? NKS / 2 : NKS > 8 && BIAS ? 2 : 4;   // (more spill)
   f32x16 next[kCols];
   uint4 kf[kFrags];
   float mx[kCols], arg0[kCols];

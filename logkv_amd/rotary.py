@@ -197,7 +197,8 @@ def log_kv_rotary(q, k, frequencies, positions=0, *, interleaved=False, amplitud
     ``frequencies [n]`` in radians per position, float64 or float32 (``rotary_frequencies``); ``positions`` the first
     token's (an int), or int64 or int32 ``[T]`` or ``[B, T]``. Pairs are features ``(i, i + n)``, or ``(2 i, 2 i + 1)``
     with ``interleaved``. Angles are formed in 64 bits, products in float32, rounded once. New tensors in the inputs'
-    dimension order; differentiable in q and k any number of times."""
+    dimension order; differentiable in q and k any number of times (captured into a HIP graph, like any backward pass, over
+    leaves that no graph of an eager call still holds)."""
     shape, dtype, index = q.shape, q.dtype, q.get_device()
     if len(shape) != 4:
         raise ValueError("q and k must be [B, heads, T, d] of one batch, length and width")
