@@ -50,9 +50,9 @@ class SharedPrefix(NamedTuple):
 
 
 def _check_pages(k_pages, v_pages, groups):
-    """(dtype code, page size) of a pool whose rows are read in 16-byte units; its device is checked too."""
-    shape, dtype = k_pages.shape, k_pages.dtype
-    if len(shape) != 4 or v_pages.ndim != 4 or shape[:3] != v_pages.shape[:3] or shape[1] != groups:
+    """(dtype code, pages, page size, key and value widths) of a pool; its device is checked too."""
+    shape, of_v, dtype = k_pages.shape, v_pages.shape, k_pages.dtype
+    if len(shape) != 4 or len(of_v) != 4 or shape[0] != of_v[0] or not shape[1] == of_v[1] == groups or shape[2] != of_v[2]:
         raise ValueError("pages must be [pages, groups, page_size, d], keys and values alike")
     page = shape[2]
     if page < MIN_PAGE or page & (page - 1):
@@ -62,15 +62,15 @@ def _check_pages(k_pages, v_pages, groups):
         raise ValueError("the pages must be bfloat16 or float16")
     if not k_pages.is_cuda:
         require_device(k_pages, "k_pages")
-    return code, page
+    return code, shape[0], page, shape[3], of_v[3]
 
 
 def _check_table(table, rows, index):
-    shape = table.shape
-    if (len(shape) != 2 or shape[0] != rows or table.dtype != torch.int32 or table.get_device() != index
-            or shape[1] > 1 and table.stride(1) != 1):
+    shape, strides = table.shape, table.stride()
+    if (len(shape) != 2 or shape[0] != rows or table.dtype is not torch.int32 or table.get_device() != index
+            or shape[1] > 1 and strides[1] != 1):
         raise ValueError(f"a page table must be int32 [{rows}, n] on the pages' device with contiguous rows")
-    return table.data_ptr(), table.stride(0), shape[1]
+    return table.data_ptr(), strides[0], shape[1]
 
 
 def _check_counts(counts, batch, index):
@@ -99,7 +99,7 @@ def log_kv_paged_append(k, v, k_pages, v_pages, table, lengths, *, q=None, frequ
         raise ValueError("new rows must be k [B, G, T, dk] and v [B, G, T, dv]")
     batch, groups, tokens, dk = k_shape
     dv = v_shape[3]
-    code, page = _check_pages(k_pages, v_pages, groups)
+    code, n_pages, page, k_width, v_width = _check_pages(k_pages, v_pages, groups)
     if v.dtype != dtype or not k.get_device() == v.get_device() == v_pages.get_device() == index:
         raise ValueError("new rows must be of one dtype, on the pages' device")
     if q is not None:
@@ -111,7 +111,7 @@ def log_kv_paged_append(k, v, k_pages, v_pages, table, lengths, *, q=None, frequ
     kp_strides, vp_strides = k_pages.stride(), v_pages.stride()
     kp_sp, kp_sg, kp_st, kp_sd = kp_strides
     vp_sp, vp_sg, vp_st, vp_sd = vp_strides
-    if k_pages.size(3) != dk or v_pages.size(3) != dv or not 1 <= dk <= MAX_WIDTH or not 1 <= dv <= MAX_WIDTH:
+    if k_width != dk or v_width != dv or not 1 <= dk <= MAX_WIDTH or not 1 <= dv <= MAX_WIDTH:
         raise ValueError(f"the pages' rows must be as wide as the new ones, up to {MAX_WIDTH} features")
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad
                                     or q is not None and q.requires_grad):
@@ -173,7 +173,7 @@ def log_kv_paged_append(k, v, k_pages, v_pages, table, lengths, *, q=None, frequ
                        k_pages.data_ptr(), kp_sp, kp_sg, kp_st, v_pages.data_ptr(), vp_sp, vp_sg, vp_st,
                        table_ptr, table_sb, n_ptr, c_ptr, freq_ptr, p_ptr, p_sb, p_st, first_ptr, first, batch, heads,
                        groups, tokens, dk, dv, rotated, _TYPES[dtype], code, int(interleaved), freq_float, p_int,
-                       len_add, page, table_len, k_pages.size(0), amplitude, 1.0)
+                       len_add, page, table_len, n_pages, amplitude, 1.0)
     _launch(paged_lib().logkv_paged_append, "logkv_paged_append", index, args)
     return q_out, k_out
 
@@ -249,9 +249,9 @@ def _paged_attention(q, k, v, k_pages, v_pages, table, lengths, scale, prefix, v
         raise ValueError("queries and rows must be 4-dimensional")
     batch, heads, tq, dk = q_shape
     groups, dv = k_shape[1], v_shape[3]
-    code, page = _check_pages(k_pages, v_pages, groups)
-    dtype, index, n_pages = k_pages.dtype, k_pages.get_device(), k_pages.size(0)
-    if k_pages.size(3) != dk or v_pages.size(3) != dv or groups < 1 or heads % groups or heads < 1 or tq < 1 or batch < 1:
+    code, n_pages, page, k_width, v_width = _check_pages(k_pages, v_pages, groups)
+    dtype, index = k_pages.dtype, k_pages.get_device()
+    if k_width != dk or v_width != dv or groups < 1 or heads % groups or heads < 1 or tq < 1 or batch < 1:
         raise ValueError("pages must be [pages, G, page_size, d] with G dividing the query heads")
     if k_shape != (batch, groups, tq, dk) or v_shape != (batch, groups, tq, dv):
         raise ValueError("the call's rows must be [B, G, T, d], one per query position")

@@ -97,8 +97,9 @@ def rotary_tables(frequencies, n, *, amplitude=1.0, dtype=torch.float32):
 def _in_and_out(x):
     """(rows with contiguous features, new ones in their dimension order, addresses and strides of both: 0 of none)."""
     y = torch.empty_like(x)
-    sb, sh, st, sd = x.stride()
-    tb, th, tt, td = y.stride()
+    sb, sh, st, sd = tb, th, tt, td = x.stride()
+    if not x.is_contiguous():
+        tb, th, tt, td = y.stride()
     if (sd != 1 or td != 1) and x.size(3) != 1:
         x = x.contiguous()
         y = torch.empty_like(x)
@@ -110,13 +111,14 @@ def _in_and_out(x):
 
 def _check_frequencies(frequencies, dim, index):
     """(address, rotated features, whether float32)."""
-    if (frequencies.ndim != 1 or frequencies.dtype not in (torch.float64, torch.float32)
-            or frequencies.get_device() != index or 2 * frequencies.size(0) > dim):
+    shape, dtype = frequencies.shape, frequencies.dtype
+    if (len(shape) != 1 or dtype is not torch.float64 and dtype is not torch.float32
+            or frequencies.get_device() != index or 2 * shape[0] > dim):
         raise ValueError("frequencies must be float64 or float32 [rotated features / 2] on the rows' device, "
                          f"for up to {dim} features")
     if frequencies.requires_grad:
         raise NotImplementedError("frequencies have no gradient")
-    return 2 * frequencies.size(0), int(frequencies.dtype == torch.float32)
+    return 2 * shape[0], int(dtype is torch.float32)
 
 
 def _check_positions(positions, batch, tokens, index):
@@ -131,16 +133,15 @@ def _check_positions(positions, batch, tokens, index):
     return positions, positions.data_ptr(), sb, st, int(positions.dtype == torch.int32), 0
 
 
-def _plan(x, heads, groups, frequencies, positions, interleaved, amplitude):
-    """What a launch needs beside its rows and its sign (for rows like ``x``), with the tensors that it points into."""
-    batch, _, tokens, dim = x.shape
-    index = x.get_device()
+def _plan(shape, groups, dtype, index, frequencies, positions, interleaved, amplitude):
+    """What a launch needs beside its rows and its sign, with the tensors that it points into."""
+    batch, heads, tokens, dim = shape
     rotated, freq_float = _check_frequencies(frequencies, dim, index)
     if not frequencies.is_contiguous():
         frequencies = frequencies.contiguous()
     positions, p_ptr, p_sb, p_st, p_int, first = _check_positions(positions, batch, tokens, index)
     rest = pack_rotary_rest(*_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0, 0, 0, 0, frequencies.data_ptr(), p_ptr, p_sb, p_st, 0, first,
-                            batch, heads, groups, tokens, dim, 0, rotated, _TYPES[x.dtype], 0, int(interleaved), freq_float,
+                            batch, heads, groups, tokens, dim, 0, rotated, _TYPES[dtype], 0, int(interleaved), freq_float,
                             p_int, 0, 0, 0, 0, amplitude)
     return rest, frequencies, positions
 
@@ -199,15 +200,16 @@ def log_kv_rotary(q, k, frequencies, positions=0, *, interleaved=False, amplitud
     with ``interleaved``. Angles are formed in 64 bits, products in float32, rounded once. New tensors in the inputs'
     dimension order; differentiable in q and k any number of times (captured into a HIP graph, like any backward pass, over
     leaves that no graph of an eager call still holds)."""
-    shape, dtype, index = q.shape, q.dtype, q.get_device()
+    shape, dtype, index, groups = q.shape, q.dtype, q.get_device(), 0
     if len(shape) != 4:
         raise ValueError("q and k must be [B, heads, T, d] of one batch, length and width")
     if k is not None:
         other = k.shape
         if len(other) != 4 or other[0] != shape[0] or other[2] != shape[2] or other[3] != shape[3]:
             raise ValueError("q and k must be [B, heads, T, d] of one batch, length and width")
-        if k.dtype != dtype or k.get_device() != index:
+        if k.dtype is not dtype or k.get_device() != index:
             raise ValueError("q and k must be of one dtype on one device")
+        groups = other[1]
     check_activation_dtype(dtype)
     if index < 0:
         require_device(q, "q")
@@ -216,8 +218,7 @@ def log_kv_rotary(q, k, frequencies, positions=0, *, interleaved=False, amplitud
     amplitude = float(amplitude)
     if not math.isfinite(amplitude):
         raise ValueError("amplitude must be finite")
-    rest, frequencies, positions = _plan(q, shape[1], 0 if k is None else k.size(1), frequencies, positions, interleaved,
-                                         amplitude)
+    rest, frequencies, positions = _plan(shape, groups, dtype, index, frequencies, positions, interleaved, amplitude)
     if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
         state = rest, index, frequencies, positions, _versions(frequencies, positions)
         return _Rotary.apply(q, k, state, 1.0)
