@@ -7,7 +7,10 @@
 // sequence's own rows are read in a second pass of few columns. Both passes are the row attention
 // kernels over a page table, in one launch where their kernels go together; this file joins their partials.
 // An infinity or NaN in V is left out of a pass's products, which would spread it to queries that do not
-// see its row, and noted behind the partial's sums; the join then adds those of the rows that a query sees.
+// see its row. Every query of a lane sees the same cache rows: a share that met some in them looks at its rows
+// once more and leaves the features that they are in, and the join adds those (time of the share once more, by
+// what the rows' loads take). Those of the call's rows, which queries see by their place or mask, the join looks
+// for in the call's rows themselves: up to tq rows a query, four at a time.
 //
 // 64 sequences of 32 heads over 16384 shared rows and 2000 of their own (8 KV groups, 128 features): 112 us, 4.1 TB/s. 8
 // sequences of 256 tokens x 16 heads over 32768 shared rows: 876 us, 630 TFLOP/s. Bound by what bounds the passes; few
@@ -28,38 +31,33 @@ int64_t align256(int64_t x) { return (x + 255) & ~int64_t(255); }
 
 }  // namespace
 
-// Values of row `at` that are infinite or NaN added to the query's features; others are in its sum.
+// Values that are infinite or NaN added to the query's features; others are in its sum.
 template <int DT>
-__device__ __forceinline__ void add_odd(const LOGKV_G uint16_t* at, f32x4& y) {
-  const uint2 x = *(const LOGKV_G uint2*)at;
+__device__ __forceinline__ void add_odd(uint2 x, f32x4& y) {
   const uint32_t v[4] = {x.x & 0xffffu, x.x >> 16, x.y & 0xffffu, x.y >> 16};
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     if ((v[k] & 0x7fffu) >= Elem<DT>::kInf) y[k] += Elem<DT>::to_f32(static_cast<uint16_t>(v[k]));
 }
 
-// Those of every row of a lane that query t sees.
+// Those of the call's rows that query t of sequence b sees.
 template <int DT>
-__device__ __forceinline__ void add_odd_rows(const logkv_rows_args& a, const RowsLaunch& r, int b, int g, int t, int d, f32x4& y) {
-  const int n = rows_in_use(a, b), own = lane_own_rows<true>(a, r, b);
-  const LOGKV_G uint16_t* base = gp(a.cache_v) + g * a.cv_sg + d;
+__device__ __forceinline__ void add_odd_rows(const logkv_rows_args& a, bool causal, int b, int g, int t, int d, f32x4& y) {
+  const int own = own_rows(a, b), n = causal ? min(own, t + 1) : own;
+  const LOGKV_G uint16_t* base = gp(a.v) + b * a.v_sb + g * a.v_sg + d;
 #pragma unroll 1
-  for (int i = 0; i < n; ++i) {
-    const int page = page_of(r, b, i);
-    bool see = page >= 0;
-    if (a.bias && see) {
-      const int64_t at = b * a.b_sb + g * a.b_sg + i * a.b_st;
-      const float x = a.bias_half ? Elem<DT>::to_f32(gp(static_cast<const uint16_t*>(a.bias))[at])
-                                  : gp(static_cast<const float*>(a.bias))[at];
-      see = x != -__builtin_inff();
+  for (int i0 = 0; i0 < n; i0 += 4) {
+    uint2 x[4];
+    bool see[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = min(i0 + k, n - 1);   // (the last row again adds nothing new)
+      x[k] = *(const LOGKV_G uint2*)(base + i * a.v_st);
+      see[k] = causal || gp(a.visible)[b * a.vis_sb + t * a.vis_st + i] != 0;
     }
-    int64_t step;
-    if (see) add_odd<DT>(page_row(r, base, a.cv_sb, a.cv_st, page, i, step), y);
-  }
-#pragma unroll 1
-  for (int i = 0; i < own; ++i) {
-    const bool see = r.causal ? i <= t : gp(a.visible)[b * a.vis_sb + t * a.vis_st + i] != 0;
-    if (see) add_odd<DT>(gp(a.v) + b * a.v_sb + g * a.v_sg + i * a.v_st + d, y);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (see[k]) add_odd<DT>(x[k], y);
   }
 }
 
@@ -70,15 +68,17 @@ struct FinishPass {
   int splits, room;
   int seqs;            // sequences of a lane, 0: no such pass
   float unit;          // the sums' scale
+  const uint32_t* odd; // what a share's note says of its cache rows (RowsLaunch)
+  int q_blocks, block_queries;
 };
-// What every block reads comes first; the passes themselves are for the rows of notes.
+// What every block reads comes first; the own pass itself is for the call's rows that a note is of.
 struct FinishArgs {
   FinishPass own, shared;
   uint16_t* out;
   int64_t o_sb, o_sh, o_st;
   const int32_t* counts;
   int n_groups, rep, tq, dv;
-  PagedPass passes[2];
+  PagedPass own_pass;
 };
 
 // TQ threads per query, four features each; the block's other factor is shared by queries and by groups of
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(kThreads) void paged_finish_kernel(FinishArgs a) {
   const int all = live ? n_own + n_shared : 0;
   float m = -__builtin_inff(), lsum = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float odd[2] = {0.f, 0.f};   // the partials' notes
+  float odd[2] = {0.f, 0.f};   // the partials' notes: of cache rows, of the call's
   // Eight partials' loads at a time, joined under the running maximum.
   for (int s0 = sg; s0 < all; s0 += 8 * SG) {
     f32x4 ml[8], x[8];
@@ -142,8 +142,8 @@ __global__ __launch_bounds__(kThreads) void paged_finish_kernel(FinishArgs a) {
       const float f = (of_own ? a.own.unit : a.shared.unit) * __builtin_amdgcn_exp2f(ml[k][0] - top);
       lsum += ml[k][1] * f;
       acc += x[k] * f;
-      odd[0] += of_own ? ml[k][2] : 0.f;
-      odd[1] += of_own ? 0.f : ml[k][2];
+      odd[0] += ml[k][2];
+      odd[1] += ml[k][3];
     }
     m = mx;
   }
@@ -176,9 +176,27 @@ __global__ __launch_bounds__(kThreads) void paged_finish_kernel(FinishArgs a) {
   f32x4 z = {0.f, 0.f, 0.f, 0.f};
   if (lsum != 0.f) z = acc / lsum;
   if (__builtin_expect(odd[0] + odd[1] > 0.f, 0)) {
-    const PagedPass &p0 = a.passes[0], &p1 = a.passes[1];
-    if (odd[0] > 0.f) add_odd_rows<DT>(p0.args, p0.launch, b, g, t, d, z);
-    if (odd[1] > 0.f) add_odd_rows<DT>(p1.args, p1.launch, b / a.shared.seqs, g, t, d, z);
+    uint32_t pos = 0, neg = 0;
+    if (odd[0] > 0.f) {
+#pragma unroll 1
+      for (int sp = 0; sp < all; ++sp) {
+        const bool of_own = sp < n_own;
+        const LOGKV_G float* at = of_own ? own + sp * own_step : shared + (sp - n_own) * shared_step;
+        if (at[a.dv + 2] == 0.f) continue;
+        const FinishPass& p = of_own ? a.own : a.shared;
+        const int run = of_own ? b : b / a.shared.seqs, q = of_own ? qc : (b - run * a.shared.seqs) * nq + qc;
+        const int64_t share = static_cast<int64_t>(run * G + g) * p.room + (of_own ? sp : sp - n_own);
+        const LOGKV_G uint32_t* words = gp(p.odd) + (share * p.q_blocks + q / p.block_queries) * 16 + d / 32;
+        pos |= words[0] >> d % 32;
+        neg |= words[8] >> d % 32;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (pos >> k & 1) z[k] += __builtin_inff();
+      if (neg >> k & 1) z[k] -= __builtin_inff();
+    }
+    if (odd[1] > 0.f) add_odd_rows<DT>(a.own_pass.args, a.own_pass.launch.causal != 0, b, g, t, d, z);
   }
   uint16_t y[4];
 #pragma unroll
@@ -194,9 +212,11 @@ template <int DT, int TQ, int SG>
 void launch_finish(const PagedLaunch& p, hipStream_t stream) {
   const logkv_rows_args& a = p.own.args;
   const int rep = a.n_heads / a.n_groups, nq = rep * a.tq, qpb = kThreads / (TQ * SG);
-  auto pass = [](const RowsLaunch& r) { return FinishPass{r.part, r.shares, r.splits, r.room, r.seqs, exp2f(-r.shift)}; };
+  auto pass = [](const RowsLaunch& r) {
+    return FinishPass{r.part, r.shares, r.splits, r.room, r.seqs, exp2f(-r.shift), r.odd, r.q_blocks, paged_block_queries(r)};
+  };
   const FinishArgs args = {pass(p.own.launch), pass(p.shared.launch), a.out, a.o_sb, a.o_sh, a.o_st, a.counts,
-                           a.n_groups, rep, a.tq, a.dv, {p.own, p.shared}};
+                           a.n_groups, rep, a.tq, a.dv, p.own};
   hipLaunchKernelGGL((paged_finish_kernel<DT, TQ, SG>), dim3((nq + qpb - 1) / qpb, a.n_batch * a.n_groups), dim3(kThreads),
                      0, stream, args);
 }
@@ -416,16 +436,18 @@ PagedLaunch paged_launch(const logkv_paged_args& a, void* ws) {
     r.bias2 = (y.bias_scale == 0.f ? 1.f : y.bias_scale) * kLog2e;
     r.causal = y.visible ? 0 : 1;
     r.shift = r.q_waves ? kTileShift : y.dtype == LOGKV_F16 ? Elem<LOGKV_F16>::kShift : Elem<LOGKV_BF16>::kShift;
-    const int block_queries = r.q_waves ? 32 * r.q_waves : 16 * r.cols;
+    const int block_queries = paged_block_queries(r);
+    r.q_blocks = static_cast<int>((nq + block_queries - 1) / block_queries);
     // Shares by length (rows_tile.hpp), as of contiguous rows.
     const bool by_length = r.q_waves && r.splits > 1 && y.n_batch > 1 && y.n_batch <= kWave;
     r.room = by_length ? 2 * r.splits : r.splits;
     r.part = take(lanes * r.room * nq * (y.dv + kRowsPartTail));
+    r.odd = reinterpret_cast<uint32_t*>(take(lanes * r.room * r.q_blocks * 16));
     if (by_length) {
       r.shares = reinterpret_cast<int*>(take(lanes));
       if (!y.lengths || !y.len_stride) r.shares = nullptr;   // rows of one length
     }
-    const int64_t blocks = lanes * r.splits * ((nq + block_queries - 1) / block_queries);
+    const int64_t blocks = lanes * r.splits * r.q_blocks;
     p.blocks += blocks;
     pass->blocks = static_cast<int>(blocks);
   }

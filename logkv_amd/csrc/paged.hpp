@@ -32,6 +32,9 @@ int launch_paged_f16_128(const PagedPass& shared, const PagedPass& own, hipStrea
 int launch_paged_f16_256(const PagedPass& shared, const PagedPass& own, hipStream_t stream);
 int launch_rotary(const logkv_rotary_args& a, bool append, hipStream_t stream);
 
+// Queries of a block: of the tiled kernel's waves, or of the streamed kernel's columns.
+inline int paged_block_queries(const RowsLaunch& r) { return r.q_waves ? 32 * r.q_waves : 16 * r.cols; }
+
 // Waves of a block: the tiled kernel's of its query waves, four of the streamed kernel alone.
 constexpr int paged_waves(int q_waves) { return q_waves > 2 ? 8 : 4; }
 

@@ -40,6 +40,10 @@ struct RowsLaunch {
   const int32_t* table;
   int64_t table_sb;
   int page_shift, pages;
+  // odd [lanes, room, q_blocks][2][8]: of a share that met infinities or NaNs in V's cache rows (its partials' third tail
+  // word), the features (bits) with +infinity and with -infinity, NaN as both; its call rows' note is the fourth word.
+  uint32_t* odd;
+  int q_blocks;   // of a lane
   int seqs;       // sequences whose queries a lane takes
   int prefix;     // rows that several sequences share: no own rows, every query sees all
 };
@@ -243,6 +247,45 @@ __device__ __forceinline__ uint4 finite_only(uint4 x) {
     *x4[j] &= (lo >= Elem<DT>::kInf ? 0u : 0xffffu) | (hi >= Elem<DT>::kInf ? 0u : 0xffff0000u);
   }
   return x;
+}
+
+// What V's cache rows [first, end) of a lane hold that is not finite, as a share's words in r.odd: those of rows that a
+// query sees (all do, but where the bias is -inf). By all threads of a block, 16 bytes each; `bits`: 16 words of LDS that
+// no thread uses any more.
+template <int DT, int THREADS>
+__device__ __forceinline__ void note_odd_rows(const logkv_rows_args& a, const RowsLaunch& r, int b, int g, int first, int end,
+                                              uint32_t* bits, uint32_t* out) {
+  const int tid = threadIdx.x, units = a.dv / 8, rows = THREADS / units, row0 = tid / units, u = tid - row0 * units;
+  __syncthreads();
+  if (tid < 16) bits[tid] = 0;
+  __syncthreads();
+  uint32_t pos = 0, neg = 0;
+  const LOGKV_G uint16_t* base = gp(a.cache_v) + g * a.cv_sg + 8 * u;
+  if (row0 < rows) {
+#pragma unroll 4
+    for (int i = first + row0; i < end; i += rows) {
+      int64_t step;
+      const uint4 x = *(const LOGKV_G uint4*)page_row(r, base, a.cv_sb, a.cv_st, page_of(r, b, i), i, step);
+      bool see = true;
+      if (a.bias) {
+        const int64_t at = b * a.b_sb + g * a.b_sg + i * a.b_st;
+        see = (a.bias_half ? Elem<DT>::to_f32(gp(static_cast<const uint16_t*>(a.bias))[at])
+                           : gp(static_cast<const float*>(a.bias))[at]) != -__builtin_inff();
+      }
+      const uint32_t x4[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t y = x4[j / 2] >> (16 * (j % 2)) & 0xffffu, mag = y & 0x7fffu;
+        if (!see || mag < Elem<DT>::kInf) continue;
+        if (mag > Elem<DT>::kInf || !(y >> 15)) pos |= 1u << j;
+        if (mag > Elem<DT>::kInf || y >> 15) neg |= 1u << j;
+      }
+    }
+    if (pos) atomicOr(bits + u / 4, pos << 8 * (u % 4));
+    if (neg) atomicOr(bits + 8 + u / 4, neg << 8 * (u % 4));
+  }
+  __syncthreads();
+  if (tid < 16) out[tid] = bits[tid];
 }
 
 }  // namespace logkv

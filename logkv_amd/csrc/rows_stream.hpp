@@ -35,7 +35,7 @@ constexpr int kWaves = 4;   // of a block over contiguous rows
 constexpr int v_stride(int blocks) { return 16 * blocks + 16; }
 
 // A block's LDS: per wave a V tile, then its sums; the waves' maxima and sums; per wave and feature, where a tile is not
-// finite, the rows (bits) with +infinity, -infinity and NaN (over pages: whether it met one).
+// finite, the rows (bits) with +infinity, -infinity and NaN (over pages: whether cache rows (1), call rows (2) held one).
 template <int NB, int NWV, bool PAGED>
 struct StreamLds {
   static constexpr int kTileBytes = kRowTile * v_stride(NB) * 2, kOutBytes = 16 * 16 * NB * 4;
@@ -48,7 +48,7 @@ struct StreamLds {
 
 // A block's share `split` of lane `lane` for its 16 NC queries from q0 on. NS 32-wide steps of dk, NB 16-wide blocks of
 // dv, NC 16-query column blocks, NWV waves. Units past dk and dv are zero. PAGED: rows in pages; infinities and NaNs of V
-// are left out and noted behind the partials' sums, for the launch that joins them.
+// are left out and noted behind the partials' sums and, by feature, in r.odd, for the launch that joins them.
 template <int DT, int NS, int NB, int NC, bool BIAS, bool PAGED, int NWV>
 __device__ __forceinline__ void rows_stream_block(const logkv_rows_args& a, const RowsLaunch& r, int split, int lane, int q0,
                                                   StreamLds<NB, NWV, PAGED>& lds) {
@@ -167,7 +167,7 @@ __device__ __forceinline__ void rows_stream_block(const logkv_rows_args& a, cons
     for (int nb = 0; nb < NB; ++nb) o[c][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   const float c2 = a.scale * kLog2e;
-  bool odd = false;   // paged: whether this wave left something out of V
+  uint32_t odd = 0;   // paged: whether this wave left something out of V, of cache rows (1) or call rows (2)
   if (begin + w < end) {
     pages(begin + w);
     load(begin + w);
@@ -199,7 +199,8 @@ __device__ __forceinline__ void rows_stream_block(const logkv_rows_args& a, cons
       if (__builtin_expect(!finite, 0)) {
 #pragma unroll
         for (int i = 0; i < kVLoads; ++i) vx[i] = finite_only<DT>(vx[i]);
-        odd = finite = true;
+        odd |= of_cache ? 1 : 2;
+        finite = true;
       }
     }
     // The wave's own V tile: written and read by this wave only (LDS accesses of a wave complete
@@ -390,11 +391,19 @@ __device__ __forceinline__ void rows_stream_block(const logkv_rows_args& a, cons
         uint32_t any = 0;
 #pragma unroll
         for (int i = 0; i < NWV; ++i) any |= odd_s[i][0][0];
-        *reinterpret_cast<f32x4*>(tail) = f32x4{mx, sum, any ? 1.f : 0.f, 0.f};
+        *reinterpret_cast<f32x4*>(tail) = f32x4{mx, sum, any & 1 ? 1.f : 0.f, any & 2 ? 1.f : 0.f};
       } else {
         *reinterpret_cast<float2*>(tail) = make_float2(mx, sum);
       }
     }
+  }
+  if constexpr (PAGED) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < NWV; ++i) any |= odd_s[i][0][0];
+    if (__builtin_expect(any & 1, 0))
+      note_odd_rows<DT, 64 * NWV>(a, r, b, g, kRowTile * begin, min(kRowTile * min(end, np), n), reinterpret_cast<uint32_t*>(buf[0]),
+                                  r.odd + ((static_cast<int64_t>(lane) * r.room + split) * r.q_blocks + q0 / (16 * NC)) * 16);
   }
 }
 

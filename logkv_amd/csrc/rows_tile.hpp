@@ -288,7 +288,7 @@ __device__ __forceinline__ bool rows_tile_share(const logkv_rows_args& a, const 
     if constexpr (PAGED) {   // infinities and NaNs are left out and noted
       if (__builtin_expect(__ballot(top[0] >= Elem<DT>::kInf || top[1] >= Elem<DT>::kInf) != 0, 0)) {
         vx[q] = finite_only<DT>(vx[q]);
-        flag_s[0] = 1;
+        flag_s[ti < np ? 0 : 1] = 1;
         top = u16x2{0, 0};
       }
     }
@@ -723,8 +723,8 @@ __device__ __forceinline__ void rows_tile_share2(const logkv_rows_args& a, const
   }
 }
 
-// A block's LDS: staged tiles, then (RW > 1) the waves' sums; the bias of the staged rows; notes of V that is not finite;
-// the waves' maxima and sums.
+// A block's LDS: staged tiles, then (RW > 1) the waves' sums; the bias of the staged rows; notes of V that is not finite
+// (over pages: of cache rows, of call rows); the waves' maxima and sums.
 template <int NKS, int NDV, int NW, int QW, int RB, bool BIAS>
 struct TileLds {
   static constexpr int RW = NW / QW / feature_waves(NDV), TR = 32 * RB * RW;
@@ -739,7 +739,7 @@ struct TileLds {
 
 // The block `id` of `q_blocks` query blocks a lane. SECOND: of the launch that follows, whose blocks do again what the
 // first left (r.redo, one flag a block). PAGED: rows in pages; infinities and NaNs of V are left out and noted behind the
-// partials' sums, for the launch that joins them.
+// partials' sums and, by feature, in r.odd, for the launch that joins them.
 template <int DT, int NKS, int NDV, int NW, int QW, int RB, bool BIAS, bool SECOND, bool PAGED>
 __device__ __forceinline__ void rows_tile_block(const logkv_rows_args& a, const RowsLaunch& r, RowsBlock id, int q_blocks,
                                                 TileLds<NKS, NDV, NW, QW, RB, BIAS>& lds) {
@@ -796,6 +796,9 @@ __device__ __forceinline__ void rows_tile_block(const logkv_rows_args& a, const 
     const bool done = rows_tile_share<DT, NKS, NDV, NW, QW, RB, BIAS, PAGED>(a, r, c, buf, lds.bias, lds.flag);
     if constexpr (PAGED) {
       __syncthreads();   // every wave's note
+      if (__builtin_expect(lds.flag[0] != 0, 0))
+        note_odd_rows<DT, kThreads>(a, r, c.b, c.g, TR * c.begin, min(TR * min(c.end, c.np), c.n), reinterpret_cast<uint32_t*>(buf),
+                                    r.odd + ((static_cast<int64_t>(lane) * r.room + id.split) * q_blocks + id.qb) * 16);
     } else {
       if (tid == 0) *redo = done ? 0 : 1;
       if (!done) return;
@@ -813,7 +816,7 @@ __device__ __forceinline__ void rows_tile_block(const logkv_rows_args& a, const 
         for (int i = 0; i < 16; ++i) c.o[k][nb][i] = 0.f;
     }
   }
-  const float note = PAGED && lds.flag[0] ? 1.f : 0.f;
+  const float note = PAGED && lds.flag[0] ? 1.f : 0.f, note_call = PAGED && lds.flag[1] ? 1.f : 0.f;
   float* part = r.part + (static_cast<int64_t>(lane) * r.room + id.split) * nq * (a.dv + kRowsPartTail);
   if constexpr (RW == 1) {
     const int fw = FW > 1 ? w / QW : 0;
@@ -823,7 +826,7 @@ __device__ __forceinline__ void rows_tile_block(const logkv_rows_args& a, const 
       if (qi >= nq) continue;
       float* out = part + static_cast<int64_t>(qi) * (a.dv + kRowsPartTail);
       if (h == 0 && fw == 0) {
-        if constexpr (PAGED) *reinterpret_cast<f32x4*>(out + a.dv) = f32x4{c.m[k], c.lsum[k], note, 0.f};
+        if constexpr (PAGED) *reinterpret_cast<f32x4*>(out + a.dv) = f32x4{c.m[k], c.lsum[k], note, note_call};
         else *reinterpret_cast<float2*>(out + a.dv) = make_float2(c.m[k], c.lsum[k]);
       }
 #pragma unroll
@@ -882,7 +885,7 @@ __device__ __forceinline__ void rows_tile_block(const logkv_rows_args& a, const 
       float sum = 0.f;
 #pragma unroll
       for (int k = 0; k < RW; ++k) sum += l_s[k * QW + tid / kQueries][tid % kQueries] * f[k];
-      *reinterpret_cast<f32x4*>(part + static_cast<int64_t>(q_first + tid) * (a.dv + kRowsPartTail) + a.dv) = f32x4{mx, sum, note, 0.f};
+      *reinterpret_cast<f32x4*>(part + static_cast<int64_t>(q_first + tid) * (a.dv + kRowsPartTail) + a.dv) = f32x4{mx, sum, note, note_call};
     }
   }
 }
