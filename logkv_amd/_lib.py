@@ -11,6 +11,7 @@ from functools import lru_cache
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "liblogkv_hip.so"
 
@@ -268,6 +269,12 @@ ACTIVATION_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 def check_activation_dtype(dtype: torch.dtype) -> None:
     if dtype not in ACTIVATION_DTYPES:
         raise NotImplementedError(f"logkv_amd takes bfloat16, float16 or float32 activations, not {dtype}")
+
+
+def refuse_tangents(*tensors):
+    """Refuses dual tensors: the kernels have no forward-mode derivative, and would drop a tangent without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("logkv_amd has no forward-mode derivatives: unpack the dual tensors")
 
 
 def as_storage(t):

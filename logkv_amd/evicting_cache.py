@@ -10,7 +10,7 @@ import math
 
 import torch
 
-from ._lib import check_activation_dtype
+from ._lib import check_activation_dtype, refuse_tangents
 from .row_attention import (_ROW_DTYPES, EvictedRows, _workspace_bytes, log_kv_evict, log_kv_tree_attention,
                             log_kv_weight_attention)
 
@@ -120,6 +120,7 @@ class EvictingKVCache:
 
     def _check_call(self, q, k, v, counts):
         """The call's tokens; refuses what any of its blocks would, before a row is dropped or stored."""
+        refuse_tangents(q, k, v)
         batch, groups, dk, dv, device = self.batch_size, self.n_groups, self.k.size(3), self.v.size(3), self.k.device
         heads, tokens = q.shape[1:3] if q.ndim == 4 else (0, 0)
         if (tokens < 1 or q.shape != (batch, heads, tokens, dk) or heads < 1 or heads % groups

@@ -28,7 +28,7 @@ from functools import lru_cache
 import torch
 
 from ._lib import (AttentionArgs, AttentionGradArgs, PackArgs, ReadoutView, SlotPackArgs, as_storage, check, lib, ptr,
-                   require_device, stream_of)
+                   refuse_tangents, require_device, stream_of)
 from .paged_attention import SharedPrefix, _paged_attention
 from .row_attention import _attention, _tree
 
@@ -142,6 +142,7 @@ def pack_mid_kv(cache, plan, k, v, dim, *, backend=None, buffers=None, skip_pool
     pooled width plus the exact, recent and current rows (reading the width
     back once per plan).
     """
+    refuse_tangents(k, v)
     if (k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16) and buffers is None:
         # float16 / float32 rows: packed at the cache's bf16 precision, returned in k's dtype.
         ka, va = pack_mid_kv(cache, plan, as_storage(k), as_storage(v), dim, backend=backend,
@@ -328,6 +329,7 @@ def log_kv_chunk_attention(cache, q_b, k_b, v_b, scale, second_order_scale=1.0, 
     rows) the packed prefix is kept on the cache and later steps re-pack only
     their new rows, as in litgpt/log_kv_cache.py:6772-6799.
     """
+    refuse_tangents(q_b, k_b, v_b)
     if q_b.dtype != torch.bfloat16 or k_b.dtype != torch.bfloat16 or v_b.dtype != torch.bfloat16:
         # float16 / float32 activations: the rows are rounded to the cache's bf16 storage and the output
         # is returned in the queries' dtype (both casts differentiable).
@@ -381,6 +383,7 @@ def log_kv_draft_attention(cache, q, k, v, visible, scale, *, pending=None):
     ``(k, v)`` of one attended but uncommitted row, which every token sees. A slot's logit is a call's,
     ``scale * (q.k + bf16(1 / scale) * log w)`` with its log-mass as packed, and the packed prefix is shared with
     ``log_kv_chunk_attention(reuse_prefix=True)``."""
+    refuse_tangents(q, k, v, *(pending or ()))
     if not cache.semantic_clusters or cache.semantic_anchor_mode != "mid":
         raise NotImplementedError("logkv_amd reads out the first-order mid-anchor path (second_order_scale=0)")
     _check_backend(cache.semantic_pack_backend)
@@ -421,6 +424,7 @@ def log_kv_prefix_attention(cache, q, k, v, k_pages, v_pages, table, lengths, sc
     are shared with ``log_kv_chunk_attention(reuse_prefix=True)``, and so a document's calls run on one stream or are
     ordered by the caller. In a HIP graph they are the graph's own, packed at each replay; the documents stay as they were at
     its capture. For inference: it has no gradient."""
+    refuse_tangents(q, k, v, k_pages, v_pages, *(pending or ()))
     if not cache.semantic_clusters or cache.semantic_anchor_mode != "mid":
         raise NotImplementedError("logkv_amd reads out the first-order mid-anchor path (second_order_scale=0)")
     _check_backend(cache.semantic_pack_backend)
@@ -531,6 +535,7 @@ def log_kv_slot_attention(q, slot_k, slot_v, slot_w, scale, mask=None, lam=1.0, 
     slots carry -10000. The slots are packed on the device (``logkv_pack_slots``) and read by the
     decode / matrix-core attention kernels. ``q [B, nh, T_q, dk]``, slots ``[B, G, S, .]``; the last
     ``causal_tail`` slots are the in-flight chunk, causal against the queries."""
+    refuse_tangents(q, slot_k, slot_v, slot_w)
     B, nh, tq, dk = q.shape
     S = slot_k.size(2)
     if S == 0:

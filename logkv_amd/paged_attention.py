@@ -24,7 +24,7 @@ from typing import NamedTuple
 
 import torch
 
-from ._lib import check_activation_dtype, require_device
+from ._lib import check_activation_dtype, refuse_tangents, require_device
 from ._paged import PagedArgs, pack_paged, pack_rotary, paged_lib
 from .rotary import MAX_WIDTH, _NO_ROWS, _TYPES, _check_frequencies, _check_positions, _in_and_out
 from .row_attention import (_LENGTH_DTYPES, _NO_STRIDES, _ROW_DTYPES, _launch, _lengths, _repeats, _small_rows, _tree,
@@ -94,6 +94,7 @@ def log_kv_paged_append(k, v, k_pages, v_pages, table, lengths, *, q=None, frequ
     Returned are the rotated queries in their dtype (None without ``q``) and the keys in the pages' dtype, as
     ``log_kv_paged_attention`` takes them beside the rows before the call. Sequences must not share the pages that a
     call writes."""
+    refuse_tangents(k, v, k_pages, v_pages, q, frequencies)
     k_shape, v_shape, dtype, index = k.shape, v.shape, k.dtype, k_pages.get_device()
     if len(k_shape) != 4 or len(v_shape) != 4 or v_shape[:3] != k_shape[:3]:
         raise ValueError("new rows must be k [B, G, T, dk] and v [B, G, T, dv]")
@@ -244,6 +245,7 @@ def log_kv_paged_attention(q, k, v, k_pages, v_pages, table, lengths, scale, *, 
 
 def _paged_attention(q, k, v, k_pages, v_pages, table, lengths, scale, prefix, visible, counts, prefix_in_use):
     """``prefix_in_use`` in place of the prefix's lengths: as ``_attention``'s ``in_use``."""
+    refuse_tangents(q, k, v, k_pages, v_pages, *(() if prefix is None else (prefix.k, prefix.v, prefix.bias)))
     q_shape, k_shape, v_shape = q.shape, k.shape, v.shape
     if not len(q_shape) == len(k_shape) == len(v_shape) == 4:
         raise ValueError("queries and rows must be 4-dimensional")

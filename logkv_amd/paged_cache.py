@@ -11,7 +11,7 @@ import math
 
 import torch
 
-from ._lib import check_activation_dtype
+from ._lib import check_activation_dtype, refuse_tangents
 from .log_kv_cache import LogStructuredKVCache
 from .log_kv_pack import log_kv_prefix_attention
 from .paged_attention import MIN_PAGE, SharedPrefix, log_kv_paged_append, log_kv_paged_attention
@@ -134,6 +134,7 @@ class PagedKVCache:
     def _check(self, q, k, v, batch, sharing):
         """A call's tokens; refuses what an append or an attention would, before a page is handed out. ``sharing``: the
         sequences whose queries read the same rows."""
+        refuse_tangents(q, k, v)
         shape = q.shape
         if len(shape) != 4 or shape[0] != batch or shape[2] < 1 or shape[1] < 1 or shape[1] % self.n_groups:
             raise ValueError("queries must be [batch, n_heads, T, k_dim] with n_groups dividing the heads")

@@ -13,7 +13,7 @@ import operator
 
 import torch
 
-from ._lib import check_activation_dtype, require_device
+from ._lib import check_activation_dtype, refuse_tangents, require_device
 from ._paged import F32, ROTARY_SIGNS, pack_rotary_rest, pack_rotary_rows, paged_lib
 from ._rows import BF16, F16
 from .row_attention import _launch
@@ -199,7 +199,8 @@ def log_kv_rotary(q, k, frequencies, positions=0, *, interleaved=False, amplitud
     token's (an int), or int64 or int32 ``[T]`` or ``[B, T]``. Pairs are features ``(i, i + n)``, or ``(2 i, 2 i + 1)``
     with ``interleaved``. Angles are formed in 64 bits, products in float32, rounded once. New tensors in the inputs'
     dimension order; differentiable in q and k any number of times (captured into a HIP graph, like any backward pass, over
-    leaves that no graph of an eager call still holds)."""
+    leaves that no graph of an eager call still holds). Dual tensors (forward mode) are refused."""
+    refuse_tangents(q, k, frequencies)
     shape, dtype, index, groups = q.shape, q.dtype, q.get_device(), 0
     if len(shape) != 4:
         raise ValueError("q and k must be [B, heads, T, d] of one batch, length and width")

@@ -25,7 +25,7 @@ from typing import NamedTuple
 
 import torch
 
-from ._lib import check, check_activation_dtype, require_device
+from ._lib import check, check_activation_dtype, refuse_tangents, require_device
 from ._rows import BF16, F16, RowsArgs, pack_evict, pack_rows, rows_lib
 
 _ROW_DTYPES = {torch.bfloat16: BF16, torch.float16: F16}
@@ -106,6 +106,7 @@ def _attention(q, k, v, cache_k, cache_v, scale, lengths, room, *, bias=None, vi
                in_use=None, bias_scale=1.0):
     """Checks and launch of both attentions. ``in_use`` in place of ``lengths``: (address, stride) of device counts
     per batch row, a second count's address (0: none) and rows to add to both. ``bias_scale``: a factor of the bias."""
+    refuse_tangents(q, k, v, cache_k, cache_v, bias, weights)
     if not q.ndim == k.ndim == v.ndim == cache_k.ndim == cache_v.ndim == 4:
         raise ValueError("queries, rows and cache must be 4-dimensional")
     batch, heads, tq, dk = q.shape
@@ -262,6 +263,7 @@ def log_kv_evict(cache_k, cache_v, weights, lengths, keep, *, recent=0, position
 
     The result is new tensors, or ``out``: an ``EvictedRows`` of buffers of at least ``keep`` rows that do not overlap
     the inputs (a cache's second buffer set), of which the first ``keep`` rows are written."""
+    refuse_tangents(cache_k, cache_v, weights)
     if cache_k.ndim != 4 or cache_v.ndim != 4 or cache_k.shape[:3] != cache_v.shape[:3]:
         raise ValueError("cache rows must be [B, G, capacity, d]")
     batch, groups, cap, dk = cache_k.shape
