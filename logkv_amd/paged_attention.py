@@ -96,8 +96,8 @@ def log_kv_paged_append(k, v, k_pages, v_pages, table, lengths, *, q=None, frequ
     call writes."""
     refuse_tangents(k, v, k_pages, v_pages, q, frequencies)
     k_shape, v_shape, dtype, index = k.shape, v.shape, k.dtype, k_pages.get_device()
-    if len(k_shape) != 4 or len(v_shape) != 4 or v_shape[:3] != k_shape[:3]:
-        raise ValueError("new rows must be k [B, G, T, dk] and v [B, G, T, dv]")
+    if len(k_shape) != 4 or len(v_shape) != 4 or v_shape[:3] != k_shape[:3] or k_shape[1] < 1:
+        raise ValueError("new rows must be k [B, G, T, dk] and v [B, G, T, dv] of at least one group")
     batch, groups, tokens, dk = k_shape
     dv = v_shape[3]
     code, n_pages, page, k_width, v_width = _check_pages(k_pages, v_pages, groups)
@@ -168,7 +168,7 @@ def log_kv_paged_append(k, v, k_pages, v_pages, table, lengths, *, q=None, frequ
     if rotated or dtype != k_pages.dtype:
         k_out = k_pages.new_empty(k_shape)
         k_to = k_out.data_ptr(), groups * tokens * dk, tokens * dk, dk
-    if batch < 1 or groups < 1 or tokens < 1:
+    if batch < 1 or tokens < 1:
         return q_out, k_out
     args = pack_rotary(*q_in, *q_to, k.data_ptr(), k_sb, k_sh, k_st, *k_to, v.data_ptr(), v_sb, v_sh, v_st,
                        k_pages.data_ptr(), kp_sp, kp_sg, kp_st, v_pages.data_ptr(), vp_sp, vp_sg, vp_st,
