@@ -34,9 +34,10 @@ class PagedKVCache:
     before the sequences' first rows.
 
     Pages are handed out as rows come and taken back by ``free``, ``trim`` and ``reset``; a call that finds too few raises
-    ``RuntimeError`` and changes nothing. ``lengths`` (int32 ``[batch]``) and the page table are on the device; the host
-    keeps an upper bound of the lengths and never waits. Calls cannot be captured into a HIP graph, since the host hands
-    out pages in them: capture ``log_kv_paged_append`` and ``log_kv_paged_attention`` on a cache's tensors instead."""
+    ``RuntimeError``, and a call that raises changes nothing. ``lengths`` (int32 ``[batch]``) and the page table are on the
+    device; the host keeps an upper bound of the lengths and never waits. Calls cannot be captured into a HIP graph, since
+    the host hands out pages in them: capture ``log_kv_paged_append`` and ``log_kv_paged_attention`` on a cache's tensors
+    instead."""
 
     def __init__(self, batch_size: int, n_groups: int, k_dim: int, v_dim: int, pages: int, *, scale: float, max_rows: int,
                  page_size: int = 64, frequencies=None, interleaved: bool = False, amplitude: float = 1.0,
@@ -118,18 +119,28 @@ class PagedKVCache:
         return host.pin_memory().to(self.lengths.device, non_blocking=True) if self.lengths.is_cuda else host
 
     def _reserve(self, lines, table, rows):
-        """Pages for ``rows[i]`` rows of every line; too few of them change nothing."""
+        """Pages for ``rows[i]`` rows of every line, returned as (line, place, page); too few of them change nothing."""
         need = [max(0, -(-n // self.page_size) - len(line)) for line, n in zip(lines, rows)]
         if sum(need) > len(self._free):
             raise RuntimeError(f"the pool has {len(self._free)} pages left, {sum(need)} are needed")
-        new = [(i, len(line) + j) for i, (line, n) in enumerate(zip(lines, need)) for j in range(n)]
-        if not new:
-            return
-        given = [self._free.pop() for _ in new]
-        for (i, _), page in zip(new, given):
+        places = [(i, len(line) + j) for i, (line, n) in enumerate(zip(lines, need)) for j in range(n)]
+        new = [(*x, page) for x, page in zip(places, reversed(self._free))]
+        if new:
+            at = self._upload(torch.tensor(list(zip(*new)), dtype=torch.int64))
+            table.index_put_((at[0], at[1]), at[2].to(torch.int32))
+            del self._free[-len(new):]
+        for i, _, page in new:
             lines[i].append(page)
-        at = self._upload(torch.tensor([list(x) for x in zip(*new)] + [given], dtype=torch.int64))
-        table.index_put_((at[0], at[1]), at[2].to(torch.int32))
+        return new
+
+    def _give_back(self, lines, table, new):
+        """Undoes a ``_reserve`` whose call failed. What is on its way to the pages comes before what others write there."""
+        for i, _, page in reversed(new):
+            lines[i].pop()
+            self._free.append(page)
+        if new:
+            at = self._upload(torch.tensor(list(zip(*new)), dtype=torch.int64))
+            table.index_put_((at[0], at[1]), torch.full_like(at[2], -1, dtype=torch.int32))
 
     def _check(self, q, k, v, batch, sharing):
         """A call's tokens; refuses what an append or an attention would, before a page is handed out. ``sharing``: the
@@ -188,10 +199,14 @@ class PagedKVCache:
         table = torch.full((runs, width), -1, dtype=torch.int32, device=self.k_pages.device)
         if self._prefix_table is not None:
             table[:, :self._prefix_table.size(1)] = self._prefix_table
-        self._reserve(lines, table, [self._prefix_rows + tokens] * runs)
-        self._prefix_pages, self._prefix_table = lines, table      # the pages are theirs also if a launch fails
-        q, stored = self._append(q, k, v, table, self._prefix_rows)
-        out = log_kv_paged_attention(q, stored, v, self.k_pages, self.v_pages, table, self._prefix_rows, self.scale)
+        new = self._reserve(lines, table, [self._prefix_rows + tokens] * runs)
+        try:
+            q, stored = self._append(q, k, v, table, self._prefix_rows)
+            out = log_kv_paged_attention(q, stored, v, self.k_pages, self.v_pages, table, self._prefix_rows, self.scale)
+        except Exception:
+            self._give_back(lines, table, new)
+            raise
+        self._prefix_pages, self._prefix_table = lines, table
         self._prefix_rows += tokens
         self._first = self._prefix_rows
         return out
@@ -235,9 +250,13 @@ class PagedKVCache:
             counts = counts.clamp(0, tokens).to(torch.int32)
         if max(self._bound) + tokens > self.max_rows:
             raise RuntimeError(f"a sequence has at most {self.max_rows} rows: {max(self._bound)} may be in use, {tokens} are new")
-        self._reserve(self._pages, self.table, [n + tokens for n in self._bound])
-        q, stored = self._append(q, k, v, self.table, self.lengths, first=self._first, counts=counts)
-        out = self._attend(q, stored, v, counts=counts)
+        new = self._reserve(self._pages, self.table, [n + tokens for n in self._bound])
+        try:
+            q, stored = self._append(q, k, v, self.table, self.lengths, first=self._first, counts=counts)
+            out = self._attend(q, stored, v, counts=counts)
+        except Exception:
+            self._give_back(self._pages, self.table, new)
+            raise
         self.lengths.add_(tokens if counts is None else counts)
         self._bound = [n + tokens for n in self._bound]
         return out

@@ -1,0 +1,78 @@
+"""A call of a PagedKVCache that fails behind its checks (memory that runs out, a launch that is refused) leaves the cache as
+it was, and the same or a smaller call can follow (no GPU: the launches are stand-ins)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from logkv_amd import paged_cache
+from test_paged_cache_refusals import B, D, DV, G, new, rows, same, state
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """Stand-ins for the launches; raise the error of the one that ``fails`` names."""
+    fails = {}
+
+    def launch(name, give):
+        def call(*args, **kw):
+            if name in fails:
+                raise fails[name]
+            return give(*args, **kw)
+        monkeypatch.setattr(paged_cache, name, call)
+
+    launch("log_kv_paged_append", lambda k, v, *a, q=None, **kw: (q, k))
+    launch("log_kv_paged_attention", lambda q, k, v, *a, **kw: q.new_zeros(*q.shape[:3], v.size(3)))
+    return fails
+
+
+def call(cache, n, batch=B, of="__call__", **kw):
+    return getattr(cache, of)(rows(batch, 4, n, D), rows(batch, G, n, D), rows(batch, G, n, DV), **kw)
+
+
+@pytest.mark.parametrize("at", ["log_kv_paged_append", "log_kv_paged_attention"])
+@pytest.mark.parametrize("error", [torch.cuda.OutOfMemoryError("no memory"), ValueError("too many blocks")], ids=["memory", "refused"])
+def test_prefixes(launches, at, error):
+    cache = new(pages=16)
+    for held in (0, 10):       # without a prefix, and behind the first block of one
+        if held:
+            call(cache, held, 2, "prefix")
+        before = state(cache)
+        launches[at] = error
+        with pytest.raises(type(error)):
+            call(cache, 70, 2, "prefix")
+        assert same(state(cache), before) and (cache._prefix_table.size(1) == 1 if held else cache._prefix_table is None)
+        del launches[at]
+    assert call(cache, 3, 2, "prefix").shape == (2, 4, 3, DV)      # fewer tokens, a narrower table
+    assert cache.prefix_rows == 2 * 13 and cache.free_pages == 14
+    launches[at] = error
+    with pytest.raises(type(error)):
+        call(cache, 1)
+    del launches[at]
+    call(cache, 5, 2, "prefix")       # no sequence has a row yet
+    assert cache.prefix_rows == 2 * 18 and cache.free_pages == 12
+
+
+@pytest.mark.parametrize("at", ["log_kv_paged_append", "log_kv_paged_attention"])
+def test_steps(launches, at):
+    cache = new(pages=16)
+    call(cache, 10)
+    before = state(cache)
+    for error in (torch.cuda.OutOfMemoryError("no memory"), ValueError("too many blocks")):
+        launches[at] = error
+        for kw in ({}, dict(counts=torch.tensor([30, 0, 1, 30], dtype=torch.int32))):
+            with pytest.raises(type(error)):
+                call(cache, 30, **kw)
+            assert same(state(cache), before)
+    del launches[at]
+    upload, cache._upload = cache._upload, None      # the table's own update fails
+    with pytest.raises(TypeError):
+        call(cache, 30)
+    cache._upload = upload
+    assert same(state(cache), before)
+    call(cache, 20)
+    assert cache.lengths.tolist() == [30] * B and cache.free_pages == 8
+    lines = sum(cache._pages, [])
+    assert len(set(lines)) == 8 and not set(lines) & set(cache._free)
+    assert all(cache.table[b, :2].tolist() == cache._pages[b] for b in range(B)) and (cache.table[:, 2:] == -1).all()
