@@ -27,7 +27,7 @@ import torch
 from ._lib import check_activation_dtype, refuse_tangents, require_device
 from ._paged import PagedArgs, pack_paged, pack_rotary, paged_lib
 from .rotary import MAX_WIDTH, _NO_ROWS, _TYPES, _check_frequencies, _check_positions, _in_and_out
-from .row_attention import (_LENGTH_DTYPES, _NO_STRIDES, _ROW_DTYPES, _launch, _lengths, _repeats, _small_rows, _tree,
+from .row_attention import (_LENGTH_DTYPES, _NO_STRIDES, _ROW_DTYPES, _int32, _launch, _lengths, _repeats, _small_rows, _tree,
                             _unit_strides)
 
 MIN_PAGE = 16
@@ -76,7 +76,7 @@ def _check_table(table, rows, index):
 def _check_counts(counts, batch, index):
     if counts.shape != (batch,) or counts.get_device() != index or counts.dtype not in _LENGTH_DTYPES:
         raise ValueError("counts must be an int32 tensor [batch] on the pages' device")
-    return counts.to(torch.int32).contiguous()
+    return _int32(counts)
 
 
 def log_kv_paged_append(k, v, k_pages, v_pages, table, lengths, *, q=None, frequencies=None, positions=None, first=0,

@@ -77,13 +77,20 @@ def _contiguous_rows(x):
     return x.stride(2) == 1 or x.size(2) == 1
 
 
+def _int32(counts):
+    """Contiguous int32 rows; int64 ones beyond its range as its ends."""
+    if counts.dtype != torch.int32:
+        counts = counts.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
+    return counts.contiguous()
+
+
 def _lengths(lengths, batch, cap, index, room=0):
     """(int32 tensor or None, its address, its stride, added rows) of an int or an int tensor ``[B]``."""
     if isinstance(lengths, torch.Tensor):
         if lengths.shape != (batch,) or lengths.get_device() != index or lengths.dtype not in _LENGTH_DTYPES:
             raise ValueError("lengths must be an int or an int32 tensor [batch] on the cache's device")
         if lengths.dtype != torch.int32 or not lengths.is_contiguous():
-            lengths = lengths.to(torch.int32).contiguous()
+            lengths = _int32(lengths)
         return lengths, lengths.data_ptr(), 1, 0
     lengths = int(lengths)
     if not 0 <= lengths <= cap - room:
@@ -228,7 +235,7 @@ def log_kv_weight_attention(q, k, v, cache_k, cache_v, weights, lengths, scale, 
         if (counts.shape != (batch,) or counts.get_device() != cache_k.get_device()
                 or counts.dtype not in _LENGTH_DTYPES):
             raise ValueError("counts must be an int32 tensor [batch] on the cache's device")
-        counts = counts.to(torch.int32).contiguous()
+        counts = _int32(counts)
     return _attention(q, k, v, cache_k, cache_v, float(scale), lengths, q.size(2), counts=counts, weights=weights)
 
 
