@@ -13,7 +13,7 @@ import torch
 
 from ._lib import check_activation_dtype, refuse_tangents
 from .log_kv_cache import LogStructuredKVCache
-from .log_kv_pack import log_kv_prefix_attention
+from .log_kv_pack import _check_backend, log_kv_prefix_attention
 from .paged_attention import MIN_PAGE, SharedPrefix, log_kv_paged_append, log_kv_paged_attention
 from .rotary import log_kv_rotary
 from .row_attention import _ROW_DTYPES
@@ -218,11 +218,14 @@ class PagedKVCache:
         cache = source.cache if engine is not None else source
         if not isinstance(cache, LogStructuredKVCache):
             raise ValueError("a shared document is a LogKVStreamingAttention or a LogStructuredKVCache")
-        if self._prefix_pages or any(self._bound):
+        if self._prefix_pages or self._compressed is not None or any(self._bound):
             raise RuntimeError("a prefix comes before the sequences' rows and beside no other one: reset() the cache first")
+        _check_backend(cache.semantic_pack_backend)
         if (self.batch_size % cache.batch_size or cache.n_groups != self.n_groups or cache.k_dim != self.k_pages.size(3)
-                or cache.v_dim != self.v_pages.size(3) or self.k_pages.dtype != torch.bfloat16):
-            raise ValueError("a shared document has this cache's groups and widths, a batch that divides it, and bfloat16 rows")
+                or cache.v_dim != self.v_pages.size(3) or self.k_pages.dtype != torch.bfloat16
+                or cache.recent_k.device != self.k_pages.device):
+            raise ValueError("a shared document has this cache's groups, widths and device, a batch that divides it, and "
+                             "bfloat16 rows")
         pending = 0 if engine is None or engine._log_kv_pending is None else engine._log_kv_pending[0].size(2)
         self._compressed, self._first = (cache, engine), cache.token_count + pending
 
