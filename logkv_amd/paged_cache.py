@@ -91,6 +91,7 @@ class PagedKVCache:
 
     def free(self, sequences=None) -> None:
         """Drop the rows of ``sequences`` (indices; all without them), whose pages others may take. Prefixes stay."""
+        self._refuse_capture()
         rows = range(self.batch_size) if sequences is None else [int(b) for b in sequences]
         if any(not 0 <= b < self.batch_size for b in rows):
             raise ValueError("sequences must be indices of the batch")
@@ -107,6 +108,7 @@ class PagedKVCache:
 
     def trim(self) -> None:
         """Take back the pages that padded batches reserved and did not fill. Waits for the device, which knows how many."""
+        self._refuse_capture()
         for b, n in enumerate(self.lengths.tolist()):
             keep = -(-n // self.page_size)
             if keep < len(self._pages[b]):
@@ -159,10 +161,13 @@ class PagedKVCache:
             raise ValueError("queries and new rows must be on the cache's device")
         if shape[1] // self.n_groups * tokens * sharing > 2 ** 19:
             raise ValueError("too many queries a KV group at once: split the call")
+        self._refuse_capture()
+        return tokens
+
+    def _refuse_capture(self):
         if self.k_pages.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a PagedKVCache's calls cannot be captured: capture log_kv_paged_append and "
                                "log_kv_paged_attention on its tensors instead")
-        return tokens
 
     def _sharing(self):
         """Sequences behind one prefix, 1 without one."""

@@ -76,3 +76,22 @@ def test_steps(launches, at):
     lines = sum(cache._pages, [])
     assert len(set(lines)) == 8 and not set(lines) & set(cache._free)
     assert all(cache.table[b, :2].tolist() == cache._pages[b] for b in range(B)) and (cache.table[:, 2:] == -1).all()
+
+
+@pytest.mark.parametrize("name", ["free", "trim", "reset", "some"])
+def test_pages_are_not_taken_back_in_a_capture(launches, monkeypatch, name):
+    """The host would hand the pages out again at once, the device forget them at a replay."""
+    cache = new(pages=16)
+    call(cache, 4, 2, "prefix")
+    call(cache, 20)
+    before, pages = state(cache), cache.k_pages
+    cache.k_pages = pages.view(pages.shape).as_subclass(OnDevice)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="captured"):
+        cache.free([1]) if name == "some" else getattr(cache, name)()
+    cache.k_pages = pages
+    assert same(state(cache), before)
+
+
+class OnDevice(torch.Tensor):
+    is_cuda = True
