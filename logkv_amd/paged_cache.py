@@ -54,8 +54,11 @@ class PagedKVCache:
             raise ValueError("the cache must be bfloat16 or float16")
         if not 0.0 < scale < math.inf or not math.isfinite(amplitude):
             raise ValueError("attention scale must be positive, amplitude finite")
-        if frequencies is not None and (frequencies.ndim != 1 or 2 * frequencies.numel() > k_dim):
-            raise ValueError("frequencies must be [rotated features / 2] for at most the keys' features")
+        if frequencies is not None and (frequencies.ndim != 1 or 2 * frequencies.numel() > k_dim
+                                        or frequencies.dtype not in (torch.float64, torch.float32)):
+            raise ValueError("frequencies must be float64 or float32 [rotated features / 2] for at most the keys' features")
+        if frequencies is not None and frequencies.requires_grad:
+            raise NotImplementedError("frequencies have no gradient")
         self.batch_size, self.n_groups, self.page_size, self.max_rows = batch_size, n_groups, page_size, max_rows
         self.scale, self.interleaved, self.amplitude = float(scale), bool(interleaved), float(amplitude)
         self.frequencies = None if frequencies is None else frequencies.to(device)

@@ -95,3 +95,11 @@ def test_pages_are_not_taken_back_in_a_capture(launches, monkeypatch, name):
 
 class OnDevice(torch.Tensor):
     is_cuda = True
+
+
+def test_frequencies_that_every_call_would_refuse():
+    for frequencies, kind in ((torch.ones(4, dtype=torch.int64), ValueError), (torch.ones(4, dtype=torch.bfloat16), ValueError),
+                              (torch.ones(4, requires_grad=True), NotImplementedError)):
+        with pytest.raises(kind, match="frequencies"):
+            new(frequencies=frequencies)
+    assert new(frequencies=torch.ones(4)).frequencies.dtype == torch.float32
