@@ -127,7 +127,8 @@ class PagedKVCache:
         """Pages for ``rows[i]`` rows of every line, returned as (line, place, page); too few of them change nothing."""
         need = [max(0, -(-n // self.page_size) - len(line)) for line, n in zip(lines, rows)]
         if sum(need) > len(self._free):
-            raise RuntimeError(f"the pool has {len(self._free)} pages left, {sum(need)} are needed")
+            raise RuntimeError(f"the pool has {len(self._free)} pages left, {sum(need)} are needed"
+                               " (trim() takes back what padded batches left unused)")
         places = [(i, len(line) + j) for i, (line, n) in enumerate(zip(lines, need)) for j in range(n)]
         new = [(*x, page) for x, page in zip(places, reversed(self._free))]
         if new:
@@ -252,7 +253,8 @@ class PagedKVCache:
     @torch.no_grad()
     def __call__(self, q, k, v, counts=None):
         """Attention ``[batch, n_heads, T, v_dim]`` of T new tokens, which join the cache. ``counts`` (int32 ``[batch]`` on
-        the device) gives the tokens that exist per sequence of a padded batch."""
+        the device) gives the tokens that exist per sequence of a padded batch; the host, which does not wait for them, counts
+        all T against ``max_rows`` and the pool until ``trim``."""
         tokens = self._check(q, k, v, self.batch_size, self._sharing())
         if counts is not None:
             if (counts.shape != (self.batch_size,) or counts.dtype not in (torch.int32, torch.int64)
@@ -260,7 +262,8 @@ class PagedKVCache:
                 raise ValueError("counts must be an int32 tensor [batch] on the cache's device")
             counts = counts.clamp(0, tokens).to(torch.int32)
         if max(self._bound) + tokens > self.max_rows:
-            raise RuntimeError(f"a sequence has at most {self.max_rows} rows: {max(self._bound)} may be in use, {tokens} are new")
+            raise RuntimeError(f"a sequence has at most {self.max_rows} rows: {max(self._bound)} may be in use, {tokens} are new"
+                               " (trim() counts anew what padded batches left unused)")
         new = self._reserve(self._pages, self.table, [n + tokens for n in self._bound])
         try:
             q, stored = self._append(q, k, v, self.table, self.lengths, first=self._first, counts=counts)

@@ -103,3 +103,22 @@ def test_frequencies_that_every_call_would_refuse():
         with pytest.raises(kind, match="frequencies"):
             new(frequencies=frequencies)
     assert new(frequencies=torch.ones(4)).frequencies.dtype == torch.float32
+
+
+def test_padded_batches_are_told_of_trim(launches):
+    """Padding counts until trim(), which the errors name; after it the calls go on."""
+    cache = new(pages=16)
+    counts = torch.tensor([1, 0, 2, 1], dtype=torch.int32)
+    for _ in range(4):
+        call(cache, 16, counts=counts)
+    with pytest.raises(RuntimeError, match=r"trim\(\)"):      # 64 of 64 rows may be in use
+        call(cache, 1)
+    cache.trim()
+    assert cache.lengths.tolist() == [4, 0, 8, 4] and cache.free_pages == 13
+    call(cache, 16)
+    cache = new(pages=4)
+    call(cache, 16, counts=counts)
+    with pytest.raises(RuntimeError, match=r"trim\(\)"):
+        call(cache, 16, counts=counts)
+    cache.trim()
+    call(cache, 1, counts=counts)
