@@ -127,6 +127,12 @@ typedef struct logkv_paged_args {
 /* Scratch of one call. */
 int64_t logkv_paged_workspace_bytes(const logkv_paged_args* args);
 
+/* How a call of these sizes is run (no buffer is needed or read), four numbers for the pass over the
+ * sequences' own rows, then four for the prefixes' (zeros without one): waves of 32 queries in a block
+ * of the tiled kernel, or 0; columns of 16 queries in a block of the streamed kernel, or 0; shares that
+ * a lane's rows are dealt in; the most that one may take where tensors of lengths deal them anew. */
+int logkv_paged_plan(const logkv_paged_args* args, int32_t plan[8]);
+
 int logkv_paged_attention(const logkv_paged_args* args, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

@@ -66,6 +66,7 @@ SIGNATURES = {
     "logkv_rotary": (_i32, [_p, _p]),
     "logkv_paged_append": (_i32, [_p, _p]),
     "logkv_paged_workspace_bytes": (_i64, [_p]),
+    "logkv_paged_plan": (_i32, [_p, _p]),
     "logkv_paged_attention": (_i32, [_p, _p, _i64, _p]),
 }
 

@@ -1012,6 +1012,21 @@ int64_t logkv_paged_workspace_bytes(const logkv_paged_args* a) {
   return p.bytes;
 }
 
+int logkv_paged_plan(const logkv_paged_args* a, int32_t* plan) {
+  if (int rc = check_paged_shape(a)) return rc;
+  if (!plan) return fail(LOGKV_EINVAL, "paged attention plan is NULL");
+  const logkv::PagedLaunch p = logkv::paged_launch(*a, nullptr);
+  if (p.blocks > logkv::kMostPagedBlocks) return too_many_blocks();
+  for (const logkv::PagedPass* pass : {&p.own, &p.shared}) {
+    const logkv::RowsLaunch& r = pass->launch;
+    *plan++ = r.q_waves;
+    *plan++ = r.q_waves ? 0 : r.cols;
+    *plan++ = r.splits;
+    *plan++ = r.room;
+  }
+  return LOGKV_OK;
+}
+
 int logkv_paged_attention(const logkv_paged_args* a, void* ws, int64_t ws_bytes, void* stream) {
   int rc = check_paged(a);
   if (rc) return rc;

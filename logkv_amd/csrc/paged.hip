@@ -8,8 +8,8 @@
 // kernels over a page table, in one launch where their kernels go together; this file joins their partials.
 // An infinity or NaN in V is left out of a pass's products, which would spread it to queries that do not
 // see its row. Every query of a lane sees the same cache rows: a share that met some in them looks at its rows
-// once more and leaves the features that they are in, and the join adds those (time of the share once more, by
-// what the rows' loads take). Those of the call's rows, which queries see by their place or mask, the join looks
+// once more and leaves the features that they are in, and the join adds those: a call with one among 32768 shared
+// rows of 128 features 76 us, without 32; among 2^19 rows of 64 265 and 95. Those of the call's rows, which queries see by their place or mask, the join looks
 // for in the call's rows themselves: up to tq rows a query, four at a time.
 //
 // 64 sequences of 32 heads over 16384 shared rows and 2000 of their own (8 KV groups, 128 features): 112 us, 4.1 TB/s. 8
