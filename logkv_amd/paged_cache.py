@@ -95,9 +95,12 @@ class PagedKVCache:
     def free(self, sequences=None) -> None:
         """Drop the rows of ``sequences`` (indices; all without them), whose pages others may take. Prefixes stay."""
         self._refuse_capture()
-        rows = range(self.batch_size) if sequences is None else [int(b) for b in sequences]
-        if any(not 0 <= b < self.batch_size for b in rows):
-            raise ValueError("sequences must be indices of the batch")
+        rows = range(self.batch_size)
+        if sequences is not None:
+            given = sequences.tolist() if hasattr(sequences, "tolist") else list(sequences)
+            rows = [b.item() if hasattr(b, "item") else b for b in (given if isinstance(given, list) else [given])]
+            if any(not isinstance(b, int) or isinstance(b, bool) or not 0 <= b < self.batch_size for b in rows):
+                raise ValueError("sequences must be indices of the batch")
         if sequences is None:
             self.lengths.zero_()
             self.table.fill_(-1)

@@ -122,3 +122,20 @@ def test_padded_batches_are_told_of_trim(launches):
         call(cache, 16, counts=counts)
     cache.trim()
     call(cache, 1, counts=counts)
+
+
+def test_sequences_to_free_are_indices(launches):
+    """A mask's truth values were taken for the indices 0 and 1, numbers with a fraction for those below."""
+    cache = new(pages=16)
+    call(cache, 20)
+    before = state(cache)
+    mask = [False, False, True, False]
+    for bad in (mask, torch.tensor(mask), [1.5], torch.tensor([1.0]), [[1]], [torch.tensor(True)], [-1], ["1"]):
+        with pytest.raises(ValueError, match="indices"):
+            cache.free(bad)
+    assert same(state(cache), before)
+    for some, left in ((torch.tensor([2]), [20, 20, 0, 20]), ((0, torch.tensor(2)), [0, 20, 0, 20]), (torch.tensor(3), [0, 20, 0, 0]),
+                       ((), [0, 20, 0, 0]), (iter([1]), [0] * B)):
+        cache.free(some)
+        assert cache.lengths.tolist() == cache._bound == left
+    assert cache.free_pages == 16
