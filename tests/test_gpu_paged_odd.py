@@ -112,3 +112,36 @@ def test_time_of_long_rows(T, H):
         want[..., 9] = math.inf
         assert torch.equal(call(p), want)
         assert ms(p) < 20 * clean[1][p] + 2.0
+
+
+@pytest.mark.parametrize("T,H", [(1, 2), (60, 4)])
+def test_captured_while_values_come_and_go(T, H):
+    """What a share left of its rows is read only beside that call's note: replays, two graphs and a side stream agree with
+    eager calls while infinities appear in the pages and vanish."""
+    c = Case(4, H, 1, T, 128, 128, 16, [33, 5, 600, 0], [700, 90])
+    c()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = c()
+        graphs.append((graph, out))
+    clean = c()
+    places = [(c.prefix_table[0, 40], 3, 7, math.inf), (c.table[2, 30], 15, 64, -math.inf), (c.prefix_table[1, 2], 0, 0, math.nan), None]
+    for place in places * 2:
+        kept = c.vp.clone()
+        if place is not None:
+            page, slot, feature, value = place
+            c.vp[page, :, slot, feature] = value
+        want = c()
+        assert torch.equal(want, clean) == (place is None)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            beside = c()
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for out in (beside, *(out for _, out in graphs)):
+            assert torch.equal(out.nan_to_num(7.0), want.nan_to_num(7.0)) and torch.equal(out.isnan(), want.isnan())
+        c.vp.copy_(kept)
