@@ -8,13 +8,13 @@
 // kernels over a page table, in one launch where their kernels go together; this file joins their partials.
 // An infinity or NaN in V is left out of a pass's products, which would spread it to queries that do not
 // see its row. Every query of a lane sees the same cache rows: a share that met some in them looks at its rows
-// once more and leaves the features that they are in, and the join adds those: a call with one among 32768 shared
-// rows of 128 features 76 us, without 32; among 2^19 rows of 64 265 and 95. Those of the call's rows, which queries see by their place or mask, the join looks
-// for in the call's rows themselves: up to tq rows a query, four at a time.
+// once more and leaves the features that they are in, and the join adds those. A call with one among 32768 shared
+// rows of 128 features takes 76 us, without 32; among 2^19 rows of 64 features 265 and 95. Those of the call's rows,
+// which queries see by their place or mask, the join looks for itself: up to tq rows a query, four at a time.
 //
-// 64 sequences of 32 heads over 16384 shared rows and 2000 of their own (8 KV groups, 128 features): 112 us, 4.1 TB/s. 8
-// sequences of 256 tokens x 16 heads over 32768 shared rows: 876 us, 630 TFLOP/s. Bound by what bounds the passes; few
-// queries by the launches, 8 us of the first and 6 of the join for 4 sequences over 2048 rows.
+// 64 sequences of 32 heads over 16384 shared rows and 2000 of their own (8 KV groups, 128 features): 110 us, 4.2 TB/s. 8
+// sequences of 256 tokens x 16 heads over 32768 shared rows: 862 - 912 us, 605 - 640 TFLOP/s. Bound by what bounds the passes; few
+// queries by the launches, 9 us of the first and 4 of the join for 4 sequences over 2048 rows.
 #include <algorithm>
 #include <array>
 #include <cmath>
@@ -317,10 +317,12 @@ double finished(double n, double tn, double m, double tm, int slots) {
   return std::max(end, best);
 }
 
-// The plan of least time for two passes in one launch, whose blocks run side by side: when the last one ends, the CUs'
-// work, memory's time (a tenth of the less of the two beside the other), and the partials' way out and in. 16 shapes of
+// The plan of least time for two passes in one launch, whose blocks run side by side: when the last one ends, the CUs' work, memory's time (a tenth of the less of the two beside the other), and the partials' way out and in. 16 shapes of
 // 24 to 256 queries over 1024 to 30000 rows ran within 5% (mean) of their best kernels and shares so. Rows wider than 128
-// features: both passes by one kernel (the two side by side take more registers than two waves a SIMD have).
+// features: both passes by one kernel (the two side by side take more registers than two waves a SIMD have). Rows are
+// taken to fill the tables, since the lengths are on the device; where they do not, shares are too few: 24 sequences of 7
+// tokens over 8192 shared rows of 64 features with 200 of their own 35 us behind a table cut to them, 134 behind one of
+// 32768 rows.
 PagedPlan plan_passes(const PagedPass& own, const PagedPass& shared) {
   static constexpr int kShares[] = {1, 2, 3, 4, 6, 8, 10, 12, 14, 16, 18, 20, 22, 24, 28, 32, 40, 48, 56, 64};
   static constexpr int kWaves[] = {0, 2, 4, 8};

@@ -237,8 +237,9 @@ def log_kv_paged_attention(q, k, v, k_pages, v_pages, table, lengths, scale, *, 
     or ``[B, T, T]``) shows it, as a drafted tree's ancestors and itself. ``counts`` (int32 ``[B]``, not with
     ``visible``) gives the tokens that exist per sequence of a padded batch: the others' outputs are zeros.
 
-    A token that sees nothing gets zeros, and what hidden rows and unused slots hold (NaN, infinities) reaches no
-    output; a table's entry outside the pool stands for a page of zeros. Queries and rows of another activation dtype are
+    Work is dealt out for rows that fill ``table`` and the prefix's capacity (lengths are not waited for): tables cut to
+    the pages in use are up to four times faster than ones with much room to grow. A token that sees nothing gets zeros, and
+    what hidden rows and unused slots hold (NaN, infinities) reaches no output; a table's entry outside the pool stands for a page of zeros. Queries and rows of another activation dtype are
     rounded to the pages', and the output is returned in the queries'. The pages are only read."""
     return _paged_attention(q, k, v, k_pages, v_pages, table, lengths, float(scale), prefix, visible, counts, None)
 
