@@ -13,8 +13,8 @@
 // which queries see by their place or mask, the join looks for itself: up to tq rows a query, four at a time.
 //
 // 64 sequences of 32 heads over 16384 shared rows and 2000 of their own (8 KV groups, 128 features): 110 us, 4.2 TB/s. 8
-// sequences of 256 tokens x 16 heads over 32768 shared rows: 862 - 912 us, 605 - 640 TFLOP/s. Bound by what bounds the passes; few
-// queries by the launches, 9 us of the first and 4 of the join for 4 sequences over 2048 rows.
+// sequences of 256 tokens x 16 heads over 32768 shared rows: 862 - 912 us, 605 - 640 TFLOP/s. Bound by what bounds the
+// passes; few queries by the launches, 9 us of the first and 4 of the join for 4 sequences over 2048 rows.
 #include <algorithm>
 #include <array>
 #include <cmath>

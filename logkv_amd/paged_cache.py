@@ -265,8 +265,8 @@ class PagedKVCache:
                 raise ValueError("counts must be an int32 tensor [batch] on the cache's device")
             counts = counts.clamp(0, tokens).to(torch.int32)
         if max(self._bound) + tokens > self.max_rows:
-            raise RuntimeError(f"a sequence has at most {self.max_rows} rows: {max(self._bound)} may be in use, {tokens} are new"
-                               " (trim() counts anew what padded batches left unused)")
+            raise RuntimeError(f"a sequence has at most {self.max_rows} rows: {max(self._bound)} may be in use, {tokens} are "
+                               "new (trim() counts anew what padded batches left unused)")
         new = self._reserve(self._pages, self.table, [n + tokens for n in self._bound])
         try:
             q, stored = self._append(q, k, v, self.table, self.lengths, first=self._first, counts=counts)
